@@ -1,0 +1,682 @@
+"""The operators of a decode step over a cache held in 4 bits, as cases to be timed.
+
+A long-context request is served in these steps: its prompt's keys are rotated
+(``rotate``) and cached in 4 bits (``write``), each new token is rotated and
+appended (``append``), attends to the 4-bit history and the exact FP16 pages
+(``attend``), and the logits of its position are shaped before the next token
+is picked (``logits``).  Shapes are those of the package's own configurations
+(32 query heads, 8 KV heads, head_dim 128, 16-token pages, 32768 tokens of
+vocabulary) and the ranges around them.
+
+``run`` computes an operator in plain torch, or where ``own`` is set calls the
+package's.  What is held in 4 bits comes back as the values it stands for.
+
+4-bit pages: ``codes`` uint8 [pages, Hkv, 2, 1024] and ``scales`` FP16
+[pages, Hkv, 4, 2, 4] (token group, K or V, token of the group).  A nibble
+holds code + 8, code in [-7, 7], and stands for code * scale of its token and
+head.  K nibbles lie as [kg 4][token 16][w 4][dims], dims 32 w + 8 kg + e; V
+nibbles as [kg 4][n 16][j 4][tokens, channels], tokens 4 kg + t of channels
+8 n + 2 j + ab.
+"""
+
+import math
+import random
+
+import torch
+
+own = False
+
+DIM, PAGE, RING = 128, 16, 16        # head_dim, tokens of a page, exact pages of a request
+WORKSPACE_BYTES = 256 << 20
+THETA = 1.0e6
+DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+def listed():
+    return [
+        # one decode step of eight requests far into a scaled context, half of
+        # each head rotated, neighbouring dims paired: latency counts
+        {"name": "rotate_b8", "op": "rotate", "tokens": 8, "q_heads": 32, "kv_heads": 8,
+         "dim": 128, "part": 64, "layout": "interleaved", "scaling": "linear", "dtype": "bf16",
+         "far": 1000000},
+        # a 16K prompt, whole heads, the context stretched in parts
+        {"name": "rotate_16k", "op": "rotate", "tokens": 16384, "q_heads": 32, "kv_heads": 8,
+         "dim": 128, "part": 128, "layout": "half", "scaling": "by_parts", "dtype": "fp16",
+         "far": 131072},
+        # a short prompt that ends inside a page, and the benchmark's 16K
+        # prompt, into the cache and back (a prompt that continues them)
+        {"name": "write_1000", "op": "write", "tokens": 1000, "kv_heads": 8, "centers": True},
+        {"name": "write_16k", "op": "write", "tokens": 16384, "kv_heads": 8, "centers": True},
+        # the cache update of eight requests that all close a page, and of a
+        # serving batch at positions of its own
+        {"name": "append_b8", "op": "append", "batch": 8, "q_heads": 32, "kv_heads": 8,
+         "closing": True, "far": 131072},
+        {"name": "append_b256", "op": "append", "batch": 256, "q_heads": 32, "kv_heads": 8,
+         "closing": False, "far": 32768},
+        # a chat turn, the benchmark's 49K request, its ragged batch of eight
+        # and its serving batch, all with exact tails
+        {"name": "attend_b1_4k", "op": "attend", "batch": 1, "low": 4096, "high": 4096,
+         "kv_heads": 8, "group": 4, "tail": True, "ragged": 0},
+        {"name": "attend_b1_49k", "op": "attend", "batch": 1, "low": 49152, "high": 49152,
+         "kv_heads": 8, "group": 4, "tail": True, "ragged": 0},
+        {"name": "attend_b8_ragged", "op": "attend", "batch": 8, "low": 4096, "high": 32768,
+         "kv_heads": 8, "group": 4, "tail": True, "ragged": 1},
+        {"name": "attend_b256", "op": "attend", "batch": 256, "low": 512, "high": 4096,
+         "kv_heads": 8, "group": 4, "tail": True, "ragged": 2},
+        # one user with a 16K history at the package's vocabulary; a serving
+        # batch at a large one
+        {"name": "logits_b1", "op": "logits", "batch": 1, "vocab": 32768, "history": 16384,
+         "biases": 16, "mask": True, "dtype": "fp32"},
+        {"name": "logits_b64", "op": "logits", "batch": 64, "vocab": 131072, "history": 4096,
+         "biases": 64, "mask": True, "dtype": "fp32"},
+    ]
+
+
+def draw(rng):
+    def spread(low, high):
+        return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+    op = rng.choice(["rotate", "write", "append", "attend", "attend", "logits"])
+    if op == "rotate":
+        kv_heads = rng.choice([1, 2, 4, 8])
+        dim = rng.choice([64, 80, 96, 128, 256])
+        group = rng.choice([1, 2, 4, 8])
+        dtype = rng.choice(["fp16", "bf16", "fp32"])
+        wide = (group + 1) * kv_heads * dim * (2 if dtype == "fp32" else 1)
+        return {"op": op, "tokens": spread(1, max(1, 16384 * 40 * 128 // max(wide, 5120))),
+                "q_heads": group * kv_heads, "kv_heads": kv_heads, "dim": dim,
+                "part": rng.choice([dim, dim, dim // 2, 32]),
+                "layout": rng.choice(["half", "interleaved"]),
+                "scaling": rng.choice(["none", "linear", "ntk", "by_parts"]), "dtype": dtype,
+                "far": spread(64, 2000000)}
+    if op == "write":
+        heads = rng.choice([1, 2, 4, 8, 8, 16])
+        return {"op": op, "tokens": spread(1, 131072 // max(8, heads)), "kv_heads": heads,
+                "centers": rng.random() < 0.75}
+    if op == "append":
+        heads = rng.choice([1, 2, 4, 8, 8])
+        return {"op": op, "batch": spread(1, 256), "q_heads": heads * rng.choice([1, 2, 4]),
+                "kv_heads": heads, "closing": rng.random() < 0.5, "far": spread(64, 1000000)}
+    if op == "attend":
+        heads, group = rng.choice([(8, 4), (8, 4), (8, 8), (4, 8), (2, 16), (16, 1), (1, 6), (5, 3)])
+        batch = spread(1, 256)
+        top = min(131072, 560000 // batch) * 8 // max(8, heads)
+        high = spread(min(1024, top), top)
+        return {"op": op, "batch": batch, "low": spread(min(288, high), high), "high": high,
+                "kv_heads": heads, "group": group, "tail": rng.random() < 0.75,
+                "ragged": rng.randrange(1 << 20)}
+    batch = spread(1, 64)
+    return {"op": op, "batch": batch, "vocab": spread(1000, 131072), "history": spread(1, 16384),
+            "biases": rng.choice([0, 1, 16, 64]), "mask": rng.random() < 0.75,
+            "dtype": rng.choice(["fp32", "fp32", "fp16", "bf16"])}
+
+
+# -- sizes -------------------------------------------------------------------
+
+def _lengths(case):
+    rng = random.Random(case["ragged"])
+    return [rng.randint(case["low"], case["high"]) for _ in range(case["batch"])]
+
+
+def _segments(case):
+    """(history tokens, exact tokens) of each request: the newest 16 pages, the
+    last perhaps partial, are exact; without a tail all are history."""
+    lengths = _lengths(case)
+    if not case["tail"]:
+        return [(n, 0) for n in lengths]
+    pages = [-(-n // PAGE) for n in lengths]
+    old = [max(0, p - RING) * PAGE for p in pages]
+    return [(o, n - o) for o, n in zip(old, lengths)]
+
+
+def work(case):
+    op = case["op"]
+    if op == "rotate":
+        size = 4 if case["dtype"] == "fp32" else 2
+        values = case["tokens"] * (case["q_heads"] + case["kv_heads"]) * case["dim"]
+        return {"bytes": 2 * values * size + 4 * case["tokens"], "flops": 3.0 * values}
+    if op == "write":
+        rows = 2 * case["tokens"] * case["kv_heads"]
+        # in FP16, the codes and scales, and back in FP16
+        return {"bytes": rows * (2 * DIM * 2 + DIM // 2 + 2), "flops": 6.0 * rows * DIM}
+    if op == "append":
+        b, hkv = case["batch"], case["kv_heads"]
+        closing = b if case["closing"] else -(-b // PAGE)
+        return {"bytes": b * (2 * case["q_heads"] * DIM * 2 + 6 * hkv * DIM * 2)
+                + closing * hkv * 2 * (PAGE * (DIM * 2 + 2 + DIM // 2))
+                + b * hkv * 2 * PAGE * (DIM // 2 + 2 + DIM * 2),
+                "flops": 8.0 * b * (case["q_heads"] + hkv) * DIM}
+    if op == "attend":
+        hkv, hq = case["kv_heads"], case["kv_heads"] * case["group"]
+        old, exact = (sum(n) for n in zip(*_segments(case)))
+        return {"bytes": old * hkv * 2 * (DIM // 2 + 2) + exact * hkv * 2 * DIM * 2
+                + (old + exact) // 4 + case["batch"] * (hq * (DIM * 4 + 4) + hkv * DIM * 2),
+                "flops": 4.0 * (old + exact) * hq * DIM}
+    size = 4 if case["dtype"] == "fp32" else 2
+    values = case["batch"] * case["vocab"]
+    return {"bytes": 2 * values * size + (values // 8 if case["mask"] else 0)
+            + case["batch"] * (6 * case["history"] + 12 * case["biases"]),
+            "flops": 6.0 * values}
+
+
+# -- inputs ------------------------------------------------------------------
+
+def _generator(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _rows(gen, *shape):
+    """Keys or values of N(0, 1), 8 times larger on 4 of 128 channels, around
+    channel means."""
+    x = torch.randn(*shape, generator=gen, device="cuda")
+    gain = torch.ones(shape[-1], device="cuda")
+    gain[torch.randperm(shape[-1], generator=gen, device="cuda")[:4]] = 8.0
+    return x.mul_(gain).add_(torch.randn(shape[-2:], generator=gen, device="cuda").mul_(0.5)).half()
+
+
+def _pool(gen, tokens, heads):
+    """Codes and scales of pages of such rows."""
+    pages = -(-tokens // PAGE)
+    k = _rows(gen, pages * PAGE, heads, DIM).float()
+    k -= k.mean(0)
+    kc, ks = _codes(k)
+    v = _rows(gen, pages * PAGE, heads, DIM).float()
+    v -= v.mean(0)
+    vc, vs = _codes(v)
+    return _pack(kc, vc), _pack_scales(ks, vs)
+
+
+def _rotary(case):
+    """Arguments of the rotary embedding of a case."""
+    return {"head_dim": case.get("dim", DIM), "rotary_dim": case.get("part", DIM), "theta": THETA,
+            "layout": case.get("layout", "half"), "scaling": case.get("scaling", "none"),
+            "factor": 1.0 if case.get("scaling", "none") == "none" else 8.0,
+            "original_context": 32768}
+
+
+def _inputs(case, seed):
+    gen = _generator(seed)
+    op = case["op"]
+    s = {"op": op}
+    if op == "rotate":
+        dtype = DTYPES[case["dtype"]]
+        tokens, hq, hkv, dim = case["tokens"], case["q_heads"], case["kv_heads"], case["dim"]
+        # query and key rows of one fused projection
+        qkv = torch.randn(tokens, (hq + 2 * hkv) * dim, generator=gen, device="cuda").to(dtype)
+        s["query"] = qkv[:, :hq * dim].view(tokens, hq, dim)
+        s["key"] = qkv[:, hq * dim:(hq + hkv) * dim].view(tokens, hkv, dim)
+        first = max(0, case["far"] - tokens)
+        s["positions"] = torch.arange(first, first + tokens, device="cuda", dtype=torch.int32)
+        s["rotary"] = _rotary(case)
+    elif op == "write":
+        tokens, heads = case["tokens"], case["kv_heads"]
+        pages = -(-tokens // PAGE)
+        s["key"] = _rows(gen, tokens, heads, DIM)
+        s["value"] = _rows(gen, tokens, heads, DIM)
+        s["centers"] = ([t.float().mean(0).half() for t in (s["key"], s["value"])]
+                        if case["centers"] else [None, None])
+        s["page_ids"] = torch.randperm(pages, generator=gen, device="cuda").int()
+        s["codes"] = torch.zeros(pages, heads, 2, 1024, device="cuda", dtype=torch.uint8)
+        s["scales"] = torch.zeros(pages, heads, 4, 2, 4, device="cuda", dtype=torch.float16)
+    elif op == "append":
+        batch, hq, hkv = case["batch"], case["q_heads"], case["kv_heads"]
+        qkv = torch.randn(batch, (hq + 2 * hkv) * DIM, generator=gen, device="cuda").half()
+        s["query"] = qkv[:, :hq * DIM].view(batch, hq, DIM)
+        s["key"] = qkv[:, hq * DIM:(hq + hkv) * DIM].view(batch, hkv, DIM)
+        s["value"] = qkv[:, (hq + hkv) * DIM:].view(batch, hkv, DIM)
+        pos = torch.randint(0, case["far"], (batch,), generator=gen, device="cuda")
+        s["positions"] = (pos // PAGE * PAGE + 15 if case["closing"] else pos).int()
+        s["centers"] = [torch.randn(batch, hkv, DIM, generator=gen, device="cuda").mul_(0.3).half()
+                        for _ in range(2)]
+        s["exact"] = [_rows(gen, batch * PAGE, hkv, DIM).view(batch, PAGE, hkv, DIM)
+                      for _ in range(2)]
+        s["exact_ids"] = torch.randperm(batch, generator=gen, device="cuda").int()
+        s["code_ids"] = torch.randperm(batch, generator=gen, device="cuda").int()
+        s["codes"], s["scales"] = _pool(gen, batch * PAGE, hkv)
+        s["rotated_query"] = torch.empty(batch, hq, DIM, device="cuda", dtype=torch.float16)
+        s["rotary"] = _rotary(case)
+    elif op == "attend":
+        batch, hkv, hq = case["batch"], case["kv_heads"], case["kv_heads"] * case["group"]
+        segments = _segments(case)
+        s["query"] = torch.randn(batch, hq, DIM, generator=gen, device="cuda").half()
+        s["center"] = torch.randn(batch, hkv, DIM, generator=gen, device="cuda").mul_(0.3).half()
+        pages = [-(-o // PAGE) for o, _ in segments]
+        s["codes"], s["scales"] = _pool(gen, max(1, sum(pages)) * PAGE, hkv)
+        s["table"] = _table(gen, pages, [o for o, _ in segments])
+        s["tail"] = s["exact"] = None
+        if case["tail"]:
+            exact = [-(-e // PAGE) for _, e in segments]
+            s["tail"] = _table(gen, exact, [e for _, e in segments])
+            s["exact"] = [_rows(gen, sum(exact) * PAGE, hkv, DIM).view(-1, PAGE, hkv, DIM)
+                          for _ in range(2)]
+    else:
+        batch, vocab, history = case["batch"], case["vocab"], case["history"]
+        s["logits"] = (torch.randn(batch, vocab, generator=gen, device="cuda") * 3).to(
+            DTYPES[case["dtype"]])
+        # frequent tokens recur: half of a history lies in 1/64 of the vocabulary
+        ids = torch.randint(0, vocab, (batch, history), generator=gen, device="cuda")
+        often = torch.rand(batch, history, generator=gen, device="cuda") < 0.5
+        s["history"] = torch.where(often, ids // 64, ids)
+        s["lengths"] = torch.randint(history // 2, history + 1, (batch,), generator=gen,
+                                     device="cuda").int()
+        s["prompts"] = s["lengths"] // 2
+        s["repetition"] = torch.rand(batch, generator=gen, device="cuda") * 0.5 + 1.0
+        s["frequency"] = torch.rand(batch, generator=gen, device="cuda") * 0.5
+        s["presence"] = torch.rand(batch, generator=gen, device="cuda")
+        s["bias_tokens"] = s["bias_values"] = s["allowed"] = None
+        if case["biases"]:
+            # distinct tokens of each request
+            spot = torch.randint(0, max(1, vocab // case["biases"]), (batch, case["biases"]),
+                                 generator=gen, device="cuda")
+            s["bias_tokens"] = spot + torch.arange(case["biases"], device="cuda") * max(
+                1, vocab // case["biases"])
+            s["bias_values"] = torch.randn(batch, case["biases"], generator=gen, device="cuda")
+        if case["mask"]:
+            s["allowed"] = torch.randint(-(1 << 31), 1 << 31, (batch, -(-vocab // 32)),
+                                         generator=gen, device="cuda").int()
+    return s
+
+
+def _table(gen, pages, tokens):
+    """A page table over a shuffled pool: host indptr, ids and last lengths."""
+    indptr = [0]
+    for p in pages:
+        indptr.append(indptr[-1] + p)
+    last = [(n - 1) % PAGE + 1 if n else 0 for n in tokens]
+    return {"indptr": torch.tensor(indptr, dtype=torch.int32),
+            "indices": torch.randperm(max(1, indptr[-1]), generator=gen, device="cuda").int(),
+            "last": torch.tensor(last, dtype=torch.int32, device="cuda")}
+
+
+def prepare(case, seed):
+    s = _inputs(case, seed)
+    if own:
+        # what a program keeps: the rotary tables, or the attention's plan
+        if case["op"] in ("rotate", "append"):
+            from pagegauge_amd.rotary import RotaryEmbedding
+
+            s["embedding"] = RotaryEmbedding(**s["rotary"], device="cuda")
+        elif case["op"] == "attend":
+            from pagegauge_amd.int4 import Int4PagedDecode
+
+            s["decode"] = Int4PagedDecode(torch.empty(WORKSPACE_BYTES, device="cuda",
+                                                      dtype=torch.uint8))
+            table, tail = s["table"], s["tail"]
+            s["decode"].plan(table["indptr"], table["indices"], table["last"],
+                             *(() if tail is None else (tail["indptr"], tail["indices"],
+                                                        tail["last"])),
+                             num_qo_heads=case["kv_heads"] * case["group"],
+                             num_kv_heads=case["kv_heads"])
+    else:
+        # its plain counterpart: each request's pages, padded to the longest
+        if case["op"] == "attend":
+            for name in ("table", "tail"):
+                if s[name] is not None:
+                    s[name].update(_padded(s[name]))
+    return s
+
+
+def run(s):
+    if own:
+        return _OWN[s["op"]](s)
+    return _PLAIN[s["op"]](s)
+
+
+# -- the package's calls -------------------------------------------------------
+
+def _own_rotate(s):
+    return s["embedding"].rotate(s["query"], s["key"], s["positions"])
+
+
+def _own_write(s):
+    from pagegauge_amd import int4
+
+    kc, vc = s["centers"]
+    int4.quantize_pages(s["key"], s["value"], s["codes"], s["scales"], page_ids=s["page_ids"],
+                        key_center=kc, value_center=vc)
+    key, value = int4.dequantize_pages(s["codes"], s["scales"], s["page_ids"],
+                                       tokens=s["key"].shape[0], key_center=kc, value_center=vc)
+    return key, value, s["scales"]
+
+
+def _own_append(s):
+    from pagegauge_amd import int4
+
+    int4.rope_append(s["embedding"], s["query"], s["key"], s["value"], s["positions"],
+                     s["exact_ids"], s["code_ids"], s["centers"][0], s["centers"][1],
+                     s["rotated_query"], s["exact"][0], s["exact"][1], s["codes"], s["scales"])
+    key, value = int4.dequantize_pages(s["codes"], s["scales"], s["code_ids"])
+    return s["rotated_query"], s["exact"][0], s["exact"][1], key, value
+
+
+def _own_attend(s):
+    return s["decode"].run(s["query"], s["codes"], s["scales"], s["exact"],
+                           value_center=s["center"], return_lse=True)
+
+
+def _own_logits(s):
+    from pagegauge_amd.logits import shape_logits
+
+    return shape_logits(s["logits"], history=s["history"], history_lengths=s["lengths"],
+                        prompt_lengths=s["prompts"], repetition=s["repetition"],
+                        frequency=s["frequency"], presence=s["presence"],
+                        bias_tokens=s["bias_tokens"], bias_values=s["bias_values"],
+                        allowed=s["allowed"])
+
+
+_OWN = {"rotate": _own_rotate, "write": _own_write, "append": _own_append, "attend": _own_attend,
+        "logits": _own_logits}
+
+
+# -- plain forms ---------------------------------------------------------------
+
+def _frequencies(rotary):
+    """Radians per position of each pair, and the amplitude, in 64 bits."""
+    r, theta, factor = rotary["rotary_dim"], rotary["theta"], rotary["factor"]
+    if rotary["scaling"] == "ntk":
+        theta = theta * factor ** (r / (r - 2))
+    f = theta ** (-torch.arange(0, r, 2, device="cuda", dtype=torch.float64) / r)
+    if rotary["scaling"] == "linear":
+        f = f / factor
+    if rotary["scaling"] != "by_parts":
+        return f, 1.0
+    # pairs that turn more than 32 times in the original context keep their
+    # frequency, those that turn less than once are stretched, a ramp between:
+    # over the pair index at which a pair turns so many times
+    def pair(turns):
+        return r * math.log(rotary["original_context"] / (turns * 2 * math.pi)) / (
+            2 * math.log(rotary["theta"]))
+
+    low, high = max(math.floor(pair(32.0)), 0), min(math.ceil(pair(1.0)), r // 2 - 1)
+    ramp = ((torch.arange(r // 2, device="cuda", dtype=torch.float64) - low)
+            / max(high - low, 0.001)).clamp(0, 1)
+    return f * (1 - ramp) + f / factor * ramp, 0.1 * math.log(factor) + 1.0
+
+
+def _rotated(rotary, x, positions, dtype):
+    """The rotation of [T, H, D] rows in ``dtype``, angles in 64 bits."""
+    f, amplitude = _frequencies(rotary)
+    angle = positions.double()[:, None] * f
+    cos = (angle.cos() * amplitude).to(dtype)[:, None, :]
+    sin = (angle.sin() * amplitude).to(dtype)[:, None, :]
+    r = rotary["rotary_dim"]
+    part, rest = x[..., :r].to(dtype), x[..., r:].to(dtype)
+    if rotary["layout"] == "half":
+        a, b = part[..., :r // 2], part[..., r // 2:]
+        turned = torch.cat((a * cos - b * sin, b * cos + a * sin), dim=-1)
+    else:
+        a, b = part[..., 0::2], part[..., 1::2]
+        turned = torch.stack((a * cos - b * sin, b * cos + a * sin), dim=-1).flatten(-2)
+    return torch.cat((turned, rest), dim=-1)
+
+
+def _plain_rotate(s):
+    return tuple(_rotated(s["rotary"], x, s["positions"], torch.float32).to(x.dtype)
+                 for x in (s["query"], s["key"]))
+
+
+def _codes(x):
+    """Codes [..., 128] in [-7, 7] and FP16 scales of centered rows in 32 bits."""
+    scale = (x.abs().amax(-1) / 7.0).clamp_min(2.0 ** -20).half()
+    q = x / scale.float()[..., None]
+    return torch.copysign((q.abs() + 0.5).floor(), q).clamp(-7, 7), scale
+
+
+def _pack(k, v):
+    """Codes of whole pages [pages * 16, H, 128] as packed pages."""
+    h = k.shape[1]
+    k = (k + 8).to(torch.uint8).view(-1, 16, h, 4, 4, 2, 2, 2)     # n h w kg i2 i1 s
+    k = k.permute(0, 2, 4, 1, 3, 7, 5, 6)                          # h kg n w s i2 i1
+    v = (v + 8).to(torch.uint8).view(-1, 4, 2, 2, h, 16, 4, 2)     # kg t2 s h n j ab
+    v = v.permute(0, 4, 1, 5, 6, 3, 7, 2)                          # h kg n j s ab t2
+    return torch.stack([(t[..., 0] | (t[..., 1] << 4)).reshape(-1, h, 1024) for t in (k, v)], 2)
+
+
+def _unpack(codes, dtype=torch.float32):
+    """Codes of packed pages, [pages, 16, H, 128] for K and for V."""
+    h = codes.shape[1]
+    both = torch.stack((codes & 15, codes >> 4), dim=-1).to(dtype) - 8
+    k = both[:, :, 0].reshape(-1, h, 4, 16, 4, 2, 2, 2).permute(0, 3, 1, 4, 2, 6, 7, 5)
+    v = both[:, :, 1].reshape(-1, h, 4, 16, 4, 2, 2, 2).permute(0, 2, 7, 5, 1, 3, 4, 6)
+    return k.reshape(-1, 16, h, DIM), v.reshape(-1, 16, h, DIM)
+
+
+def _pack_scales(ks, vs):
+    """Scales [pages * 16, H] of K and V as [pages, H, 4, 2, 4]."""
+    h = ks.shape[1]
+    return torch.stack([t.view(-1, 4, 4, h).permute(0, 3, 1, 2) for t in (ks, vs)], dim=3)
+
+
+def _values(codes, scales, dtype=torch.float32):
+    """What packed pages stand for, [pages, 16, H, 128] for K and for V."""
+    k, v = _unpack(codes, dtype)
+    s = scales.to(dtype).permute(3, 0, 2, 4, 1).flatten(2, 3)[..., None]
+    return k * s[0], v * s[1]
+
+
+def _filled(x, pages):
+    """Rows [T, H, 128] in 32 bits up to whole pages, the missing ones zero."""
+    missing = pages * PAGE - x.shape[0]
+    return torch.cat((x, x.new_zeros(missing, *x.shape[1:]))) if missing else x
+
+
+def _plain_write(s):
+    pages, tokens = s["codes"].shape[0], s["key"].shape[0]
+    ids = s["page_ids"].long()
+    centered = [x.float() if c is None else x.float() - c.float()
+                for x, c in zip((s["key"], s["value"]), s["centers"])]
+    (kc, ks), (vc, vs) = (_codes(x) for x in centered)
+    s["codes"].index_copy_(0, ids, _pack(_filled(kc, pages), _filled(vc, pages)))
+    s["scales"].index_copy_(0, ids, _pack_scales(_filled(ks, pages), _filled(vs, pages)))
+    rows = [t.flatten(0, 1)[:tokens] for t in _values(s["codes"][ids], s["scales"][ids])]
+    key, value = (t.half() if c is None else (t + c.float()).half()
+                  for t, c in zip(rows, s["centers"]))
+    return key, value, s["scales"]
+
+
+def _plain_append(s):
+    batch = s["query"].shape[0]
+    exact, code = s["exact_ids"].long(), s["code_ids"].long()
+    offset = s["positions"].long() % PAGE
+    s["rotated_query"].copy_(_rotated(s["rotary"], s["query"], s["positions"], torch.float32))
+    rows = (_rotated(s["rotary"], s["key"], s["positions"], torch.float32), s["value"].float())
+    for pool, row, center in zip(s["exact"], rows, s["centers"]):
+        pool[exact, offset] = (row - center.float()).half()
+    (kc, ks), (vc, vs) = (_codes(pool[exact].float().flatten(0, 1)) for pool in s["exact"])
+    closes = offset == PAGE - 1
+    s["codes"][code] = torch.where(closes.view(batch, 1, 1, 1), _pack(kc, vc), s["codes"][code])
+    s["scales"][code] = torch.where(closes.view(batch, 1, 1, 1, 1), _pack_scales(ks, vs),
+                                    s["scales"][code])
+    key, value = (t.flatten(0, 1).half() for t in _values(s["codes"][code], s["scales"][code]))
+    return s["rotated_query"], s["exact"][0], s["exact"][1], key, value
+
+
+def _padded(table):
+    """Page ids [B, P] of each request, filled with its pool's first page, and
+    the visible tokens [B, P * 16]."""
+    counts = table["indptr"][1:] - table["indptr"][:-1]
+    most = max(1, int(counts.max()))
+    at = torch.arange(most)
+    spot = (table["indptr"][:-1, None] + at).clamp_max(max(0, int(table["indptr"][-1]) - 1))
+    last = table["last"].cpu()
+    tokens = torch.where(counts > 0, (counts - 1) * PAGE + last, 0)
+    visible = torch.arange(most * PAGE) < tokens[:, None]
+    return {"pages": table["indices"][spot.cuda().long()].long(), "visible": visible.cuda()}
+
+
+def _attend(s, dtype):
+    """(out, lse) in ``dtype``: one softmax over each request's history and tail."""
+    q = s["query"].to(dtype)
+    batch, hq, _ = q.shape
+    hkv = s["codes"].shape[1]
+    keys, values, visible = [], [], []
+    parts = [(s["table"], _values(s["codes"], s["scales"], dtype))]
+    if s["tail"] is not None:
+        parts.append((s["tail"], tuple(t.to(dtype) for t in s["exact"])))
+    for table, (k, v) in parts:
+        where = (batch, -1, hkv, DIM)
+        keys.append(k[table["pages"]].view(*where))
+        values.append(v[table["pages"]].view(*where))
+        visible.append(table["visible"])
+    k = torch.cat(keys, 1).transpose(1, 2)                    # [B, Hkv, T, 128]
+    v = torch.cat(values, 1).transpose(1, 2).contiguous()
+    seen = torch.cat(visible, 1)[:, None, None, :]
+    grouped = q.view(batch, hkv, hq // hkv, DIM)
+    scores = torch.matmul(grouped, k.transpose(2, 3).contiguous()) * DIM ** -0.5
+    scores = scores.masked_fill(~seen, -math.inf)
+    most = scores.amax(-1, keepdim=True)
+    p = (scores - most).exp()
+    total = p.sum(-1, keepdim=True)
+    out = torch.matmul(p, v) / total + s["center"].to(dtype)[:, :, None, :]
+    lse = ((most + total.log()) / math.log(2.0)).view(batch, hq)
+    return out.view(batch, hq, DIM), lse
+
+
+def _plain_attend(s):
+    out, lse = _attend(s, torch.float32)
+    return out.half(), lse
+
+
+def _shaped(s, dtype):
+    x = s["logits"].to(dtype)
+    batch, vocab = x.shape
+    at = torch.arange(s["history"].shape[1], device="cuda")
+    inside = at < s["lengths"][:, None]
+    made = inside & (at >= s["prompts"][:, None])
+    seen = torch.zeros(batch, vocab, device="cuda").scatter_add_(1, s["history"], inside.float())
+    count = torch.zeros(batch, vocab, device="cuda").scatter_add_(1, s["history"], made.float())
+    rep = s["repetition"].to(dtype)[:, None]
+    x = torch.where(seen > 0, torch.where(x > 0, x / rep, x * rep), x)
+    x = x - s["frequency"].to(dtype)[:, None] * count.to(dtype)
+    x = x - s["presence"].to(dtype)[:, None] * (count > 0).to(dtype)
+    if s["bias_tokens"] is not None:
+        x = x.scatter_add(1, s["bias_tokens"], s["bias_values"].to(dtype))
+    if s["allowed"] is not None:
+        bits = (s["allowed"][:, :, None] >> torch.arange(32, device="cuda")) & 1
+        x = x.masked_fill(bits.flatten(1)[:, :vocab] == 0, -math.inf)
+    return x
+
+
+def _plain_logits(s):
+    return _shaped(s, torch.float32).to(s["logits"].dtype)
+
+
+_PLAIN = {"rotate": _plain_rotate, "write": _plain_write, "append": _plain_append,
+          "attend": _plain_attend, "logits": _plain_logits}
+
+
+# -- in 64 bits ------------------------------------------------------------------
+
+def _exact_turn(rotary, x, positions):
+    """Each pair as a complex number, turned by a unit complex number."""
+    r, theta, factor = rotary["rotary_dim"], rotary["theta"], rotary["factor"]
+    exponent = [-2.0 * i / r for i in range(r // 2)]
+    if rotary["scaling"] == "ntk":
+        theta *= factor ** (r / (r - 2.0))
+    freqs, amplitude = [theta ** e for e in exponent], 1.0
+    if rotary["scaling"] == "linear":
+        freqs = [f / factor for f in freqs]
+    elif rotary["scaling"] == "by_parts":
+        ends = [r / 2 * math.log(rotary["original_context"] / (2 * math.pi * turns), theta)
+                for turns in (32.0, 1.0)]
+        low, high = max(0, math.floor(ends[0])), min(r // 2 - 1, math.ceil(ends[1]))
+        share = [min(1.0, max(0.0, (i - low) / max(high - low, 0.001))) for i in range(r // 2)]
+        freqs = [f * (1 - g) + f * g / factor for f, g in zip(freqs, share)]
+        amplitude += 0.1 * math.log(factor)
+    angle = torch.outer(positions.double(), torch.tensor(freqs, device="cuda", dtype=torch.float64))
+    turn = torch.polar(torch.full_like(angle, amplitude), angle)[:, None]
+    out = x.double().clone()
+    if rotary["layout"] == "half":
+        z = torch.complex(out[..., :r // 2].clone(), out[..., r // 2:r].clone()) * turn
+        out[..., :r // 2], out[..., r // 2:r] = z.real, z.imag
+    else:
+        z = torch.complex(out[..., 0:r:2].clone(), out[..., 1:r:2].clone()) * turn
+        out[..., 0:r:2], out[..., 1:r:2] = z.real, z.imag
+    return out
+
+
+def _exact_held(x):
+    """What centered rows are held as, and their scales, in 64 bits: the code
+    of a row is the nearest multiple of its stored scale, halves away from
+    zero, at most 7 steps."""
+    scale = torch.maximum(x.abs().amax(-1) / 7, torch.tensor(2.0 ** -20, device="cuda",
+                                                             dtype=torch.float64))
+    stored = scale.half().double()[..., None]
+    steps = torch.floor(x.abs() / stored + 0.5).clamp_max(7)
+    return steps * stored * x.sign(), scale
+
+
+def exact(case, seed):
+    s = _inputs(case, seed)
+    op = case["op"]
+    if op == "rotate":
+        return tuple(_exact_turn(s["rotary"], s[n], s["positions"]) for n in ("query", "key"))
+    if op == "write":
+        rows, scales = [], []
+        for x, c in zip((s["key"], s["value"]), s["centers"]):
+            c = 0.0 if c is None else c.double()
+            held, scale = _exact_held(x.double() - c)
+            rows.append(held + c)
+            scales.append(scale)
+        pages, heads = s["codes"].shape[:2]
+        laid = torch.zeros(pages * PAGE, heads, 2, device="cuda", dtype=torch.float64)
+        laid[:case["tokens"]] = torch.stack(scales, -1)
+        laid = laid.view(pages, 4, 4, heads, 2).permute(0, 3, 1, 4, 2)
+        placed = torch.zeros_like(laid)
+        placed[s["page_ids"].long()] = laid
+        return rows[0], rows[1], placed
+    if op == "append":
+        batch = case["batch"]
+        turned = [_exact_turn(s["rotary"], s[n], s["positions"]) for n in ("query", "key")]
+        where = (s["exact_ids"].long(), s["positions"].long() % PAGE)
+        rings, read = [], []
+        before = _values(s["codes"], s["scales"], torch.float64)
+        closes = (where[1] == PAGE - 1).view(batch, 1, 1, 1)
+        for ring, row, c, was in zip(s["exact"], (turned[1], s["value"].double()), s["centers"],
+                                     before):
+            new = ring.double()
+            new[where] = row - c.double()
+            rings.append(new)
+            held, _ = _exact_held(new.half().double()[where[0]])
+            read.append(torch.where(closes, held, was[s["code_ids"].long()]).flatten(0, 1))
+        return turned[0], rings[0], rings[1], read[0], read[1]
+    if op == "attend":
+        if case["batch"] * case["high"] * case["kv_heads"] > 16 << 20:
+            return None
+        # per request, without padding
+        hkv, hq = case["kv_heads"], case["kv_heads"] * case["group"]
+        pools = [(s["table"], _values(s["codes"], s["scales"], torch.float64))]
+        if s["tail"] is not None:
+            pools.append((s["tail"], [t.double() for t in s["exact"]]))
+        outs, lses = [], []
+        for b in range(case["batch"]):
+            k, v = [], []
+            for table, (pk, pv) in pools:
+                low, high = (int(n) for n in table["indptr"][b:b + 2])
+                tokens = (high - low - 1) * PAGE + int(table["last"][b]) if high > low else 0
+                ids = table["indices"][low:high].long()
+                k.append(pk[ids].flatten(0, 1)[:tokens])
+                v.append(pv[ids].flatten(0, 1)[:tokens])
+            k, v = (torch.cat(t).permute(1, 0, 2).contiguous() for t in (k, v))
+            q = s["query"][b].double().view(hkv, -1, DIM)
+            score = torch.matmul(q, k.transpose(1, 2).contiguous()) / math.sqrt(DIM)
+            lses.append(torch.logsumexp(score, -1).view(hq) / math.log(2.0))
+            mixed = torch.matmul(torch.softmax(score, -1), v)
+            outs.append((mixed + s["center"][b].double()[:, None]).reshape(hq, DIM))
+        return torch.stack(outs), torch.stack(lses)
+    # logits: counts by row from the sorted history
+    x = s["logits"].double()
+    for b in range(case["batch"]):
+        n, p = int(s["lengths"][b]), int(s["prompts"][b])
+        seen = torch.unique(s["history"][b, :n])
+        rep = float(s["repetition"][b])
+        x[b, seen] = torch.where(x[b, seen] > 0, x[b, seen] / rep, x[b, seen] * rep)
+        made, count = torch.unique(s["history"][b, p:n], return_counts=True)
+        x[b, made] -= float(s["frequency"][b]) * count.double() + float(s["presence"][b])
+        if s["bias_tokens"] is not None:
+            x[b, s["bias_tokens"][b]] += s["bias_values"][b].double()
+    if s["allowed"] is not None:
+        token = torch.arange(case["vocab"], device="cuda")
+        word = s["allowed"].long()[:, token // 32]
+        x[(word >> (token % 32)) & 1 == 0] = -math.inf
+    return x
