@@ -444,7 +444,7 @@ def _unpack(codes, dtype=torch.float32):
 def _pack_scales(ks, vs):
     """Scales [pages * 16, H] of K and V as [pages, H, 4, 2, 4]."""
     h = ks.shape[1]
-    return torch.stack([t.view(-1, 4, 4, h).permute(0, 3, 1, 2) for t in (ks, vs)], dim=3)
+    return torch.stack([t.view(-1, 4, 4, h).permute(0, 3, 1, 2) for t in (ks, vs)], dim=3).contiguous()
 
 
 def _values(codes, scales, dtype=torch.float32):
