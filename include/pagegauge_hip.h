@@ -16,6 +16,7 @@
  *   FP16 and INT8 page caches  NHD [pages, 16, Hkv, 128]
  *   page scales                fp16 [pages, Hkv]
  *   centers                    fp16 [B, Hkv, 128] (or [Hkv, 128] when B == 1)
+ *   4-bit page caches          codes and scales, further down
  *   lse                        float32 [B, Hq], base 2 (log2-sum-exp2 of
  *                              sm_scale*log2(e)*q.k)
  */
@@ -35,6 +36,9 @@ enum {
   PG_ERROR_UNSUPPORTED = 3,
   PG_ERROR_WORKSPACE = 4
 };
+
+/* Types of rows and logits, where an entry point takes several. */
+enum { PG_DTYPE_FP16 = 0, PG_DTYPE_BF16 = 1, PG_DTYPE_FP32 = 2 };
 
 /* Message of the last failing call on this thread ("" if none). */
 const char* pg_last_error(void);
@@ -616,6 +620,166 @@ int32_t pg_decoder_gemm_rope_append(const void* weight, int32_t k, const void* x
  * workgroup per row. */
 int32_t pg_argmax_f32(const float* x, int32_t rows, int32_t n, int64_t row_stride, int64_t* out,
                       void* stream);
+
+/* ------------------------------------------------------------------------
+ * Rotary positions from 64-bit angles.
+ * ---------------------------------------------------------------------- */
+
+/* Turns pairs (i, i + rotary_dim/2), or (2i, 2i + 1) with interleaved != 0,
+ * of the first rotary_dim dims of each head by positions[t] * turns[i]
+ * revolutions and multiplies them by amplitude; the other dims are copied.
+ * Rows [tokens, heads, head_dim] of dtype (PG_DTYPE_*), token and head strides
+ * in elements; key_heads may be 0 (then its pointers are not used).  Outputs
+ * may be the inputs themselves, query and key alike.  positions is int32 or
+ * int64 (position_bytes 4 or 8), turns float64 [rotary_dim/2].  Angles are
+ * reduced in 64 bits, the rotation is float32, rounded once. */
+int32_t pg_rotate(const void* query, int64_t query_token_stride, int64_t query_head_stride,
+                  int32_t query_heads, const void* key, int64_t key_token_stride,
+                  int64_t key_head_stride, int32_t key_heads, void* out_query,
+                  int64_t out_query_token_stride, int64_t out_query_head_stride, void* out_key,
+                  int64_t out_key_token_stride, int64_t out_key_head_stride,
+                  const void* positions, int32_t position_bytes, const double* turns,
+                  float amplitude, int64_t tokens, int32_t head_dim, int32_t rotary_dim,
+                  int32_t interleaved, int32_t dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The cache held in 4 bits.
+ *
+ *   codes   uint8 [pages, Hkv, 2 (K, V), 1024], 16-byte aligned
+ *   scales  fp16  [pages, Hkv, 4, 2 (K, V), 4], 16-byte aligned: tokens
+ *           4g .. 4g + 3 of group g
+ *
+ * A nibble holds code + 8 with code in [-7, 7] and stands for code * scale of
+ * its token, head and part.  Nibble i of a dword is bits 4i .. 4i + 3.  The
+ * dword at byte 16*(16*kg + n) + 4*w of a K part holds token n: dim
+ * 32w + 8kg + 2i in nibble i and dim 32w + 8kg + 2i + 1 in nibble i + 4, i < 4.
+ * The dword at byte 16*(16*kg + n) + 4*j of a V part holds tokens 4kg .. 4kg + 3
+ * of channel 8n + 2j in nibbles 0, 4, 1, 5 and of channel 8n + 2j + 1 in nibbles
+ * 2, 6, 3, 7.
+ * ---------------------------------------------------------------------- */
+
+/* Holds token-major rows [tokens, heads, 128] (fp16, dense heads, token stride
+ * in elements) in 4 bits: source page i (tokens 16i ..) goes to code page
+ * page_ids[i] (page_ids NULL: i).  Per token and head, of the float32 rows
+ * minus the centers [heads, 128] (both NULL: none): scale
+ * fp16(max(amax * (1/7), 2^-20)), codes sign * floor(|x/scale| + 0.5).  Rows past
+ * the last token of a partial page get scale 0.  With exact_page_ids, source
+ * page i is also stored, centered and rounded to fp16, in exact page
+ * exact_page_ids[i] of the [num_exact_pages, 16, heads, 128] pages (rows past
+ * the last token are left as they were).  Ids outside their pool skip the
+ * store. */
+int32_t pg_int4_quantize_pages(const void* key, int64_t key_token_stride, const void* value,
+                               int64_t value_token_stride, const void* key_center,
+                               const void* value_center, void* codes, void* scales,
+                               int64_t num_code_pages, const int32_t* page_ids,
+                               const int32_t* exact_page_ids, void* exact_key_pages,
+                               void* exact_value_pages, int64_t num_exact_pages, int64_t tokens,
+                               int32_t heads, void* stream);
+
+/* The inverse: fp16(code * scale + center) of the first ``tokens`` tokens of
+ * pages page_ids[0], page_ids[1], ... (NULL: 0, 1, ...) into token-major rows
+ * [tokens, heads, 128].  Pages whose id lies outside the pool give zeros. */
+int32_t pg_int4_dequantize_pages(const void* codes, const void* scales, int64_t num_code_pages,
+                                 const int32_t* page_ids, const void* key_center,
+                                 const void* value_center, void* key, int64_t key_token_stride,
+                                 void* value, int64_t value_token_stride, int64_t tokens,
+                                 int32_t heads, void* stream);
+
+/* The cache update of one token per request: query and key rows [B, H, 128]
+ * (fp16, dense heads, batch strides in elements) turned as by pg_rotate, the
+ * rotated query stored, the centered key and value stored in row
+ * positions[r] % 16 of exact page exact_page_ids[r], and on a page's 16th token
+ * that page held in 4 bits in code page code_page_ids[r].  Centers
+ * [B, kv_heads, 128].  A row with a negative position is skipped; ids outside
+ * their pool skip the store.  Rows of one call must have exact and code pages of
+ * their own. */
+int32_t pg_int4_rope_append(const void* query, const void* key, const void* value,
+                            int64_t query_batch_stride, int64_t key_batch_stride,
+                            int64_t value_batch_stride, const int32_t* positions,
+                            const double* turns, float amplitude, int32_t rotary_dim,
+                            int32_t interleaved, const int32_t* exact_page_ids,
+                            const int32_t* code_page_ids, const void* key_center,
+                            const void* value_center, void* rotated_query, void* exact_key_pages,
+                            void* exact_value_pages, int64_t num_exact_pages, void* codes,
+                            void* scales, int64_t num_code_pages, int32_t batch_size,
+                            int32_t query_heads, int32_t kv_heads, void* stream);
+
+/* Plan of the attention over such a cache (opaque to the caller; copied by
+ * value).  Offsets lie in the workspace. */
+typedef struct pg_int4_plan {
+  int32_t batch_size;
+  int32_t num_qo_heads;
+  int32_t num_kv_heads;
+  int32_t has_history;
+  int32_t has_tail;
+  int32_t num_items;
+  int32_t max_items_per_request;
+  int32_t reserved;
+  int64_t items_offset;
+  int64_t item_ptr_offset;
+  int64_t partial_offset;
+  int64_t workspace_bytes;
+} pg_int4_plan_t;
+
+/* Cuts a batch into work items: history pages host_indptr[b] .. [b + 1] and,
+ * with host_tail_indptr, exact FP16 pages, 1 to 16 query heads per KV head.  The
+ * work list is copied into the workspace, and the copy waited for. */
+int32_t pg_int4_plan(const int32_t* host_indptr, const int32_t* host_tail_indptr,
+                     int32_t batch_size, int32_t num_qo_heads, int32_t num_kv_heads,
+                     int32_t num_cus, void* workspace, int64_t workspace_bytes,
+                     pg_int4_plan_t* plan, void* stream);
+
+/* The same on the host alone: items_out (NULL, or at least items_capacity
+ * items of 8 int32: request, first and end history page, the request's last
+ * one, first and end tail page, the last one, items of the request) and
+ * item_ptr_out [B + 1]. */
+int32_t pg_int4_plan_host(const int32_t* host_indptr, const int32_t* host_tail_indptr,
+                          int32_t batch_size, int32_t num_qo_heads, int32_t num_kv_heads,
+                          int32_t num_cus, pg_int4_plan_t* plan, int32_t* items_out,
+                          int64_t items_capacity, int32_t* item_ptr_out);
+
+/* Attention of query rows [B, Hq, 128] (fp16, dense heads) over each request's
+ * history (codes and scales of pages indices[...], the last one holding
+ * last_page_len[b] tokens) and exact tail pages [pages, 16, Hkv, 128], plus the
+ * value center [B, Hkv, 128] (or NULL).  out fp16 [B, Hq, 128]; lse float32
+ * [B, Hq] base 2, or NULL.  A request without tokens gives its center and an
+ * lse of -inf.  last_page_len and tail_last_len are read on the device.  Runs
+ * that share a workspace must not overlap. */
+int32_t pg_int4_decode_run(const pg_int4_plan_t* plan, const void* query,
+                           int64_t query_batch_stride, const void* codes, const void* scales,
+                           const int32_t* indices, const int32_t* last_page_len,
+                           const void* tail_k, const void* tail_v, const int32_t* tail_indices,
+                           const int32_t* tail_last_len, const void* value_center,
+                           int64_t center_batch_stride, void* out, float* lse, float sm_scale,
+                           void* workspace, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Logits.
+ * ---------------------------------------------------------------------- */
+
+/* Shapes a batch of logits [batch, vocab] (dtype PG_DTYPE_*, row strides in
+ * elements) before a token is picked; out may be logits itself.  In order, in
+ * float32, each part left out where its pointer is NULL:
+ *   x > 0 ? x / repetition[b] : x * repetition[b] for tokens of
+ *     history[b, 0 .. history_lengths[b]);
+ *   x - frequency[b] * c - presence[b] * (c > 0), c the count of the token in
+ *     history[b, prompt_lengths[b] .. history_lengths[b]) (prompt_lengths NULL:
+ *     from 0);
+ *   x + bias_values[b, i] for token bias_tokens[b, i] (the last i of a token
+ *     counts);
+ *   -inf where bit t % 32 of allowed[b, t / 32] is clear.
+ * history (rows of history_capacity tokens, stride in elements) and
+ * bias_tokens [batch, biases] are int32 or int64 (token_bytes 4 or 8);
+ * lengths beyond the capacity are cut to it, and tokens outside the vocabulary
+ * ignored. */
+int32_t pg_shape_logits(const void* logits, int64_t logits_stride, void* out, int64_t out_stride,
+                        int32_t dtype, int32_t batch, int32_t vocab, const void* history,
+                        int64_t history_stride, int64_t history_capacity,
+                        const int32_t* history_lengths, const int32_t* prompt_lengths,
+                        const float* repetition, const float* frequency, const float* presence,
+                        const void* bias_tokens, const float* bias_values, int32_t biases,
+                        int32_t token_bytes, const int32_t* allowed, int64_t allowed_stride,
+                        void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,6 +20,9 @@ PG_OK = 0
 PG_KV_INT8 = 0
 PG_KV_FP16 = 1
 PG_KV_HETEROGENEOUS = 2
+PG_DTYPE_FP16 = 0
+PG_DTYPE_BF16 = 1
+PG_DTYPE_FP32 = 2
 
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -50,6 +53,25 @@ class DecodePlan(ctypes.Structure):
         ("cf_tail_pages", _i32),
         ("cf_primary_begin", _i32),
         ("cf_primary_pages", _i32),
+        ("reserved", _i32),
+        ("items_offset", _i64),
+        ("item_ptr_offset", _i64),
+        ("partial_offset", _i64),
+        ("workspace_bytes", _i64),
+    ]
+
+
+class Int4Plan(ctypes.Structure):
+    """Mirror of ``pg_int4_plan_t``."""
+
+    _fields_ = [
+        ("batch_size", _i32),
+        ("num_qo_heads", _i32),
+        ("num_kv_heads", _i32),
+        ("has_history", _i32),
+        ("has_tail", _i32),
+        ("num_items", _i32),
+        ("max_items_per_request", _i32),
         ("reserved", _i32),
         ("items_offset", _i64),
         ("item_ptr_offset", _i64),
@@ -124,6 +146,21 @@ PROTOTYPES = {
     "pg_decoder_qkv_rope_append": (_i32, [_p, _i32, _p, _i64, _i32, _p, _f32, _i32, _i32, _p, _p,
                                           _i64, _i32, _p, _i32, _p, _p, _p, _p, _p, _i64, _i32,
                                           _i32, _i32, _p]),
+    "pg_rotate": (_i32, [_p, _i64, _i64, _i32, _p, _i64, _i64, _i32, _p, _i64, _i64, _p, _i64, _i64,
+                         _p, _i32, _p, _f32, _i64, _i32, _i32, _i32, _i32, _p]),
+    "pg_int4_quantize_pages": (_i32, [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _p, _p, _p, _p, _i64,
+                                      _i64, _i32, _p]),
+    "pg_int4_dequantize_pages": (_i32, [_p, _p, _i64, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i32,
+                                        _p]),
+    "pg_int4_rope_append": (_i32, [_p, _p, _p, _i64, _i64, _i64, _p, _p, _f32, _i32, _i32, _p, _p, _p,
+                                   _p, _p, _p, _p, _i64, _p, _p, _i64, _i32, _i32, _i32, _p]),
+    "pg_int4_plan": (_i32, [_p, _p, _i32, _i32, _i32, _i32, _p, _i64, ctypes.POINTER(Int4Plan), _p]),
+    "pg_int4_plan_host": (_i32, [_p, _p, _i32, _i32, _i32, _i32, ctypes.POINTER(Int4Plan), _p, _i64,
+                                 _p]),
+    "pg_int4_decode_run": (_i32, [ctypes.POINTER(Int4Plan), _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p,
+                                  _p, _i64, _p, _p, _f32, _p, _p]),
+    "pg_shape_logits": (_i32, [_p, _i64, _p, _i64, _i32, _i32, _i32, _p, _i64, _i64, _p, _p, _p, _p,
+                               _p, _p, _p, _i32, _i32, _p, _i64, _p]),
     "pg_argmax_f32": (_i32, [_p, _i32, _i32, _i64, _p, _p]),
     "pg_merge_state_in_place": (_i32, [_p, _p, _p, _p, _p, _i32, _i32, _i32, _p]),
     "pg_exact_tail_merge_center": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32,
@@ -207,6 +244,15 @@ def current_stream() -> int:
     stream object that ``torch.cuda.current_stream()`` builds (2.5 us a call,
     a sixth of a small decode call's host time)."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def require_current_device(*tensors) -> None:
+    """ValueError unless every tensor (None aside) is on the current CUDA
+    device, on whose current stream the kernels are launched."""
+    device = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else None
+    for t in tensors:
+        if t is not None and (device is None or t.get_device() != device):
+            raise ValueError("all tensors must be on the current CUDA device")
 
 
 def last_error() -> str:

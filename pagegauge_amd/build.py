@@ -67,6 +67,12 @@ SOURCES = {
     "pg_decode.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"],
     "pg_decoder.hip": [],
     "pg_prefill.hip": [],
+    "pg_rotary.hip": [],
+    "pg_int4_plan.cpp": [],
+    # the quantizer's quotients round operation by operation
+    "pg_int4_cache.hip": ["-ffp-contract=off"],
+    "pg_int4_decode.hip": [],
+    "pg_logits.hip": [],
 }
 
 BENCH_SOURCES = {

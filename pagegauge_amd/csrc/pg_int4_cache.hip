@@ -1,0 +1,486 @@
+// Writers and reader-back of the cache held in 4 bits (layout: pg_int4.h).
+//
+// A token's row x (128 dims of a KV head, K or V, minus the request's channel
+// center) is held as code * scale:
+//   scale = fp16(max(max|x| * (1/7), 2^-20)),
+//   code  = sign(x) floor(|x / scale| + 0.5) clamped to [-7, 7], a NaN giving 0,
+// in float32, 1/7 rounded to it and the quotient IEEE's: the INT8 pages' finalize
+// with 7 steps for 127, and a product for its division by the steps.  A scale
+// per token and head costs 1/32 of the codes and keeps an outlying token
+// to itself; a scale per page would share it with 15 others.
+//
+// All kernels are bound by HBM.  One wave takes one K or V part of a block and
+// holds it in registers in the lane order of the packed layout, so that codes
+// leave as one 1 KiB store of 16 bytes per lane.
+#include "pg_int4.h"
+#include "pg_rotary.h"
+
+namespace pg {
+namespace {
+
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+constexpr int kWavesPerBlock = 4;
+
+__device__ __forceinline__ uint16_t int4_scale_bits(float maximum) {
+  return __half_as_ushort(__float2half_rn(fmaxf(maximum * (1.0f / 7.0f), 0x1p-20f)));
+}
+
+// code + 8 of x / scale
+__device__ __forceinline__ uint32_t int4_nibble(float x, float scale) {
+  const float q = x / scale;
+  const float steps = fminf(floorf(fabsf(q) + 0.5f), 7.0f);
+  const int code = static_cast<int>(__builtin_copysignf(steps, q));   // a NaN converts to 0
+  return static_cast<uint32_t>((q != q ? 0 : code) + 8);
+}
+
+__device__ __forceinline__ float half_at(const v4u& v, int e) {
+  return half_bits_to_float(static_cast<uint16_t>(v[e >> 1] >> (16 * (e & 1))));
+}
+
+// Eight FP16 values at ``p``, which need only be aligned to 2 bytes unless kWide.
+template <bool kWide>
+__device__ __forceinline__ v4u load8(const uint16_t* p) {
+  if (kWide) return *reinterpret_cast<const v4u*>(p);
+  v4u v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = p[2 * i] | static_cast<uint32_t>(p[2 * i + 1]) << 16;
+  return v;
+}
+
+template <bool kWide>
+__device__ __forceinline__ void store8(uint16_t* p, const v4u& v) {
+  if (kWide) {
+    *reinterpret_cast<v4u*>(p) = v;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    p[2 * i] = static_cast<uint16_t>(v[i]);
+    p[2 * i + 1] = static_cast<uint16_t>(v[i] >> 16);
+  }
+}
+
+// Packs one part from the wave's registers: x[g][e] is dim 32 g + 8 kg + e of
+// token n (K), or channel 8 n + e of token 4 kg + g (V).  Rows at or past
+// ``visible`` are stored as scale 0.
+template <bool kValue>
+__device__ __forceinline__ void pack_part(const float (&x)[4][8], int visible, uint8_t* codes,
+                                          uint16_t* scales, int lane) {
+  const int n = lane & 15, kg = lane >> 4;
+  v4u word = {0u, 0u, 0u, 0u};
+  if (!kValue) {
+    float m = 0.0f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[g][e]));
+    m = fmaxf(m, __shfl_xor(m, 16, kWave));
+    m = fmaxf(m, __shfl_xor(m, 32, kWave));
+    const uint16_t bits = int4_scale_bits(m);
+    const float scale = half_bits_to_float(bits);
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        word[g] |= int4_nibble(x[g][e], scale) << (4 * ((e >> 1) + 4 * (e & 1)));
+    if (kg == 0) scales[int4_scale_index(0, n)] = n < visible ? bits : 0;
+  } else {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      float m = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[t][e]));
+      const uint16_t bits = int4_scale_bits(row16_max(m));
+      const float scale = half_bits_to_float(bits);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        word[e >> 1] |= int4_nibble(x[t][e], scale) << (4 * ((t >> 1) + 2 * (e & 1) + 4 * (t & 1)));
+      if (n == 0) scales[int4_scale_index(1, 4 * kg + t)] = 4 * kg + t < visible ? bits : 0;
+    }
+  }
+  *reinterpret_cast<v4u*>(codes + 16 * lane) = word;
+}
+
+// The row of part registers x[g] and its first dim, of the lane order above.
+template <bool kValue>
+__device__ __forceinline__ int part_row(int g, int lane) {
+  return kValue ? 4 * (lane >> 4) + g : lane & 15;
+}
+template <bool kValue>
+__device__ __forceinline__ int part_dim(int g, int lane) {
+  return kValue ? 8 * (lane & 15) : 32 * g + 8 * (lane >> 4);
+}
+
+struct QuantizeArgs {
+  const uint16_t* source[2];       // token-major K and V rows
+  int64_t token_stride[2];
+  const uint16_t* center[2];       // [Hkv, 128] or null
+  uint8_t* codes;
+  uint16_t* scales;
+  const int32_t* page_ids;         // code page of each source page, or null: the same
+  const int32_t* exact_ids;        // exact page of each source page, or null
+  uint16_t* exact[2];
+  int64_t tokens, pages, num_code_pages, num_exact_pages;
+  int heads;
+};
+
+template <bool kWide, bool kValue>
+__device__ __forceinline__ void quantize_part(const QuantizeArgs& a, int64_t page, int head, int lane) {
+  const int64_t code_page = a.page_ids ? a.page_ids[page] : page;
+  const int64_t exact_page = a.exact_ids ? a.exact_ids[page] : -1;
+  const int visible = static_cast<int>(min(static_cast<int64_t>(kPageSize), a.tokens - page * kPageSize));
+  const uint16_t* source = a.source[kValue] + page * kPageSize * a.token_stride[kValue] + head * kHeadDim;
+  const uint16_t* center = a.center[kValue];
+  float x[4][8];
+  v4u raw[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int row = part_row<kValue>(g, lane);
+    const int64_t at = min(row, visible - 1) * a.token_stride[kValue] + part_dim<kValue>(g, lane);
+    raw[g] = load8<kWide>(source + at);
+  }
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const bool in = part_row<kValue>(g, lane) < visible;
+    v4u c = {0u, 0u, 0u, 0u};
+    if (center) c = load8<kWide>(center + head * kHeadDim + part_dim<kValue>(g, lane));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[g][e] = in ? half_at(raw[g], e) - half_at(c, e) : 0.0f;
+  }
+  if (exact_page >= 0 && exact_page < a.num_exact_pages) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int row = part_row<kValue>(g, lane);
+      if (row >= visible) continue;
+      v4u out;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        out[i] = __half_as_ushort(__float2half_rn(x[g][2 * i])) |
+                 static_cast<uint32_t>(__half_as_ushort(__float2half_rn(x[g][2 * i + 1]))) << 16;
+      store8<kWide>(a.exact[kValue] + ((exact_page * kPageSize + row) * a.heads + head) * kHeadDim +
+                        part_dim<kValue>(g, lane), out);
+    }
+  }
+  if (code_page < 0 || code_page >= a.num_code_pages) return;
+  const int64_t block = code_page * a.heads + head;
+  pack_part<kValue>(x, visible, a.codes + block * kInt4BlockBytes + kValue * kInt4PartBytes,
+                    a.scales + block * kInt4BlockScales, lane);
+}
+
+// Grid (blocks of 4 waves, 2): a wave per (page, head), K and V by blockIdx.y.
+template <bool kWide>
+__global__ __launch_bounds__(kWave * kWavesPerBlock) void int4_quantize_kernel(QuantizeArgs a) {
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + threadIdx.x / kWave;
+  if (unit >= a.pages * a.heads) return;
+  const int64_t page = unit / a.heads;
+  const int head = static_cast<int>(unit - page * a.heads);
+  if (blockIdx.y == 0)
+    quantize_part<kWide, false>(a, page, head, threadIdx.x % kWave);
+  else
+    quantize_part<kWide, true>(a, page, head, threadIdx.x % kWave);
+}
+
+struct DequantizeArgs {
+  const uint8_t* codes;
+  const uint16_t* scales;
+  const int32_t* page_ids;
+  const uint16_t* center[2];
+  uint16_t* out[2];
+  int64_t token_stride[2];
+  int64_t tokens, pages, num_code_pages;
+  int heads;
+};
+
+template <bool kWide, bool kValue>
+__device__ __forceinline__ void dequantize_part(const DequantizeArgs& a, int64_t page, int head, int lane) {
+  const int64_t code_page = a.page_ids ? a.page_ids[page] : page;
+  const int64_t visible = a.tokens - page * kPageSize;
+  const bool held = code_page >= 0 && code_page < a.num_code_pages;
+  const int64_t block = (held ? code_page : 0) * a.heads + head;
+  const v4u word = *reinterpret_cast<const v4u*>(a.codes + block * kInt4BlockBytes +
+                                                 kValue * kInt4PartBytes + 16 * lane);
+  const uint16_t* center = a.center[kValue];
+  uint16_t* out = a.out[kValue] + page * kPageSize * a.token_stride[kValue] + head * kHeadDim;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int row = part_row<kValue>(g, lane);
+    const float scale = half_bits_to_float(a.scales[block * kInt4BlockScales + int4_scale_index(kValue, row)]);
+    v4u c = {0u, 0u, 0u, 0u};
+    if (center) c = load8<kWide>(center + head * kHeadDim + part_dim<kValue>(g, lane));
+    v4u packed = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t w = kValue ? word[e >> 1] : word[g];
+      const int nibble = kValue ? (g >> 1) + 2 * (e & 1) + 4 * (g & 1) : (e >> 1) + 4 * (e & 1);
+      const int code = static_cast<int>(w >> (4 * nibble) & 15u) - 8;
+      const float value = held ? static_cast<float>(code) * scale + half_at(c, e) : 0.0f;
+      packed[e >> 1] |= static_cast<uint32_t>(__half_as_ushort(__float2half_rn(value))) << (16 * (e & 1));
+    }
+    if (row < visible) store8<kWide>(out + row * a.token_stride[kValue] + part_dim<kValue>(g, lane), packed);
+  }
+}
+
+template <bool kWide>
+__global__ __launch_bounds__(kWave * kWavesPerBlock) void int4_dequantize_kernel(DequantizeArgs a) {
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + threadIdx.x / kWave;
+  if (unit >= a.pages * a.heads) return;
+  const int64_t page = unit / a.heads;
+  const int head = static_cast<int>(unit - page * a.heads);
+  if (blockIdx.y == 0)
+    dequantize_part<kWide, false>(a, page, head, threadIdx.x % kWave);
+  else
+    dequantize_part<kWide, true>(a, page, head, threadIdx.x % kWave);
+}
+
+struct AppendArgs {
+  const uint16_t* rows[3];         // query, key, value [B, H, 128]
+  int64_t batch_stride[3];
+  uint16_t* rotated_query;
+  const int32_t* positions;
+  const double* turns;
+  float amplitude;
+  int rotary_dim, interleaved;
+  const int32_t* exact_ids;
+  const int32_t* code_ids;
+  const uint16_t* center[2];       // [B, Hkv, 128]
+  uint16_t* exact[2];
+  uint8_t* codes;
+  uint16_t* scales;
+  int64_t num_exact_pages, num_code_pages;
+  int query_heads, kv_heads;
+};
+
+// Rows of the part from the exact page, the token's own row (15) from LDS.
+template <bool kValue>
+__device__ __forceinline__ void finalize_part(const AppendArgs& a, int64_t exact_page, int64_t code_page,
+                                              int head, const uint16_t* own_row, int lane) {
+  const uint16_t* page = a.exact[kValue] + (exact_page * kPageSize * a.kv_heads + head) * kHeadDim;
+  float x[4][8];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int row = part_row<kValue>(g, lane);
+    const int dim = part_dim<kValue>(g, lane);
+    // row 15 was stored by this wave just now: read row 14 in its place
+    const v4u held = *reinterpret_cast<const v4u*>(
+        page + static_cast<int64_t>(min(row, kPageSize - 2)) * a.kv_heads * kHeadDim + dim);
+    const v4u own = *reinterpret_cast<const v4u*>(own_row + dim);
+    const v4u raw = row == kPageSize - 1 ? own : held;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[g][e] = half_at(raw, e);
+  }
+  const int64_t block = code_page * a.kv_heads + head;
+  pack_part<kValue>(x, kPageSize, a.codes + block * kInt4BlockBytes + kValue * kInt4PartBytes,
+                    a.scales + block * kInt4BlockScales, lane);
+}
+
+// One wave per row of a request (query heads, then K, then V heads): lane p
+// holds pair p of the rotated part, or two dims past it.
+__global__ __launch_bounds__(kWave * kWavesPerBlock) void int4_rope_append_kernel(AppendArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t own[kWavesPerBlock][kHeadDim];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int row = blockIdx.y * kWavesPerBlock + wave;
+  if (row >= a.query_heads + 2 * a.kv_heads) return;   // whole waves; no barrier below
+  const int request = blockIdx.x;
+  const int32_t position = a.positions[request];
+  if (position < 0) return;
+  const int kind = row < a.query_heads ? 0 : row < a.query_heads + a.kv_heads ? 1 : 2;
+  const int head = kind == 0 ? row : kind == 1 ? row - a.query_heads : row - a.query_heads - a.kv_heads;
+  const uint16_t* in = a.rows[kind] + request * a.batch_stride[kind] + head * kHeadDim;
+  const bool turned = lane < a.rotary_dim / 2;
+  const int first = turned && !a.interleaved ? lane : 2 * lane;
+  const int second = turned && !a.interleaved ? lane + a.rotary_dim / 2 : 2 * lane + 1;
+  float x = half_bits_to_float(in[first]);
+  float y = half_bits_to_float(in[second]);
+  if (kind < 2 && turned) {
+    const float2 pair = rotate_pair(x, y, rotary_cos_sin(position, a.turns[lane], a.amplitude));
+    x = pair.x;
+    y = pair.y;
+  }
+  if (kind == 0) {
+    uint16_t* out = a.rotated_query + (static_cast<int64_t>(request) * a.query_heads + head) * kHeadDim;
+    out[first] = __half_as_ushort(__float2half_rn(x));
+    out[second] = __half_as_ushort(__float2half_rn(y));
+    return;
+  }
+  const int64_t exact_page = a.exact_ids[request];
+  if (exact_page < 0 || exact_page >= a.num_exact_pages) return;
+  const uint16_t* center = a.center[kind - 1] + (static_cast<int64_t>(request) * a.kv_heads + head) * kHeadDim;
+  const uint16_t xb = __half_as_ushort(__float2half_rn(x - half_bits_to_float(center[first])));
+  const uint16_t yb = __half_as_ushort(__float2half_rn(y - half_bits_to_float(center[second])));
+  const int offset = position % kPageSize;
+  uint16_t* out = a.exact[kind - 1] +
+                  ((exact_page * kPageSize + offset) * a.kv_heads + head) * kHeadDim;
+  out[first] = xb;
+  out[second] = yb;
+  if (offset != kPageSize - 1) return;
+  const int64_t code_page = a.code_ids[request];
+  if (code_page < 0 || code_page >= a.num_code_pages) return;
+  own[wave][first] = xb;
+  own[wave][second] = yb;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  if (kind == 1)
+    finalize_part<false>(a, exact_page, code_page, head, own[wave], lane);
+  else
+    finalize_part<true>(a, exact_page, code_page, head, own[wave], lane);
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int32_t check_pool(const void* codes, const void* scales, int64_t num_code_pages, int32_t heads) {
+  if (!codes || !scales) return fail(PG_ERROR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!aligned16(codes) || !aligned16(scales))
+    return fail(PG_ERROR_INVALID_ARGUMENT, "4-bit codes and scales must be 16-byte aligned");
+  if (num_code_pages < 0 || heads <= 0)
+    return fail(PG_ERROR_INVALID_ARGUMENT, "page and head counts must be positive");
+  if (heads > 65535) return fail(PG_ERROR_UNSUPPORTED, "at most 65535 KV heads");
+  return PG_OK;
+}
+
+}  // namespace
+}  // namespace pg
+
+using namespace pg;
+
+extern "C" int32_t pg_int4_quantize_pages(const void* key, int64_t key_token_stride, const void* value,
+                                          int64_t value_token_stride, const void* key_center,
+                                          const void* value_center, void* codes, void* scales,
+                                          int64_t num_code_pages, const int32_t* page_ids,
+                                          const int32_t* exact_page_ids, void* exact_key_pages,
+                                          void* exact_value_pages, int64_t num_exact_pages,
+                                          int64_t tokens, int32_t heads, void* stream) {
+  clear_error();
+  if (!key || !value) return fail(PG_ERROR_INVALID_ARGUMENT, "null tensor pointer");
+  if (int32_t rc = check_pool(codes, scales, num_code_pages, heads)) return rc;
+  if ((key_center == nullptr) != (value_center == nullptr))
+    return fail(PG_ERROR_INVALID_ARGUMENT, "key and value centers go together");
+  if (exact_page_ids && (!exact_key_pages || !exact_value_pages || num_exact_pages < 0))
+    return fail(PG_ERROR_INVALID_ARGUMENT, "exact page ids need exact key/value pages");
+  if (tokens < 0) return fail(PG_ERROR_INVALID_ARGUMENT, "token count must be nonnegative");
+  if (tokens == 0) return PG_OK;
+  QuantizeArgs a{};
+  a.source[0] = static_cast<const uint16_t*>(key);
+  a.source[1] = static_cast<const uint16_t*>(value);
+  a.token_stride[0] = key_token_stride;
+  a.token_stride[1] = value_token_stride;
+  a.center[0] = static_cast<const uint16_t*>(key_center);
+  a.center[1] = static_cast<const uint16_t*>(value_center);
+  a.codes = static_cast<uint8_t*>(codes);
+  a.scales = static_cast<uint16_t*>(scales);
+  a.page_ids = page_ids;
+  a.exact_ids = exact_page_ids;
+  a.exact[0] = static_cast<uint16_t*>(exact_key_pages);
+  a.exact[1] = static_cast<uint16_t*>(exact_value_pages);
+  a.tokens = tokens;
+  a.pages = (tokens - 1) / kPageSize + 1;
+  a.num_code_pages = num_code_pages;
+  a.num_exact_pages = exact_page_ids ? num_exact_pages : 0;
+  a.heads = heads;
+  const int64_t blocks = (a.pages * heads + kWavesPerBlock - 1) / kWavesPerBlock;
+  if (blocks > INT32_MAX) return fail(PG_ERROR_UNSUPPORTED, "too many pages for one call");
+  bool wide = key_token_stride % 8 == 0 && value_token_stride % 8 == 0;
+  for (const void* p : {key, value, key_center, value_center,
+                        static_cast<const void*>(exact_key_pages), static_cast<const void*>(exact_value_pages)})
+    wide = wide && aligned16(p);
+  const dim3 grid(static_cast<uint32_t>(blocks), 2);
+  if (wide)
+    hipLaunchKernelGGL(int4_quantize_kernel<true>, grid, dim3(kWave * kWavesPerBlock), 0, as_stream(stream), a);
+  else
+    hipLaunchKernelGGL(int4_quantize_kernel<false>, grid, dim3(kWave * kWavesPerBlock), 0, as_stream(stream), a);
+  return check_launch("int4_quantize_pages");
+}
+
+extern "C" int32_t pg_int4_dequantize_pages(const void* codes, const void* scales,
+                                            int64_t num_code_pages, const int32_t* page_ids,
+                                            const void* key_center, const void* value_center,
+                                            void* key, int64_t key_token_stride, void* value,
+                                            int64_t value_token_stride, int64_t tokens,
+                                            int32_t heads, void* stream) {
+  clear_error();
+  if (!key || !value) return fail(PG_ERROR_INVALID_ARGUMENT, "null tensor pointer");
+  if (int32_t rc = check_pool(codes, scales, num_code_pages, heads)) return rc;
+  if ((key_center == nullptr) != (value_center == nullptr))
+    return fail(PG_ERROR_INVALID_ARGUMENT, "key and value centers go together");
+  if (tokens < 0) return fail(PG_ERROR_INVALID_ARGUMENT, "token count must be nonnegative");
+  if (tokens == 0) return PG_OK;
+  if (num_code_pages == 0) return fail(PG_ERROR_INVALID_ARGUMENT, "the pool holds no pages");
+  DequantizeArgs a{};
+  a.codes = static_cast<const uint8_t*>(codes);
+  a.scales = static_cast<const uint16_t*>(scales);
+  a.page_ids = page_ids;
+  a.center[0] = static_cast<const uint16_t*>(key_center);
+  a.center[1] = static_cast<const uint16_t*>(value_center);
+  a.out[0] = static_cast<uint16_t*>(key);
+  a.out[1] = static_cast<uint16_t*>(value);
+  a.token_stride[0] = key_token_stride;
+  a.token_stride[1] = value_token_stride;
+  a.tokens = tokens;
+  a.pages = (tokens - 1) / kPageSize + 1;
+  a.num_code_pages = num_code_pages;
+  a.heads = heads;
+  const int64_t blocks = (a.pages * heads + kWavesPerBlock - 1) / kWavesPerBlock;
+  if (blocks > INT32_MAX) return fail(PG_ERROR_UNSUPPORTED, "too many pages for one call");
+  bool wide = key_token_stride % 8 == 0 && value_token_stride % 8 == 0;
+  for (const void* p : {key_center, value_center, static_cast<const void*>(key), static_cast<const void*>(value)})
+    wide = wide && aligned16(p);
+  const dim3 grid(static_cast<uint32_t>(blocks), 2);
+  if (wide)
+    hipLaunchKernelGGL(int4_dequantize_kernel<true>, grid, dim3(kWave * kWavesPerBlock), 0, as_stream(stream), a);
+  else
+    hipLaunchKernelGGL(int4_dequantize_kernel<false>, grid, dim3(kWave * kWavesPerBlock), 0, as_stream(stream), a);
+  return check_launch("int4_dequantize_pages");
+}
+
+extern "C" int32_t pg_int4_rope_append(
+    const void* query, const void* key, const void* value, int64_t query_batch_stride,
+    int64_t key_batch_stride, int64_t value_batch_stride, const int32_t* positions,
+    const double* turns, float amplitude, int32_t rotary_dim, int32_t interleaved,
+    const int32_t* exact_page_ids, const int32_t* code_page_ids, const void* key_center,
+    const void* value_center, void* rotated_query, void* exact_key_pages, void* exact_value_pages,
+    int64_t num_exact_pages, void* codes, void* scales, int64_t num_code_pages,
+    int32_t batch_size, int32_t query_heads, int32_t kv_heads, void* stream) {
+  clear_error();
+  if (!query || !key || !value || !positions || !turns || !exact_page_ids || !code_page_ids ||
+      !key_center || !value_center || !rotated_query || !exact_key_pages || !exact_value_pages)
+    return fail(PG_ERROR_INVALID_ARGUMENT, "null tensor pointer");
+  if (int32_t rc = check_pool(codes, scales, num_code_pages, kv_heads)) return rc;
+  if (!aligned16(exact_key_pages) || !aligned16(exact_value_pages))
+    return fail(PG_ERROR_INVALID_ARGUMENT, "exact pages must be 16-byte aligned");
+  if (batch_size < 0 || num_exact_pages < 0 || query_heads <= 0)
+    return fail(PG_ERROR_INVALID_ARGUMENT, "batch, head and page counts must be positive");
+  if (rotary_dim <= 0 || rotary_dim % 2 || rotary_dim > kHeadDim)
+    return fail(PG_ERROR_INVALID_ARGUMENT, "the rotated part must be an even number of a head's dims");
+  const int64_t row_blocks = (static_cast<int64_t>(query_heads) + 2 * kv_heads + kWavesPerBlock - 1) / kWavesPerBlock;
+  if (row_blocks > 65535) return fail(PG_ERROR_UNSUPPORTED, "too many heads for one call");
+  if (batch_size == 0) return PG_OK;
+  AppendArgs a{};
+  a.rows[0] = static_cast<const uint16_t*>(query);
+  a.rows[1] = static_cast<const uint16_t*>(key);
+  a.rows[2] = static_cast<const uint16_t*>(value);
+  a.batch_stride[0] = query_batch_stride;
+  a.batch_stride[1] = key_batch_stride;
+  a.batch_stride[2] = value_batch_stride;
+  a.rotated_query = static_cast<uint16_t*>(rotated_query);
+  a.positions = positions;
+  a.turns = turns;
+  a.amplitude = amplitude;
+  a.rotary_dim = rotary_dim;
+  a.interleaved = interleaved;
+  a.exact_ids = exact_page_ids;
+  a.code_ids = code_page_ids;
+  a.center[0] = static_cast<const uint16_t*>(key_center);
+  a.center[1] = static_cast<const uint16_t*>(value_center);
+  a.exact[0] = static_cast<uint16_t*>(exact_key_pages);
+  a.exact[1] = static_cast<uint16_t*>(exact_value_pages);
+  a.codes = static_cast<uint8_t*>(codes);
+  a.scales = static_cast<uint16_t*>(scales);
+  a.num_exact_pages = num_exact_pages;
+  a.num_code_pages = num_code_pages;
+  a.query_heads = query_heads;
+  a.kv_heads = kv_heads;
+  hipLaunchKernelGGL(int4_rope_append_kernel, dim3(batch_size, static_cast<uint32_t>(row_blocks)),
+                     dim3(kWave * kWavesPerBlock), 0, as_stream(stream), a);
+  return check_launch("int4_rope_append");
+}

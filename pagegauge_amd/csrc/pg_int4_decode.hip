@@ -1,0 +1,546 @@
+// Attention of single tokens over pages held in 4 bits and exact FP16 pages
+// (layout: pg_int4.h), split over the context, with the value center added back.
+//
+//   out = sum_t p_t sV_t v_t / sum_t p_t + cV,  p_t = exp2(sm log2(e) sK_t q . k_t - m)
+//
+// over codes k, v in [-7, 7] and one scale per token, head and part.  The key
+// center shifts all of a request's scores alike and is left out.
+//
+// A workgroup takes one KV head, up to 8 of its query heads and a range of
+// pages; its 8 waves take groups of 4 pages in turn and meet in LDS once, at the
+// end.  Everything else stays in registers, with no exchange between lanes but
+// two steps of the running maximum:
+//  * QK as K Q^T: tokens are the MFMA's rows, heads its columns, so lane (kg, n)
+//    gets the scores of tokens 4 kg .. 4 kg + 3 for head n % 8.
+//  * These are, pair of pages by pair, exactly the k slots that the lane feeds
+//    as the A operand of P V: probabilities never leave their lane.  Columns
+//    n < 8 hand over the FP16 part of a probability and columns n >= 8 (the same
+//    heads again) its remainder, so rows r and r + 8 of the product add up to
+//    one of about 22 bits.
+//  * Codes become FP16 exactly: a nibble u under the exponent of 1024 is
+//    1024 + u, minus 1032.  K and V are used as small integers; the scales
+//    multiply scores and probabilities in float32.
+//
+// Probabilities times V's scales are carried relative to a power of two that
+// puts the largest of the wave's scales near 2^14, so that FP16's range holds
+// them (a weight 2^-28 of the largest is still a normal number).
+#include "pg_int4.h"
+#include "pg_int4_plan.h"
+
+#include <algorithm>
+
+namespace pg {
+namespace {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+constexpr float kNegInf = -__builtin_huge_valf();
+constexpr int kThreads = kWave * kInt4Waves;
+constexpr int kHeads = kInt4HeadsPerWave;
+
+struct Int4Args {
+  const uint16_t* query;
+  int64_t query_batch_stride;
+  const uint8_t* codes;
+  const uint16_t* scales;
+  const int32_t* indices;
+  const int32_t* last_page_len;
+  const uint16_t* tail_k;
+  const uint16_t* tail_v;
+  const int32_t* tail_indices;
+  const int32_t* tail_last_len;
+  const uint16_t* value_center;
+  int64_t center_batch_stride;
+  const Int4Item* items;
+  float* partial_o;                // [items][Hq][128]
+  float* partial_m;                // [items][Hq], base-2 scores
+  float* partial_l;
+  uint16_t* out;
+  float* lse;
+  float sm_scale_log2;
+  int num_qo_heads, num_kv_heads, group, subs;
+};
+
+__device__ __forceinline__ v2h as_half2(uint32_t bits) { return __builtin_bit_cast(v2h, bits); }
+
+// The codes of nibbles i and i + 4 as FP16.
+__device__ __forceinline__ v2h codes2(uint32_t word, int i) {
+  const uint32_t bits = (word >> (4 * i) & 0x000f000fu) | 0x64006400u;
+  return as_half2(bits) - v2h{static_cast<_Float16>(1032.0f), static_cast<_Float16>(1032.0f)};
+}
+
+__device__ __forceinline__ v8h join(v2h a, v2h b, v2h c, v2h d) {
+  return v8h{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// Running state of one wave.  Lane (kg, n): m, l of head n % 8 (l over its own
+// tokens), acc[nb][r] = row 4 kg + r of the product, channel 8 n + nb.
+struct State {
+  float m, l;
+  v4f acc[8];
+};
+
+// Softmax step over kPages pages: s are the lane's scores (already scaled),
+// w the weights of V (v_scale: V's scale of each, times 2^e), masked scores -inf.
+template <int kPages>
+__device__ __forceinline__ void softmax_step(State& st, const float (&s)[kPages][4],
+                                             const float (&v_scale)[kPages][4], float low_part,
+                                             int lane, v8h (&p)[kPages / 2]) {
+  float top = kNegInf;
+#pragma unroll
+  for (int i = 0; i < kPages; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][r]);
+  top = fmaxf(top, __shfl_xor(top, 16, kWave));
+  top = fmaxf(top, __shfl_xor(top, 32, kWave));
+  const float m = fmaxf(st.m, top);
+  const float base = m == kNegInf ? 0.0f : m;    // nothing visible yet: every p is 0
+  const float alpha = __builtin_amdgcn_exp2f(st.m - base);
+  if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+    const int kg = lane >> 4;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float f = __shfl(alpha, (4 * kg + r) & 7, kWave);
+#pragma unroll
+      for (int nb = 0; nb < 8; ++nb) st.acc[nb][r] *= f;
+    }
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kPages / 2; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = __builtin_amdgcn_exp2f(s[2 * j + (e >> 2)][e & 3] - base);
+      sum += x;
+      // a masked token's scale may be anything
+      const float w = x == 0.0f ? 0.0f : x * v_scale[2 * j + (e >> 2)][e & 3];
+      const _Float16 high = static_cast<_Float16>(w);
+      p[j][e] = static_cast<_Float16>(w - low_part * static_cast<float>(high));
+    }
+  st.l = st.l * alpha + sum;
+  st.m = m;
+}
+
+// MFMA operand A of K rows or V columns in FP16, for pages of the tail.
+__device__ __forceinline__ uint32_t pick(uint32_t a, uint32_t b, bool high) {
+  // the low or the high halves of two words, side by side
+  return high ? __builtin_amdgcn_perm(b, a, 0x07060302u) : __builtin_amdgcn_perm(b, a, 0x05040100u);
+}
+
+struct Group {
+  v4u k[kInt4GroupPages], v[kInt4GroupPages], s[kInt4GroupPages];
+};
+
+__global__ __launch_bounds__(kThreads) void int4_decode_kernel(Int4Args a) {
+  __shared__ float part_o[kInt4Waves][kHeads][kHeadDim];
+  __shared__ float part_m[kInt4Waves][kHeads];
+  __shared__ float part_l[kInt4Waves][kHeads];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
+  const int n = lane & 15, kg = lane >> 4;
+  const Int4Item it = a.items[blockIdx.x];
+  const int kv = blockIdx.y / a.subs;
+  const int first_head = (blockIdx.y % a.subs) * kHeads;     // within the KV head's group
+  const int heads = min(kHeads, a.group - first_head);
+  const int hkv = a.num_kv_heads;
+
+  // query: B operand, column n = head n % 8, dims 32 w + 8 kg ..
+  v8h q[4];
+  {
+    const bool in = (n & 7) < heads;
+    const uint16_t* row = a.query + it.request * a.query_batch_stride +
+                          static_cast<int64_t>(kv * a.group + first_head + (in ? n & 7 : 0)) * kHeadDim;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      q[w] = *reinterpret_cast<const v8h*>(row + 32 * w + 8 * kg);
+      if (!in) q[w] = v8h{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+  }
+  const float low_part = n < 8 ? 0.0f : 1.0f;
+
+  State st;
+  st.m = kNegInf;
+  st.l = 0.0f;
+#pragma unroll
+  for (int nb = 0; nb < 8; ++nb) st.acc[nb] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  int scale_exp = 0;               // st.acc is held times 2^scale_exp
+
+  // ---- history: groups wave, wave + 8, ... of the item's pages
+  const int count = it.page_end - it.page_begin;
+  const int all_groups = (count + kInt4GroupPages - 1) / kInt4GroupPages;
+  const int groups = (all_groups - wave + kInt4Waves - 1) / kInt4Waves;
+  if (groups > 0) {
+    // lane l: slot l of the wave, page 4 (8 (l / 4) + wave) + l % 4 of the item
+    const int slot_page = kInt4GroupPages * (kInt4Waves * (lane / kInt4GroupPages) + wave) +
+                          lane % kInt4GroupPages;
+    const bool held = slot_page < count;
+    const int my_page = a.indices[it.page_begin + min(slot_page, count - 1)];
+    const int last_len = min(a.last_page_len[it.request], kPageSize);
+    auto visible = [&](int page) {     // tokens of the item's page ``page``
+      return page >= count ? 0 : it.page_begin + page == it.last_page ? last_len : kPageSize;
+    };
+    Group buf[2];
+    auto issue = [&](int g, Group& dst) {
+#pragma unroll
+      for (int i = 0; i < kInt4GroupPages; ++i) {
+        const int page = __builtin_amdgcn_readlane(my_page, g * kInt4GroupPages + i);
+        const int64_t block = static_cast<int64_t>(page) * hkv + kv;
+        const uint8_t* codes = a.codes + block * kInt4BlockBytes;
+        dst.k[i] = *reinterpret_cast<const v4u*>(codes + 16 * lane);
+        dst.v[i] = *reinterpret_cast<const v4u*>(codes + kInt4PartBytes + 16 * lane);
+        dst.s[i] = *reinterpret_cast<const v4u*>(a.scales + block * kInt4BlockScales + 8 * kg);
+      }
+    };
+    issue(0, buf[0]);
+    // the largest visible V scale of the wave's pages fixes the power of two
+    float top = 0.0f;
+    {
+      const uint16_t* scales = a.scales + (static_cast<int64_t>(my_page) * hkv + kv) * kInt4BlockScales;
+      const int limit = held ? visible(slot_page) : 0;
+      v2u raw[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) raw[g] = *reinterpret_cast<const v2u*>(scales + 8 * g + 4);
+#pragma unroll
+      for (int t = 0; t < kPageSize; ++t) {
+        const float s = half_bits_to_float(static_cast<uint16_t>(raw[t >> 2][(t & 3) >> 1] >> (16 * (t & 1))));
+        top = fmaxf(top, t < limit ? s : 0.0f);
+      }
+      top = wave_max(top);
+    }
+    int e = 0;
+    if (top > 0.0f) frexpf(top, &e);
+    scale_exp = 14 - e;
+    const float unit = ldexpf(1.0f, scale_exp);
+
+    auto compute = [&](int g, const Group& cur) {
+      float s[kInt4GroupPages][4], v_scale[kInt4GroupPages][4];
+#pragma unroll
+      for (int i = 0; i < kInt4GroupPages; ++i) {
+        v4f dot = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t x = cur.k[i][w];
+          dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              join(codes2(x, 0), codes2(x, 1), codes2(x, 2), codes2(x, 3)), q[w], dot, 0, 0, 0);
+        }
+        const int limit = visible(kInt4GroupPages * (kInt4Waves * g + wave) + i);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float ks = half_bits_to_float(static_cast<uint16_t>(cur.s[i][r >> 1] >> (16 * (r & 1))));
+          const float vs = half_bits_to_float(static_cast<uint16_t>(cur.s[i][2 + (r >> 1)] >> (16 * (r & 1))));
+          s[i][r] = 4 * kg + r < limit ? dot[r] * (ks * a.sm_scale_log2) : kNegInf;
+          v_scale[i][r] = vs * unit;
+        }
+      }
+      v8h p[kInt4GroupPages / 2];
+      softmax_step<kInt4GroupPages>(st, s, v_scale, low_part, lane, p);
+#pragma unroll
+      for (int j = 0; j < kInt4GroupPages / 2; ++j)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t x = cur.v[2 * j][w], y = cur.v[2 * j + 1][w];
+          st.acc[2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              p[j], join(codes2(x, 0), codes2(x, 1), codes2(y, 0), codes2(y, 1)), st.acc[2 * w], 0, 0, 0);
+          st.acc[2 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              p[j], join(codes2(x, 2), codes2(x, 3), codes2(y, 2), codes2(y, 3)), st.acc[2 * w + 1], 0, 0, 0);
+        }
+    };
+    int g = 0;
+    for (; g + 2 < groups; g += 2) {
+      issue(g + 1, buf[1]);
+      compute(g, buf[0]);
+      issue(g + 2, buf[0]);
+      compute(g + 1, buf[1]);
+    }
+    if (g + 1 < groups) {
+      issue(g + 1, buf[1]);
+      compute(g, buf[0]);
+      compute(g + 1, buf[1]);
+    } else {
+      compute(g, buf[0]);
+    }
+  }
+
+  // ---- exact tail: pairs wave, wave + 8, ... of the item's tail pages
+  const int tail_count = it.tail_end - it.tail_begin;
+  if (2 * wave < tail_count) {
+    const float change = ldexpf(1.0f, 14 - scale_exp);     // p alone is at most 1
+#pragma unroll
+    for (int nb = 0; nb < 8; ++nb) st.acc[nb] *= change;
+    scale_exp = 14;
+    const int64_t row_stride = static_cast<int64_t>(hkv) * kHeadDim;
+    const int last_len = min(a.tail_last_len[it.request], kPageSize);
+    for (int page = 2 * wave; page < tail_count; page += 2 * kInt4Waves) {
+      float s[2][4], ones[2][4];
+      v4u k[2][4], v[2][4];
+      int limit[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = it.tail_begin + min(page + i, tail_count - 1);
+        const int64_t base = static_cast<int64_t>(a.tail_indices[at]) * kPageSize * row_stride + kv * kHeadDim;
+        limit[i] = page + i >= tail_count ? 0 : at == it.last_tail ? last_len : kPageSize;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          k[i][w] = *reinterpret_cast<const v4u*>(a.tail_k + base + n * row_stride + 32 * w + 8 * kg);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          v[i][t] = *reinterpret_cast<const v4u*>(a.tail_v + base + (4 * kg + t) * row_stride + 8 * n);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        v4f dot = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, k[i][w]), q[w], dot, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[i][r] = 4 * kg + r < limit[i] ? dot[r] * a.sm_scale_log2 : kNegInf;
+          ones[i][r] = 0x1p14f;
+          // a row not yet written may hold anything: 0 times it must be 0
+          if (4 * kg + r >= limit[i]) v[i][r] = v4u{0u, 0u, 0u, 0u};
+        }
+      }
+      v8h p[1];
+      softmax_step<2>(st, s, ones, low_part, lane, p);
+#pragma unroll
+      for (int nb = 0; nb < 8; ++nb) {
+        v4u cols;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          cols[2 * i] = pick(v[i][0][nb >> 1], v[i][1][nb >> 1], nb & 1);
+          cols[2 * i + 1] = pick(v[i][2][nb >> 1], v[i][3][nb >> 1], nb & 1);
+        }
+        st.acc[nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[0], __builtin_bit_cast(v8h, cols), st.acc[nb], 0, 0, 0);
+      }
+    }
+  }
+
+  // ---- the waves meet: rows r and r + 8 of the product, then 8 partial states
+  st.l += __shfl_xor(st.l, 16, kWave);
+  st.l += __shfl_xor(st.l, 32, kWave);
+  if (kg == 0 && n < kHeads) {
+    part_m[wave][n] = st.m;
+    part_l[wave][n] = st.l;
+  }
+  const float scale = ldexpf(1.0f, -scale_exp);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    float o[8];
+#pragma unroll
+    for (int nb = 0; nb < 8; ++nb) o[nb] = (st.acc[nb][r] + __shfl_xor(st.acc[nb][r], 32, kWave)) * scale;
+    if (kg < 2) {
+      float* dst = &part_o[wave][4 * kg + r][8 * n];
+      *reinterpret_cast<float4*>(dst) = make_float4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<float4*>(dst + 4) = make_float4(o[4], o[5], o[6], o[7]);
+    }
+  }
+  __syncthreads();
+  if (wave >= heads) return;       // wave h finishes head h, two dims per lane
+  float m = kNegInf;
+#pragma unroll
+  for (int w = 0; w < kInt4Waves; ++w) m = fmaxf(m, part_m[w][wave]);
+  const float base = m == kNegInf ? 0.0f : m;
+  float l = 0.0f;
+  float2 o = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int w = 0; w < kInt4Waves; ++w) {
+    const float f = __builtin_amdgcn_exp2f(part_m[w][wave] - base);
+    const float2 x = *reinterpret_cast<const float2*>(&part_o[w][wave][2 * lane]);
+    l += f * part_l[w][wave];
+    o.x += f * x.x;
+    o.y += f * x.y;
+  }
+  const int head = kv * a.group + first_head + wave;
+  if (it.items_in_request > 1) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * a.num_qo_heads + head;
+    *reinterpret_cast<float2*>(a.partial_o + row * kHeadDim + 2 * lane) = o;
+    if (lane == 0) {
+      a.partial_m[row] = m;
+      a.partial_l[row] = l;
+    }
+    return;
+  }
+  const int64_t row = static_cast<int64_t>(it.request) * a.num_qo_heads + head;
+  float2 c = make_float2(0.0f, 0.0f);
+  if (a.value_center) {
+    const uint32_t bits = *reinterpret_cast<const uint32_t*>(
+        a.value_center + it.request * a.center_batch_stride + kv * kHeadDim + 2 * lane);
+    c = make_float2(half_bits_to_float(static_cast<uint16_t>(bits)),
+                    half_bits_to_float(static_cast<uint16_t>(bits >> 16)));
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;      // no token: the center alone
+  *reinterpret_cast<__half2*>(a.out + row * kHeadDim + 2 * lane) =
+      __floats2half2_rn(o.x * inv + c.x, o.y * inv + c.y);
+  if (lane == 0 && a.lse) a.lse[row] = l == 0.0f ? kNegInf : log2f(l) + m;
+}
+
+struct Int4CombineArgs {
+  const float* partial_o;
+  const float* partial_m;
+  const float* partial_l;
+  const int32_t* item_ptr;
+  const uint16_t* value_center;
+  int64_t center_batch_stride;
+  uint16_t* out;
+  float* lse;
+  int num_qo_heads, group;
+};
+
+// Joins the partial states of one (request, query head): 4 waves take its
+// items in turn, two dims per lane.
+__global__ __launch_bounds__(4 * kWave) void int4_combine_kernel(Int4CombineArgs a) {
+  __shared__ float part_o[4][kHeadDim];
+  __shared__ float part_m[4], part_l[4];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int request = blockIdx.x, head = blockIdx.y;
+  const int begin = a.item_ptr[request], end = a.item_ptr[request + 1];
+  if (end - begin <= 1) return;    // its only workgroup wrote the output
+  float m = kNegInf, l = 0.0f;
+  float2 o = make_float2(0.0f, 0.0f);
+  for (int i = begin + wave; i < end; i += 4) {
+    const int64_t row = static_cast<int64_t>(i) * a.num_qo_heads + head;
+    const float mi = a.partial_m[row];
+    const float2 x = *reinterpret_cast<const float2*>(a.partial_o + row * kHeadDim + 2 * lane);
+    const float top = fmaxf(m, mi), base = top == kNegInf ? 0.0f : top;
+    const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(mi - base);
+    l = l * f + a.partial_l[row] * g;
+    o.x = o.x * f + x.x * g;
+    o.y = o.y * f + x.y * g;
+    m = top;
+  }
+  *reinterpret_cast<float2*>(&part_o[wave][2 * lane]) = o;
+  if (lane == 0) {
+    part_m[wave] = m;
+    part_l[wave] = l;
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  m = fmaxf(fmaxf(part_m[0], part_m[1]), fmaxf(part_m[2], part_m[3]));
+  const float base = m == kNegInf ? 0.0f : m;
+  l = 0.0f;
+  o = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = __builtin_amdgcn_exp2f(part_m[w] - base);
+    const float2 x = *reinterpret_cast<const float2*>(&part_o[w][2 * lane]);
+    l += f * part_l[w];
+    o.x += f * x.x;
+    o.y += f * x.y;
+  }
+  const int64_t row = static_cast<int64_t>(request) * a.num_qo_heads + head;
+  float2 c = make_float2(0.0f, 0.0f);
+  if (a.value_center) {
+    const uint32_t bits = *reinterpret_cast<const uint32_t*>(
+        a.value_center + request * a.center_batch_stride + (head / a.group) * kHeadDim + 2 * lane);
+    c = make_float2(half_bits_to_float(static_cast<uint16_t>(bits)),
+                    half_bits_to_float(static_cast<uint16_t>(bits >> 16)));
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  *reinterpret_cast<__half2*>(a.out + row * kHeadDim + 2 * lane) =
+      __floats2half2_rn(o.x * inv + c.x, o.y * inv + c.y);
+  if (lane == 0 && a.lse) a.lse[row] = l == 0.0f ? kNegInf : log2f(l) + m;
+}
+
+}  // namespace
+}  // namespace pg
+
+using namespace pg;
+
+extern "C" int32_t pg_int4_plan(const int32_t* host_indptr, const int32_t* host_tail_indptr,
+                                int32_t batch_size, int32_t num_qo_heads, int32_t num_kv_heads,
+                                int32_t num_cus, void* workspace, int64_t workspace_bytes,
+                                pg_int4_plan_t* plan, void* stream) {
+  clear_error();
+  if (!plan || !workspace) return fail(PG_ERROR_INVALID_ARGUMENT, "null plan argument");
+  return guarded([&]() -> int32_t {
+    std::vector<Int4Item> items;
+    std::vector<int32_t> item_ptr;
+    pg_int4_plan_t p{};
+    if (int32_t rc = build_int4_plan(host_indptr, host_tail_indptr, batch_size, num_qo_heads,
+                                     num_kv_heads, num_cus, items, item_ptr, p))
+      return rc;
+    if (p.workspace_bytes > workspace_bytes)
+      return fail(PG_ERROR_WORKSPACE, "decode workspace too small: need " +
+                                          std::to_string(p.workspace_bytes) + " bytes, have " +
+                                          std::to_string(workspace_bytes));
+    hipStream_t s = as_stream(stream);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    if (hipMemcpyAsync(ws + p.items_offset, items.data(), items.size() * sizeof(Int4Item),
+                       hipMemcpyHostToDevice, s) != hipSuccess ||
+        hipMemcpyAsync(ws + p.item_ptr_offset, item_ptr.data(), item_ptr.size() * sizeof(int32_t),
+                       hipMemcpyHostToDevice, s) != hipSuccess ||
+        hipStreamSynchronize(s) != hipSuccess)
+      return fail(PG_ERROR_LAUNCH, "plan copy failed");
+    *plan = p;
+    return PG_OK;
+  });
+}
+
+extern "C" int32_t pg_int4_decode_run(const pg_int4_plan_t* plan, const void* query,
+                                      int64_t query_batch_stride, const void* codes,
+                                      const void* scales, const int32_t* indices,
+                                      const int32_t* last_page_len, const void* tail_k,
+                                      const void* tail_v, const int32_t* tail_indices,
+                                      const int32_t* tail_last_len, const void* value_center,
+                                      int64_t center_batch_stride, void* out, float* lse,
+                                      float sm_scale, void* workspace, void* stream) {
+  clear_error();
+  if (!plan || !query || !out || !workspace) return fail(PG_ERROR_INVALID_ARGUMENT, "null run argument");
+  if (plan->has_history && (!codes || !scales || !indices || !last_page_len))
+    return fail(PG_ERROR_INVALID_ARGUMENT, "history segment tensors missing");
+  if (plan->has_tail && (!tail_k || !tail_v || !tail_indices || !tail_last_len))
+    return fail(PG_ERROR_INVALID_ARGUMENT, "tail segment tensors missing");
+  if (!(sm_scale > 0.0f) || !__builtin_isfinite(sm_scale))
+    return fail(PG_ERROR_INVALID_ARGUMENT, "sm_scale must be positive and finite");
+  if (plan->num_items <= 0 || plan->batch_size <= 0 || plan->num_kv_heads <= 0 ||
+      plan->num_qo_heads % plan->num_kv_heads || plan->num_qo_heads / plan->num_kv_heads > 16)
+    return fail(PG_ERROR_INVALID_ARGUMENT, "the plan is not one of pg_int4_plan");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  Int4Args a{};
+  a.query = static_cast<const uint16_t*>(query);
+  a.query_batch_stride = query_batch_stride;
+  a.codes = static_cast<const uint8_t*>(codes);
+  a.scales = static_cast<const uint16_t*>(scales);
+  a.indices = indices;
+  a.last_page_len = last_page_len;
+  a.tail_k = static_cast<const uint16_t*>(tail_k);
+  a.tail_v = static_cast<const uint16_t*>(tail_v);
+  a.tail_indices = tail_indices;
+  a.tail_last_len = tail_last_len;
+  a.value_center = static_cast<const uint16_t*>(value_center);
+  a.center_batch_stride = center_batch_stride;
+  a.items = reinterpret_cast<const Int4Item*>(ws + plan->items_offset);
+  const int64_t rows = static_cast<int64_t>(plan->num_items) * plan->num_qo_heads;
+  a.partial_o = reinterpret_cast<float*>(ws + plan->partial_offset);
+  a.partial_m = a.partial_o + rows * kHeadDim;
+  a.partial_l = a.partial_m + rows;
+  a.out = static_cast<uint16_t*>(out);
+  a.lse = lse;
+  a.sm_scale_log2 = sm_scale * 1.4426950408889634f;
+  a.num_qo_heads = plan->num_qo_heads;
+  a.num_kv_heads = plan->num_kv_heads;
+  a.group = plan->num_qo_heads / plan->num_kv_heads;
+  a.subs = (a.group + kHeads - 1) / kHeads;
+  hipLaunchKernelGGL(int4_decode_kernel, dim3(plan->num_items, plan->num_kv_heads * a.subs),
+                     dim3(kThreads), 0, as_stream(stream), a);
+  if (int32_t rc = check_launch("int4_decode")) return rc;
+  if (plan->max_items_per_request <= 1) return PG_OK;
+  Int4CombineArgs c{};
+  c.partial_o = a.partial_o;
+  c.partial_m = a.partial_m;
+  c.partial_l = a.partial_l;
+  c.item_ptr = reinterpret_cast<const int32_t*>(ws + plan->item_ptr_offset);
+  c.value_center = a.value_center;
+  c.center_batch_stride = center_batch_stride;
+  c.out = a.out;
+  c.lse = lse;
+  c.num_qo_heads = plan->num_qo_heads;
+  c.group = a.group;
+  hipLaunchKernelGGL(int4_combine_kernel, dim3(plan->batch_size, plan->num_qo_heads),
+                     dim3(4 * kWave), 0, as_stream(stream), c);
+  return check_launch("int4_combine");
+}

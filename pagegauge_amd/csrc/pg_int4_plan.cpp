@@ -1,0 +1,137 @@
+// Planner of the attention over the cache held in 4 bits (host only).
+#include "pg_int4_plan.h"
+
+#include <algorithm>
+#include <cstring>
+#include <string>
+
+namespace pg {
+namespace {
+
+int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// A request's pages, weighted by their bytes in 4-bit pages, as one sequence:
+// the history, then the exact tail.
+struct Request {
+  int64_t pages, tail;
+  int64_t weight() const { return pages + kInt4TailWeight * tail; }
+  int64_t cuts(int64_t cap) const { return std::max<int64_t>(1, ceil_div(weight(), cap)); }
+};
+
+}  // namespace
+
+int32_t build_int4_plan(const int32_t* host_indptr, const int32_t* host_tail_indptr,
+                        int32_t batch_size, int32_t num_qo_heads, int32_t num_kv_heads,
+                        int32_t num_cus, std::vector<Int4Item>& items,
+                        std::vector<int32_t>& item_ptr, pg_int4_plan_t& p) {
+  if (!host_indptr) return fail(PG_ERROR_INVALID_ARGUMENT, "null plan argument");
+  if (batch_size <= 0) return fail(PG_ERROR_INVALID_ARGUMENT, "batch size must be positive");
+  if (num_kv_heads <= 0 || num_qo_heads <= 0 || num_qo_heads % num_kv_heads)
+    return fail(PG_ERROR_INVALID_ARGUMENT, "query heads must be a positive multiple of KV heads");
+  if (num_qo_heads / num_kv_heads > 16)
+    return fail(PG_ERROR_UNSUPPORTED, "at most 16 query heads per KV head");
+  if (num_kv_heads > 1024) return fail(PG_ERROR_UNSUPPORTED, "at most 1024 KV heads");
+  std::vector<Request> requests(batch_size);
+  int64_t total = 0, history = 0, exact_pages = 0;
+  for (int32_t b = 0; b < batch_size; ++b) {
+    Request& r = requests[b];
+    r.pages = static_cast<int64_t>(host_indptr[b + 1]) - host_indptr[b];
+    r.tail = host_tail_indptr ? static_cast<int64_t>(host_tail_indptr[b + 1]) - host_tail_indptr[b] : 0;
+    if (host_indptr[b] < 0 || r.pages < 0 || r.tail < 0 || (host_tail_indptr && host_tail_indptr[b] < 0))
+      return fail(PG_ERROR_INVALID_ARGUMENT, "indptr must be nonnegative and non-decreasing");
+    total += r.weight();
+    history += r.pages;
+    exact_pages += r.tail;
+  }
+  // The largest share of a workgroup (``cap``, in weighted pages) for which
+  // the batch fills about two workgroups per CU, but at least one group of
+  // pages per wave, and at most the pages that an item can hold.
+  const int64_t groups = static_cast<int64_t>(num_kv_heads) *
+                         ceil_div(num_qo_heads / num_kv_heads, kInt4HeadsPerWave);
+  const int64_t cus = num_cus > 0 ? num_cus : 256;
+  const int64_t target = std::max<int64_t>(batch_size, 2 * cus / groups);
+  int64_t low = kInt4Waves * kInt4GroupPages;
+  int64_t high = std::min<int64_t>(std::max(low, total), kInt4MaxItemPages);
+  auto count = [&](int64_t cap) {
+    int64_t n = 0;
+    for (const Request& r : requests) n += r.cuts(cap);
+    return n;
+  };
+  while (low < high) {
+    const int64_t mid = low + (high - low) / 2;
+    if (count(mid) <= target) high = mid; else low = mid + 1;
+  }
+  items.clear();
+  item_ptr.assign(batch_size + 1, 0);
+  int64_t most = 0;
+  for (int32_t b = 0; b < batch_size; ++b) {
+    const Request& r = requests[b];
+    const int64_t cuts = r.cuts(high);
+    if (cuts > kInt4MaxItemsPerRequest)
+      return fail(PG_ERROR_UNSUPPORTED, "too many pages in one request");
+    item_ptr[b] = static_cast<int32_t>(items.size());
+    const int32_t begin = host_indptr[b], tail = host_tail_indptr ? host_tail_indptr[b] : 0;
+    // cut i ends at weight w = (i + 1) W / cuts: its history page, or the
+    // tail page that w falls into
+    int64_t page = 0, exact = 0;
+    for (int64_t i = 0; i < cuts; ++i) {
+      const int64_t w = (i + 1) * r.weight() / cuts;
+      int64_t page_end = std::min(r.pages, w);
+      int64_t exact_end = w <= r.pages ? 0 : (w - r.pages) / kInt4TailWeight;
+      if (i + 1 == cuts) { page_end = r.pages; exact_end = r.tail; }
+      items.push_back({b, static_cast<int32_t>(begin + page), static_cast<int32_t>(begin + page_end),
+                       static_cast<int32_t>(begin + r.pages - 1), static_cast<int32_t>(tail + exact),
+                       static_cast<int32_t>(tail + exact_end), static_cast<int32_t>(tail + r.tail - 1),
+                       static_cast<int32_t>(cuts)});
+      page = page_end;
+      exact = exact_end;
+    }
+    most = std::max(most, cuts);
+  }
+  if (items.size() > INT32_MAX / 2) return fail(PG_ERROR_UNSUPPORTED, "too many work items");
+  item_ptr[batch_size] = static_cast<int32_t>(items.size());
+  p = pg_int4_plan_t{};
+  p.batch_size = batch_size;
+  p.num_qo_heads = num_qo_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.has_tail = exact_pages > 0;
+  p.has_history = history > 0;
+  p.num_items = static_cast<int32_t>(items.size());
+  p.max_items_per_request = static_cast<int32_t>(most);
+  p.items_offset = 0;
+  p.item_ptr_offset = align_up(static_cast<int64_t>(items.size() * sizeof(Int4Item)), 256);
+  p.partial_offset = p.item_ptr_offset + align_up((batch_size + 1) * 4, 256);
+  const int64_t rows = most > 1 ? static_cast<int64_t>(items.size()) * num_qo_heads : 0;
+  p.workspace_bytes = p.partial_offset + rows * (kHeadDim + 2) * 4;
+  return PG_OK;
+}
+
+}  // namespace pg
+
+using namespace pg;
+
+extern "C" int32_t pg_int4_plan_host(const int32_t* host_indptr, const int32_t* host_tail_indptr,
+                                     int32_t batch_size, int32_t num_qo_heads, int32_t num_kv_heads,
+                                     int32_t num_cus, pg_int4_plan_t* plan, int32_t* items_out,
+                                     int64_t items_capacity, int32_t* item_ptr_out) {
+  clear_error();
+  if (!plan) return fail(PG_ERROR_INVALID_ARGUMENT, "null plan argument");
+  return guarded([&]() -> int32_t {
+    std::vector<Int4Item> items;
+    std::vector<int32_t> item_ptr;
+    pg_int4_plan_t p{};
+    if (int32_t rc = build_int4_plan(host_indptr, host_tail_indptr, batch_size, num_qo_heads,
+                                     num_kv_heads, num_cus, items, item_ptr, p))
+      return rc;
+    if (items_out) {
+      if (items_capacity < static_cast<int64_t>(items.size()))
+        return fail(PG_ERROR_INVALID_ARGUMENT, "work-item buffer too small: need " +
+                                                   std::to_string(items.size()) + " items");
+      std::memcpy(items_out, items.data(), items.size() * sizeof(Int4Item));
+    }
+    if (item_ptr_out) std::memcpy(item_ptr_out, item_ptr.data(), item_ptr.size() * sizeof(int32_t));
+    *plan = p;
+    return PG_OK;
+  });
+}

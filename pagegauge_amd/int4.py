@@ -1,0 +1,351 @@
+"""The KV cache held in 4 bits: writers, reader-back and attention.
+
+Beside the INT8 pages of ``update`` and ``decode``, the same page tables, exact
+FP16 pages and centers over pages of half the bytes.  A page of 16 tokens holds
+per KV head one code in [-7, 7] per value and one FP16 scale per token, K and V
+apart, of rows centered on the request's channel means:
+
+* ``allocate_pages`` -- the pool: ``codes`` uint8 [pages, Hkv, 2, 1024] and
+  ``scales`` FP16 [pages, Hkv, 4, 2, 4] (``include/pagegauge_hip.h`` gives the
+  order of the nibbles);
+* ``quantize_pages`` -- a prompt's token-major K and V into pages, with the
+  centered FP16 copies of its exact pages (the 4-bit ``update.prefill_page_gauge``);
+* ``dequantize_pages`` -- back to FP16, for a prompt that continues a cached
+  prefix;
+* ``rope_append`` -- one token per request: rotation, centered append to the
+  exact pages, and the page that a token completed held in 4 bits (the 4-bit
+  ``rope_append_page_gauge_slots``, with ``rotary.RotaryEmbedding``);
+* ``Int4PagedDecode`` -- attention of one token per request over 4-bit pages,
+  an exact FP16 tail and the value center, planned like
+  ``decode.PageGaugeSegmentedDecode``, for 1 to 16 query heads per KV head.
+
+Everything runs on the current stream and nothing but ``plan`` synchronises.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from . import _capi
+from .decode import (_check_cache, _check_index, _check_page_ids, _check_query, _host_i32,
+                     _host_tables, _num_cus, _page_id_range)
+from .rotary import RotaryEmbedding
+
+DIM = 128
+PAGE = 16
+BLOCK_SHAPE = (2, 1024)
+SCALE_SHAPE = (4, 2, 4)
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def allocate_pages(pages: int, kv_heads: int, device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of a pool, zeroed (every value -8 times a scale of 0)."""
+    return (torch.zeros(pages, kv_heads, *BLOCK_SHAPE, device=device, dtype=torch.uint8),
+            torch.zeros(pages, kv_heads, *SCALE_SHAPE, device=device, dtype=torch.float16))
+
+
+def _check_pool(codes: torch.Tensor, scales: torch.Tensor, heads: int) -> int:
+    pages = codes.shape[0] if codes.dim() == 4 else -1
+    if codes.dtype != torch.uint8 or codes.shape != (pages, heads, *BLOCK_SHAPE) \
+            or not codes.is_contiguous():
+        raise ValueError(f"4-bit codes must be contiguous uint8 [pages,{heads},2,1024]")
+    if scales.dtype != torch.float16 or scales.shape != (pages, heads, *SCALE_SHAPE) \
+            or not scales.is_contiguous():
+        raise ValueError(f"4-bit scales must be contiguous float16 [{pages},{heads},4,2,4]")
+    return pages
+
+
+def _check_ids(ids: Optional[torch.Tensor], count: int, what: str) -> None:
+    if ids is not None and (ids.dtype != torch.int32 or ids.shape != (count,) or not ids.is_contiguous()):
+        raise ValueError(f"{what} must be contiguous int32 [{count}]")
+
+
+def _token_rows(t: torch.Tensor, what: str) -> int:
+    """Token stride of FP16 rows [T, H, 128] whose heads are dense."""
+    if t.dtype != torch.float16 or t.dim() != 3 or t.shape[2] != DIM or t.shape[1] == 0 \
+            or t.stride(2) != 1 or t.stride(1) != DIM and t.shape[1] > 1:
+        raise ValueError(f"{what} must be float16 [T,Hkv,128] rows of dense heads")
+    return t.stride(0)
+
+
+def _check_centers(key_center, value_center, shape: tuple) -> None:
+    if (key_center is None) != (value_center is None):
+        raise ValueError("key and value centers go together")
+    for c in (key_center, value_center):
+        if c is not None and (c.dtype != torch.float16 or tuple(c.shape) != shape
+                              or not c.is_contiguous()):
+            raise ValueError(f"centers must be contiguous float16 {list(shape)}")
+
+
+def _check_exact(pages: torch.Tensor, heads: int, what: str) -> int:
+    if pages.dtype != torch.float16 or pages.dim() != 4 or pages.shape[1:] != (PAGE, heads, DIM) \
+            or not pages.is_contiguous():
+        raise ValueError(f"{what} must be contiguous float16 [pages,16,{heads},128]")
+    return pages.shape[0]
+
+
+def quantize_pages(key: torch.Tensor, value: torch.Tensor, codes: torch.Tensor,
+                   scales: torch.Tensor, *, page_ids: Optional[torch.Tensor] = None,
+                   key_center: Optional[torch.Tensor] = None,
+                   value_center: Optional[torch.Tensor] = None,
+                   exact_page_ids: Optional[torch.Tensor] = None,
+                   exact_key: Optional[torch.Tensor] = None,
+                   exact_value: Optional[torch.Tensor] = None) -> None:
+    """Hold token-major rows ``key``, ``value`` [T, Hkv, 128] in 4 bits: tokens
+    16i .. 16i + 15 in page ``page_ids[i]`` of the pool (device int32
+    [ceil(T / 16)]; None: page i), centered on ``key_center``, ``value_center``
+    [Hkv, 128] where given.  The rows of a partial last page past T get scale
+    0.  With ``exact_page_ids`` those pages are also stored, centered and
+    rounded to FP16, in pages ``exact_page_ids[i]`` of ``exact_key`` and
+    ``exact_value`` [pages, 16, Hkv, 128].  Ids outside their pool (-1) skip
+    the store.  Rows may be strided by token."""
+    if key.shape != value.shape:
+        raise ValueError("token-major K/V must have identical [T,Hkv,128] shapes")
+    key_stride, value_stride = _token_rows(key, "K"), _token_rows(value, "V")
+    tokens, heads = key.shape[0], key.shape[1]
+    pages = (tokens + PAGE - 1) // PAGE
+    pool = _check_pool(codes, scales, heads)
+    _check_ids(page_ids, pages, "page_ids")
+    _check_ids(exact_page_ids, pages, "exact_page_ids")
+    if page_ids is None and pages > pool:
+        raise ValueError(f"{pages} pages do not fit a pool of {pool}")
+    _check_centers(key_center, value_center, (heads, DIM))
+    exact_pages = 0
+    if exact_page_ids is not None:
+        if exact_key is None or exact_value is None:
+            raise ValueError("exact page ids need exact key/value pages")
+        exact_pages = min(_check_exact(exact_key, heads, "exact_key"),
+                          _check_exact(exact_value, heads, "exact_value"))
+    else:
+        exact_key = exact_value = None
+    _capi.require_current_device(key, value, codes, scales, page_ids, key_center, value_center,
+                                 exact_page_ids, exact_key, exact_value)
+    if tokens == 0 or pool == 0 and exact_pages == 0:
+        return
+    if pool == 0 or exact_page_ids is not None and exact_pages == 0:
+        raise ValueError("a pool without pages holds nothing")
+    _capi.call("pg_int4_quantize_pages", key.data_ptr(), key_stride, value.data_ptr(), value_stride,
+               _ptr(key_center), _ptr(value_center), codes.data_ptr(), scales.data_ptr(), pool,
+               _ptr(page_ids), _ptr(exact_page_ids), _ptr(exact_key), _ptr(exact_value), exact_pages,
+               tokens, heads, _capi.current_stream())
+
+
+def dequantize_pages(codes: torch.Tensor, scales: torch.Tensor,
+                     page_ids: Optional[torch.Tensor] = None, *, tokens: Optional[int] = None,
+                     key_center: Optional[torch.Tensor] = None,
+                     value_center: Optional[torch.Tensor] = None,
+                     key: Optional[torch.Tensor] = None,
+                     value: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(K, V) rows [tokens, Hkv, 128] in FP16 that pages ``page_ids`` (device
+    int32; None: the whole pool in order) stand for, ``code * scale + center``.
+    ``tokens`` defaults to whole pages.  Ids outside the pool give zeros.
+    ``key`` and ``value`` may be given (token rows may be strided)."""
+    if codes.dim() != 4 or codes.shape[1] == 0:
+        raise ValueError("4-bit codes must be contiguous uint8 [pages,Hkv,2,1024]")
+    heads = codes.shape[1]
+    pool = _check_pool(codes, scales, heads)
+    pages = pool if page_ids is None else page_ids.numel()
+    _check_ids(page_ids, pages, "page_ids")
+    tokens = pages * PAGE if tokens is None else int(tokens)
+    if not 0 <= tokens <= pages * PAGE:
+        raise ValueError(f"{pages} pages hold at most {pages * PAGE} tokens, asked for {tokens}")
+    _check_centers(key_center, value_center, (heads, DIM))
+    strides = []
+    rows = []
+    for t in (key, value):
+        if t is None:
+            t = torch.empty(tokens, heads, DIM, device=codes.device, dtype=torch.float16)
+        elif t.shape != (tokens, heads, DIM):
+            raise ValueError(f"K and V rows must be [{tokens},{heads},128]")
+        strides.append(_token_rows(t, "K and V"))
+        if tokens > 1 and strides[-1] < heads * DIM:
+            raise ValueError("K and V rows must not overlap")
+        rows.append(t)
+    _capi.require_current_device(codes, scales, page_ids, key_center, value_center, *rows)
+    if tokens:
+        _capi.call("pg_int4_dequantize_pages", codes.data_ptr(), scales.data_ptr(), pool,
+                   _ptr(page_ids), _ptr(key_center), _ptr(value_center), rows[0].data_ptr(),
+                   strides[0], rows[1].data_ptr(), strides[1], tokens, heads,
+                   _capi.current_stream())
+    return rows[0], rows[1]
+
+
+def rope_append(rotary: RotaryEmbedding, query: torch.Tensor, key: torch.Tensor,
+                value: torch.Tensor, positions: torch.Tensor, exact_page_ids: torch.Tensor,
+                code_page_ids: torch.Tensor, key_center: torch.Tensor, value_center: torch.Tensor,
+                rotated_query: torch.Tensor, exact_key: torch.Tensor, exact_value: torch.Tensor,
+                codes: torch.Tensor, scales: torch.Tensor) -> None:
+    """The cache update of one token per request, in one launch: ``query``
+    [B, Hq, 128] and ``key`` [B, Hkv, 128] rotated at ``positions`` (device
+    int32 [B]), the query into ``rotated_query``, key and ``value`` minus their
+    centers [B, Hkv, 128] into row ``positions % 16`` of page
+    ``exact_page_ids[b]`` of ``exact_key`` / ``exact_value``
+    [pages, 16, Hkv, 128], and where that is row 15, the completed page in 4
+    bits into page ``code_page_ids[b]`` of the pool.
+
+    The tables are ``serving.decode_tables``' or the caller's own.  A request
+    with a negative position (padding of a captured batch) is left out whole;
+    ids outside their pool skip the store.  The pages of one call must differ
+    from each other."""
+    if rotary.head_dim != DIM:
+        raise ValueError("the cache holds heads of 128 dims")
+    strides = []
+    for t, what in ((query, "query"), (key, "key"), (value, "value")):
+        strides.append(_token_rows(t, what))
+    batch, heads = key.shape[0], key.shape[1]
+    if value.shape != key.shape or query.shape[0] != batch:
+        raise ValueError("query, key and value must have a row per request")
+    for ids, what in ((positions, "positions"), (exact_page_ids, "exact_page_ids"),
+                      (code_page_ids, "code_page_ids")):
+        _check_ids(ids, batch, what)
+    if key_center is None:
+        raise ValueError("key and value centers are required")
+    _check_centers(key_center, value_center, (batch, heads, DIM))
+    if rotated_query.shape != query.shape or rotated_query.dtype != torch.float16 \
+            or not rotated_query.is_contiguous():
+        raise ValueError("rotated_query must be contiguous float16, shaped like the query")
+    exact_pages = min(_check_exact(exact_key, heads, "exact_key"),
+                      _check_exact(exact_value, heads, "exact_value"))
+    pool = _check_pool(codes, scales, heads)
+    _capi.require_current_device(rotary.turns, query, key, value, positions, exact_page_ids,
+                                 code_page_ids, key_center, value_center, rotated_query, exact_key,
+                                 exact_value, codes, scales)
+    if batch == 0:
+        return
+    if pool == 0 or exact_pages == 0:
+        raise ValueError("a pool without pages holds nothing")
+    _capi.call("pg_int4_rope_append", query.data_ptr(), key.data_ptr(), value.data_ptr(), strides[0],
+               strides[1], strides[2], positions.data_ptr(), rotary.turns.data_ptr(),
+               rotary.amplitude, rotary.rotary_dim, int(rotary.interleaved),
+               exact_page_ids.data_ptr(), code_page_ids.data_ptr(), key_center.data_ptr(),
+               value_center.data_ptr(), rotated_query.data_ptr(), exact_key.data_ptr(),
+               exact_value.data_ptr(), exact_pages, codes.data_ptr(), scales.data_ptr(), pool, batch,
+               query.shape[1], heads, _capi.current_stream())
+
+
+def plan_work_items(indptr, tail_indptr=None, num_qo_heads: int = 32, num_kv_heads: int = 8,
+                    num_cus: int = 256):
+    """Run the planner on the host only: ``(plan, items [n, 8], item_ptr)``."""
+    lib = _capi.library()
+    host = _host_i32(indptr)
+    tail = None if tail_indptr is None else _host_i32(tail_indptr)
+    if host.dim() != 1 or host.numel() < 2 or tail is not None and tail.shape != host.shape:
+        raise ValueError("indptr must be a 1-D tensor of batch_size + 1 >= 2 entries")
+    batch = host.numel() - 1
+    plan = _capi.Int4Plan()
+    args = (host.data_ptr(), _ptr(tail), batch, num_qo_heads, num_kv_heads, num_cus,
+            ctypes.byref(plan))
+    _capi.check(lib.pg_int4_plan_host(*args, None, 0, None), "decode plan")
+    items = torch.empty(plan.num_items, 8, dtype=torch.int32)
+    item_ptr = torch.empty(batch + 1, dtype=torch.int32)
+    _capi.check(lib.pg_int4_plan_host(*args, items.data_ptr(), items.shape[0], item_ptr.data_ptr()),
+                "decode plan")
+    return plan, items, item_ptr
+
+
+class Int4PagedDecode:
+    """Attention of one token per request over 4-bit history pages, an exact
+    FP16 tail and the value center (``plan`` / ``run`` as
+    ``decode.PageGaugeSegmentedDecode``).  Runs of one object share its
+    workspace and must not overlap on different streams."""
+
+    def __init__(self, workspace: torch.Tensor) -> None:
+        if not workspace.is_cuda or workspace.dtype != torch.uint8 or not workspace.is_contiguous() \
+                or workspace.data_ptr() % 256:
+            raise ValueError("workspace must be a contiguous CUDA uint8 tensor, 256-byte aligned")
+        self.workspace = workspace
+        self._plan = _capi.Int4Plan()
+        self._planned = False
+
+    def plan(self, indptr, indices: torch.Tensor, last_page_len: torch.Tensor,
+             tail_indptr=None, tail_indices: Optional[torch.Tensor] = None,
+             tail_last_page_len: Optional[torch.Tensor] = None, num_qo_heads: int = 32,
+             num_kv_heads: int = 8, sm_scale: Optional[float] = None,
+             num_cus: Optional[int] = None) -> None:
+        """CSR page tables of the history and, with ``tail_indptr``, of the
+        exact pages; either may be empty for a request.  ``indices`` and the
+        last lengths (device int32) must stay alive until the next ``plan``
+        and are re-read by every run.  Waits for the GPU."""
+        if (tail_indptr is None) != (tail_indices is None) or (tail_indptr is None) != (
+                tail_last_page_len is None):
+            raise ValueError("tail indptr, indices and last_page_len go together")
+        _check_index(indices, "indices")
+        _check_index(last_page_len, "last_page_len")
+        host, _ = _host_tables(indptr, last_page_len, indices)
+        tail = tail_range = None
+        if tail_indptr is not None:
+            _check_index(tail_indices, "tail_indices")
+            _check_index(tail_last_page_len, "tail_last_page_len")
+            tail, _ = _host_tables(tail_indptr, tail_last_page_len, tail_indices, "tail")
+            if tail.numel() != host.numel():
+                raise ValueError("history and tail page tables must cover the same batch")
+            tail_range = _page_id_range(tail_indices, tail)
+        _capi.require_current_device(self.workspace, indices, last_page_len, tail_indices,
+                                     tail_last_page_len)
+        _capi.call("pg_int4_plan", host.data_ptr(), _ptr(tail), host.numel() - 1, num_qo_heads,
+                   num_kv_heads, int(num_cus or _num_cus(indices.device)), self.workspace.data_ptr(),
+                   self.workspace.numel(), ctypes.byref(self._plan), _capi.current_stream())
+        self._planned = True
+        self._tables = (indices, last_page_len, tail_indices, tail_last_page_len)
+        self._table_ptrs = tuple(_ptr(t) for t in self._tables)
+        self._id_ranges = (_page_id_range(indices, host), tail_range)
+        self._batch = host.numel() - 1
+        self._num_qo_heads, self._num_kv_heads = num_qo_heads, num_kv_heads
+        self._sm_scale = sm_scale if sm_scale is not None else 1.0 / math.sqrt(DIM)
+
+    @property
+    def num_work_items(self) -> int:
+        return int(self._plan.num_items)
+
+    def run(self, q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, exact_cache=None,
+            value_center: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None,
+            out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+            return_lse: bool = False):
+        """Attention of ``q`` [B, Hq, 128] (FP16, dense heads): ``out`` FP16
+        [B, Hq, 128], with ``return_lse`` also the base-2 lse float32 [B, Hq].
+        ``exact_cache`` is the (K, V) pages of the tail, ``value_center``
+        [B, Hkv, 128].  A request without tokens gives its center (or zeros)
+        and an lse of -inf."""
+        if not self._planned:
+            raise RuntimeError("plan() must be called before run()")
+        hkv = self._num_kv_heads
+        _check_query(q, self._batch, self._num_qo_heads)
+        pool = _check_pool(codes, scales, hkv)
+        exact_k = exact_v = None
+        if self._tables[2] is not None:
+            if exact_cache is None:
+                raise ValueError("a plan with a tail needs the exact pages")
+            exact_k, exact_v = exact_cache
+            _check_cache(exact_k, "exact_k", torch.float16, hkv)
+            _check_cache(exact_v, "exact_v", torch.float16, hkv)
+            _check_page_ids(self._id_ranges[1], min(exact_k.shape[0], exact_v.shape[0]), "exact tail")
+        _check_page_ids(self._id_ranges[0], pool, "4-bit")
+        if value_center is not None and (value_center.dtype != torch.float16
+                                         or value_center.shape != (self._batch, hkv, DIM)
+                                         or not value_center.is_contiguous()):
+            raise ValueError(f"value_center must be contiguous float16 [B,{hkv},128]")
+        if out is None:
+            out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        elif out.shape != q.shape or out.dtype != torch.float16 or not out.is_contiguous():
+            raise ValueError("out must be contiguous float16, shaped like q")
+        if lse is None:
+            if return_lse:
+                lse = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32)
+        elif lse.shape != q.shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous():
+            raise ValueError("lse must be contiguous float32 [B,Hq]")
+        _capi.require_current_device(self.workspace, q, codes, scales, exact_k, exact_v, value_center,
+                                     out, lse)
+        indices, last, tail_indices, tail_last = self._table_ptrs
+        _capi.call("pg_int4_decode_run", ctypes.byref(self._plan), q.data_ptr(), q.stride(0),
+                   codes.data_ptr(), scales.data_ptr(), indices, last, _ptr(exact_k), _ptr(exact_v),
+                   tail_indices, tail_last, _ptr(value_center), hkv * DIM, out.data_ptr(), _ptr(lse),
+                   float(self._sm_scale if sm_scale is None else sm_scale),
+                   self.workspace.data_ptr(), _capi.current_stream())
+        return (out, lse) if return_lse else out
