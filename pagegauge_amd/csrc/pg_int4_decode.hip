@@ -17,9 +17,8 @@
 //    n < 8 hand over the FP16 part of a probability and columns n >= 8 (the same
 //    heads again) its remainder, so rows r and r + 8 of the product add up to
 //    one of about 22 bits.
-//  * Codes become FP16 exactly: a nibble u under the exponent of 1024 is
-//    1024 + u, minus 1032.  K and V are used as small integers; the scales
-//    multiply scores and probabilities in float32.
+//  * Codes become FP16 exactly, 9 operations for 8 of them.  K and V are used as
+//    small integers; the scales multiply scores and probabilities in float32.
 //
 // Probabilities times V's scales are carried relative to a power of two that
 // puts the largest of the wave's scales near 2^14, so that FP16's range holds
@@ -67,29 +66,66 @@ struct Int4Args {
 
 __device__ __forceinline__ v2h as_half2(uint32_t bits) { return __builtin_bit_cast(v2h, bits); }
 
-// The codes of nibbles i and i + 4 as FP16.
-__device__ __forceinline__ v2h codes2(uint32_t word, int i) {
-  const uint32_t bits = (word >> (4 * i) & 0x000f000fu) | 0x64006400u;
-  return as_half2(bits) - v2h{static_cast<_Float16>(1032.0f), static_cast<_Float16>(1032.0f)};
+__device__ __forceinline__ v2h splat(float x) {
+  return v2h{static_cast<_Float16>(x), static_cast<_Float16>(x)};
 }
+
+// Codes of a dword as FP16, two at a time.  The masks and the exponent sit in
+// registers, out of the compiler's sight: it would otherwise write each
+// and-or as two operations with a literal each.
+struct Unpack {
+  uint32_t low, high, magic;
+
+  __device__ __forceinline__ Unpack() {
+    asm("s_mov_b32 %0, 0x000f000f" : "=s"(low));
+    asm("s_mov_b32 %0, 0x00f000f0" : "=s"(high));
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(magic));
+  }
+  // nibbles 0 and 4: u under the exponent of 1024 is 1024 + u, minus 1032
+  __device__ __forceinline__ v2h even(uint32_t word) const {
+    return as_half2((word & low) | magic) - splat(1032.0f);
+  }
+  // nibbles 1 and 5: 1024 + 16 u, times 1/16 minus 72 (one exact fused
+  // operation, which spares the shift)
+  __device__ __forceinline__ v2h odd(uint32_t word) const {
+    return __builtin_elementwise_fma(as_half2((word & high) | magic), splat(0.0625f), splat(-72.0f));
+  }
+};
 
 __device__ __forceinline__ v8h join(v2h a, v2h b, v2h c, v2h d) {
   return v8h{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-// Running state of one wave.  Lane (kg, n): m, l of head n % 8 (l over its own
-// tokens), acc[nb][r] = row 4 kg + r of the product, channel 8 n + nb.
+// x times one half of ``pair``: one mixed-precision operation, no conversion.
+__device__ __forceinline__ float times_half(float x, uint32_t pair, int which) {
+  return fmaf(x, static_cast<float>(as_half2(pair)[which]), 0.0f);
+}
+
+// Running state of one wave.  Lane (kg, n): m is the largest score of head n % 8
+// before the softmax scale, l the sum of the lane's own tokens' probabilities,
+// acc[nb][r] row 4 kg + r of the product, channel 8 n + nb; l and acc are held
+// times 2^exponent.
 struct State {
-  float m, l;
+  float m, l, exponent;
   v4f acc[8];
 };
 
-// Softmax step over kPages pages: s are the lane's scores (already scaled),
-// w the weights of V (v_scale: V's scale of each, times 2^e), masked scores -inf.
-template <int kPages>
+// Brings l and acc to another exponent.
+__device__ __forceinline__ void set_exponent(State& st, int exponent) {
+  const float change = __builtin_amdgcn_exp2f(static_cast<float>(exponent) - st.exponent);
+  st.exponent = static_cast<float>(exponent);
+  st.l *= change;
+#pragma unroll
+  for (int nb = 0; nb < 8; ++nb) st.acc[nb] *= change;
+}
+
+// Softmax step over kPages pages: s are the lane's scores, masked ones -inf,
+// v_scale pairs of V's scales (FP16; 0 where masked), ``scale`` the softmax scale
+// in base 2.  p: the lane's rows of the A operand of P V.
+template <int kPages, bool kScaled>
 __device__ __forceinline__ void softmax_step(State& st, const float (&s)[kPages][4],
-                                             const float (&v_scale)[kPages][4], float low_part,
-                                             int lane, v8h (&p)[kPages / 2]) {
+                                             const uint32_t (&v_scale)[kPages][2], float scale,
+                                             float low_part, int lane, v8h (&p)[kPages / 2]) {
   float top = kNegInf;
 #pragma unroll
   for (int i = 0; i < kPages; ++i)
@@ -99,9 +135,10 @@ __device__ __forceinline__ void softmax_step(State& st, const float (&s)[kPages]
   top = fmaxf(top, __shfl_xor(top, 32, kWave));
   const float m = fmaxf(st.m, top);
   const float base = m == kNegInf ? 0.0f : m;    // nothing visible yet: every p is 0
-  const float alpha = __builtin_amdgcn_exp2f(st.m - base);
+  const float alpha = __builtin_amdgcn_exp2f((st.m - base) * scale);
   if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
     const int kg = lane >> 4;
+    st.l *= alpha;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float f = __shfl(alpha, (4 * kg + r) & 7, kWave);
@@ -109,26 +146,39 @@ __device__ __forceinline__ void softmax_step(State& st, const float (&s)[kPages]
       for (int nb = 0; nb < 8; ++nb) st.acc[nb][r] *= f;
     }
   }
-  float sum = 0.0f;
-#pragma unroll
-  for (int j = 0; j < kPages / 2; ++j)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = __builtin_amdgcn_exp2f(s[2 * j + (e >> 2)][e & 3] - base);
-      sum += x;
-      // a masked token's scale may be anything
-      const float w = x == 0.0f ? 0.0f : x * v_scale[2 * j + (e >> 2)][e & 3];
-      const _Float16 high = static_cast<_Float16>(w);
-      p[j][e] = static_cast<_Float16>(w - low_part * static_cast<float>(high));
-    }
-  st.l = st.l * alpha + sum;
   st.m = m;
+  const float offset = fmaf(-base, scale, st.exponent);
+#pragma unroll
+  for (int j = 0; j < kPages / 2; ++j) {
+    uint32_t words[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const int page = 2 * j + (h >> 1), r = 2 * (h & 1);
+      const float x0 = __builtin_amdgcn_exp2f(fmaf(s[page][r], scale, offset));
+      const float x1 = __builtin_amdgcn_exp2f(fmaf(s[page][r + 1], scale, offset));
+      st.l += x0 + x1;
+      const float w0 = kScaled ? times_half(x0, v_scale[page][h & 1], 0) : x0;
+      const float w1 = kScaled ? times_half(x1, v_scale[page][h & 1], 1) : x1;
+      // the FP16 part, or what it leaves (rounding down costs the second 2^-21)
+      const v2h high = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(w0, w1));
+      words[h] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(
+          fmaf(-low_part, static_cast<float>(high.x), w0), fmaf(-low_part, static_cast<float>(high.y), w1)));
+    }
+    p[j] = __builtin_bit_cast(v8h, v4u{words[0], words[1], words[2], words[3]});
+  }
 }
 
-// MFMA operand A of K rows or V columns in FP16, for pages of the tail.
+// The low or the high halves of two words, side by side.
 __device__ __forceinline__ uint32_t pick(uint32_t a, uint32_t b, bool high) {
-  // the low or the high halves of two words, side by side
   return high ? __builtin_amdgcn_perm(b, a, 0x07060302u) : __builtin_amdgcn_perm(b, a, 0x05040100u);
+}
+
+// Pins ``x`` here: the wait for its load is placed at this point, not earlier.
+template <typename T>
+__device__ __forceinline__ void consume_point(T& x) {
+  T value = x;
+  asm volatile("" : "+v"(value));
+  x = value;
 }
 
 struct Group {
@@ -149,25 +199,29 @@ __global__ __launch_bounds__(kThreads) void int4_decode_kernel(Int4Args a) {
   const int hkv = a.num_kv_heads;
 
   // query: B operand, column n = head n % 8, dims 32 w + 8 kg ..
+  const bool has_query = (n & 7) < heads;
   v8h q[4];
   {
-    const bool in = (n & 7) < heads;
     const uint16_t* row = a.query + it.request * a.query_batch_stride +
-                          static_cast<int64_t>(kv * a.group + first_head + (in ? n & 7 : 0)) * kHeadDim;
+                          static_cast<int64_t>(kv * a.group + first_head + (has_query ? n & 7 : 0)) * kHeadDim;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) q[w] = *reinterpret_cast<const v8h*>(row + 32 * w + 8 * kg);
+  }
+  auto take_query = [&]() {        // once the first pages are on their way
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      q[w] = *reinterpret_cast<const v8h*>(row + 32 * w + 8 * kg);
-      if (!in) q[w] = v8h{0, 0, 0, 0, 0, 0, 0, 0};
+      consume_point(q[w]);
+      if (!has_query) q[w] = v8h{0, 0, 0, 0, 0, 0, 0, 0};
     }
-  }
+  };
   const float low_part = n < 8 ? 0.0f : 1.0f;
 
   State st;
   st.m = kNegInf;
   st.l = 0.0f;
+  st.exponent = 0.0f;
 #pragma unroll
   for (int nb = 0; nb < 8; ++nb) st.acc[nb] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  int scale_exp = 0;               // st.acc is held times 2^scale_exp
 
   // ---- history: groups wave, wave + 8, ... of the item's pages
   const int count = it.page_end - it.page_begin;
@@ -177,12 +231,14 @@ __global__ __launch_bounds__(kThreads) void int4_decode_kernel(Int4Args a) {
     // lane l: slot l of the wave, page 4 (8 (l / 4) + wave) + l % 4 of the item
     const int slot_page = kInt4GroupPages * (kInt4Waves * (lane / kInt4GroupPages) + wave) +
                           lane % kInt4GroupPages;
-    const bool held = slot_page < count;
     const int my_page = a.indices[it.page_begin + min(slot_page, count - 1)];
     const int last_len = min(a.last_page_len[it.request], kPageSize);
     auto visible = [&](int page) {     // tokens of the item's page ``page``
       return page >= count ? 0 : it.page_begin + page == it.last_page ? last_len : kPageSize;
     };
+    const int whole = visible(count - 1) == kPageSize ? count : count - 1;   // leading whole pages
+    const uint32_t lane_bytes = 16 * lane, lane_scales = 16 * kg;
+    const Unpack unpack;
     Group buf[2];
     auto issue = [&](int g, Group& dst) {
 #pragma unroll
@@ -190,65 +246,82 @@ __global__ __launch_bounds__(kThreads) void int4_decode_kernel(Int4Args a) {
         const int page = __builtin_amdgcn_readlane(my_page, g * kInt4GroupPages + i);
         const int64_t block = static_cast<int64_t>(page) * hkv + kv;
         const uint8_t* codes = a.codes + block * kInt4BlockBytes;
-        dst.k[i] = *reinterpret_cast<const v4u*>(codes + 16 * lane);
-        dst.v[i] = *reinterpret_cast<const v4u*>(codes + kInt4PartBytes + 16 * lane);
-        dst.s[i] = *reinterpret_cast<const v4u*>(a.scales + block * kInt4BlockScales + 8 * kg);
+        const uint8_t* scales = reinterpret_cast<const uint8_t*>(a.scales + block * kInt4BlockScales);
+        dst.k[i] = *reinterpret_cast<const v4u*>(codes + lane_bytes);
+        dst.v[i] = *reinterpret_cast<const v4u*>(codes + kInt4PartBytes + lane_bytes);
+        dst.s[i] = *reinterpret_cast<const v4u*>(scales + lane_scales);
       }
     };
     issue(0, buf[0]);
     // the largest visible V scale of the wave's pages fixes the power of two
-    float top = 0.0f;
     {
       const uint16_t* scales = a.scales + (static_cast<int64_t>(my_page) * hkv + kv) * kInt4BlockScales;
-      const int limit = held ? visible(slot_page) : 0;
+      const int limit = visible(slot_page);
       v2u raw[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) raw[g] = *reinterpret_cast<const v2u*>(scales + 8 * g + 4);
+      take_query();
+      float top = 0.0f;
 #pragma unroll
-      for (int t = 0; t < kPageSize; ++t) {
-        const float s = half_bits_to_float(static_cast<uint16_t>(raw[t >> 2][(t & 3) >> 1] >> (16 * (t & 1))));
-        top = fmaxf(top, t < limit ? s : 0.0f);
-      }
+      for (int t = 0; t < kPageSize; ++t)
+        top = fmaxf(top, t < limit ? static_cast<float>(as_half2(raw[t >> 2][(t & 3) >> 1])[t & 1]) : 0.0f);
       top = wave_max(top);
+      int e = 0;
+      if (top > 0.0f) frexpf(top, &e);
+      st.exponent = static_cast<float>(14 - e);
     }
-    int e = 0;
-    if (top > 0.0f) frexpf(top, &e);
-    scale_exp = 14 - e;
-    const float unit = ldexpf(1.0f, scale_exp);
 
-    auto compute = [&](int g, const Group& cur) {
-      float s[kInt4GroupPages][4], v_scale[kInt4GroupPages][4];
+    auto compute = [&](int g, Group& cur) {
+      const int first = kInt4GroupPages * (kInt4Waves * g + wave);
+      float s[kInt4GroupPages][4];
 #pragma unroll
       for (int i = 0; i < kInt4GroupPages; ++i) {
+        consume_point(cur.k[i]);
+        consume_point(cur.s[i]);
         v4f dot = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const uint32_t x = cur.k[i][w];
+          const uint32_t x = cur.k[i][w], y = x >> 8;
           dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              join(codes2(x, 0), codes2(x, 1), codes2(x, 2), codes2(x, 3)), q[w], dot, 0, 0, 0);
+              join(unpack.even(x), unpack.odd(x), unpack.even(y), unpack.odd(y)), q[w], dot, 0, 0, 0);
         }
-        const int limit = visible(kInt4GroupPages * (kInt4Waves * g + wave) + i);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float ks = half_bits_to_float(static_cast<uint16_t>(cur.s[i][r >> 1] >> (16 * (r & 1))));
-          const float vs = half_bits_to_float(static_cast<uint16_t>(cur.s[i][2 + (r >> 1)] >> (16 * (r & 1))));
-          s[i][r] = 4 * kg + r < limit ? dot[r] * (ks * a.sm_scale_log2) : kNegInf;
-          v_scale[i][r] = vs * unit;
+        for (int r = 0; r < 4; ++r) s[i][r] = times_half(dot[r], cur.s[i][r >> 1], r & 1);
+      }
+      uint32_t v_scale[kInt4GroupPages][2];
+#pragma unroll
+      for (int i = 0; i < kInt4GroupPages; ++i) {
+        v_scale[i][0] = cur.s[i][2];
+        v_scale[i][1] = cur.s[i][3];
+      }
+      if (first + kInt4GroupPages > whole) {     // a partial or a missing page
+#pragma unroll
+        for (int i = 0; i < kInt4GroupPages; ++i) {
+          const int limit = visible(first + i) - 4 * kg;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            s[i][r] = r < limit ? s[i][r] : kNegInf;
+            v_scale[i][r >> 1] &= r < limit ? ~0u : r & 1 ? 0x0000ffffu : 0xffff0000u;
+          }
         }
       }
       v8h p[kInt4GroupPages / 2];
-      softmax_step<kInt4GroupPages>(st, s, v_scale, low_part, lane, p);
+      softmax_step<kInt4GroupPages, true>(st, s, v_scale, a.sm_scale_log2, low_part, lane, p);
+#pragma unroll
+      for (int i = 0; i < kInt4GroupPages; ++i) consume_point(cur.v[i]);
 #pragma unroll
       for (int j = 0; j < kInt4GroupPages / 2; ++j)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const uint32_t x = cur.v[2 * j][w], y = cur.v[2 * j + 1][w];
           st.acc[2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              p[j], join(codes2(x, 0), codes2(x, 1), codes2(y, 0), codes2(y, 1)), st.acc[2 * w], 0, 0, 0);
+              p[j], join(unpack.even(x), unpack.odd(x), unpack.even(y), unpack.odd(y)), st.acc[2 * w], 0, 0, 0);
           st.acc[2 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              p[j], join(codes2(x, 2), codes2(x, 3), codes2(y, 2), codes2(y, 3)), st.acc[2 * w + 1], 0, 0, 0);
+              p[j], join(unpack.even(x >> 8), unpack.odd(x >> 8), unpack.even(y >> 8), unpack.odd(y >> 8)),
+              st.acc[2 * w + 1], 0, 0, 0);
         }
     };
+    // the loads of group g + 1 are in flight while group g is computed
     int g = 0;
     for (; g + 2 < groups; g += 2) {
       issue(g + 1, buf[1]);
@@ -263,26 +336,25 @@ __global__ __launch_bounds__(kThreads) void int4_decode_kernel(Int4Args a) {
     } else {
       compute(g, buf[0]);
     }
+  } else {
+    take_query();
   }
 
   // ---- exact tail: pairs wave, wave + 8, ... of the item's tail pages
   const int tail_count = it.tail_end - it.tail_begin;
   if (2 * wave < tail_count) {
-    const float change = ldexpf(1.0f, 14 - scale_exp);     // p alone is at most 1
-#pragma unroll
-    for (int nb = 0; nb < 8; ++nb) st.acc[nb] *= change;
-    scale_exp = 14;
+    set_exponent(st, 14);          // probabilities alone are at most 1
     const int64_t row_stride = static_cast<int64_t>(hkv) * kHeadDim;
     const int last_len = min(a.tail_last_len[it.request], kPageSize);
     for (int page = 2 * wave; page < tail_count; page += 2 * kInt4Waves) {
-      float s[2][4], ones[2][4];
+      float s[2][4];
       v4u k[2][4], v[2][4];
       int limit[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int at = it.tail_begin + min(page + i, tail_count - 1);
         const int64_t base = static_cast<int64_t>(a.tail_indices[at]) * kPageSize * row_stride + kv * kHeadDim;
-        limit[i] = page + i >= tail_count ? 0 : at == it.last_tail ? last_len : kPageSize;
+        limit[i] = (page + i >= tail_count ? 0 : at == it.last_tail ? last_len : kPageSize) - 4 * kg;
 #pragma unroll
         for (int w = 0; w < 4; ++w)
           k[i][w] = *reinterpret_cast<const v4u*>(a.tail_k + base + n * row_stride + 32 * w + 8 * kg);
@@ -298,14 +370,14 @@ __global__ __launch_bounds__(kThreads) void int4_decode_kernel(Int4Args a) {
           dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, k[i][w]), q[w], dot, 0, 0, 0);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          s[i][r] = 4 * kg + r < limit[i] ? dot[r] * a.sm_scale_log2 : kNegInf;
-          ones[i][r] = 0x1p14f;
+          s[i][r] = r < limit[i] ? dot[r] : kNegInf;
           // a row not yet written may hold anything: 0 times it must be 0
-          if (4 * kg + r >= limit[i]) v[i][r] = v4u{0u, 0u, 0u, 0u};
+          if (r >= limit[i]) v[i][r] = v4u{0u, 0u, 0u, 0u};
         }
       }
       v8h p[1];
-      softmax_step<2>(st, s, ones, low_part, lane, p);
+      const uint32_t unscaled[2][2] = {};
+      softmax_step<2, false>(st, s, unscaled, a.sm_scale_log2, low_part, lane, p);
 #pragma unroll
       for (int nb = 0; nb < 8; ++nb) {
         v4u cols;
@@ -322,11 +394,11 @@ __global__ __launch_bounds__(kThreads) void int4_decode_kernel(Int4Args a) {
   // ---- the waves meet: rows r and r + 8 of the product, then 8 partial states
   st.l += __shfl_xor(st.l, 16, kWave);
   st.l += __shfl_xor(st.l, 32, kWave);
+  const float scale = __builtin_amdgcn_exp2f(-st.exponent);
   if (kg == 0 && n < kHeads) {
-    part_m[wave][n] = st.m;
-    part_l[wave][n] = st.l;
+    part_m[wave][n] = st.m * a.sm_scale_log2;
+    part_l[wave][n] = st.l * scale;
   }
-  const float scale = ldexpf(1.0f, -scale_exp);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     float o[8];

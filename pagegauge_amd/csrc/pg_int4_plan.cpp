@@ -45,12 +45,12 @@ int32_t build_int4_plan(const int32_t* host_indptr, const int32_t* host_tail_ind
     exact_pages += r.tail;
   }
   // The largest share of a workgroup (``cap``, in weighted pages) for which
-  // the batch fills about two workgroups per CU, but at least one group of
+  // the batch fills about one workgroup per CU, but at least one group of
   // pages per wave, and at most the pages that an item can hold.
   const int64_t groups = static_cast<int64_t>(num_kv_heads) *
                          ceil_div(num_qo_heads / num_kv_heads, kInt4HeadsPerWave);
   const int64_t cus = num_cus > 0 ? num_cus : 256;
-  const int64_t target = std::max<int64_t>(batch_size, 2 * cus / groups);
+  const int64_t target = std::max<int64_t>(batch_size, cus / groups);
   int64_t low = kInt4Waves * kInt4GroupPages;
   int64_t high = std::min<int64_t>(std::max(low, total), kInt4MaxItemPages);
   auto count = [&](int64_t cap) {
