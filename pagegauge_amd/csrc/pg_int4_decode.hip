@@ -185,7 +185,7 @@ struct Group {
   v4u k[kInt4GroupPages], v[kInt4GroupPages], s[kInt4GroupPages];
 };
 
-__global__ __launch_bounds__(kThreads) void int4_decode_kernel(Int4Args a) {
+__global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
   __shared__ float part_o[kInt4Waves][kHeads][kHeadDim];
   __shared__ float part_m[kInt4Waves][kHeads];
   __shared__ float part_l[kInt4Waves][kHeads];
@@ -297,7 +297,8 @@ __global__ __launch_bounds__(kThreads) void int4_decode_kernel(Int4Args a) {
       if (first + kInt4GroupPages > whole) {     // a partial or a missing page
 #pragma unroll
         for (int i = 0; i < kInt4GroupPages; ++i) {
-          const int limit = visible(first + i) - 4 * kg;
+          int limit = visible(first + i) - 4 * kg;
+          consume_point(limit);     // keeps this a branch: whole groups skip the selects
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             s[i][r] = r < limit ? s[i][r] : kNegInf;
@@ -411,22 +412,23 @@ __global__ __launch_bounds__(kThreads) void int4_decode_kernel(Int4Args a) {
     }
   }
   __syncthreads();
-  if (wave >= heads) return;       // wave h finishes head h, two dims per lane
+  // wave w finishes heads w, w + 4, two dims per lane
+  for (int h = wave; h < heads; h += kInt4Waves) {
   float m = kNegInf;
 #pragma unroll
-  for (int w = 0; w < kInt4Waves; ++w) m = fmaxf(m, part_m[w][wave]);
+  for (int w = 0; w < kInt4Waves; ++w) m = fmaxf(m, part_m[w][h]);
   const float base = m == kNegInf ? 0.0f : m;
   float l = 0.0f;
   float2 o = make_float2(0.0f, 0.0f);
 #pragma unroll
   for (int w = 0; w < kInt4Waves; ++w) {
-    const float f = __builtin_amdgcn_exp2f(part_m[w][wave] - base);
-    const float2 x = *reinterpret_cast<const float2*>(&part_o[w][wave][2 * lane]);
-    l += f * part_l[w][wave];
+    const float f = __builtin_amdgcn_exp2f(part_m[w][h] - base);
+    const float2 x = *reinterpret_cast<const float2*>(&part_o[w][h][2 * lane]);
+    l += f * part_l[w][h];
     o.x += f * x.x;
     o.y += f * x.y;
   }
-  const int head = kv * a.group + first_head + wave;
+  const int head = kv * a.group + first_head + h;
   if (it.items_in_request > 1) {
     const int64_t row = static_cast<int64_t>(blockIdx.x) * a.num_qo_heads + head;
     *reinterpret_cast<float2*>(a.partial_o + row * kHeadDim + 2 * lane) = o;
@@ -434,7 +436,7 @@ __global__ __launch_bounds__(kThreads) void int4_decode_kernel(Int4Args a) {
       a.partial_m[row] = m;
       a.partial_l[row] = l;
     }
-    return;
+    continue;
   }
   const int64_t row = static_cast<int64_t>(it.request) * a.num_qo_heads + head;
   float2 c = make_float2(0.0f, 0.0f);
@@ -448,6 +450,7 @@ __global__ __launch_bounds__(kThreads) void int4_decode_kernel(Int4Args a) {
   *reinterpret_cast<__half2*>(a.out + row * kHeadDim + 2 * lane) =
       __floats2half2_rn(o.x * inv + c.x, o.y * inv + c.y);
   if (lane == 0 && a.lse) a.lse[row] = l == 0.0f ? kNegInf : log2f(l) + m;
+  }
 }
 
 struct Int4CombineArgs {
@@ -460,61 +463,99 @@ struct Int4CombineArgs {
   uint16_t* out;
   float* lse;
   int num_qo_heads, group;
+  int single;                      // one request: its items (item_ptr is not read)
 };
 
-// Joins the partial states of one (request, query head): 4 waves take its
-// items in turn, two dims per lane.
-__global__ __launch_bounds__(4 * kWave) void int4_combine_kernel(Int4CombineArgs a) {
-  __shared__ float part_o[4][kHeadDim];
-  __shared__ float part_m[4], part_l[4];
+// Joins the partial states of one (request, query head), 64 dims a workgroup:
+// thread (row, column) = (tid / 16, tid % 16) takes items row, row + 16, ... of
+// four dims.  The first 64 items are requested together, so a join of that many
+// is one trip to memory after the item range.
+constexpr int kCombineThreads = 256;
+constexpr int kCombineRows = kCombineThreads / 16;
+constexpr int kCombineInFlight = 4;
+
+__global__ __launch_bounds__(kCombineThreads) void int4_combine_kernel(Int4CombineArgs a) {
+  constexpr int kWaves = kCombineThreads / kWave;
+  __shared__ float part_o[kWaves][64];
+  __shared__ float part_m[kWaves], part_l[kWaves];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int row = threadIdx.x / 16, dim = 64 * blockIdx.z + 4 * (threadIdx.x % 16);
   const int request = blockIdx.x, head = blockIdx.y;
-  const int begin = a.item_ptr[request], end = a.item_ptr[request + 1];
+  const int begin = a.single ? 0 : a.item_ptr[request];
+  const int end = a.single ? a.single : a.item_ptr[request + 1];
   if (end - begin <= 1) return;    // its only workgroup wrote the output
   float m = kNegInf, l = 0.0f;
-  float2 o = make_float2(0.0f, 0.0f);
-  for (int i = begin + wave; i < end; i += 4) {
-    const int64_t row = static_cast<int64_t>(i) * a.num_qo_heads + head;
-    const float mi = a.partial_m[row];
-    const float2 x = *reinterpret_cast<const float2*>(a.partial_o + row * kHeadDim + 2 * lane);
-    const float top = fmaxf(m, mi), base = top == kNegInf ? 0.0f : top;
-    const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(mi - base);
-    l = l * f + a.partial_l[row] * g;
-    o.x = o.x * f + x.x * g;
-    o.y = o.y * f + x.y * g;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int first = begin + row; first < end; first += kCombineRows * kCombineInFlight) {
+    float mi[kCombineInFlight], li[kCombineInFlight];
+    float4 x[kCombineInFlight];
+#pragma unroll
+    for (int k = 0; k < kCombineInFlight; ++k) {
+      const int item = first + k * kCombineRows;
+      const int64_t at = static_cast<int64_t>(min(item, end - 1)) * a.num_qo_heads + head;
+      mi[k] = a.partial_m[at];
+      li[k] = a.partial_l[at];
+      x[k] = *reinterpret_cast<const float4*>(a.partial_o + at * kHeadDim + dim);
+    }
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < kCombineInFlight; ++k) {
+      if (first + k * kCombineRows >= end) mi[k] = kNegInf;
+      top = fmaxf(top, mi[k]);
+    }
+    const float base = top == kNegInf ? 0.0f : top;
+    const float f = __builtin_amdgcn_exp2f(m - base);
+    l *= f;
+    o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+#pragma unroll
+    for (int k = 0; k < kCombineInFlight; ++k) {
+      if (first + k * kCombineRows >= end) break;
+      const float g = __builtin_amdgcn_exp2f(mi[k] - base);
+      l = fmaf(g, li[k], l);
+      o.x = fmaf(g, x[k].x, o.x);
+      o.y = fmaf(g, x[k].y, o.y);
+      o.z = fmaf(g, x[k].z, o.z);
+      o.w = fmaf(g, x[k].w, o.w);
+    }
     m = top;
   }
-  *reinterpret_cast<float2*>(&part_o[wave][2 * lane]) = o;
+  // the wave's four rows, then the waves
+  float top = fmaxf(m, __shfl_xor(m, 16, kWave));
+  top = fmaxf(top, __shfl_xor(top, 32, kWave));
+  const float base = top == kNegInf ? 0.0f : top;
+  const float f = __builtin_amdgcn_exp2f(m - base);
+  float sums[5] = {l * f, o.x * f, o.y * f, o.z * f, o.w * f};
+#pragma unroll
+  for (float& x : sums) {
+    x += __shfl_xor(x, 16, kWave);
+    x += __shfl_xor(x, 32, kWave);
+  }
+  if (lane < 16)
+    *reinterpret_cast<float4*>(&part_o[wave][4 * lane]) = make_float4(sums[1], sums[2], sums[3], sums[4]);
   if (lane == 0) {
-    part_m[wave] = m;
-    part_l[wave] = l;
+    part_m[wave] = top;
+    part_l[wave] = sums[0];
   }
   __syncthreads();
   if (wave != 0) return;
-  m = fmaxf(fmaxf(part_m[0], part_m[1]), fmaxf(part_m[2], part_m[3]));
-  const float base = m == kNegInf ? 0.0f : m;
-  l = 0.0f;
-  o = make_float2(0.0f, 0.0f);
+  float all = kNegInf;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float f = __builtin_amdgcn_exp2f(part_m[w] - base);
-    const float2 x = *reinterpret_cast<const float2*>(&part_o[w][2 * lane]);
-    l += f * part_l[w];
-    o.x += f * x.x;
-    o.y += f * x.y;
+  for (int w = 0; w < kWaves; ++w) all = fmaxf(all, part_m[w]);
+  const float all_base = all == kNegInf ? 0.0f : all;
+  float sum = 0.0f, out = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float g = __builtin_amdgcn_exp2f(part_m[w] - all_base);
+    sum = fmaf(g, part_l[w], sum);
+    out = fmaf(g, part_o[w][lane], out);
   }
-  const int64_t row = static_cast<int64_t>(request) * a.num_qo_heads + head;
-  float2 c = make_float2(0.0f, 0.0f);
-  if (a.value_center) {
-    const uint32_t bits = *reinterpret_cast<const uint32_t*>(
-        a.value_center + request * a.center_batch_stride + (head / a.group) * kHeadDim + 2 * lane);
-    c = make_float2(half_bits_to_float(static_cast<uint16_t>(bits)),
-                    half_bits_to_float(static_cast<uint16_t>(bits >> 16)));
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  *reinterpret_cast<__half2*>(a.out + row * kHeadDim + 2 * lane) =
-      __floats2half2_rn(o.x * inv + c.x, o.y * inv + c.y);
-  if (lane == 0 && a.lse) a.lse[row] = l == 0.0f ? kNegInf : log2f(l) + m;
+  const int64_t at = static_cast<int64_t>(request) * a.num_qo_heads + head;
+  const int d = 64 * blockIdx.z + lane;
+  const float center = a.value_center ? half_bits_to_float(a.value_center[
+      request * a.center_batch_stride + (head / a.group) * kHeadDim + d]) : 0.0f;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  a.out[at * kHeadDim + d] = __half_as_ushort(__float2half_rn(out * inv + center));
+  if (d == 0 && a.lse) a.lse[at] = sum == 0.0f ? kNegInf : log2f(sum) + all;
 }
 
 }  // namespace
@@ -612,7 +653,8 @@ extern "C" int32_t pg_int4_decode_run(const pg_int4_plan_t* plan, const void* qu
   c.lse = lse;
   c.num_qo_heads = plan->num_qo_heads;
   c.group = a.group;
-  hipLaunchKernelGGL(int4_combine_kernel, dim3(plan->batch_size, plan->num_qo_heads),
-                     dim3(4 * kWave), 0, as_stream(stream), c);
+  c.single = plan->batch_size == 1 ? plan->num_items : 0;
+  hipLaunchKernelGGL(int4_combine_kernel, dim3(plan->batch_size, plan->num_qo_heads, kHeadDim / 64),
+                     dim3(kCombineThreads), 0, as_stream(stream), c);
   return check_launch("int4_combine");
 }

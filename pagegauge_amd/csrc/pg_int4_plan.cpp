@@ -16,7 +16,11 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct Request {
   int64_t pages, tail;
   int64_t weight() const { return pages + kInt4TailWeight * tail; }
-  int64_t cuts(int64_t cap) const { return std::max<int64_t>(1, ceil_div(weight(), cap)); }
+  // Cuts of at most ``cap``; no item may get more pages than its waves can hold.
+  int64_t cuts(int64_t cap) const {
+    if (pages > kInt4MaxItemPages) cap = std::min<int64_t>(cap, kInt4MaxItemPages);
+    return std::max<int64_t>(1, ceil_div(weight(), cap));
+  }
 };
 
 }  // namespace
@@ -46,13 +50,13 @@ int32_t build_int4_plan(const int32_t* host_indptr, const int32_t* host_tail_ind
   }
   // The largest share of a workgroup (``cap``, in weighted pages) for which
   // the batch fills about one workgroup per CU, but at least one group of
-  // pages per wave, and at most the pages that an item can hold.
+  // pages per wave.
   const int64_t groups = static_cast<int64_t>(num_kv_heads) *
                          ceil_div(num_qo_heads / num_kv_heads, kInt4HeadsPerWave);
   const int64_t cus = num_cus > 0 ? num_cus : 256;
-  const int64_t target = std::max<int64_t>(batch_size, cus / groups);
+  const int64_t target = std::max<int64_t>(batch_size, kInt4TargetPerCu * cus / groups);
   int64_t low = kInt4Waves * kInt4GroupPages;
-  int64_t high = std::min<int64_t>(std::max(low, total), kInt4MaxItemPages);
+  int64_t high = std::max(low, total);
   auto count = [&](int64_t cap) {
     int64_t n = 0;
     for (const Request& r : requests) n += r.cuts(cap);
