@@ -17,12 +17,18 @@
 //    n < 8 hand over the FP16 part of a probability and columns n >= 8 (the same
 //    heads again) its remainder, so rows r and r + 8 of the product add up to
 //    one of about 22 bits.
-//  * Codes become FP16 exactly, 9 operations for 8 of them.  K and V are used as
-//    small integers; the scales multiply scores and probabilities in float32.
+//  * A nibble u = code + 8 masked out of its dword is the FP16 subnormal
+//    u * 2^-24, or 16 u * 2^-24 one nibble further up, and MFMAs multiply
+//    subnormals exactly: 5 operations make 8 operands.  The offset of 8 comes off
+//    the products: of K as the accumulators' start, -8 sum(q), of V as one more
+//    column of the product, against 8s.  The scales multiply scores and
+//    probabilities in float32.
+//  * The softmax's base follows the running maximum lazily: it moves when a
+//    score passes it by 2^4, so most groups of pages need no exchange at all.
 //
 // Probabilities times V's scales are carried relative to a power of two that
-// puts the largest of the wave's scales near 2^14, so that FP16's range holds
-// them (a weight 2^-28 of the largest is still a normal number).
+// puts the largest of the wave's scales near 2^10 (2^14 with the base's slack), so
+// that two FP16 parts hold them to 2^-34 of the largest.
 #include "pg_int4.h"
 #include "pg_int4_plan.h"
 
@@ -70,101 +76,92 @@ __device__ __forceinline__ v2h splat(float x) {
   return v2h{static_cast<_Float16>(x), static_cast<_Float16>(x)};
 }
 
-// Codes of a dword as FP16, two at a time.  The masks and the exponent sit in
-// registers, out of the compiler's sight: it would otherwise write each
-// and-or as two operations with a literal each.
-struct Unpack {
-  uint32_t low, high, magic;
-
-  __device__ __forceinline__ Unpack() {
-    asm("s_mov_b32 %0, 0x000f000f" : "=s"(low));
-    asm("s_mov_b32 %0, 0x00f000f0" : "=s"(high));
-    asm("v_mov_b32 %0, 0x64006400" : "=v"(magic));
-  }
-  // nibbles 0 and 4: u under the exponent of 1024 is 1024 + u, minus 1032
-  __device__ __forceinline__ v2h even(uint32_t word) const {
-    return as_half2((word & low) | magic) - splat(1032.0f);
-  }
-  // nibbles 1 and 5: 1024 + 16 u, times 1/16 minus 72 (one exact fused
-  // operation, which spares the shift)
-  __device__ __forceinline__ v2h odd(uint32_t word) const {
-    return __builtin_elementwise_fma(as_half2((word & high) | magic), splat(0.0625f), splat(-72.0f));
-  }
-};
-
-__device__ __forceinline__ v8h join(v2h a, v2h b, v2h c, v2h d) {
-  return v8h{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+__device__ __forceinline__ v8h operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(v8h, v4u{a, b, c, d});
 }
+
+// Nibbles 0 and 4 of a dword as FP16 u * 2^-24, and 1 and 5 as 16 u * 2^-24.
+__device__ __forceinline__ uint32_t even(uint32_t word) { return word & 0x000f000fu; }
+__device__ __forceinline__ uint32_t odd(uint32_t word) { return word & 0x00f000f0u; }
+constexpr uint32_t kEvenEights = 0x00080008u, kOddEights = 0x00800080u;     // u = 8
 
 // x times one half of ``pair``: one mixed-precision operation, no conversion.
 __device__ __forceinline__ float times_half(float x, uint32_t pair, int which) {
   return fmaf(x, static_cast<float>(as_half2(pair)[which]), 0.0f);
 }
 
-// Running state of one wave.  Lane (kg, n): m is the largest score of head n % 8
-// before the softmax scale, l the sum of the lane's own tokens' probabilities,
-// acc[nb][r] row 4 kg + r of the product, channel 8 n + nb; l and acc are held
-// times 2^exponent.
+constexpr float kSlack = 4.0f;     // how far (base 2) a score may pass the base
+
+// Running state of one wave.  Lane (kg, n) has head n % 8's: base (before the
+// softmax scale), limit past which it moves, and offset, the exponent of the sums
+// minus the scaled base; l0 and l1 sum the lane's own tokens 4 kg, 4 kg + 1 and, in
+// sixteenths, 4 kg + 2, 4 kg + 3.  acc[nb][r] is row 4 kg + r of the product,
+// channel 8 n + nb, and eights[r] that row's sum of weights times 8.
 struct State {
-  float m, l, exponent;
-  v4f acc[8];
+  float base, limit, offset;
+  float l0, l1;
+  v4f acc[8], eights;
 };
 
-// Brings l and acc to another exponent.
-__device__ __forceinline__ void set_exponent(State& st, int exponent) {
-  const float change = __builtin_amdgcn_exp2f(static_cast<float>(exponent) - st.exponent);
-  st.exponent = static_cast<float>(exponent);
-  st.l *= change;
+__device__ __forceinline__ void scale_sums(State& st, const float (&f)[4]) {
 #pragma unroll
-  for (int nb = 0; nb < 8; ++nb) st.acc[nb] *= change;
+  for (int r = 0; r < 4; ++r) {
+    st.eights[r] *= f[r];
+#pragma unroll
+    for (int nb = 0; nb < 8; ++nb) st.acc[nb][r] *= f[r];
+  }
 }
 
 // Softmax step over kPages pages: s are the lane's scores, masked ones -inf,
 // v_scale pairs of V's scales (FP16; 0 where masked), ``scale`` the softmax scale
-// in base 2.  p: the lane's rows of the A operand of P V.
-template <int kPages, bool kScaled>
+// in base 2, ``exponent`` that of the sums.  p: the lane's rows of the A operand
+// of P V, tokens 4 kg + 2, 4 kg + 3 in sixteenths with kCodes.
+template <int kPages, bool kCodes>
 __device__ __forceinline__ void softmax_step(State& st, const float (&s)[kPages][4],
                                              const uint32_t (&v_scale)[kPages][2], float scale,
-                                             float low_part, int lane, v8h (&p)[kPages / 2]) {
+                                             float exponent, float low_part, int lane,
+                                             v8h (&p)[kPages / 2]) {
   float top = kNegInf;
 #pragma unroll
   for (int i = 0; i < kPages; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][r]);
-  top = fmaxf(top, __shfl_xor(top, 16, kWave));
-  top = fmaxf(top, __shfl_xor(top, 32, kWave));
-  const float m = fmaxf(st.m, top);
-  const float base = m == kNegInf ? 0.0f : m;    // nothing visible yet: every p is 0
-  const float alpha = __builtin_amdgcn_exp2f((st.m - base) * scale);
-  if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+  if (__builtin_amdgcn_ballot_w64(top > st.limit)) {
+    top = fmaxf(top, __shfl_xor(top, 16, kWave));
+    top = fmaxf(top, __shfl_xor(top, 32, kWave));
+    const float base = fmaxf(st.base, top);
+    // a head with nothing visible yet keeps a base of -inf and an offset of 0
+    const float alpha = base == kNegInf ? 1.0f : __builtin_amdgcn_exp2f((st.base - base) * scale);
+    st.base = base;
+    st.limit = base + kSlack / scale;
+    st.offset = base == kNegInf ? exponent : fmaf(-base, scale, exponent);
+    st.l0 *= alpha;
+    st.l1 *= alpha;
     const int kg = lane >> 4;
-    st.l *= alpha;
+    float f[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float f = __shfl(alpha, (4 * kg + r) & 7, kWave);
-#pragma unroll
-      for (int nb = 0; nb < 8; ++nb) st.acc[nb][r] *= f;
-    }
+    for (int r = 0; r < 4; ++r) f[r] = __shfl(alpha, (4 * kg + r) & 7, kWave);
+    scale_sums(st, f);
   }
-  st.m = m;
-  const float offset = fmaf(-base, scale, st.exponent);
+  const float offset1 = kCodes ? st.offset - 4.0f : st.offset;
 #pragma unroll
   for (int j = 0; j < kPages / 2; ++j) {
     uint32_t words[4];
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
       const int page = 2 * j + (h >> 1), r = 2 * (h & 1);
+      const float offset = h & 1 ? offset1 : st.offset;
       const float x0 = __builtin_amdgcn_exp2f(fmaf(s[page][r], scale, offset));
       const float x1 = __builtin_amdgcn_exp2f(fmaf(s[page][r + 1], scale, offset));
-      st.l += x0 + x1;
-      const float w0 = kScaled ? times_half(x0, v_scale[page][h & 1], 0) : x0;
-      const float w1 = kScaled ? times_half(x1, v_scale[page][h & 1], 1) : x1;
+      if (h & 1) st.l1 += x0 + x1; else st.l0 += x0 + x1;
+      const float w0 = kCodes ? times_half(x0, v_scale[page][h & 1], 0) : x0;
+      const float w1 = kCodes ? times_half(x1, v_scale[page][h & 1], 1) : x1;
       // the FP16 part, or what it leaves (rounding down costs the second 2^-21)
       const v2h high = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(w0, w1));
       words[h] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(
           fmaf(-low_part, static_cast<float>(high.x), w0), fmaf(-low_part, static_cast<float>(high.y), w1)));
     }
-    p[j] = __builtin_bit_cast(v8h, v4u{words[0], words[1], words[2], words[3]});
+    p[j] = operand(words[0], words[1], words[2], words[3]);
   }
 }
 
@@ -217,18 +214,19 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
   const float low_part = n < 8 ? 0.0f : 1.0f;
 
   State st;
-  st.m = kNegInf;
-  st.l = 0.0f;
-  st.exponent = 0.0f;
+  st.base = st.limit = kNegInf;
+  st.offset = st.l0 = st.l1 = 0.0f;
+  st.eights = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int nb = 0; nb < 8; ++nb) st.acc[nb] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  float exponent = 0.0f, acc_exponent = 0.0f;    // of the sums l and acc
 
-  // ---- history: groups wave, wave + 8, ... of the item's pages
+  // ---- history: groups wave, wave + 4, ... of the item's pages
   const int count = it.page_end - it.page_begin;
   const int all_groups = (count + kInt4GroupPages - 1) / kInt4GroupPages;
   const int groups = (all_groups - wave + kInt4Waves - 1) / kInt4Waves;
   if (groups > 0) {
-    // lane l: slot l of the wave, page 4 (8 (l / 4) + wave) + l % 4 of the item
+    // lane l: slot l of the wave, page 4 (4 (l / 4) + wave) + l % 4 of the item
     const int slot_page = kInt4GroupPages * (kInt4Waves * (lane / kInt4GroupPages) + wave) +
                           lane % kInt4GroupPages;
     const int my_page = a.indices[it.page_begin + min(slot_page, count - 1)];
@@ -237,30 +235,53 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
       return page >= count ? 0 : it.page_begin + page == it.last_page ? last_len : kPageSize;
     };
     const int whole = visible(count - 1) == kPageSize ? count : count - 1;   // leading whole pages
+    // byte offset of the slot's block of codes; its scales are at 1/32 of that
+    static_assert(kInt4BlockBytes == 32 * 2 * kInt4BlockScales, "scales of a block");
+    const int64_t my_block = (static_cast<int64_t>(my_page) * hkv + kv) * kInt4BlockBytes;
+    const int my_low = static_cast<int>(my_block), my_high = static_cast<int>(my_block >> 32);
     const uint32_t lane_bytes = 16 * lane, lane_scales = 16 * kg;
-    const Unpack unpack;
+    const uint8_t* scale_bytes = reinterpret_cast<const uint8_t*>(a.scales);
     Group buf[2];
     auto issue = [&](int g, Group& dst) {
 #pragma unroll
       for (int i = 0; i < kInt4GroupPages; ++i) {
-        const int page = __builtin_amdgcn_readlane(my_page, g * kInt4GroupPages + i);
-        const int64_t block = static_cast<int64_t>(page) * hkv + kv;
-        const uint8_t* codes = a.codes + block * kInt4BlockBytes;
-        const uint8_t* scales = reinterpret_cast<const uint8_t*>(a.scales + block * kInt4BlockScales);
+        const int slot = g * kInt4GroupPages + i;
+        const uint64_t block = static_cast<uint32_t>(__builtin_amdgcn_readlane(my_low, slot)) |
+                               static_cast<uint64_t>(__builtin_amdgcn_readlane(my_high, slot)) << 32;
+        const uint8_t* codes = a.codes + block;
         dst.k[i] = *reinterpret_cast<const v4u*>(codes + lane_bytes);
         dst.v[i] = *reinterpret_cast<const v4u*>(codes + kInt4PartBytes + lane_bytes);
-        dst.s[i] = *reinterpret_cast<const v4u*>(scales + lane_scales);
+        dst.s[i] = *reinterpret_cast<const v4u*>(scale_bytes + (block >> 5) + lane_scales);
       }
     };
     issue(0, buf[0]);
     // the largest visible V scale of the wave's pages fixes the power of two
-    {
-      const uint16_t* scales = a.scales + (static_cast<int64_t>(my_page) * hkv + kv) * kInt4BlockScales;
-      const int limit = visible(slot_page);
-      v2u raw[4];
+    v2u raw[4];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) raw[g] = *reinterpret_cast<const v2u*>(scales + 8 * g + 4);
-      take_query();
+    for (int g = 0; g < 4; ++g)
+      raw[g] = *reinterpret_cast<const v2u*>(scale_bytes + (my_block >> 5) + 16 * g + 8);
+    take_query();
+    // q against the even and the odd nibbles of two dwords, and the products'
+    // start, -8 sum(q) over the same dims of all four lanes of the head
+    v8h q_even[2], q_odd[2];
+    float start_even = 0.0f, start_odd = 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const v4u x = __builtin_bit_cast(v4u, q[2 * h]), y = __builtin_bit_cast(v4u, q[2 * h + 1]);
+      q_even[h] = operand(x[0], x[2], y[0], y[2]);
+      q_odd[h] = operand(x[1], x[3], y[1], y[3]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        start_even += static_cast<float>(q_even[h][e]);
+        start_odd += static_cast<float>(q_odd[h][e]);
+      }
+    }
+    start_even += __shfl_xor(start_even, 16, kWave);
+    start_odd += __shfl_xor(start_odd, 16, kWave);
+    start_even = (start_even + __shfl_xor(start_even, 32, kWave)) * -0x1p-21f;
+    start_odd = (start_odd + __shfl_xor(start_odd, 32, kWave)) * -0x1p-17f;
+    {
+      const int limit = visible(slot_page);
       float top = 0.0f;
 #pragma unroll
       for (int t = 0; t < kPageSize; ++t)
@@ -268,8 +289,9 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
       top = wave_max(top);
       int e = 0;
       if (top > 0.0f) frexpf(top, &e);
-      st.exponent = static_cast<float>(14 - e);
+      exponent = st.offset = static_cast<float>(10 - e);
     }
+    const float scale = a.sm_scale_log2 * 0x1p20f;       // the products are dots times 2^-20
 
     auto compute = [&](int g, Group& cur) {
       const int first = kInt4GroupPages * (kInt4Waves * g + wave);
@@ -278,15 +300,19 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
       for (int i = 0; i < kInt4GroupPages; ++i) {
         consume_point(cur.k[i]);
         consume_point(cur.s[i]);
-        v4f dot = {0.0f, 0.0f, 0.0f, 0.0f};
+        v4f dot_even = {start_even, start_even, start_even, start_even};
+        v4f dot_odd = {start_odd, start_odd, start_odd, start_odd};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t x = cur.k[i][w], y = x >> 8;
-          dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              join(unpack.even(x), unpack.odd(x), unpack.even(y), unpack.odd(y)), q[w], dot, 0, 0, 0);
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t x = cur.k[i][2 * h], y = cur.k[i][2 * h + 1];
+          dot_even = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              operand(even(x), even(x >> 8), even(y), even(y >> 8)), q_even[h], dot_even, 0, 0, 0);
+          dot_odd = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              operand(odd(x), odd(x >> 8), odd(y), odd(y >> 8)), q_odd[h], dot_odd, 0, 0, 0);
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[i][r] = times_half(dot[r], cur.s[i][r >> 1], r & 1);
+        for (int r = 0; r < 4; ++r)
+          s[i][r] = times_half(fmaf(dot_even[r], 16.0f, dot_odd[r]), cur.s[i][r >> 1], r & 1);
       }
       uint32_t v_scale[kInt4GroupPages][2];
 #pragma unroll
@@ -307,20 +333,22 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
         }
       }
       v8h p[kInt4GroupPages / 2];
-      softmax_step<kInt4GroupPages, true>(st, s, v_scale, a.sm_scale_log2, low_part, lane, p);
+      softmax_step<kInt4GroupPages, true>(st, s, v_scale, scale, exponent, low_part, lane, p);
 #pragma unroll
       for (int i = 0; i < kInt4GroupPages; ++i) consume_point(cur.v[i]);
 #pragma unroll
-      for (int j = 0; j < kInt4GroupPages / 2; ++j)
+      for (int j = 0; j < kInt4GroupPages / 2; ++j) {
+        st.eights = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            p[j], operand(kEvenEights, kOddEights, kEvenEights, kOddEights), st.eights, 0, 0, 0);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const uint32_t x = cur.v[2 * j][w], y = cur.v[2 * j + 1][w];
           st.acc[2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              p[j], join(unpack.even(x), unpack.odd(x), unpack.even(y), unpack.odd(y)), st.acc[2 * w], 0, 0, 0);
+              p[j], operand(even(x), odd(x), even(y), odd(y)), st.acc[2 * w], 0, 0, 0);
           st.acc[2 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              p[j], join(unpack.even(x >> 8), unpack.odd(x >> 8), unpack.even(y >> 8), unpack.odd(y >> 8)),
-              st.acc[2 * w + 1], 0, 0, 0);
+              p[j], operand(even(x >> 8), odd(x >> 8), even(y >> 8), odd(y >> 8)), st.acc[2 * w + 1], 0, 0, 0);
         }
+      }
     };
     // the loads of group g + 1 are in flight while group g is computed
     int g = 0;
@@ -337,14 +365,28 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
     } else {
       compute(g, buf[0]);
     }
+#pragma unroll
+    for (int nb = 0; nb < 8; ++nb) st.acc[nb] -= st.eights;
+    st.l0 = fmaf(st.l1, 16.0f, st.l0);
+    st.l1 = 0.0f;
+    st.base *= 0x1p20f;            // as the dots themselves
+    st.limit *= 0x1p20f;
+    acc_exponent = exponent - 24.0f;
   } else {
     take_query();
   }
 
-  // ---- exact tail: pairs wave, wave + 8, ... of the item's tail pages
+  // ---- exact tail: pairs wave, wave + 4, ... of the item's tail pages
   const int tail_count = it.tail_end - it.tail_begin;
   if (2 * wave < tail_count) {
-    set_exponent(st, 14);          // probabilities alone are at most 1
+    // probabilities alone: their largest is 1, or 2^4 with the base's slack
+    const float change_l = __builtin_amdgcn_exp2f(10.0f - exponent);
+    const float change = __builtin_amdgcn_exp2f(10.0f - acc_exponent);
+    st.l0 *= change_l;
+    st.offset += 10.0f - exponent;
+    const float f[4] = {change, change, change, change};
+    scale_sums(st, f);
+    exponent = acc_exponent = 10.0f;
     const int64_t row_stride = static_cast<int64_t>(hkv) * kHeadDim;
     const int last_len = min(a.tail_last_len[it.request], kPageSize);
     for (int page = 2 * wave; page < tail_count; page += 2 * kInt4Waves) {
@@ -378,7 +420,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
       }
       v8h p[1];
       const uint32_t unscaled[2][2] = {};
-      softmax_step<2, false>(st, s, unscaled, a.sm_scale_log2, low_part, lane, p);
+      softmax_step<2, false>(st, s, unscaled, a.sm_scale_log2, exponent, low_part, lane, p);
 #pragma unroll
       for (int nb = 0; nb < 8; ++nb) {
         v4u cols;
@@ -393,12 +435,13 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
   }
 
   // ---- the waves meet: rows r and r + 8 of the product, then 8 partial states
-  st.l += __shfl_xor(st.l, 16, kWave);
-  st.l += __shfl_xor(st.l, 32, kWave);
-  const float scale = __builtin_amdgcn_exp2f(-st.exponent);
+  float l_sum = st.l0 + st.l1;
+  l_sum += __shfl_xor(l_sum, 16, kWave);
+  l_sum += __shfl_xor(l_sum, 32, kWave);
+  const float scale = __builtin_amdgcn_exp2f(-acc_exponent);
   if (kg == 0 && n < kHeads) {
-    part_m[wave][n] = st.m * a.sm_scale_log2;
-    part_l[wave][n] = st.l * scale;
+    part_m[wave][n] = st.base * a.sm_scale_log2;
+    part_l[wave][n] = l_sum * __builtin_amdgcn_exp2f(-exponent);
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
