@@ -42,6 +42,7 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef uint16_t v2s __attribute__((ext_vector_type(2)));
 
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr int kThreads = kWave * kInt4Waves;
@@ -71,6 +72,8 @@ struct Int4Args {
 };
 
 __device__ __forceinline__ v2h as_half2(uint32_t bits) { return __builtin_bit_cast(v2h, bits); }
+
+__device__ __forceinline__ v2s as_short2(uint32_t bits) { return __builtin_bit_cast(v2s, bits); }
 
 __device__ __forceinline__ v2h splat(float x) {
   return v2h{static_cast<_Float16>(x), static_cast<_Float16>(x)};
@@ -195,21 +198,18 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
   const int heads = min(kHeads, a.group - first_head);
   const int hkv = a.num_kv_heads;
 
-  // query: B operand, column n = head n % 8, dims 32 w + 8 kg ..
-  const bool has_query = (n & 7) < heads;
+  // query: B operand, column n = head n % 8, dims 32 w + 8 kg ..; columns past
+  // the heads repeat the first one and are dropped at the end
   v8h q[4];
   {
     const uint16_t* row = a.query + it.request * a.query_batch_stride +
-                          static_cast<int64_t>(kv * a.group + first_head + (has_query ? n & 7 : 0)) * kHeadDim;
+                          static_cast<int64_t>(kv * a.group + first_head + ((n & 7) < heads ? n & 7 : 0)) * kHeadDim;
 #pragma unroll
     for (int w = 0; w < 4; ++w) q[w] = *reinterpret_cast<const v8h*>(row + 32 * w + 8 * kg);
   }
   auto take_query = [&]() {        // once the first pages are on their way
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      consume_point(q[w]);
-      if (!has_query) q[w] = v8h{0, 0, 0, 0, 0, 0, 0, 0};
-    }
+    for (int w = 0; w < 4; ++w) consume_point(q[w]);
   };
   const float low_part = n < 8 ? 0.0f : 1.0f;
 
@@ -271,9 +271,9 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
       q_even[h] = operand(x[0], x[2], y[0], y[2]);
       q_odd[h] = operand(x[1], x[3], y[1], y[3]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        start_even += static_cast<float>(q_even[h][e]);
-        start_odd += static_cast<float>(q_odd[h][e]);
+      for (int e = 0; e < 4; ++e) {
+        start_even = __builtin_amdgcn_fdot2(as_half2(e < 2 ? x[2 * e] : y[2 * e - 4]), splat(1.0f), start_even, false);
+        start_odd = __builtin_amdgcn_fdot2(as_half2(e < 2 ? x[2 * e + 1] : y[2 * e - 3]), splat(1.0f), start_odd, false);
       }
     }
     start_even += __shfl_xor(start_even, 16, kWave);
@@ -281,14 +281,22 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
     start_even = (start_even + __shfl_xor(start_even, 32, kWave)) * -0x1p-21f;
     start_odd = (start_odd + __shfl_xor(start_odd, 32, kWave)) * -0x1p-17f;
     {
-      const int limit = visible(slot_page);
-      float top = 0.0f;
+      // positive FP16 values order as their bits do
+      if (whole < count) {
+        const int limit = visible(slot_page);
 #pragma unroll
-      for (int t = 0; t < kPageSize; ++t)
-        top = fmaxf(top, t < limit ? static_cast<float>(as_half2(raw[t >> 2][(t & 3) >> 1])[t & 1]) : 0.0f);
-      top = wave_max(top);
+        for (int t = 0; t < kPageSize; t += 2)
+          raw[t >> 2][(t & 3) >> 1] &= t + 1 < limit ? ~0u : t < limit ? 0x0000ffffu : 0u;
+      }
+      v2s top = as_short2(raw[0][0]);
+#pragma unroll
+      for (int d = 1; d < 8; ++d) top = __builtin_elementwise_max(top, as_short2(raw[d >> 1][d & 1]));
+      float largest = fmaxf(half_bits_to_float(top.x), half_bits_to_float(top.y));
+      largest = row16_max(largest);
+      largest = fmaxf(largest, __shfl_xor(largest, 16, kWave));
+      largest = fmaxf(largest, __shfl_xor(largest, 32, kWave));
       int e = 0;
-      if (top > 0.0f) frexpf(top, &e);
+      if (largest > 0.0f) frexpf(largest, &e);
       exponent = st.offset = static_cast<float>(10 - e);
     }
     const float scale = a.sm_scale_log2 * 0x1p20f;       // the products are dots times 2^-20
@@ -443,16 +451,20 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
     part_m[wave][n] = st.base * a.sm_scale_log2;
     part_l[wave][n] = l_sum * __builtin_amdgcn_exp2f(-exponent);
   }
+  // a swap of two registers' halves adds rows r and r + 8 of two channels at
+  // once: lanes below 32 end with channel 8 n + 2 p, the others with the next
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    float o[8];
+    float o[4];
 #pragma unroll
-    for (int nb = 0; nb < 8; ++nb) o[nb] = (st.acc[nb][r] + __shfl_xor(st.acc[nb][r], 32, kWave)) * scale;
-    if (kg < 2) {
-      float* dst = &part_o[wave][4 * kg + r][8 * n];
-      *reinterpret_cast<float4*>(dst) = make_float4(o[0], o[1], o[2], o[3]);
-      *reinterpret_cast<float4*>(dst + 4) = make_float4(o[4], o[5], o[6], o[7]);
+    for (int p = 0; p < 4; ++p) {
+      const v2u x = __builtin_amdgcn_permlane32_swap(__float_as_uint(st.acc[2 * p][r]),
+                                                     __float_as_uint(st.acc[2 * p + 1][r]), false, false);
+      o[p] = (__uint_as_float(x.x) + __uint_as_float(x.y)) * scale;
     }
+    // part_o[..][64 b + c]: dim 2 c + b
+    *reinterpret_cast<float4*>(&part_o[wave][4 * (kg & 1) + r][64 * (lane >> 5) + 4 * n]) =
+        make_float4(o[0], o[1], o[2], o[3]);
   }
   __syncthreads();
   // wave w finishes heads w, w + 4, two dims per lane
@@ -466,7 +478,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
 #pragma unroll
   for (int w = 0; w < kInt4Waves; ++w) {
     const float f = __builtin_amdgcn_exp2f(part_m[w][h] - base);
-    const float2 x = *reinterpret_cast<const float2*>(&part_o[w][h][2 * lane]);
+    const float2 x = make_float2(part_o[w][h][lane], part_o[w][h][64 + lane]);
     l += f * part_l[w][h];
     o.x += f * x.x;
     o.y += f * x.y;
