@@ -249,10 +249,16 @@ def current_stream() -> int:
 def require_current_device(*tensors) -> None:
     """ValueError unless every tensor (None aside) is on the current CUDA
     device, on whose current stream the kernels are launched."""
-    device = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else None
+    device = None
     for t in tensors:
-        if t is not None and (device is None or t.get_device() != device):
-            raise ValueError("all tensors must be on the current CUDA device")
+        if t is not None:
+            at = t.get_device()
+            if device is None:
+                device = at
+            if at != device or at < 0:
+                raise ValueError("all tensors must be on the current CUDA device")
+    if device is not None and device != torch._C._cuda_getDevice():
+        raise ValueError("all tensors must be on the current CUDA device")
 
 
 def last_error() -> str:

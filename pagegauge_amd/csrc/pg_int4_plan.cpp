@@ -48,30 +48,33 @@ int32_t build_int4_plan(const int32_t* host_indptr, const int32_t* host_tail_ind
     history += r.pages;
     exact_pages += r.tail;
   }
-  // The largest share of a workgroup (``cap``, in weighted pages) for which
-  // the batch fills about one workgroup per CU, but at least one group of
-  // pages per wave.
+  // The smallest largest share (``cap``, in weighted pages) with which the batch
+  // takes no more workgroups than ``target``, but at least one group of pages per
+  // wave.  One workgroup per CU is the better plan as long as its waves can hold
+  // their pages (49K tokens: 32 items 15.5 us, 64 items 17.2; 64K 18.1 and 20.0),
+  // and two where they cannot (128K tokens: 33 items, an uneven round, 44.7 us, 64
+  // items 33.0; 16 requests of 8K 37.1 and 33.9).
   const int64_t groups = static_cast<int64_t>(num_kv_heads) *
                          ceil_div(num_qo_heads / num_kv_heads, kInt4HeadsPerWave);
   const int64_t cus = num_cus > 0 ? num_cus : 256;
-  const int64_t target = std::max<int64_t>(batch_size, kInt4TargetPerCu * cus / groups);
-  int64_t low = kInt4Waves * kInt4GroupPages;
-  int64_t high = std::max(low, total);
-  auto count = [&](int64_t cap) {
-    int64_t n = 0;
-    for (const Request& r : requests) n += r.cuts(cap);
-    return n;
+  auto balanced = [&](int64_t target) {
+    int64_t low = kInt4Waves * kInt4GroupPages, high = std::max(low, total);
+    while (low < high) {
+      const int64_t cap = low + (high - low) / 2;
+      int64_t n = 0;
+      for (const Request& r : requests) n += r.cuts(cap);
+      if (n <= target) high = cap; else low = cap + 1;
+    }
+    return high;
   };
-  while (low < high) {
-    const int64_t mid = low + (high - low) / 2;
-    if (count(mid) <= target) high = mid; else low = mid + 1;
-  }
+  int64_t cap = balanced(std::max<int64_t>(batch_size, cus / groups));
+  if (cap > kInt4MaxItemPages) cap = balanced(std::max<int64_t>(batch_size, 2 * cus / groups));
   items.clear();
   item_ptr.assign(batch_size + 1, 0);
   int64_t most = 0;
   for (int32_t b = 0; b < batch_size; ++b) {
     const Request& r = requests[b];
-    const int64_t cuts = r.cuts(high);
+    const int64_t cuts = r.cuts(cap);
     if (cuts > kInt4MaxItemsPerRequest)
       return fail(PG_ERROR_UNSUPPORTED, "too many pages in one request");
     item_ptr[b] = static_cast<int32_t>(items.size());

@@ -10,7 +10,6 @@
 
 namespace pg {
 
-constexpr int kInt4TargetPerCu = 2;
 constexpr int kInt4Waves = 4;           // waves of a workgroup, sharing one item's pages
 constexpr int kInt4GroupPages = 4;      // consecutive pages a wave takes at a time
 constexpr int kInt4MaxItemPages = kInt4Waves * 64;   // a wave holds its page ids one per lane

@@ -52,14 +52,14 @@ def allocate_pages(pages: int, kv_heads: int, device="cuda") -> tuple[torch.Tens
 
 
 def _check_pool(codes: torch.Tensor, scales: torch.Tensor, heads: int) -> int:
-    pages = codes.shape[0] if codes.dim() == 4 else -1
-    if codes.dtype != torch.uint8 or codes.shape != (pages, heads, *BLOCK_SHAPE) \
-            or not codes.is_contiguous():
+    shape = codes.shape
+    if codes.dtype is not torch.uint8 or len(shape) != 4 or shape[1] != heads \
+            or shape[2:] != BLOCK_SHAPE or not codes.is_contiguous():
         raise ValueError(f"4-bit codes must be contiguous uint8 [pages,{heads},2,1024]")
-    if scales.dtype != torch.float16 or scales.shape != (pages, heads, *SCALE_SHAPE) \
+    if scales.dtype is not torch.float16 or scales.shape != (shape[0], heads, 4, 2, 4) \
             or not scales.is_contiguous():
-        raise ValueError(f"4-bit scales must be contiguous float16 [{pages},{heads},4,2,4]")
-    return pages
+        raise ValueError(f"4-bit scales must be contiguous float16 [{shape[0]},{heads},4,2,4]")
+    return shape[0]
 
 
 def _check_ids(ids: Optional[torch.Tensor], count: int, what: str) -> None:
@@ -69,10 +69,12 @@ def _check_ids(ids: Optional[torch.Tensor], count: int, what: str) -> None:
 
 def _token_rows(t: torch.Tensor, what: str) -> int:
     """Token stride of FP16 rows [T, H, 128] whose heads are dense."""
-    if t.dtype != torch.float16 or t.dim() != 3 or t.shape[2] != DIM or t.shape[1] == 0 \
-            or t.stride(2) != 1 or t.stride(1) != DIM and t.shape[1] > 1:
-        raise ValueError(f"{what} must be float16 [T,Hkv,128] rows of dense heads")
-    return t.stride(0)
+    shape = t.shape
+    if t.dtype is torch.float16 and len(shape) == 3 and shape[2] == DIM and shape[1] > 0:
+        token, head, dim = t.stride()
+        if dim == 1 and (head == DIM or shape[1] == 1):
+            return token
+    raise ValueError(f"{what} must be float16 [T,Hkv,128] rows of dense heads")
 
 
 def _check_centers(key_center, value_center, shape: tuple) -> None:
@@ -161,7 +163,8 @@ def dequantize_pages(codes: torch.Tensor, scales: torch.Tensor,
     rows = []
     for t in (key, value):
         if t is None:
-            t = torch.empty(tokens, heads, DIM, device=codes.device, dtype=torch.float16)
+            t = torch.empty_strided((tokens, heads, DIM), (heads * DIM, DIM, 1), dtype=torch.float16,
+                                    device=codes.device)
         elif t.shape != (tokens, heads, DIM):
             raise ValueError(f"K and V rows must be [{tokens},{heads},128]")
         strides.append(_token_rows(t, "K and V"))
@@ -315,8 +318,8 @@ class Int4PagedDecode:
         and an lse of -inf."""
         if not self._planned:
             raise RuntimeError("plan() must be called before run()")
-        hkv = self._num_kv_heads
-        _check_query(q, self._batch, self._num_qo_heads)
+        hkv, batch = self._num_kv_heads, self._batch
+        _check_query(q, batch, self._num_qo_heads)
         pool = _check_pool(codes, scales, hkv)
         exact_k = exact_v = None
         if self._tables[2] is not None:
@@ -325,20 +328,27 @@ class Int4PagedDecode:
             exact_k, exact_v = exact_cache
             _check_cache(exact_k, "exact_k", torch.float16, hkv)
             _check_cache(exact_v, "exact_v", torch.float16, hkv)
-            _check_page_ids(self._id_ranges[1], min(exact_k.shape[0], exact_v.shape[0]), "exact tail")
-        _check_page_ids(self._id_ranges[0], pool, "4-bit")
-        if value_center is not None and (value_center.dtype != torch.float16
-                                         or value_center.shape != (self._batch, hkv, DIM)
+            if self._id_ranges[1] is not None:
+                _check_page_ids(self._id_ranges[1], min(exact_k.shape[0], exact_v.shape[0]),
+                                "exact tail")
+        if self._id_ranges[0] is not None:
+            _check_page_ids(self._id_ranges[0], pool, "4-bit")
+        if value_center is not None and (value_center.dtype is not torch.float16
+                                         or value_center.shape != (batch, hkv, DIM)
                                          or not value_center.is_contiguous()):
             raise ValueError(f"value_center must be contiguous float16 [B,{hkv},128]")
         if out is None:
-            out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        elif out.shape != q.shape or out.dtype != torch.float16 or not out.is_contiguous():
+            out = torch.empty_like(q)
+            if not out.is_contiguous():
+                out = torch.empty(q.shape, device=q.device, dtype=torch.float16)
+        elif out.shape != q.shape or out.dtype is not torch.float16 or not out.is_contiguous():
             raise ValueError("out must be contiguous float16, shaped like q")
         if lse is None:
             if return_lse:
-                lse = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32)
-        elif lse.shape != q.shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous():
+                lse = torch.empty_strided((batch, self._num_qo_heads), (self._num_qo_heads, 1),
+                                          dtype=torch.float32, device=q.device)
+        elif lse.shape != (batch, self._num_qo_heads) or lse.dtype is not torch.float32 \
+                or not lse.is_contiguous():
             raise ValueError("lse must be contiguous float32 [B,Hq]")
         _capi.require_current_device(self.workspace, q, codes, scales, exact_k, exact_v, value_center,
                                      out, lse)

@@ -57,7 +57,9 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
         raise ValueError("logits must be FP16, BF16 or float32 [B, V] rows")
     batch, vocab = logits.shape
     if out is None:
-        out = torch.empty((batch, vocab), device=logits.device, dtype=logits.dtype)
+        out = torch.empty_like(logits)
+        if vocab > 1 and out.stride(1) != 1:
+            out = torch.empty((batch, vocab), device=logits.device, dtype=logits.dtype)
     elif out.shape != logits.shape or out.dtype != logits.dtype or vocab > 1 and out.stride(1) != 1 \
             or batch > 1 and out.stride(0) < vocab:
         raise ValueError("shaped logits must be rows like the logits")
@@ -73,11 +75,13 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
             raise ValueError("history must be int32 or int64 [B, capacity] rows")
         if history_lengths is None:
             raise ValueError("a history needs its lengths")
-    for t, dt in ((history_lengths, torch.int32), (prompt_lengths, torch.int32),
-                  (repetition, torch.float32), (frequency, torch.float32),
-                  (presence, torch.float32)):
-        if t is not None and (t.dtype != dt or t.shape != (batch,) or not t.is_contiguous()):
-            raise ValueError("lengths must be int32 and penalties float32, contiguous [B]")
+    for t in (history_lengths, prompt_lengths):
+        if t is not None and (t.dtype is not torch.int32 or t.shape != (batch,) or not t.is_contiguous()):
+            raise ValueError("lengths must be contiguous int32 [B]")
+    for t in (repetition, frequency, presence):
+        if t is not None and (t.dtype is not torch.float32 or t.shape != (batch,)
+                              or not t.is_contiguous()):
+            raise ValueError("penalties must be contiguous float32 [B]")
     if (bias_tokens is None) != (bias_values is None):
         raise ValueError("bias tokens and values go together")
     biases = 0

@@ -31,6 +31,8 @@ from . import _capi
 
 _DTYPES = {torch.float16: _capi.PG_DTYPE_FP16, torch.bfloat16: _capi.PG_DTYPE_BF16,
            torch.float32: _capi.PG_DTYPE_FP32}
+_POSITIONS = (torch.int32, torch.int64)
+_NO_ROWS = (None, 0, 0, 0, None, 0, 0)
 LAYOUTS = ("half", "interleaved")
 SCALINGS = ("none", "linear", "ntk", "by_parts")
 
@@ -103,47 +105,54 @@ class RotaryEmbedding:
         dtype = _DTYPES.get(query.dtype)
         if dtype is None:
             raise ValueError("rotary rows must be FP16, BF16 or FP32")
-        if positions.dim() != 1 or positions.dtype not in (torch.int32, torch.int64) \
-                or positions.stride(0) != 1 and positions.shape[0] > 1:
+        if positions.dim() != 1 or positions.dtype not in _POSITIONS or not positions.is_contiguous():
             raise ValueError("positions must be contiguous int32 or int64 [T]")
-        if out_query is None:
-            out_query = torch.empty(query.shape, device=query.device, dtype=query.dtype)
-        if key is not None and out_key is None:
-            out_key = torch.empty(key.shape, device=key.device, dtype=key.dtype)
         tokens = positions.shape[0]
-        rows = []
-        for x, out in ((query, out_query), (key, out_key)):
-            if x is None:
-                rows.append((None, 0, 0, 0, None, 0, 0))
-                continue
-            if x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != self.head_dim \
-                    or x.dtype != query.dtype:
-                raise ValueError(f"rotary rows must be [T, H, {self.head_dim}] of one type, with a "
-                                 "position each")
-            if out.shape != x.shape or out.dtype != x.dtype:
-                raise ValueError("rotated rows must be shaped and typed like the rows")
-            xs, os = x.stride(), out.stride()
-            if xs[2] != 1 or os[2] != 1:
-                raise ValueError("a head's dims must be contiguous")
-            xp, op = x.data_ptr(), out.data_ptr()
-            # rows of the output, [T, H] of head_dim dims, must lie apart
-            (near, inner), (far, _) = sorted(((os[0], tokens), (os[1], x.shape[1])))
-            if tokens > 1 and x.shape[1] > 1:
-                apart = near >= self.head_dim and far >= near * (inner - 1) + self.head_dim
-            else:
-                apart = (os[0] if tokens > 1 else os[1]) >= self.head_dim or tokens * x.shape[1] <= 1
-            if not apart:
-                raise ValueError("rotated rows must not overlap each other")
-            if xp == op and xs != os:
-                raise ValueError("rows rotated in place must keep their strides")
-            rows.append((xp, xs[0], xs[1], x.shape[1], op, os[0], os[1]))
-        if key is not None and (rows[0][0] == rows[0][4]) != (rows[1][0] == rows[1][4]):
-            raise ValueError("query and key are rotated in place together or not at all")
+        out_query, query_args, in_place = self._rows(query, out_query, tokens, query.dtype)
+        key_args = _NO_ROWS
+        if key is not None:
+            out_key, key_args, key_in_place = self._rows(key, out_key, tokens, query.dtype)
+            if in_place != key_in_place:
+                raise ValueError("query and key are rotated in place together or not at all")
         _capi.require_current_device(self.turns, positions, query, out_query, key, out_key)
-        (q, qt, qh, hq, oq, oqt, oqh), (k, kt, kh, hk, ok, okt, okh) = rows
-        if tokens and hq + hk:
-            _capi.call("pg_rotate", q, qt, qh, hq, k, kt, kh, hk, oq, oqt, oqh, ok, okt, okh,
+        if tokens and query_args[3] + key_args[3]:
+            _capi.call("pg_rotate", *query_args[:4], *key_args[:4], *query_args[4:], *key_args[4:],
                        positions.data_ptr(), positions.element_size(), self.turns.data_ptr(),
                        self.amplitude, tokens, self.head_dim, self.rotary_dim,
                        int(self.interleaved), dtype, _capi.current_stream())
         return out_query, out_key
+
+    def _rows(self, x: torch.Tensor, out: Optional[torch.Tensor], tokens: int, dtype):
+        """(out, (x, token and head strides, heads, out, its strides), in place)."""
+        shape = x.shape
+        if len(shape) != 3 or shape[0] != tokens or shape[2] != self.head_dim or x.dtype != dtype:
+            raise ValueError(f"rotary rows must be [T, H, {self.head_dim}] of one type, with a "
+                             "position each")
+        token, head, dim = x.stride()
+        if dim != 1:
+            raise ValueError("a head's dims must be contiguous")
+        heads = shape[1]
+        at = x.data_ptr()
+        if out is None:
+            out = torch.empty_like(x)
+            if not out.is_contiguous():
+                out = torch.empty(shape, device=x.device, dtype=dtype)
+            return out, (at, token, head, heads, out.data_ptr(), heads * self.head_dim,
+                         self.head_dim), False
+        if out.shape != shape or out.dtype != dtype:
+            raise ValueError("rotated rows must be shaped and typed like the rows")
+        out_token, out_head, out_dim = out.stride()
+        if out_dim != 1:
+            raise ValueError("a head's dims must be contiguous")
+        # the [T, H] rows of head_dim dims must lie apart
+        (near, inner), (far, _) = sorted(((out_token, tokens), (out_head, heads)))
+        if tokens > 1 and heads > 1:
+            apart = near >= self.head_dim and far >= near * (inner - 1) + self.head_dim
+        else:
+            apart = tokens * heads <= 1 or (out_token if tokens > 1 else out_head) >= self.head_dim
+        if not apart:
+            raise ValueError("rotated rows must not overlap each other")
+        in_place = out.data_ptr() == at
+        if in_place and (out_token, out_head) != (token, head):
+            raise ValueError("rows rotated in place must keep their strides")
+        return out, (at, token, head, heads, out.data_ptr(), out_token, out_head), in_place

@@ -33,14 +33,14 @@ def _check_plan(pages, tail, hq, hkv, cus):
             assert own[0][begin] == lo and own[-1][end] == hi
             assert all(x[end] == y[begin] for x, y in zip(own, own[1:]))
             assert all(x[begin] <= x[end] and x[last] == hi - 1 for x in own)
-        assert all(i[2] - i[1] <= 512 for i in own)       # page ids a wave's lanes can hold
+        assert all(i[2] - i[1] <= 256 for i in own)       # page ids a wave's lanes can hold
     assert plan.max_items_per_request == most
     assert plan.workspace_bytes >= plan.partial_offset + (most > 1) * len(items) * hq * 130 * 4
 
 
 @pytest.mark.parametrize("pages,tail,hq,hkv", [
     ([1], [0], 32, 8), ([0], [0], 32, 8), ([3056], [16], 32, 8), ([0], [4000], 32, 8),
-    ([0, 5, 0, 100000], [0, 0, 16, 16], 64, 4), ([512], [16], 32, 8), ([513], [0], 8, 8)])
+    ([0, 5, 0, 100000], [0, 0, 16, 16], 64, 4), ([256], [16], 32, 8), ([257], [0], 8, 8), ([512], [16], 32, 8)])
 def test_plan_covers_every_page_once(pages, tail, hq, hkv):
     for cus in (1, 64, 256):
         _check_plan(pages, tail, hq, hkv, cus)

@@ -24,9 +24,9 @@ _H = torch.zeros(2, 5, dtype=torch.int64)
     (None, dict(history=_H), "needs its lengths"),
     (None, dict(history=_H.float(), history_lengths=_N), "int32 or int64"),
     (None, dict(history=_H[:1], history_lengths=_N), "int32 or int64"),
-    (None, dict(history=_H, history_lengths=_N.long()), "int32 and penalties float32"),
-    (None, dict(history=_H, history_lengths=_N, presence=_F.double()), "penalties float32"),
-    (None, dict(history=_H, history_lengths=_N, frequency=torch.zeros(3)), "penalties float32"),
+    (None, dict(history=_H, history_lengths=_N.long()), "lengths must be contiguous int32"),
+    (None, dict(history=_H, history_lengths=_N, presence=_F.double()), "penalties must be contiguous float32"),
+    (None, dict(history=_H, history_lengths=_N, frequency=torch.zeros(3)), "penalties must be contiguous float32"),
     (None, dict(bias_tokens=_H), "go together"),
     (None, dict(bias_tokens=_H, bias_values=torch.zeros(2, 4)), "biases must be"),
     (None, dict(history=_H.int(), history_lengths=_N, bias_tokens=_H, bias_values=torch.zeros(2, 5)),
