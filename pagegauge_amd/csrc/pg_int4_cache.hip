@@ -26,12 +26,30 @@ __device__ __forceinline__ uint16_t int4_scale_bits(float maximum) {
   return __half_as_ushort(__float2half_rn(fmaxf(maximum * (1.0f / 7.0f), 0x1p-20f)));
 }
 
-// code + 8 of x / scale
-__device__ __forceinline__ uint32_t int4_nibble(float x, float scale) {
-  const float q = x / scale;
-  const float steps = fminf(floorf(fabsf(q) + 0.5f), 7.0f);
-  const int code = static_cast<int>(__builtin_copysignf(steps, q));   // a NaN converts to 0
-  return static_cast<uint32_t>((q != q ? 0 : code) + 8);
+// Code of x / scale, given r = 1 / scale rounded: the quotient is the IEEE one,
+// by three operations instead of a division.  With q0 = RN(x * r), within 2 ulp
+// of it, the residual e = x - q0 * scale is exact (the scale has the 11 bits of an
+// FP16 value, and x lies far from float32's limits), and RN(q0 + e * r) is the
+// quotient with a relative error of 2^-24 of its last bits before it is rounded;
+// a 24-bit number over an 11-bit one is never that near a midpoint of two floats.
+// An infinite scale gives NaN for every x where the division gives 0 or NaN, and
+// both have code 0.
+//
+// sign(q) floor(|q| + 0.5) is the truncation of q + copysign(0.5, q).  The
+// conversion instruction saturates and takes a NaN to 0 (C++ leaves that open).
+__device__ __forceinline__ int int4_code(float x, float scale, float r) {
+  const float q0 = x * r;
+  const float q = fmaf(fmaf(-q0, scale, x), r, q0);
+  int code;
+  asm("v_cvt_i32_f32 %0, %1" : "=v"(code) : "v"(q + __builtin_copysignf(0.5f, q)));
+  return max(-7, min(7, code));
+}
+
+// Eight nibbles, code + 8 each, start at 8 8 ... 8; adding a code at its place
+// never carries out of it.
+constexpr uint32_t kNibbles8 = 0x88888888u;
+__device__ __forceinline__ uint32_t put_code(uint32_t word, int code, int nibble) {
+  return word + (static_cast<uint32_t>(code) << (4 * nibble));
 }
 
 __device__ __forceinline__ float half_at(const v4u& v, int e) {
@@ -68,7 +86,7 @@ template <bool kValue>
 __device__ __forceinline__ void pack_part(const float (&x)[4][8], int visible, uint8_t* codes,
                                           uint16_t* scales, int lane) {
   const int n = lane & 15, kg = lane >> 4;
-  v4u word = {0u, 0u, 0u, 0u};
+  v4u word = {kNibbles8, kNibbles8, kNibbles8, kNibbles8};
   if (!kValue) {
     float m = 0.0f;
 #pragma unroll
@@ -78,12 +96,12 @@ __device__ __forceinline__ void pack_part(const float (&x)[4][8], int visible, u
     m = fmaxf(m, __shfl_xor(m, 16, kWave));
     m = fmaxf(m, __shfl_xor(m, 32, kWave));
     const uint16_t bits = int4_scale_bits(m);
-    const float scale = half_bits_to_float(bits);
+    const float scale = half_bits_to_float(bits), r = 1.0f / scale;
 #pragma unroll
     for (int g = 0; g < 4; ++g)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        word[g] |= int4_nibble(x[g][e], scale) << (4 * ((e >> 1) + 4 * (e & 1)));
+        word[g] = put_code(word[g], int4_code(x[g][e], scale, r), (e >> 1) + 4 * (e & 1));
     if (kg == 0) scales[int4_scale_index(0, n)] = n < visible ? bits : 0;
   } else {
 #pragma unroll
@@ -92,10 +110,10 @@ __device__ __forceinline__ void pack_part(const float (&x)[4][8], int visible, u
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[t][e]));
       const uint16_t bits = int4_scale_bits(row16_max(m));
-      const float scale = half_bits_to_float(bits);
+      const float scale = half_bits_to_float(bits), r = 1.0f / scale;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        word[e >> 1] |= int4_nibble(x[t][e], scale) << (4 * ((t >> 1) + 2 * (e & 1) + 4 * (t & 1)));
+        word[e >> 1] = put_code(word[e >> 1], int4_code(x[t][e], scale, r), (t >> 1) + 2 * (e & 1) + 4 * (t & 1));
       if (n == 0) scales[int4_scale_index(1, 4 * kg + t)] = 4 * kg + t < visible ? bits : 0;
     }
   }
@@ -251,49 +269,54 @@ struct AppendArgs {
   int query_heads, kv_heads;
 };
 
-// Rows of the part from the exact page, the token's own row (15) from LDS.
-template <bool kValue>
-__device__ __forceinline__ void finalize_part(const AppendArgs& a, int64_t exact_page, int64_t code_page,
-                                              int head, const uint16_t* own_row, int lane) {
-  const uint16_t* page = a.exact[kValue] + (exact_page * kPageSize * a.kv_heads + head) * kHeadDim;
-  float x[4][8];
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int row = part_row<kValue>(g, lane);
-    const int dim = part_dim<kValue>(g, lane);
-    // row 15 was stored by this wave just now: read row 14 in its place
-    const v4u held = *reinterpret_cast<const v4u*>(
-        page + static_cast<int64_t>(min(row, kPageSize - 2)) * a.kv_heads * kHeadDim + dim);
-    const v4u own = *reinterpret_cast<const v4u*>(own_row + dim);
-    const v4u raw = row == kPageSize - 1 ? own : held;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[g][e] = half_at(raw, e);
-  }
-  const int64_t block = code_page * a.kv_heads + head;
-  pack_part<kValue>(x, kPageSize, a.codes + block * kInt4BlockBytes + kValue * kInt4PartBytes,
-                    a.scales + block * kInt4BlockScales, lane);
-}
-
 // One wave per row of a request (query heads, then K, then V heads): lane p
-// holds pair p of the rotated part, or two dims past it.
+// holds pair p of the rotated part, or two dims past it.  What the row needs is
+// requested at once, the rows of a page that closes included: the kernel's time
+// is that of its trips to memory, one for the request's position and ids and one
+// for everything else (as a chain of five, 256 requests took 10.4 us).
 __global__ __launch_bounds__(kWave * kWavesPerBlock) void int4_rope_append_kernel(AppendArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t own[kWavesPerBlock][kHeadDim];
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int row = blockIdx.y * kWavesPerBlock + wave;
   if (row >= a.query_heads + 2 * a.kv_heads) return;   // whole waves; no barrier below
   const int request = blockIdx.x;
-  const int32_t position = a.positions[request];
-  if (position < 0) return;
   const int kind = row < a.query_heads ? 0 : row < a.query_heads + a.kv_heads ? 1 : 2;
   const int head = kind == 0 ? row : kind == 1 ? row - a.query_heads : row - a.query_heads - a.kv_heads;
   const uint16_t* in = a.rows[kind] + request * a.batch_stride[kind] + head * kHeadDim;
   const bool turned = lane < a.rotary_dim / 2;
   const int first = turned && !a.interleaved ? lane : 2 * lane;
   const int second = turned && !a.interleaved ? lane + a.rotary_dim / 2 : 2 * lane + 1;
-  float x = half_bits_to_float(in[first]);
-  float y = half_bits_to_float(in[second]);
+  const int32_t position = a.positions[request];
+  const int64_t exact_page = a.exact_ids[request], code_page = a.code_ids[request];
+  const uint16_t x_bits = in[first], y_bits = in[second];
+  const double turns = a.turns[turned ? lane : 0];
+  if (position < 0) return;
+  const int offset = position % kPageSize;
+  const bool stored = kind > 0 && exact_page >= 0 && exact_page < a.num_exact_pages;
+  const bool closes = stored && offset == kPageSize - 1 && code_page >= 0 && code_page < a.num_code_pages;
+
+  // rows of the page in the packed order; row 15 is this token's own and comes
+  // from LDS, row 14 is read in its place
+  v4u held[4];
+  const int64_t row_stride = static_cast<int64_t>(a.kv_heads) * kHeadDim;
+  uint16_t* page = stored ? a.exact[kind - 1] + exact_page * kPageSize * row_stride + head * kHeadDim : nullptr;
+  if (closes) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int r = kind == 1 ? part_row<false>(g, lane) : part_row<true>(g, lane);
+      const int dim = kind == 1 ? part_dim<false>(g, lane) : part_dim<true>(g, lane);
+      held[g] = *reinterpret_cast<const v4u*>(page + min(r, kPageSize - 2) * row_stride + dim);
+    }
+  }
+  float cx = 0.0f, cy = 0.0f;
+  if (stored) {
+    const uint16_t* center = a.center[kind - 1] + (static_cast<int64_t>(request) * a.kv_heads + head) * kHeadDim;
+    cx = half_bits_to_float(center[first]);
+    cy = half_bits_to_float(center[second]);
+  }
+  float x = half_bits_to_float(x_bits), y = half_bits_to_float(y_bits);
   if (kind < 2 && turned) {
-    const float2 pair = rotate_pair(x, y, rotary_cos_sin(position, a.turns[lane], a.amplitude));
+    const float2 pair = rotate_pair(x, y, rotary_cos_sin(position, turns, a.amplitude));
     x = pair.x;
     y = pair.y;
   }
@@ -303,28 +326,34 @@ __global__ __launch_bounds__(kWave * kWavesPerBlock) void int4_rope_append_kerne
     out[second] = __half_as_ushort(__float2half_rn(y));
     return;
   }
-  const int64_t exact_page = a.exact_ids[request];
-  if (exact_page < 0 || exact_page >= a.num_exact_pages) return;
-  const uint16_t* center = a.center[kind - 1] + (static_cast<int64_t>(request) * a.kv_heads + head) * kHeadDim;
-  const uint16_t xb = __half_as_ushort(__float2half_rn(x - half_bits_to_float(center[first])));
-  const uint16_t yb = __half_as_ushort(__float2half_rn(y - half_bits_to_float(center[second])));
-  const int offset = position % kPageSize;
-  uint16_t* out = a.exact[kind - 1] +
-                  ((exact_page * kPageSize + offset) * a.kv_heads + head) * kHeadDim;
-  out[first] = xb;
-  out[second] = yb;
-  if (offset != kPageSize - 1) return;
-  const int64_t code_page = a.code_ids[request];
-  if (code_page < 0 || code_page >= a.num_code_pages) return;
+  if (!stored) return;
+  const uint16_t xb = __half_as_ushort(__float2half_rn(x - cx));
+  const uint16_t yb = __half_as_ushort(__float2half_rn(y - cy));
+  page[offset * row_stride + first] = xb;
+  page[offset * row_stride + second] = yb;
+  if (!closes) return;
   own[wave][first] = xb;
   own[wave][second] = yb;
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  const int64_t block = code_page * a.kv_heads + head;
+  uint8_t* codes = a.codes + block * kInt4BlockBytes;
+  uint16_t* scales = a.scales + block * kInt4BlockScales;
+  float rows[4][8];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int r = kind == 1 ? part_row<false>(g, lane) : part_row<true>(g, lane);
+    const int dim = kind == 1 ? part_dim<false>(g, lane) : part_dim<true>(g, lane);
+    const v4u mine = *reinterpret_cast<const v4u*>(own[wave] + dim);
+    const v4u raw = r == kPageSize - 1 ? mine : held[g];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) rows[g][e] = half_at(raw, e);
+  }
   if (kind == 1)
-    finalize_part<false>(a, exact_page, code_page, head, own[wave], lane);
+    pack_part<false>(rows, kPageSize, codes, scales, lane);
   else
-    finalize_part<true>(a, exact_page, code_page, head, own[wave], lane);
+    pack_part<true>(rows, kPageSize, codes + kInt4PartBytes, scales, lane);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }

@@ -25,7 +25,8 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kMaxTile = 8192;
 constexpr int kMinTile = 1024;
-constexpr uint32_t kSeen = 0x80000000u;    // in the history, made or not; low bits: times made
+// a token's count: times made, and whether the history or the biases have it
+constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u;
 constexpr float kNegInf = -__builtin_huge_valf();
 
 struct LogitsArgs {
@@ -63,76 +64,121 @@ struct alignas(sizeof(T) * kVec) Vec {
 };
 
 // Grid (tiles, rows); kVec 1 for rows that are not 16-byte aligned.
+//
+// The tile's logits and the first tokens of the history are requested before
+// anything else, so that the trips to memory overlap (64 x 131072 with
+// histories of 4096: 20.5 us one after the other).
 template <typename T, typename Token, int kVec>
 __global__ __launch_bounds__(kThreads) void shape_logits_kernel(LogitsArgs a) {
+  constexpr int kSteps = kVec > 1 ? kMaxTile / (kThreads * kVec) : 1;
+  constexpr int kBatch = 4;                                    // tokens of a thread in flight
   extern __shared__ uint32_t lds[];
-  uint32_t* counts = lds;                                      // with a history
-  int* bias_at = reinterpret_cast<int*>(lds) + (a.history ? a.tile : 0);   // with biases
+  uint32_t* counts = lds;
+  int* bias_at = reinterpret_cast<int*>(lds) + a.tile;         // of the tokens that have a bias
   const int row = blockIdx.y;
   const int base = blockIdx.x * a.tile;
   const int size = min(a.tile, a.vocab - base);
   const int tid = threadIdx.x;
-  if (a.history)
-    for (int i = tid; i < a.tile; i += kThreads) counts[i] = 0u;
-  if (a.biases)
-    for (int i = tid; i < a.tile; i += kThreads) bias_at[i] = -1;
-  __syncthreads();
-  if (a.history) {
-    const int64_t length = min(static_cast<int64_t>(a.history_lengths[row]), a.history_capacity);
-    const int64_t prompt = a.prompt_lengths ? a.prompt_lengths[row] : 0;
-    const Token* tokens = static_cast<const Token*>(a.history) + row * a.history_stride;
-#pragma unroll 8
-    for (int64_t i = tid; i < length; i += kThreads) {
-      const int64_t at = static_cast<int64_t>(tokens[i]) - base;
-      if (at < 0 || at >= size) continue;
-      if (i >= prompt) atomicAdd(&counts[at], 1u); else atomicOr(&counts[at], kSeen);
+  const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride + base;
+  // the mask's bits of a vector: tiles and vectors are aligned to its words
+  const int32_t* allowed = a.allowed ? a.allowed + row * a.allowed_stride + (base >> 5) : nullptr;
+  auto bits = [&](int i) { return allowed ? static_cast<uint32_t>(allowed[i >> 5]) >> (i & 31) : ~0u; };
+  Vec<T, kVec> held[kSteps];
+  uint32_t words[kSteps];
+  if (kVec > 1 && size >= kVec) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      // a vector past the row's end is read from its start, and not used
+      const int i = (tid + s * kThreads) * kVec, at = i + kVec <= size ? i : 0;
+      held[s] = *reinterpret_cast<const Vec<T, kVec>*>(in + at);
+      words[s] = bits(at);
     }
   }
-  if (a.biases) {
-    const Token* tokens = static_cast<const Token*>(a.bias_tokens) + static_cast<int64_t>(row) * a.biases;
-    for (int i = tid; i < a.biases; i += kThreads) {
-      const int64_t at = static_cast<int64_t>(tokens[i]) - base;
-      if (at >= 0 && at < size) atomicMax(&bias_at[at], i);
-    }
-  }
-  __syncthreads();
   const float repetition = a.repetition ? a.repetition[row] : 1.0f;
   const float frequency = a.frequency ? a.frequency[row] : 0.0f;
   const float presence = a.presence ? a.presence[row] : 0.0f;
-  const float* bias_values = a.bias_values + static_cast<int64_t>(row) * a.biases;
-  const int32_t* allowed = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-  auto shape = [&](float x, int at) {
-    if (a.history) {
-      const uint32_t c = counts[at];
-      if (c) {
-        if (a.repetition) x = x > 0.0f ? x / repetition : x * repetition;
-        const uint32_t made = c & ~kSeen;
-        if (made) {
-          if (a.frequency) x -= frequency * static_cast<float>(made);
-          if (a.presence) x -= presence;
-        }
+  const bool counted = a.history || a.biases;
+  const Token* tokens = static_cast<const Token*>(a.history) + row * a.history_stride;
+  int64_t length = 0, prompt = 0;
+  Token batch[kBatch];
+  auto request_tokens = [&](int64_t first) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int64_t i = first + tid + k * kThreads;
+      batch[k] = tokens[i < length ? i : length - 1];
+    }
+  };
+  if (a.history) {
+    length = max(int64_t{0}, min(static_cast<int64_t>(a.history_lengths[row]), a.history_capacity));
+    if (a.prompt_lengths) prompt = a.prompt_lengths[row];
+    if (length > 0) request_tokens(0);
+  }
+  const Token* bias_tokens = static_cast<const Token*>(a.bias_tokens) + static_cast<int64_t>(row) * a.biases;
+  if (counted) {
+    for (int i = tid; i < a.tile / 4; i += kThreads) reinterpret_cast<uint4*>(counts)[i] = uint4{0u, 0u, 0u, 0u};
+    for (int i = tid; i < a.biases; i += kThreads) {
+      const int64_t at = static_cast<int64_t>(bias_tokens[i]) - base;
+      if (at >= 0 && at < size) bias_at[at] = -1;
+    }
+    __syncthreads();
+    for (int64_t first = 0; first < length; first += kBatch * kThreads) {
+      if (first) request_tokens(first);
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int64_t i = first + tid + k * kThreads;
+        const int64_t at = static_cast<int64_t>(batch[k]) - base;
+        if (i >= length || at < 0 || at >= size) continue;
+        if (i >= prompt) atomicAdd(&counts[at], 1u); else atomicOr(&counts[at], kSeen);
       }
     }
-    if (a.biases) {
-      const int b = bias_at[at];
-      if (b >= 0) x += bias_values[b];
+    for (int i = tid; i < a.biases; i += kThreads) {
+      const int64_t at = static_cast<int64_t>(bias_tokens[i]) - base;
+      if (at < 0 || at >= size) continue;
+      atomicMax(&bias_at[at], i);
+      atomicOr(&counts[at], kBiased);
     }
+    __syncthreads();
+  }
+  const float* bias_values = a.bias_values + static_cast<int64_t>(row) * a.biases;
+  auto shape = [&](float x, uint32_t c, int at) {
+    if (c == 0) return x;
+    const uint32_t made = c & ~(kSeen | kBiased);
+    if (a.repetition && (c & ~kBiased)) x = x > 0.0f ? x / repetition : x * repetition;
+    if (made && a.frequency) x -= frequency * static_cast<float>(made);
+    if (made && a.presence) x -= presence;
+    if (c & kBiased) x += bias_values[bias_at[at]];
     return x;
   };
-  const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride + base;
   T* out = static_cast<T*>(a.out) + row * a.out_stride + base;
-  for (int i = tid * kVec; i < size; i += kThreads * kVec) {
-    // tiles and vectors are aligned to 32-token words of the mask
-    const uint32_t word = allowed ? static_cast<uint32_t>(allowed[(base + i) >> 5]) >> (i & 31) : ~0u;
-    if (kVec > 1 && i + kVec > size) {
-      for (int e = 0; i + e < size; ++e)
-        out[i + e] = word >> e & 1u ? from_float<T>(shape(to_float(in[i + e]), i + e)) : from_float<T>(kNegInf);
+  auto one = [&](int i, uint32_t bit) {
+    out[i] = bit & 1u ? from_float<T>(shape(to_float(in[i]), counted ? counts[i] : 0u, i)) : from_float<T>(kNegInf);
+  };
+  if (kVec == 1) {
+    for (int i = tid; i < size; i += kThreads) one(i, bits(i));
+    return;
+  }
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int i = (tid + s * kThreads) * kVec;
+    if (i >= size) break;
+    if (i + kVec > size) {
+      for (int e = 0; i + e < size; ++e) one(i + e, bits(i + e));
       break;
     }
-    Vec<T, kVec> x = *reinterpret_cast<const Vec<T, kVec>*>(in + i);
+    const uint32_t word = words[s];
+    uint32_t c[kVec];
+#pragma unroll
+    for (int e = 0; e < kVec; e += 4) {
+      const uint4 q = counted ? *reinterpret_cast<const uint4*>(counts + i + e) : uint4{0u, 0u, 0u, 0u};
+      c[e] = q.x;
+      c[e + 1] = q.y;
+      c[e + 2] = q.z;
+      c[e + 3] = q.w;
+    }
+    Vec<T, kVec> x = held[s];
 #pragma unroll
     for (int e = 0; e < kVec; ++e)
-      x.v[e] = word >> e & 1u ? from_float<T>(shape(to_float(x.v[e]), i + e)) : from_float<T>(kNegInf);
+      x.v[e] = word >> e & 1u ? from_float<T>(shape(to_float(x.v[e]), c[e], i + e)) : from_float<T>(kNegInf);
     *reinterpret_cast<Vec<T, kVec>*>(out + i) = x;
   }
 }
@@ -141,7 +187,7 @@ template <typename T, typename Token>
 int32_t launch(const LogitsArgs& a, int batch, bool wide, void* stream) {
   constexpr int kWide = 16 / sizeof(T);
   const dim3 grid((a.vocab + a.tile - 1) / a.tile, batch);
-  const size_t lds = sizeof(uint32_t) * a.tile * ((a.history ? 1 : 0) + (a.biases ? 1 : 0));
+  const size_t lds = sizeof(uint32_t) * a.tile * (a.biases ? 2 : a.history ? 1 : 0);
   if (wide)
     hipLaunchKernelGGL((shape_logits_kernel<T, Token, kWide>), grid, dim3(kThreads), lds, as_stream(stream), a);
   else
