@@ -15,34 +15,38 @@
 #include "pg_int4.h"
 #include "pg_rotary.h"
 
+#include <algorithm>
+
 namespace pg {
 namespace {
 
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr int kWavesPerBlock = 4;
+constexpr int64_t kMaxBlocks = UINT32_MAX / (kWave * kWavesPerBlock);   // of a launch, a dimension
 
 __device__ __forceinline__ uint16_t int4_scale_bits(float maximum) {
   return __half_as_ushort(__float2half_rn(fmaxf(maximum * (1.0f / 7.0f), 0x1p-20f)));
 }
 
-// Code of x / scale, given r = 1 / scale rounded: the quotient is the IEEE one,
-// by three operations instead of a division.  With q0 = RN(x * r), within 2 ulp
-// of it, the residual e = x - q0 * scale is exact (the scale has the 11 bits of an
-// FP16 value, and x lies far from float32's limits), and RN(q0 + e * r) is the
-// quotient with a relative error of 2^-24 of its last bits before it is rounded;
-// a 24-bit number over an 11-bit one is never that near a midpoint of two floats.
-// An infinite scale gives NaN for every x where the division gives 0 or NaN, and
-// both have code 0.
+// Code of x / scale, given r = 1 / scale to an ulp: the quotient is the IEEE one,
+// by three operations instead of a division.  q0 = RN(x * r) is within 3 ulp of
+// it, the residual e = x - q0 * scale is exact (the scale has the 11 bits of an
+// FP16 value, so e has 13; x lies far from float32's limits), and q0 + e * r is
+// the quotient to 2^-20 ulp before it is rounded; a 24-bit number over an 11-bit
+// one is never within 2^-12 ulp of a midpoint of two floats.  An infinite scale
+// gives NaN for every x where the division gives 0 or NaN, and both have code 0.
 //
-// sign(q) floor(|q| + 0.5) is the truncation of q + copysign(0.5, q).  The
-// conversion instruction saturates and takes a NaN to 0 (C++ leaves that open).
+// sign(q) floor(|q| + 0.5) is the truncation of q + copysign(0.5, q).  No clamp
+// is needed: a stored scale is at least (1 - 2^-5) max|x| / 7 (2^-20 is a subnormal
+// FP16 number), so |q| < 7.25.  The conversion instruction takes a NaN to 0 (C++
+// leaves that open).
 __device__ __forceinline__ int int4_code(float x, float scale, float r) {
   const float q0 = x * r;
   const float q = fmaf(fmaf(-q0, scale, x), r, q0);
   int code;
   asm("v_cvt_i32_f32 %0, %1" : "=v"(code) : "v"(q + __builtin_copysignf(0.5f, q)));
-  return max(-7, min(7, code));
+  return code;
 }
 
 // Eight nibbles, code + 8 each, start at 8 8 ... 8; adding a code at its place
@@ -50,6 +54,15 @@ __device__ __forceinline__ int int4_code(float x, float scale, float r) {
 constexpr uint32_t kNibbles8 = 0x88888888u;
 __device__ __forceinline__ uint32_t put_code(uint32_t word, int code, int nibble) {
   return word + (static_cast<uint32_t>(code) << (4 * nibble));
+}
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+// Value e of eight minus center e, rounded to float32: one mixed-precision
+// operation (``one`` is 1, where the compiler does not see it).
+__device__ __forceinline__ float centered_at(const v4u& v, const v4u& c, int e, float one) {
+  return fmaf(static_cast<float>(__builtin_bit_cast(v8h, v)[e]), one,
+              -static_cast<float>(__builtin_bit_cast(v8h, c)[e]));
 }
 
 __device__ __forceinline__ float half_at(const v4u& v, int e) {
@@ -96,7 +109,7 @@ __device__ __forceinline__ void pack_part(const float (&x)[4][8], int visible, u
     m = fmaxf(m, __shfl_xor(m, 16, kWave));
     m = fmaxf(m, __shfl_xor(m, 32, kWave));
     const uint16_t bits = int4_scale_bits(m);
-    const float scale = half_bits_to_float(bits), r = 1.0f / scale;
+    const float scale = half_bits_to_float(bits), r = __builtin_amdgcn_rcpf(scale);
 #pragma unroll
     for (int g = 0; g < 4; ++g)
 #pragma unroll
@@ -110,7 +123,7 @@ __device__ __forceinline__ void pack_part(const float (&x)[4][8], int visible, u
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[t][e]));
       const uint16_t bits = int4_scale_bits(row16_max(m));
-      const float scale = half_bits_to_float(bits), r = 1.0f / scale;
+      const float scale = half_bits_to_float(bits), r = __builtin_amdgcn_rcpf(scale);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         word[e >> 1] = put_code(word[e >> 1], int4_code(x[t][e], scale, r), (t >> 1) + 2 * (e & 1) + 4 * (t & 1));
@@ -158,13 +171,20 @@ __device__ __forceinline__ void quantize_part(const QuantizeArgs& a, int64_t pag
     const int64_t at = min(row, visible - 1) * a.token_stride[kValue] + part_dim<kValue>(g, lane);
     raw[g] = load8<kWide>(source + at);
   }
+  float one = 1.0f;
+  asm("" : "+v"(one));
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const bool in = part_row<kValue>(g, lane) < visible;
     v4u c = {0u, 0u, 0u, 0u};
     if (center) c = load8<kWide>(center + head * kHeadDim + part_dim<kValue>(g, lane));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[g][e] = in ? half_at(raw[g], e) - half_at(c, e) : 0.0f;
+    for (int e = 0; e < 8; ++e) x[g][e] = centered_at(raw[g], c, e, one);
+  }
+  if (visible < kPageSize) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[g][e] = part_row<kValue>(g, lane) < visible ? x[g][e] : 0.0f;
   }
   if (exact_page >= 0 && exact_page < a.num_exact_pages) {
 #pragma unroll
@@ -186,14 +206,14 @@ __device__ __forceinline__ void quantize_part(const QuantizeArgs& a, int64_t pag
                     a.scales + block * kInt4BlockScales, lane);
 }
 
-// Grid (blocks of 4 waves, 2): a wave per (page, head), K and V by blockIdx.y.
+// Grid (pages, blocks of up to 4 heads, 2): a wave per (page, head), K and V by
+// blockIdx.z.
 template <bool kWide>
 __global__ __launch_bounds__(kWave * kWavesPerBlock) void int4_quantize_kernel(QuantizeArgs a) {
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + threadIdx.x / kWave;
-  if (unit >= a.pages * a.heads) return;
-  const int64_t page = unit / a.heads;
-  const int head = static_cast<int>(unit - page * a.heads);
-  if (blockIdx.y == 0)
+  const int64_t page = blockIdx.x;
+  const int head = blockIdx.y * (blockDim.x / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  if (head >= a.heads) return;
+  if (blockIdx.z == 0)
     quantize_part<kWide, false>(a, page, head, threadIdx.x % kWave);
   else
     quantize_part<kWide, true>(a, page, head, threadIdx.x % kWave);
@@ -241,11 +261,10 @@ __device__ __forceinline__ void dequantize_part(const DequantizeArgs& a, int64_t
 
 template <bool kWide>
 __global__ __launch_bounds__(kWave * kWavesPerBlock) void int4_dequantize_kernel(DequantizeArgs a) {
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + threadIdx.x / kWave;
-  if (unit >= a.pages * a.heads) return;
-  const int64_t page = unit / a.heads;
-  const int head = static_cast<int>(unit - page * a.heads);
-  if (blockIdx.y == 0)
+  const int64_t page = blockIdx.x;
+  const int head = blockIdx.y * (blockDim.x / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  if (head >= a.heads) return;
+  if (blockIdx.z == 0)
     dequantize_part<kWide, false>(a, page, head, threadIdx.x % kWave);
   else
     dequantize_part<kWide, true>(a, page, head, threadIdx.x % kWave);
@@ -407,17 +426,17 @@ extern "C" int32_t pg_int4_quantize_pages(const void* key, int64_t key_token_str
   a.num_code_pages = num_code_pages;
   a.num_exact_pages = exact_page_ids ? num_exact_pages : 0;
   a.heads = heads;
-  const int64_t blocks = (a.pages * heads + kWavesPerBlock - 1) / kWavesPerBlock;
-  if (blocks > INT32_MAX) return fail(PG_ERROR_UNSUPPORTED, "too many pages for one call");
+  if (a.pages > kMaxBlocks) return fail(PG_ERROR_UNSUPPORTED, "too many pages for one call");
   bool wide = key_token_stride % 8 == 0 && value_token_stride % 8 == 0;
   for (const void* p : {key, value, key_center, value_center,
                         static_cast<const void*>(exact_key_pages), static_cast<const void*>(exact_value_pages)})
     wide = wide && aligned16(p);
-  const dim3 grid(static_cast<uint32_t>(blocks), 2);
+  const int waves = std::min(heads, kWavesPerBlock);
+  const dim3 grid(static_cast<uint32_t>(a.pages), (heads + waves - 1) / waves, 2);
   if (wide)
-    hipLaunchKernelGGL(int4_quantize_kernel<true>, grid, dim3(kWave * kWavesPerBlock), 0, as_stream(stream), a);
+    hipLaunchKernelGGL(int4_quantize_kernel<true>, grid, dim3(kWave * waves), 0, as_stream(stream), a);
   else
-    hipLaunchKernelGGL(int4_quantize_kernel<false>, grid, dim3(kWave * kWavesPerBlock), 0, as_stream(stream), a);
+    hipLaunchKernelGGL(int4_quantize_kernel<false>, grid, dim3(kWave * waves), 0, as_stream(stream), a);
   return check_launch("int4_quantize_pages");
 }
 
@@ -449,16 +468,16 @@ extern "C" int32_t pg_int4_dequantize_pages(const void* codes, const void* scale
   a.pages = (tokens - 1) / kPageSize + 1;
   a.num_code_pages = num_code_pages;
   a.heads = heads;
-  const int64_t blocks = (a.pages * heads + kWavesPerBlock - 1) / kWavesPerBlock;
-  if (blocks > INT32_MAX) return fail(PG_ERROR_UNSUPPORTED, "too many pages for one call");
+  if (a.pages > kMaxBlocks) return fail(PG_ERROR_UNSUPPORTED, "too many pages for one call");
   bool wide = key_token_stride % 8 == 0 && value_token_stride % 8 == 0;
   for (const void* p : {key_center, value_center, static_cast<const void*>(key), static_cast<const void*>(value)})
     wide = wide && aligned16(p);
-  const dim3 grid(static_cast<uint32_t>(blocks), 2);
+  const int waves = std::min(heads, kWavesPerBlock);
+  const dim3 grid(static_cast<uint32_t>(a.pages), (heads + waves - 1) / waves, 2);
   if (wide)
-    hipLaunchKernelGGL(int4_dequantize_kernel<true>, grid, dim3(kWave * kWavesPerBlock), 0, as_stream(stream), a);
+    hipLaunchKernelGGL(int4_dequantize_kernel<true>, grid, dim3(kWave * waves), 0, as_stream(stream), a);
   else
-    hipLaunchKernelGGL(int4_dequantize_kernel<false>, grid, dim3(kWave * kWavesPerBlock), 0, as_stream(stream), a);
+    hipLaunchKernelGGL(int4_dequantize_kernel<false>, grid, dim3(kWave * waves), 0, as_stream(stream), a);
   return check_launch("int4_dequantize_pages");
 }
 
@@ -483,6 +502,7 @@ extern "C" int32_t pg_int4_rope_append(
     return fail(PG_ERROR_INVALID_ARGUMENT, "the rotated part must be an even number of a head's dims");
   const int64_t row_blocks = (static_cast<int64_t>(query_heads) + 2 * kv_heads + kWavesPerBlock - 1) / kWavesPerBlock;
   if (row_blocks > 65535) return fail(PG_ERROR_UNSUPPORTED, "too many heads for one call");
+  if (batch_size > kMaxBlocks) return fail(PG_ERROR_UNSUPPORTED, "too many requests for one call");
   if (batch_size == 0) return PG_OK;
   AppendArgs a{};
   a.rows[0] = static_cast<const uint16_t*>(query);

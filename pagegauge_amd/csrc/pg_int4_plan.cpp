@@ -96,7 +96,7 @@ int32_t build_int4_plan(const int32_t* host_indptr, const int32_t* host_tail_ind
     }
     most = std::max(most, cuts);
   }
-  if (items.size() > INT32_MAX / 2) return fail(PG_ERROR_UNSUPPORTED, "too many work items");
+  if (items.size() > UINT32_MAX / (kInt4Waves * 64)) return fail(PG_ERROR_UNSUPPORTED, "too many work items");
   item_ptr[batch_size] = static_cast<int32_t>(items.size());
   p = pg_int4_plan_t{};
   p.batch_size = batch_size;

@@ -123,7 +123,7 @@ int32_t dispatch(RotaryArgs a, int vec, int head_dim, bool interleaved, void* st
   const bool copies = a.rows[0].in != a.rows[0].out || (a.rows[1].heads && a.rows[1].in != a.rows[1].out);
   a.units = a.turned_units + (copies ? (head_dim - a.rotary_dim) / (2 * vec) : 0);
   const int64_t blocks = (a.tokens * a.units + kThreads - 1) / kThreads;
-  if (blocks > INT32_MAX) return fail(PG_ERROR_UNSUPPORTED, "too many rows for one rotation");
+  if (blocks > UINT32_MAX / kThreads) return fail(PG_ERROR_UNSUPPORTED, "too many rows for one rotation");
   const int heads = a.rows[0].heads + a.rows[1].heads;
   // few tokens: the heads of a token over several workgroups
   int slices = static_cast<int>(std::min<int64_t>(heads, std::max<int64_t>(1, 2048 / blocks)));
