@@ -19,10 +19,11 @@
 //    one of about 22 bits.
 //  * A nibble u = code + 8 masked out of its dword is the FP16 subnormal
 //    u * 2^-24, or 16 u * 2^-24 one nibble further up, and MFMAs multiply
-//    subnormals exactly: 5 operations make 8 operands.  The offset of 8 comes off
-//    the products: of K as the accumulators' start, -8 sum(q), of V as one more
-//    column of the product, against 8s.  The scales multiply scores and
-//    probabilities in float32.
+//    subnormals exactly: 5 operations make 8 operands of V.  Its offset of 8 comes
+//    off the product, as one more column against 8s.  K's comes off the operands,
+//    4 operations more: off its product it costs the scores two bits (lse 1e-6 off
+//    instead of 3e-7, for 15.5 us against 16.6 at 49K tokens).  The scales
+//    multiply scores and probabilities in float32.
 //  * The softmax's base follows the running maximum lazily: it moves when a
 //    score passes it by 2^4, so most groups of pages need no exchange at all.
 //
@@ -75,10 +76,6 @@ __device__ __forceinline__ v2h as_half2(uint32_t bits) { return __builtin_bit_ca
 
 __device__ __forceinline__ v2s as_short2(uint32_t bits) { return __builtin_bit_cast(v2s, bits); }
 
-__device__ __forceinline__ v2h splat(float x) {
-  return v2h{static_cast<_Float16>(x), static_cast<_Float16>(x)};
-}
-
 __device__ __forceinline__ v8h operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __builtin_bit_cast(v8h, v4u{a, b, c, d});
 }
@@ -87,6 +84,14 @@ __device__ __forceinline__ v8h operand(uint32_t a, uint32_t b, uint32_t c, uint3
 __device__ __forceinline__ uint32_t even(uint32_t word) { return word & 0x000f000fu; }
 __device__ __forceinline__ uint32_t odd(uint32_t word) { return word & 0x00f000f0u; }
 constexpr uint32_t kEvenEights = 0x00080008u, kOddEights = 0x00800080u;     // u = 8
+
+// The same of codes, u - 8: exact, as all of it is a multiple of 2^-24.
+__device__ __forceinline__ uint32_t even_codes(uint32_t word) {
+  return __builtin_bit_cast(uint32_t, as_half2(even(word)) - as_half2(kEvenEights));
+}
+__device__ __forceinline__ uint32_t odd_codes(uint32_t word) {
+  return __builtin_bit_cast(uint32_t, as_half2(odd(word)) - as_half2(kOddEights));
+}
 
 // x times one half of ``pair``: one mixed-precision operation, no conversion.
 __device__ __forceinline__ float times_half(float x, uint32_t pair, int which) {
@@ -261,25 +266,14 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
     for (int g = 0; g < 4; ++g)
       raw[g] = *reinterpret_cast<const v2u*>(scale_bytes + (my_block >> 5) + 16 * g + 8);
     take_query();
-    // q against the even and the odd nibbles of two dwords, and the products'
-    // start, -8 sum(q) over the same dims of all four lanes of the head
+    // q against the even and the odd nibbles of two dwords
     v8h q_even[2], q_odd[2];
-    float start_even = 0.0f, start_odd = 0.0f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const v4u x = __builtin_bit_cast(v4u, q[2 * h]), y = __builtin_bit_cast(v4u, q[2 * h + 1]);
       q_even[h] = operand(x[0], x[2], y[0], y[2]);
       q_odd[h] = operand(x[1], x[3], y[1], y[3]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        start_even = __builtin_amdgcn_fdot2(as_half2(e < 2 ? x[2 * e] : y[2 * e - 4]), splat(1.0f), start_even, false);
-        start_odd = __builtin_amdgcn_fdot2(as_half2(e < 2 ? x[2 * e + 1] : y[2 * e - 3]), splat(1.0f), start_odd, false);
-      }
     }
-    start_even += __shfl_xor(start_even, 16, kWave);
-    start_odd += __shfl_xor(start_odd, 16, kWave);
-    start_even = (start_even + __shfl_xor(start_even, 32, kWave)) * -0x1p-21f;
-    start_odd = (start_odd + __shfl_xor(start_odd, 32, kWave)) * -0x1p-17f;
     {
       // positive FP16 values order as their bits do
       if (whole < count) {
@@ -308,15 +302,15 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
       for (int i = 0; i < kInt4GroupPages; ++i) {
         consume_point(cur.k[i]);
         consume_point(cur.s[i]);
-        v4f dot_even = {start_even, start_even, start_even, start_even};
-        v4f dot_odd = {start_odd, start_odd, start_odd, start_odd};
+        v4f dot_even = {0.0f, 0.0f, 0.0f, 0.0f};
+        v4f dot_odd = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t x = cur.k[i][2 * h], y = cur.k[i][2 * h + 1];
           dot_even = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              operand(even(x), even(x >> 8), even(y), even(y >> 8)), q_even[h], dot_even, 0, 0, 0);
+              operand(even_codes(x), even_codes(x >> 8), even_codes(y), even_codes(y >> 8)), q_even[h], dot_even, 0, 0, 0);
           dot_odd = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              operand(odd(x), odd(x >> 8), odd(y), odd(y >> 8)), q_odd[h], dot_odd, 0, 0, 0);
+              operand(odd_codes(x), odd_codes(x >> 8), odd_codes(y), odd_codes(y >> 8)), q_odd[h], dot_odd, 0, 0, 0);
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r)
