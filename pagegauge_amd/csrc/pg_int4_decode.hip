@@ -7,9 +7,9 @@
 // center shifts all of a request's scores alike and is left out.
 //
 // A workgroup takes one KV head, up to 8 of its query heads and a range of
-// pages; its 8 waves take groups of 4 pages in turn and meet in LDS once, at the
-// end.  Everything else stays in registers, with no exchange between lanes but
-// two steps of the running maximum:
+// pages; its 4 waves take groups of 4 pages in turn and meet in LDS once, at the
+// end.  Everything else stays in registers, with hardly an exchange between
+// lanes:
 //  * QK as K Q^T: tokens are the MFMA's rows, heads its columns, so lane (kg, n)
 //    gets the scores of tokens 4 kg .. 4 kg + 3 for head n % 8.
 //  * These are, pair of pages by pair, exactly the k slots that the lane feeds
@@ -30,6 +30,16 @@
 // Probabilities times V's scales are carried relative to a power of two that
 // puts the largest of the wave's scales near 2^10 (2^14 with the base's slack), so
 // that two FP16 parts hold them to 2^-34 of the largest.
+//
+// Bound by HBM once a wave has several groups, by a chain of trips to memory
+// (work item, page ids, pages, partial rows) before.  Kernel times on MI355X, and
+// of the same walk without its arithmetic: 256 requests (829 MB) 169 and 165 us,
+// 8 requests of 4K to 32K (164 MB) 34 and 32, one of 49K tokens (53 MB) 14.8 and
+// 12.3, of 4K (5 MB) 5.5 and 4.6; a join adds 2.3 to 4.6 us.  Measured and not
+// taken: 8 waves a workgroup (one fits a CU, and nothing covers its start and
+// end: 256 requests 191 us), and a join by the workgroup that ends last (49K
+// tokens 18.7 us a call against 17.2 with the second launch, before the last
+// steps: counting across XCDs costs what the launch does).
 #include "pg_int4.h"
 #include "pg_int4_plan.h"
 
@@ -436,7 +446,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
     }
   }
 
-  // ---- the waves meet: rows r and r + 8 of the product, then 8 partial states
+  // ---- the waves meet: rows r and r + 8 of the product, then 4 partial states
   float l_sum = st.l0 + st.l1;
   l_sum += __shfl_xor(l_sum, 16, kWave);
   l_sum += __shfl_xor(l_sum, 32, kWave);
@@ -463,42 +473,42 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
   __syncthreads();
   // wave w finishes heads w, w + 4, two dims per lane
   for (int h = wave; h < heads; h += kInt4Waves) {
-  float m = kNegInf;
+    float m = kNegInf;
 #pragma unroll
-  for (int w = 0; w < kInt4Waves; ++w) m = fmaxf(m, part_m[w][h]);
-  const float base = m == kNegInf ? 0.0f : m;
-  float l = 0.0f;
-  float2 o = make_float2(0.0f, 0.0f);
+    for (int w = 0; w < kInt4Waves; ++w) m = fmaxf(m, part_m[w][h]);
+    const float base = m == kNegInf ? 0.0f : m;
+    float l = 0.0f;
+    float2 o = make_float2(0.0f, 0.0f);
 #pragma unroll
-  for (int w = 0; w < kInt4Waves; ++w) {
-    const float f = __builtin_amdgcn_exp2f(part_m[w][h] - base);
-    const float2 x = make_float2(part_o[w][h][lane], part_o[w][h][64 + lane]);
-    l += f * part_l[w][h];
-    o.x += f * x.x;
-    o.y += f * x.y;
-  }
-  const int head = kv * a.group + first_head + h;
-  if (it.items_in_request > 1) {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * a.num_qo_heads + head;
-    *reinterpret_cast<float2*>(a.partial_o + row * kHeadDim + 2 * lane) = o;
-    if (lane == 0) {
-      a.partial_m[row] = m;
-      a.partial_l[row] = l;
+    for (int w = 0; w < kInt4Waves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(part_m[w][h] - base);
+      const float2 x = make_float2(part_o[w][h][lane], part_o[w][h][64 + lane]);
+      l += f * part_l[w][h];
+      o.x += f * x.x;
+      o.y += f * x.y;
     }
-    continue;
-  }
-  const int64_t row = static_cast<int64_t>(it.request) * a.num_qo_heads + head;
-  float2 c = make_float2(0.0f, 0.0f);
-  if (a.value_center) {
-    const uint32_t bits = *reinterpret_cast<const uint32_t*>(
-        a.value_center + it.request * a.center_batch_stride + kv * kHeadDim + 2 * lane);
-    c = make_float2(half_bits_to_float(static_cast<uint16_t>(bits)),
-                    half_bits_to_float(static_cast<uint16_t>(bits >> 16)));
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;      // no token: the center alone
-  *reinterpret_cast<__half2*>(a.out + row * kHeadDim + 2 * lane) =
-      __floats2half2_rn(o.x * inv + c.x, o.y * inv + c.y);
-  if (lane == 0 && a.lse) a.lse[row] = l == 0.0f ? kNegInf : log2f(l) + m;
+    const int head = kv * a.group + first_head + h;
+    if (it.items_in_request > 1) {
+      const int64_t row = static_cast<int64_t>(blockIdx.x) * a.num_qo_heads + head;
+      *reinterpret_cast<float2*>(a.partial_o + row * kHeadDim + 2 * lane) = o;
+      if (lane == 0) {
+        a.partial_m[row] = m;
+        a.partial_l[row] = l;
+      }
+      continue;
+    }
+    const int64_t row = static_cast<int64_t>(it.request) * a.num_qo_heads + head;
+    float2 c = make_float2(0.0f, 0.0f);
+    if (a.value_center) {
+      const uint32_t bits = *reinterpret_cast<const uint32_t*>(
+          a.value_center + it.request * a.center_batch_stride + kv * kHeadDim + 2 * lane);
+      c = make_float2(half_bits_to_float(static_cast<uint16_t>(bits)),
+                      half_bits_to_float(static_cast<uint16_t>(bits >> 16)));
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;      // no token: the center alone
+    *reinterpret_cast<__half2*>(a.out + row * kHeadDim + 2 * lane) =
+        __floats2half2_rn(o.x * inv + c.x, o.y * inv + c.y);
+    if (lane == 0 && a.lse) a.lse[row] = l == 0.0f ? kNegInf : log2f(l) + m;
   }
 }
 
@@ -656,8 +666,16 @@ extern "C" int32_t pg_int4_decode_run(const pg_int4_plan_t* plan, const void* qu
     return fail(PG_ERROR_INVALID_ARGUMENT, "history segment tensors missing");
   if (plan->has_tail && (!tail_k || !tail_v || !tail_indices || !tail_last_len))
     return fail(PG_ERROR_INVALID_ARGUMENT, "tail segment tensors missing");
-  if (!(sm_scale > 0.0f) || !__builtin_isfinite(sm_scale))
-    return fail(PG_ERROR_INVALID_ARGUMENT, "sm_scale must be positive and finite");
+  // the kernel multiplies it by 2^20 log2(e)
+  if (!(sm_scale > 0.0f) || !(sm_scale < 0x1p100f))
+    return fail(PG_ERROR_INVALID_ARGUMENT, "sm_scale must be positive and below 2^100");
+  for (const void* p : {query, codes, scales, tail_k, tail_v})
+    if (reinterpret_cast<uintptr_t>(p) % 16)
+      return fail(PG_ERROR_INVALID_ARGUMENT, "queries and pages must be 16-byte aligned");
+  if (query_batch_stride % 8) return fail(PG_ERROR_INVALID_ARGUMENT, "query rows must be 16-byte aligned");
+  for (const void* p : {value_center, static_cast<const void*>(out)})
+    if (reinterpret_cast<uintptr_t>(p) % 4)
+      return fail(PG_ERROR_INVALID_ARGUMENT, "centers and outputs must be 4-byte aligned");
   if (plan->num_items <= 0 || plan->batch_size <= 0 || plan->num_kv_heads <= 0 ||
       plan->num_qo_heads % plan->num_kv_heads || plan->num_qo_heads / plan->num_kv_heads > 16)
     return fail(PG_ERROR_INVALID_ARGUMENT, "the plan is not one of pg_int4_plan");

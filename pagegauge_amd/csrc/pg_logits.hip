@@ -224,6 +224,7 @@ extern "C" int32_t pg_shape_logits(const void* logits, int64_t logits_stride, vo
     return fail(PG_ERROR_INVALID_ARGUMENT, "logits must be FP16, BF16 or FP32");
   if (history && (!history_lengths || history_capacity < 0))
     return fail(PG_ERROR_INVALID_ARGUMENT, "a history needs its lengths");
+  if (history_capacity >= 1 << 30) return fail(PG_ERROR_UNSUPPORTED, "histories must be shorter than 2^30 tokens");
   if (!history && (repetition || frequency || presence))
     return fail(PG_ERROR_INVALID_ARGUMENT, "penalties need a history");
   if (biases < 0 || (biases && (!bias_tokens || !bias_values)))

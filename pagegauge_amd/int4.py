@@ -93,6 +93,12 @@ def _check_exact(pages: torch.Tensor, heads: int, what: str) -> int:
     return pages.shape[0]
 
 
+def _check_last(indptr: torch.Tensor, last: torch.Tensor, what: str) -> None:
+    """The last length of every request with pages lies in [1, 16] (host tensors)."""
+    if bool(((indptr[1:] > indptr[:-1]) & ((last < 1) | (last > PAGE))).any()):
+        raise ValueError(f"{what} must lie in [1, {PAGE}]")
+
+
 def quantize_pages(key: torch.Tensor, value: torch.Tensor, codes: torch.Tensor,
                    scales: torch.Tensor, *, page_ids: Optional[torch.Tensor] = None,
                    key_center: Optional[torch.Tensor] = None,
@@ -107,7 +113,8 @@ def quantize_pages(key: torch.Tensor, value: torch.Tensor, codes: torch.Tensor,
     0.  With ``exact_page_ids`` those pages are also stored, centered and
     rounded to FP16, in pages ``exact_page_ids[i]`` of ``exact_key`` and
     ``exact_value`` [pages, 16, Hkv, 128].  Ids outside their pool (-1) skip
-    the store.  Rows may be strided by token."""
+    the store; the others must differ from each other.  Rows may be strided
+    by token."""
     if key.shape != value.shape:
         raise ValueError("token-major K/V must have identical [T,Hkv,128] shapes")
     key_stride, value_stride = _token_rows(key, "K"), _token_rows(value, "V")
@@ -275,18 +282,21 @@ class Int4PagedDecode:
         """CSR page tables of the history and, with ``tail_indptr``, of the
         exact pages; either may be empty for a request.  ``indices`` and the
         last lengths (device int32) must stay alive until the next ``plan``
-        and are re-read by every run.  Waits for the GPU."""
+        and are re-read by every run (lengths within [0, 16] may move), so a
+        captured run stays valid until the next ``plan``.  Waits for the GPU."""
         if (tail_indptr is None) != (tail_indices is None) or (tail_indptr is None) != (
                 tail_last_page_len is None):
             raise ValueError("tail indptr, indices and last_page_len go together")
         _check_index(indices, "indices")
         _check_index(last_page_len, "last_page_len")
-        host, _ = _host_tables(indptr, last_page_len, indices)
+        host, last = _host_tables(indptr, last_page_len, indices)
+        _check_last(host, last, "last_page_len")
         tail = tail_range = None
         if tail_indptr is not None:
             _check_index(tail_indices, "tail_indices")
             _check_index(tail_last_page_len, "tail_last_page_len")
-            tail, _ = _host_tables(tail_indptr, tail_last_page_len, tail_indices, "tail")
+            tail, last = _host_tables(tail_indptr, tail_last_page_len, tail_indices, "tail")
+            _check_last(tail, last, "tail_last_page_len")
             if tail.numel() != host.numel():
                 raise ValueError("history and tail page tables must cover the same batch")
             tail_range = _page_id_range(tail_indices, tail)

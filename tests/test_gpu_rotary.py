@@ -128,3 +128,25 @@ def test_infinities_stay_in_their_pair(cuda):
     bad = ~torch.isfinite(got)
     assert bad[0, 0].nonzero().flatten().tolist() == [3, 35]
     assert bad[1, 0].nonzero().flatten().tolist() == [100]
+
+
+def test_negative_positions_and_missing_heads(cuda):
+    """Positions below zero turn back; a call without query heads turns the keys."""
+    from pagegauge_amd import rotary
+
+    emb = rotary.RotaryEmbedding(128, 96, layout="interleaved")
+    f = rotary.frequencies(96, 1.0e6)
+    x = _rows(cuda, torch.float32, 3, 2, 128, 6)
+    positions = torch.tensor([-1, -70000, -2 ** 40], device=cuda)
+    _check(emb, f, x, positions, emb.rotate(x, None, positions)[0])
+    none, got = emb.rotate(x[:, :0], x, positions)
+    assert none.shape == (3, 0, 128)
+    assert torch.equal(got, emb.rotate(x, None, positions)[0])
+
+
+def test_tensors_of_another_device_are_refused(cuda):
+    from pagegauge_amd import rotary
+
+    x = _rows(cuda, torch.float16, 1, 1, 128, 1)
+    with pytest.raises(ValueError, match="current CUDA device"):
+        rotary.RotaryEmbedding(128).rotate(x, None, torch.zeros(1, dtype=torch.int32))

@@ -198,3 +198,32 @@ def test_decode_refuses_memory_of_the_host():
 def test_c_entry_points_refuse(name, args, code, message):
     rc = getattr(_capi.library(), name)(*args)
     assert rc == code and message in _capi.last_error()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="host-only checks of the C entry points")
+@pytest.mark.parametrize("over,message", [
+    (dict(query=None), "null run argument"), (dict(codes=None), "history segment"),
+    (dict(tail_k=None), "tail segment"), (dict(sm_scale=0.0), "sm_scale"),
+    (dict(sm_scale=float("inf")), "sm_scale"), (dict(sm_scale=float("nan")), "sm_scale"),
+    (dict(query=4104), "16-byte aligned"), (dict(scales=4100), "16-byte aligned"),
+    (dict(stride=4), "16-byte aligned"), (dict(center=4098), "4-byte aligned"),
+    (dict(heads=0), "not one of")])
+def test_decode_run_refuses(over, message):
+    plan, _, _ = int4.plan_work_items([0, 40], [0, 16])
+    a = dict(query=4096, stride=4096, codes=4096, scales=4096, indices=4096, last=4096, tail_k=4096,
+             tail_v=4096, tail_indices=4096, tail_last=4096, center=None, center_stride=0, out=4096,
+             lse=None, sm_scale=0.1, workspace=4096, stream=None)
+    a.update(over)
+    if "heads" in a:
+        plan.num_kv_heads = a.pop("heads")
+    a["sm_scale"] = ctypes.c_float(a["sm_scale"])
+    rc = _capi.library().pg_int4_decode_run(ctypes.byref(plan), *a.values())
+    assert rc == 1 and message in _capi.last_error()
+
+
+def test_last_lengths_are_checked_where_there_are_pages():
+    indptr = torch.tensor([0, 2, 2, 3])
+    int4._check_last(indptr, torch.tensor([16, 99, 1]), "last")
+    for bad in ([0, 1, 1], [17, 1, 1], [1, 1, -1]):
+        with pytest.raises(ValueError, match="last must lie"):
+            int4._check_last(indptr, torch.tensor(bad), "last")

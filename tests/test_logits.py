@@ -45,7 +45,7 @@ def test_refusals(logits, over, message):
     (dict(logits=None), 1, "null tensor"), (dict(vocab=0), 1, "must be positive"),
     (dict(batch=70000), 3, "65535 rows"), (dict(dtype=3), 1, "FP16, BF16 or FP32"),
     (dict(history=4096), 1, "lengths"), (dict(presence=4096), 1, "need a history"),
-    (dict(biases=1), 1, "go together"),
+    (dict(biases=1), 1, "go together"), (dict(history=4096, lengths=4096, capacity=1 << 30), 3, "2^30"),
     (dict(biases=1, bias_tokens=4096, bias_values=4096, token_bytes=2), 1, "int32 or int64")])
 def test_c_entry_point_refuses(over, code, message):
     a = dict(logits=4096, logits_stride=32, out=4096, out_stride=32, dtype=2, batch=1, vocab=32,
