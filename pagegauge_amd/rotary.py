@@ -16,7 +16,8 @@ was trained on:
   pairs between, and both rows scaled by ``0.1 ln(factor) + 1`` (unless
   ``attention_factor`` is given).
 
-The angles are worked out in the kernel, so nothing grows with the context;
+The angles are worked out in the kernel, so nothing grows with the context; they
+are good to 2^-22 of a turn at position 2^31 (and to 2^-51 of themselves beyond);
 ``int4.rope_append`` uses the same object.
 """
 

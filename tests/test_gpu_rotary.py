@@ -27,7 +27,10 @@ def _check(emb, frequencies, x, positions, got):
     """Half a rounding of the row's type; the angle is reduced in 64 bits and
     rounded once (2^-25 of a turn, 2 pi 2^-25 < 2^-22), its sine and cosine are
     within 2^-22 and the products and sum round three times (2^-24 each): below
-    2^-20 of the pair's absolute sum.  2^-25 is half a subnormal step of FP16."""
+    2^-20 of the pair's absolute sum.  The angle itself, in radians, is off by
+    2^-51 of its size: revolutions per position round twice (f / 2 pi), their
+    product with the position once, and the angle here once, 2^-53 each.  2^-25
+    is half a subnormal step of FP16."""
     x, positions, got = x.cpu(), positions.cpu(), got.cpu().double()
     want = _turned(emb, frequencies, x, positions)
     r = emb.rotary_dim
@@ -39,8 +42,14 @@ def _check(emb, frequencies, x, positions, got):
     else:
         both = size[..., 0:r:2] + size[..., 1:r:2]
         pair[..., 0:r:2], pair[..., 1:r:2] = both, both
+    angle = torch.zeros_like(size)
+    turned = (positions.double().abs()[:, None] * frequencies)[:, None, :].expand(*size.shape[:2], r // 2)
+    if emb.layout == "half":
+        angle[..., :r // 2], angle[..., r // 2:r] = turned, turned
+    else:
+        angle[..., 0:r:2], angle[..., 1:r:2] = turned, turned
     eps = torch.finfo(x.dtype).eps
-    allowed = want.abs() * eps / 2 * (1 + eps) + pair * abs(emb.amplitude) * 2.0 ** -20 + (
+    allowed = pair * abs(emb.amplitude) * angle * 2.0 ** -51 + want.abs() * eps / 2 * (1 + eps) + pair * abs(emb.amplitude) * 2.0 ** -20 + (
         2.0 ** -25 if x.dtype == torch.float16 else 0.0)
     assert ((got - want).abs() <= allowed).all()
     assert torch.equal(got[..., r:], x[..., r:].double())
