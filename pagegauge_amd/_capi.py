@@ -183,6 +183,8 @@ TRACE_PROTOTYPES = {
     "pg_trace_set_buffer": (_i32, [_p, _i64]),
 }
 
+DEVICE_ERROR = "all tensors must be on the current CUDA device"
+
 _lock = threading.Lock()
 _library = None
 _bench_library = None
@@ -248,17 +250,34 @@ def current_stream() -> int:
 
 def require_current_device(*tensors) -> None:
     """ValueError unless every tensor (None aside) is on the current CUDA
-    device, on whose current stream the kernels are launched."""
+    device."""
     device = None
     for t in tensors:
         if t is not None:
             at = t.get_device()
             if device is None:
                 device = at
-            if at != device or at < 0:
-                raise ValueError("all tensors must be on the current CUDA device")
-    if device is not None and device != torch._C._cuda_getDevice():
-        raise ValueError("all tensors must be on the current CUDA device")
+            if at != device:
+                raise ValueError(DEVICE_ERROR)
+    if device is not None:
+        check_device(device)
+
+
+def pointer(t: torch.Tensor, dtype, shape: tuple, device: int, what: str) -> int:
+    """Address of a contiguous tensor of this type, shape and device; ``what``
+    is the ValueError of another one."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(what)
+    if t.get_device() != device:
+        raise ValueError(DEVICE_ERROR)
+    return t.data_ptr()
+
+
+def check_device(device: int) -> None:
+    """ValueError unless ``device``, where a call's tensors are, is the current
+    CUDA device, on whose current stream the kernels are launched."""
+    if device < 0 or device != torch._C._cuda_getDevice():
+        raise ValueError(DEVICE_ERROR)
 
 
 def last_error() -> str:

@@ -31,14 +31,24 @@ from typing import Optional
 import torch
 
 from . import _capi
-from .decode import (_check_cache, _check_index, _check_page_ids, _check_query, _host_i32,
-                     _host_tables, _num_cus, _page_id_range)
+from .decode import (_check_index, _check_page_ids, _check_query, _host_i32, _host_tables, _num_cus,
+                     _page_id_range)
 from .rotary import RotaryEmbedding
 
 DIM = 128
 PAGE = 16
 BLOCK_SHAPE = (2, 1024)
 SCALE_SHAPE = (4, 2, 4)
+
+# what the checks below say
+_CODES = "4-bit codes must be contiguous uint8 [pages,Hkv,2,1024]"
+_SCALES = "4-bit scales must be contiguous float16 [pages,Hkv,4,2,4]"
+_CENTERS = "centers must be contiguous float16, [Hkv,128] of each request"
+_EXACT_KEY = "exact_key must be contiguous float16 [pages,16,Hkv,128]"
+_EXACT_VALUE = "exact_value must be contiguous float16 [pages,16,Hkv,128]"
+_PAGE_IDS = "page_ids must be contiguous int32, one per page"
+_EXACT_IDS = "exact_page_ids must be contiguous int32, one per page or request"
+_CODE_IDS = "code_page_ids must be contiguous int32, one per request"
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -51,20 +61,17 @@ def allocate_pages(pages: int, kv_heads: int, device="cuda") -> tuple[torch.Tens
             torch.zeros(pages, kv_heads, *SCALE_SHAPE, device=device, dtype=torch.float16))
 
 
-def _check_pool(codes: torch.Tensor, scales: torch.Tensor, heads: int) -> int:
-    shape = codes.shape
-    if codes.dtype is not torch.uint8 or len(shape) != 4 or shape[1] != heads \
-            or shape[2:] != BLOCK_SHAPE or not codes.is_contiguous():
-        raise ValueError(f"4-bit codes must be contiguous uint8 [pages,{heads},2,1024]")
-    if scales.dtype is not torch.float16 or scales.shape != (shape[0], heads, 4, 2, 4) \
-            or not scales.is_contiguous():
-        raise ValueError(f"4-bit scales must be contiguous float16 [{shape[0]},{heads},4,2,4]")
-    return shape[0]
+def _pool(codes: torch.Tensor, scales: torch.Tensor, heads: int, device: int) -> tuple[int, int, int]:
+    """(pages, codes' address, scales' address) of a pool."""
+    if codes.dim() != 4:
+        raise ValueError(_CODES)
+    pages = codes.shape[0]
+    return (pages, _capi.pointer(codes, torch.uint8, (pages, heads, 2, 1024), device, _CODES),
+            _capi.pointer(scales, torch.float16, (pages, heads, 4, 2, 4), device, _SCALES))
 
 
-def _check_ids(ids: Optional[torch.Tensor], count: int, what: str) -> None:
-    if ids is not None and (ids.dtype != torch.int32 or ids.shape != (count,) or not ids.is_contiguous()):
-        raise ValueError(f"{what} must be contiguous int32 [{count}]")
+def _ids(ids: Optional[torch.Tensor], count: int, device: int, what: str) -> Optional[int]:
+    return None if ids is None else _capi.pointer(ids, torch.int32, (count,), device, what)
 
 
 def _token_rows(t: torch.Tensor, what: str) -> int:
@@ -77,20 +84,21 @@ def _token_rows(t: torch.Tensor, what: str) -> int:
     raise ValueError(f"{what} must be float16 [T,Hkv,128] rows of dense heads")
 
 
-def _check_centers(key_center, value_center, shape: tuple) -> None:
-    if (key_center is None) != (value_center is None):
+def _centers(key_center, value_center, shape: tuple, device: int):
+    if key_center is None and value_center is None:
+        return None, None
+    if key_center is None or value_center is None:
         raise ValueError("key and value centers go together")
-    for c in (key_center, value_center):
-        if c is not None and (c.dtype != torch.float16 or tuple(c.shape) != shape
-                              or not c.is_contiguous()):
-            raise ValueError(f"centers must be contiguous float16 {list(shape)}")
+    return (_capi.pointer(key_center, torch.float16, shape, device, _CENTERS),
+            _capi.pointer(value_center, torch.float16, shape, device, _CENTERS))
 
 
-def _check_exact(pages: torch.Tensor, heads: int, what: str) -> int:
-    if pages.dtype != torch.float16 or pages.dim() != 4 or pages.shape[1:] != (PAGE, heads, DIM) \
-            or not pages.is_contiguous():
-        raise ValueError(f"{what} must be contiguous float16 [pages,16,{heads},128]")
-    return pages.shape[0]
+def _exact(pages: torch.Tensor, heads: int, device: int, what: str) -> tuple[int, int]:
+    """(pages, address) of exact FP16 pages."""
+    if pages.dim() != 4:
+        raise ValueError(what)
+    count = pages.shape[0]
+    return count, _capi.pointer(pages, torch.float16, (count, PAGE, heads, DIM), device, what)
 
 
 def _check_last(indptr: torch.Tensor, last: torch.Tensor, what: str) -> None:
@@ -118,32 +126,32 @@ def quantize_pages(key: torch.Tensor, value: torch.Tensor, codes: torch.Tensor,
     if key.shape != value.shape:
         raise ValueError("token-major K/V must have identical [T,Hkv,128] shapes")
     key_stride, value_stride = _token_rows(key, "K"), _token_rows(value, "V")
-    tokens, heads = key.shape[0], key.shape[1]
+    tokens, heads, _ = key.shape
     pages = (tokens + PAGE - 1) // PAGE
-    pool = _check_pool(codes, scales, heads)
-    _check_ids(page_ids, pages, "page_ids")
-    _check_ids(exact_page_ids, pages, "exact_page_ids")
+    device = key.get_device()
+    pool, codes_at, scales_at = _pool(codes, scales, heads, device)
+    ids_at = _ids(page_ids, pages, device, _PAGE_IDS)
+    exact_ids_at = _ids(exact_page_ids, pages, device, _EXACT_IDS)
     if page_ids is None and pages > pool:
         raise ValueError(f"{pages} pages do not fit a pool of {pool}")
-    _check_centers(key_center, value_center, (heads, DIM))
-    exact_pages = 0
+    key_center_at, value_center_at = _centers(key_center, value_center, (heads, DIM), device)
+    exact_pages, exact_key_at, exact_value_at = 0, None, None
     if exact_page_ids is not None:
         if exact_key is None or exact_value is None:
             raise ValueError("exact page ids need exact key/value pages")
-        exact_pages = min(_check_exact(exact_key, heads, "exact_key"),
-                          _check_exact(exact_value, heads, "exact_value"))
-    else:
-        exact_key = exact_value = None
-    _capi.require_current_device(key, value, codes, scales, page_ids, key_center, value_center,
-                                 exact_page_ids, exact_key, exact_value)
+        exact_pages, exact_key_at = _exact(exact_key, heads, device, _EXACT_KEY)
+        count, exact_value_at = _exact(exact_value, heads, device, _EXACT_VALUE)
+        exact_pages = min(exact_pages, count)
+    if value.get_device() != device:
+        raise ValueError(_capi.DEVICE_ERROR)
+    _capi.check_device(device)
     if tokens == 0 or pool == 0 and exact_pages == 0:
         return
     if pool == 0 or exact_page_ids is not None and exact_pages == 0:
         raise ValueError("a pool without pages holds nothing")
     _capi.call("pg_int4_quantize_pages", key.data_ptr(), key_stride, value.data_ptr(), value_stride,
-               _ptr(key_center), _ptr(value_center), codes.data_ptr(), scales.data_ptr(), pool,
-               _ptr(page_ids), _ptr(exact_page_ids), _ptr(exact_key), _ptr(exact_value), exact_pages,
-               tokens, heads, _capi.current_stream())
+               key_center_at, value_center_at, codes_at, scales_at, pool, ids_at, exact_ids_at,
+               exact_key_at, exact_value_at, exact_pages, tokens, heads, _capi.current_stream())
 
 
 def dequantize_pages(codes: torch.Tensor, scales: torch.Tensor,
@@ -157,34 +165,38 @@ def dequantize_pages(codes: torch.Tensor, scales: torch.Tensor,
     ``tokens`` defaults to whole pages.  Ids outside the pool give zeros.
     ``key`` and ``value`` may be given (token rows may be strided)."""
     if codes.dim() != 4 or codes.shape[1] == 0:
-        raise ValueError("4-bit codes must be contiguous uint8 [pages,Hkv,2,1024]")
-    heads = codes.shape[1]
-    pool = _check_pool(codes, scales, heads)
+        raise ValueError(_CODES)
+    heads, device = codes.shape[1], codes.get_device()
+    pool, codes_at, scales_at = _pool(codes, scales, heads, device)
     pages = pool if page_ids is None else page_ids.numel()
-    _check_ids(page_ids, pages, "page_ids")
+    ids_at = _ids(page_ids, pages, device, _PAGE_IDS)
     tokens = pages * PAGE if tokens is None else int(tokens)
     if not 0 <= tokens <= pages * PAGE:
         raise ValueError(f"{pages} pages hold at most {pages * PAGE} tokens, asked for {tokens}")
-    _check_centers(key_center, value_center, (heads, DIM))
+    key_center_at, value_center_at = _centers(key_center, value_center, (heads, DIM), device)
+    shape, dense = (tokens, heads, DIM), (heads * DIM, DIM, 1)
     strides = []
-    rows = []
     for t in (key, value):
-        if t is None:
-            t = torch.empty_strided((tokens, heads, DIM), (heads * DIM, DIM, 1), dtype=torch.float16,
-                                    device=codes.device)
-        elif t.shape != (tokens, heads, DIM):
-            raise ValueError(f"K and V rows must be [{tokens},{heads},128]")
-        strides.append(_token_rows(t, "K and V"))
-        if tokens > 1 and strides[-1] < heads * DIM:
-            raise ValueError("K and V rows must not overlap")
-        rows.append(t)
-    _capi.require_current_device(codes, scales, page_ids, key_center, value_center, *rows)
+        stride = heads * DIM
+        if t is not None:
+            if t.shape != shape:
+                raise ValueError(f"K and V rows must be [{tokens},{heads},128]")
+            stride = _token_rows(t, "K and V")
+            if tokens > 1 and stride < heads * DIM:
+                raise ValueError("K and V rows must not overlap")
+            if t.get_device() != device:
+                raise ValueError(_capi.DEVICE_ERROR)
+        strides.append(stride)
+    _capi.check_device(device)
+    if key is None:
+        key = torch.empty_strided(shape, dense, dtype=torch.float16, device=codes.device)
+    if value is None:
+        value = torch.empty_strided(shape, dense, dtype=torch.float16, device=codes.device)
     if tokens:
-        _capi.call("pg_int4_dequantize_pages", codes.data_ptr(), scales.data_ptr(), pool,
-                   _ptr(page_ids), _ptr(key_center), _ptr(value_center), rows[0].data_ptr(),
-                   strides[0], rows[1].data_ptr(), strides[1], tokens, heads,
-                   _capi.current_stream())
-    return rows[0], rows[1]
+        _capi.call("pg_int4_dequantize_pages", codes_at, scales_at, pool, ids_at, key_center_at,
+                   value_center_at, key.data_ptr(), strides[0], value.data_ptr(), strides[1], tokens,
+                   heads, _capi.current_stream())
+    return key, value
 
 
 def rope_append(rotary: RotaryEmbedding, query: torch.Tensor, key: torch.Tensor,
@@ -206,38 +218,37 @@ def rope_append(rotary: RotaryEmbedding, query: torch.Tensor, key: torch.Tensor,
     from each other."""
     if rotary.head_dim != DIM:
         raise ValueError("the cache holds heads of 128 dims")
-    strides = []
-    for t, what in ((query, "query"), (key, "key"), (value, "value")):
-        strides.append(_token_rows(t, what))
-    batch, heads = key.shape[0], key.shape[1]
+    query_stride, key_stride = _token_rows(query, "query"), _token_rows(key, "key")
+    value_stride = _token_rows(value, "value")
+    batch, heads, _ = key.shape
     if value.shape != key.shape or query.shape[0] != batch:
         raise ValueError("query, key and value must have a row per request")
-    for ids, what in ((positions, "positions"), (exact_page_ids, "exact_page_ids"),
-                      (code_page_ids, "code_page_ids")):
-        _check_ids(ids, batch, what)
+    device = key.get_device()
+    positions_at = _ids(positions, batch, device, "positions must be contiguous int32, one per request")
+    exact_ids_at = _ids(exact_page_ids, batch, device, _EXACT_IDS)
+    code_ids_at = _ids(code_page_ids, batch, device, _CODE_IDS)
     if key_center is None:
         raise ValueError("key and value centers are required")
-    _check_centers(key_center, value_center, (batch, heads, DIM))
-    if rotated_query.shape != query.shape or rotated_query.dtype != torch.float16 \
-            or not rotated_query.is_contiguous():
-        raise ValueError("rotated_query must be contiguous float16, shaped like the query")
-    exact_pages = min(_check_exact(exact_key, heads, "exact_key"),
-                      _check_exact(exact_value, heads, "exact_value"))
-    pool = _check_pool(codes, scales, heads)
-    _capi.require_current_device(rotary.turns, query, key, value, positions, exact_page_ids,
-                                 code_page_ids, key_center, value_center, rotated_query, exact_key,
-                                 exact_value, codes, scales)
+    key_center_at, value_center_at = _centers(key_center, value_center, (batch, heads, DIM), device)
+    rotated_at = _capi.pointer(rotated_query, torch.float16, query.shape, device,
+                               "rotated_query must be contiguous float16, shaped like the query")
+    exact_pages, exact_key_at = _exact(exact_key, heads, device, _EXACT_KEY)
+    count, exact_value_at = _exact(exact_value, heads, device, _EXACT_VALUE)
+    pool, codes_at, scales_at = _pool(codes, scales, heads, device)
+    if query.get_device() != device or value.get_device() != device \
+            or rotary.turns.get_device() != device:
+        raise ValueError(_capi.DEVICE_ERROR)
+    _capi.check_device(device)
     if batch == 0:
         return
+    exact_pages = min(exact_pages, count)
     if pool == 0 or exact_pages == 0:
         raise ValueError("a pool without pages holds nothing")
-    _capi.call("pg_int4_rope_append", query.data_ptr(), key.data_ptr(), value.data_ptr(), strides[0],
-               strides[1], strides[2], positions.data_ptr(), rotary.turns.data_ptr(),
-               rotary.amplitude, rotary.rotary_dim, int(rotary.interleaved),
-               exact_page_ids.data_ptr(), code_page_ids.data_ptr(), key_center.data_ptr(),
-               value_center.data_ptr(), rotated_query.data_ptr(), exact_key.data_ptr(),
-               exact_value.data_ptr(), exact_pages, codes.data_ptr(), scales.data_ptr(), pool, batch,
-               query.shape[1], heads, _capi.current_stream())
+    _capi.call("pg_int4_rope_append", query.data_ptr(), key.data_ptr(), value.data_ptr(), query_stride,
+               key_stride, value_stride, positions_at, rotary.turns.data_ptr(), rotary.amplitude,
+               rotary.rotary_dim, int(rotary.interleaved), exact_ids_at, code_ids_at, key_center_at,
+               value_center_at, rotated_at, exact_key_at, exact_value_at, exact_pages, codes_at,
+               scales_at, pool, batch, query.shape[1], heads, _capi.current_stream())
 
 
 def plan_work_items(indptr, tail_indptr=None, num_qo_heads: int = 32, num_kv_heads: int = 8,
@@ -271,7 +282,9 @@ class Int4PagedDecode:
                 or workspace.data_ptr() % 256:
             raise ValueError("workspace must be a contiguous CUDA uint8 tensor, 256-byte aligned")
         self.workspace = workspace
+        self._device = workspace.get_device()
         self._plan = _capi.Int4Plan()
+        self._plan_ref = ctypes.byref(self._plan)
         self._planned = False
 
     def plan(self, indptr, indices: torch.Tensor, last_page_len: torch.Tensor,
@@ -304,7 +317,7 @@ class Int4PagedDecode:
                                      tail_last_page_len)
         _capi.call("pg_int4_plan", host.data_ptr(), _ptr(tail), host.numel() - 1, num_qo_heads,
                    num_kv_heads, int(num_cus or _num_cus(indices.device)), self.workspace.data_ptr(),
-                   self.workspace.numel(), ctypes.byref(self._plan), _capi.current_stream())
+                   self.workspace.numel(), self._plan_ref, _capi.current_stream())
         self._planned = True
         self._tables = (indices, last_page_len, tail_indices, tail_last_page_len)
         self._table_ptrs = tuple(_ptr(t) for t in self._tables)
@@ -328,44 +341,40 @@ class Int4PagedDecode:
         and an lse of -inf."""
         if not self._planned:
             raise RuntimeError("plan() must be called before run()")
-        hkv, batch = self._num_kv_heads, self._batch
-        _check_query(q, batch, self._num_qo_heads)
-        pool = _check_pool(codes, scales, hkv)
-        exact_k = exact_v = None
+        hkv, hq, batch = self._num_kv_heads, self._num_qo_heads, self._batch
+        _check_query(q, batch, hq)
+        device = q.get_device()
+        pool, codes_at, scales_at = _pool(codes, scales, hkv, device)
+        exact_k_at = exact_v_at = center_at = lse_at = None
         if self._tables[2] is not None:
             if exact_cache is None:
                 raise ValueError("a plan with a tail needs the exact pages")
             exact_k, exact_v = exact_cache
-            _check_cache(exact_k, "exact_k", torch.float16, hkv)
-            _check_cache(exact_v, "exact_v", torch.float16, hkv)
+            pages, exact_k_at = _exact(exact_k, hkv, device, _EXACT_KEY)
+            count, exact_v_at = _exact(exact_v, hkv, device, _EXACT_VALUE)
             if self._id_ranges[1] is not None:
-                _check_page_ids(self._id_ranges[1], min(exact_k.shape[0], exact_v.shape[0]),
-                                "exact tail")
+                _check_page_ids(self._id_ranges[1], min(pages, count), "exact tail")
         if self._id_ranges[0] is not None:
             _check_page_ids(self._id_ranges[0], pool, "4-bit")
-        if value_center is not None and (value_center.dtype is not torch.float16
-                                         or value_center.shape != (batch, hkv, DIM)
-                                         or not value_center.is_contiguous()):
-            raise ValueError(f"value_center must be contiguous float16 [B,{hkv},128]")
+        if value_center is not None:
+            center_at = _capi.pointer(value_center, torch.float16, (batch, hkv, DIM), device, _CENTERS)
         if out is None:
             out = torch.empty_like(q)
             if not out.is_contiguous():
                 out = torch.empty(q.shape, device=q.device, dtype=torch.float16)
-        elif out.shape != q.shape or out.dtype is not torch.float16 or not out.is_contiguous():
-            raise ValueError("out must be contiguous float16, shaped like q")
-        if lse is None:
-            if return_lse:
-                lse = torch.empty_strided((batch, self._num_qo_heads), (self._num_qo_heads, 1),
-                                          dtype=torch.float32, device=q.device)
-        elif lse.shape != (batch, self._num_qo_heads) or lse.dtype is not torch.float32 \
-                or not lse.is_contiguous():
-            raise ValueError("lse must be contiguous float32 [B,Hq]")
-        _capi.require_current_device(self.workspace, q, codes, scales, exact_k, exact_v, value_center,
-                                     out, lse)
+        out_at = _capi.pointer(out, torch.float16, q.shape, device,
+                               "out must be contiguous float16, shaped like q")
+        if lse is None and return_lse:
+            lse = torch.empty_strided((batch, hq), (hq, 1), dtype=torch.float32, device=q.device)
+        if lse is not None:
+            lse_at = _capi.pointer(lse, torch.float32, (batch, hq), device,
+                                   "lse must be contiguous float32 [B,Hq]")
+        if self._device != device:
+            raise ValueError(_capi.DEVICE_ERROR)
+        _capi.check_device(device)
         indices, last, tail_indices, tail_last = self._table_ptrs
-        _capi.call("pg_int4_decode_run", ctypes.byref(self._plan), q.data_ptr(), q.stride(0),
-                   codes.data_ptr(), scales.data_ptr(), indices, last, _ptr(exact_k), _ptr(exact_v),
-                   tail_indices, tail_last, _ptr(value_center), hkv * DIM, out.data_ptr(), _ptr(lse),
-                   float(self._sm_scale if sm_scale is None else sm_scale),
+        _capi.call("pg_int4_decode_run", self._plan_ref, q.data_ptr(), q.stride(0), codes_at, scales_at,
+                   indices, last, exact_k_at, exact_v_at, tail_indices, tail_last, center_at, hkv * DIM,
+                   out_at, lse_at, float(self._sm_scale if sm_scale is None else sm_scale),
                    self.workspace.data_ptr(), _capi.current_stream())
         return (out, lse) if return_lse else out

@@ -18,10 +18,9 @@ from . import _capi
 _DTYPES = {torch.float16: _capi.PG_DTYPE_FP16, torch.bfloat16: _capi.PG_DTYPE_BF16,
            torch.float32: _capi.PG_DTYPE_FP32}
 _TOKENS = (torch.int32, torch.int64)
-
-
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+_LENGTHS = "lengths must be contiguous int32 [B]"
+_PENALTIES = "penalties must be contiguous float32 [B]"
+_BIASES = "biases must be contiguous int32 or int64 tokens and float32 values [B, n]"
 
 
 def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
@@ -53,18 +52,27 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
     the vocabulary (padding) are ignored.  Computed in float32; ``out`` may be
     ``logits``.  Returns ``out``."""
     dtype = _DTYPES.get(logits.dtype)
-    if dtype is None or logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] > 1:
+    if dtype is None or logits.dim() != 2:
         raise ValueError("logits must be FP16, BF16 or float32 [B, V] rows")
-    batch, vocab = logits.shape
+    batch, vocab = shape = logits.shape
+    row, one = logits.stride()
+    if one != 1 and vocab > 1:
+        raise ValueError("logits must be FP16, BF16 or float32 [B, V] rows")
+    device, at = logits.get_device(), logits.data_ptr()
     if out is None:
         out = torch.empty_like(logits)
         if vocab > 1 and out.stride(1) != 1:
-            out = torch.empty((batch, vocab), device=logits.device, dtype=logits.dtype)
-    elif out.shape != logits.shape or out.dtype != logits.dtype or vocab > 1 and out.stride(1) != 1 \
+            out = torch.empty(shape, device=logits.device, dtype=logits.dtype)
+    elif out.shape != shape or out.dtype != logits.dtype or vocab > 1 and out.stride(1) != 1 \
             or batch > 1 and out.stride(0) < vocab:
         raise ValueError("shaped logits must be rows like the logits")
-    elif out.data_ptr() == logits.data_ptr() and out.stride() != logits.stride():
+    elif out.data_ptr() == at and out.stride() != (row, one):
         raise ValueError("logits shaped in place must keep their strides")
+    elif out.get_device() != device:
+        raise ValueError(_capi.DEVICE_ERROR)
+    rows = (batch,)
+    token_bytes = capacity = history_row = 0
+    history_at = lengths_at = prompts_at = None
     if history is None:
         if history_lengths is not None or prompt_lengths is not None or repetition is not None \
                 or frequency is not None or presence is not None:
@@ -75,43 +83,44 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
             raise ValueError("history must be int32 or int64 [B, capacity] rows")
         if history_lengths is None:
             raise ValueError("a history needs its lengths")
-    for t in (history_lengths, prompt_lengths):
-        if t is not None and (t.dtype is not torch.int32 or t.shape != (batch,) or not t.is_contiguous()):
-            raise ValueError("lengths must be contiguous int32 [B]")
-    for t in (repetition, frequency, presence):
-        if t is not None and (t.dtype is not torch.float32 or t.shape != (batch,)
-                              or not t.is_contiguous()):
-            raise ValueError("penalties must be contiguous float32 [B]")
+        if history.get_device() != device:
+            raise ValueError(_capi.DEVICE_ERROR)
+        lengths_at = _capi.pointer(history_lengths, torch.int32, rows, device, _LENGTHS)
+        if prompt_lengths is not None:
+            prompts_at = _capi.pointer(prompt_lengths, torch.int32, rows, device, _LENGTHS)
+        capacity, token_bytes = history.shape[1], history.element_size()
+        history_at, history_row = history.data_ptr(), history.stride(0)
+    repetition_at, frequency_at, presence_at = (
+        None if t is None else _capi.pointer(t, torch.float32, rows, device, _PENALTIES)
+        for t in (repetition, frequency, presence))
     if (bias_tokens is None) != (bias_values is None):
         raise ValueError("bias tokens and values go together")
-    biases = 0
+    biases, tokens_at, values_at = 0, None, None
     if bias_tokens is not None:
-        if bias_tokens.dtype not in _TOKENS or bias_tokens.dim() != 2 or bias_tokens.shape[0] != batch \
-                or bias_values.shape != bias_tokens.shape or bias_values.dtype != torch.float32 \
-                or not bias_tokens.is_contiguous() or not bias_values.is_contiguous():
-            raise ValueError("biases must be int32 or int64 tokens and float32 values [B, n]")
+        if bias_tokens.dtype not in _TOKENS or bias_tokens.dim() != 2 or bias_tokens.shape[0] != batch:
+            raise ValueError(_BIASES)
         if history is not None and history.dtype != bias_tokens.dtype:
             raise ValueError("history and bias tokens must have one type")
-        biases = bias_tokens.shape[1]
-    if allowed is not None and (allowed.dtype != torch.int32 or allowed.dim() != 2
-                                or allowed.shape != (batch, (vocab + 31) // 32)
-                                or allowed.shape[1] > 1 and allowed.stride(1) != 1):
-        raise ValueError("allowed must be int32 [B, ceil(V / 32)] rows of bits")
-    _capi.require_current_device(logits, out, history, history_lengths, prompt_lengths, repetition,
-                                 frequency, presence, bias_tokens, bias_values, allowed)
+        tokens_at = _capi.pointer(bias_tokens, bias_tokens.dtype, bias_tokens.shape, device, _BIASES)
+        values_at = _capi.pointer(bias_values, torch.float32, bias_tokens.shape, device, _BIASES)
+        biases, token_bytes = bias_tokens.shape[1], bias_tokens.element_size()
+    allowed_at, allowed_row = None, 0
+    if allowed is not None:
+        if allowed.dtype is not torch.int32 or allowed.shape != (batch, (vocab + 31) // 32) \
+                or allowed.shape[1] > 1 and allowed.stride(1) != 1:
+            raise ValueError("allowed must be int32 [B, ceil(V / 32)] rows of bits")
+        if allowed.get_device() != device:
+            raise ValueError(_capi.DEVICE_ERROR)
+        allowed_at, allowed_row = allowed.data_ptr(), allowed.stride(0)
+    _capi.check_device(device)
     if batch == 0 or vocab == 0:
         return out
-    tokens = history if history is not None else bias_tokens
-    # a history of no tokens has no address
-    with_history = history is not None and history.shape[1] > 0
-    _capi.call("pg_shape_logits", logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0),
-               dtype, batch, vocab, history.data_ptr() if with_history else None,
-               history.stride(0) if with_history else 0, history.shape[1] if with_history else 0,
-               _ptr(history_lengths) if with_history else None,
-               _ptr(prompt_lengths) if with_history else None,
-               _ptr(repetition) if with_history else None, _ptr(frequency) if with_history else None,
-               _ptr(presence) if with_history else None,
-               _ptr(bias_tokens) if biases else None, _ptr(bias_values) if biases else None, biases,
-               0 if tokens is None else tokens.element_size(), _ptr(allowed),
-               0 if allowed is None else allowed.stride(0), _capi.current_stream())
+    if capacity == 0:       # a history of no tokens has no address
+        history_at = lengths_at = prompts_at = repetition_at = frequency_at = presence_at = None
+    if biases == 0:
+        tokens_at = values_at = None
+    _capi.call("pg_shape_logits", at, row, out.data_ptr(), out.stride(0), dtype, batch, vocab,
+               history_at, history_row, capacity, lengths_at, prompts_at, repetition_at, frequency_at,
+               presence_at, tokens_at, values_at, biases, token_bytes, allowed_at, allowed_row,
+               _capi.current_stream())
     return out
