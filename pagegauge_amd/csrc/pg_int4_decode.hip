@@ -33,13 +33,15 @@
 //
 // Bound by HBM once a wave has several groups, by a chain of trips to memory
 // (work item, page ids, pages, partial rows) before.  Kernel times on MI355X, and
-// of the same walk without its arithmetic: 256 requests (829 MB) 169 and 165 us,
-// 8 requests of 4K to 32K (164 MB) 34 and 32, one of 49K tokens (53 MB) 14.8 and
-// 12.3, of 4K (5 MB) 5.5 and 4.6; a join adds 2.3 to 4.6 us.  Measured and not
+// of the same walk without its arithmetic: 256 requests (829 MB) 168 and 165 us,
+// 8 requests of 4K to 32K (164 MB) 34 and 32, one of 49K tokens (53 MB) 14.4 and
+// 12.3, of 4K (5 MB) 5.4 and 4.6; a join adds 2.4 to 4.6 us.  Measured and not
 // taken: 8 waves a workgroup (one fits a CU, and nothing covers its start and
 // end: 256 requests 191 us), and a join by the workgroup that ends last (49K
 // tokens 18.7 us a call against 17.2 with the second launch, before the last
-// steps: counting across XCDs costs what the launch does).
+// steps: counting across XCDs costs what the launch does), and pages requested two
+// groups ahead (19.0 us a call at 49K tokens against 16.6, 190 at 256 requests:
+// the clamped or checked addresses cost more than the wait).
 #include "pg_int4.h"
 #include "pg_int4_plan.h"
 

@@ -51,9 +51,9 @@ int32_t build_int4_plan(const int32_t* host_indptr, const int32_t* host_tail_ind
   // The smallest largest share (``cap``, in weighted pages) with which the batch
   // takes no more workgroups than ``target``, but at least one group of pages per
   // wave.  One workgroup per CU is the better plan as long as its waves can hold
-  // their pages (49K tokens: 32 items 15.5 us, 64 items 17.2; 64K 18.1 and 20.0),
-  // and two where they cannot (128K tokens: 33 items, an uneven round, 44.7 us, 64
-  // items 33.0; 16 requests of 8K 37.1 and 33.9).
+  // their pages (49K tokens: 32 items 16.6 us, 64 items 18.1; 64K 18.9 and 20.8),
+  // and two where they cannot (128K tokens: 33 items, an uneven round, 46.8 us, 64
+  // items 33.6; 16 requests of 8K 38.3 and 34.4).
   const int64_t groups = static_cast<int64_t>(num_kv_heads) *
                          ceil_div(num_qo_heads / num_kv_heads, kInt4HeadsPerWave);
   const int64_t cus = num_cus > 0 ? num_cus : 256;

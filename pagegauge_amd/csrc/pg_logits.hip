@@ -13,6 +13,14 @@
 // the whole history, which L2 serves to all tiles but the first; that is cheaper
 // than counts of the whole vocabulary in memory, 4 bytes per logit and a
 // launch to clear them.
+//
+// Bound by HBM and, in turn, by the steps before the logits can leave: 64 rows of
+// 131072 float32 logits (70 MB) with histories of 4096, 64 biases and a mask take
+// 17.0 to 17.8 us, where a copy of as many bytes takes 13.5.  Of these the mask
+// costs 2, cleared counts and barriers 1.7, the histories 3.5 and the biases 0.5
+// to 1.  One row of 32768 takes 5.6 us.  Measured and not taken at 64 rows: 512
+// threads with tiles of 4096 or 8192 (19.5, 20.5 us), 256 with 4096 (22.3), and
+// two tiles per workgroup with the tokens kept in registers (21.2).
 #include "pg_common.h"
 
 #include <hip/hip_bf16.h>
@@ -238,9 +246,11 @@ extern "C" int32_t pg_shape_logits(const void* logits, int64_t logits_stride, vo
   a.logits_stride = logits_stride;
   a.out_stride = out_stride;
   a.vocab = vocab;
-  // tiles of 1024 to 8192 tokens, small ones where the batch leaves CUs idle
+  // tiles of 8192 tokens, which read the history least often, down to 1024 where
+  // 256 CUs would not get one each (histories of 4096: 8 rows of 131072 4.5 us, with
+  // tiles of 8192 5.3; 4 of 32768 3.8 and 4.9; but 16 of 131072 6.4 with 4096, 6.0)
   a.tile = kMaxTile;
-  while (a.tile > kMinTile && static_cast<int64_t>(batch) * ((vocab + a.tile - 1) / a.tile) < 512) a.tile /= 2;
+  while (a.tile > kMinTile && static_cast<int64_t>(batch) * ((vocab + a.tile - 1) / a.tile) < 256) a.tile /= 2;
   a.history = history && (repetition || frequency || presence) ? history : nullptr;
   a.history_stride = history_stride;
   a.history_capacity = history_capacity;

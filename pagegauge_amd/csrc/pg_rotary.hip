@@ -8,6 +8,12 @@
 // context stretched in parts.  The angles come from float64 frequencies (no
 // table of positions is read or kept), and a thread turns the same kVec pairs
 // of several heads of one token, so their sines are worked out once for them.
+//
+// Bound by HBM, and for few tokens by one trip to it.  16384 tokens of 32 query
+// and 8 KV heads in FP16 (336 MB) take 70 to 72 us, 4.7 TB/s, where a copy of as
+// many bytes takes 65; 8 tokens 3.7 us.  Measured and not taken at that size:
+// one slice of all heads 75.5 us, 8 and 20 slices 72.8 and 79.7 (the sines over
+// again), nontemporal stores 72.9, 2 or 10 heads in flight for 4 the same.
 #include "pg_rotary.h"
 
 #include <hip/hip_bf16.h>
@@ -125,7 +131,8 @@ int32_t dispatch(RotaryArgs a, int vec, int head_dim, bool interleaved, void* st
   const int64_t blocks = (a.tokens * a.units + kThreads - 1) / kThreads;
   if (blocks > UINT32_MAX / kThreads) return fail(PG_ERROR_UNSUPPORTED, "too many rows for one rotation");
   const int heads = a.rows[0].heads + a.rows[1].heads;
-  // few tokens: the heads of a token over several workgroups
+  // few tokens: the heads of a token over several workgroups, up to 2048 in all (40
+  // heads of 8 tokens 2.8 us, in one slice 17.5; of 1024 6.6 and 20.1)
   int slices = static_cast<int>(std::min<int64_t>(heads, std::max<int64_t>(1, 2048 / blocks)));
   a.heads_per_slice = (heads + slices - 1) / slices;
   slices = (heads + a.heads_per_slice - 1) / a.heads_per_slice;
