@@ -12,6 +12,11 @@ call signatures:
   ``merge_state_in_place``) and the split scheduler (``plan_work_items``);
 * ``update`` -- the paged append / finalize, bulk quantizers, prefill
   population and exact centers;
+* ``rotary`` -- rotary positions from 64-bit angles: both layouts, part of the
+  head, frequencies scaled for long contexts;
+* ``int4`` -- the cache held in 4 bits: prompt writer, reader-back, append with
+  the rotation on the way, attention;
+* ``logits`` -- penalties, biases and masks before a token is picked;
 * ``page_table`` -- the page-table algebra of the decoder harness;
 * ``decoder`` -- the Mistral-shaped decoder over these kernels;
 * ``serving`` / ``serving_bridge`` -- request slots, decode-batch tables and
@@ -19,5 +24,5 @@ call signatures:
 * ``workloads`` -- the seeded benchmark configurations.
 """
 
-__all__ = ["runtime", "decode", "update", "page_table", "decoder", "serving", "serving_bridge",
-           "workloads"]
+__all__ = ["runtime", "decode", "update", "rotary", "int4", "logits", "page_table", "decoder",
+           "serving", "serving_bridge", "workloads"]

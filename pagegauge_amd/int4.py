@@ -122,7 +122,7 @@ def quantize_pages(key: torch.Tensor, value: torch.Tensor, codes: torch.Tensor,
     rounded to FP16, in pages ``exact_page_ids[i]`` of ``exact_key`` and
     ``exact_value`` [pages, 16, Hkv, 128].  Ids outside their pool (-1) skip
     the store; the others must differ from each other.  Rows may be strided
-    by token."""
+    by token, and may not lie in the exact pages."""
     if key.shape != value.shape:
         raise ValueError("token-major K/V must have identical [T,Hkv,128] shapes")
     key_stride, value_stride = _token_rows(key, "K"), _token_rows(value, "V")
@@ -275,7 +275,8 @@ class Int4PagedDecode:
     """Attention of one token per request over 4-bit history pages, an exact
     FP16 tail and the value center (``plan`` / ``run`` as
     ``decode.PageGaugeSegmentedDecode``).  Runs of one object share its
-    workspace and must not overlap on different streams."""
+    workspace and must not overlap on different streams; it belongs to this
+    object alone (another one's plan would replace the work list in it)."""
 
     def __init__(self, workspace: torch.Tensor) -> None:
         if not workspace.is_cuda or workspace.dtype != torch.uint8 or not workspace.is_contiguous() \

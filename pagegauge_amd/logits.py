@@ -50,7 +50,7 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
     ``history`` is int32 or int64 [B, capacity], each row's tokens first;
     lengths are int32 [B], the penalties and biases float32.  Tokens outside
     the vocabulary (padding) are ignored.  Computed in float32; ``out`` may be
-    ``logits``.  Returns ``out``."""
+    ``logits``, but not otherwise overlap them.  Returns ``out``."""
     dtype = _DTYPES.get(logits.dtype)
     if dtype is None or logits.dim() != 2:
         raise ValueError("logits must be FP16, BF16 or float32 [B, V] rows")
