@@ -260,7 +260,7 @@ def require_current_device(*tensors) -> None:
             if at != device:
                 raise ValueError(DEVICE_ERROR)
     if device is not None:
-        check_device(device)
+        launch_stream(device)
 
 
 def pointer(t: torch.Tensor, dtype, shape: tuple, device: int, what: str) -> int:
@@ -273,11 +273,12 @@ def pointer(t: torch.Tensor, dtype, shape: tuple, device: int, what: str) -> int
     return t.data_ptr()
 
 
-def check_device(device: int) -> None:
-    """ValueError unless ``device``, where a call's tensors are, is the current
-    CUDA device, on whose current stream the kernels are launched."""
+def launch_stream(device: int) -> int:
+    """Raw handle of the current stream; ValueError unless ``device``, where a
+    call's tensors are, is the current CUDA device."""
     if device < 0 or device != torch._C._cuda_getDevice():
         raise ValueError(DEVICE_ERROR)
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def last_error() -> str:
@@ -291,4 +292,6 @@ def check(rc: int, what: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(library(), name)(*args), name)
+    rc = getattr(_library or library(), name)(*args)
+    if rc != PG_OK:
+        check(rc, name)

@@ -144,14 +144,14 @@ def quantize_pages(key: torch.Tensor, value: torch.Tensor, codes: torch.Tensor,
         exact_pages = min(exact_pages, count)
     if value.get_device() != device:
         raise ValueError(_capi.DEVICE_ERROR)
-    _capi.check_device(device)
+    stream = _capi.launch_stream(device)
     if tokens == 0 or pool == 0 and exact_pages == 0:
         return
     if pool == 0 or exact_page_ids is not None and exact_pages == 0:
         raise ValueError("a pool without pages holds nothing")
     _capi.call("pg_int4_quantize_pages", key.data_ptr(), key_stride, value.data_ptr(), value_stride,
                key_center_at, value_center_at, codes_at, scales_at, pool, ids_at, exact_ids_at,
-               exact_key_at, exact_value_at, exact_pages, tokens, heads, _capi.current_stream())
+               exact_key_at, exact_value_at, exact_pages, tokens, heads, stream)
 
 
 def dequantize_pages(codes: torch.Tensor, scales: torch.Tensor,
@@ -187,7 +187,7 @@ def dequantize_pages(codes: torch.Tensor, scales: torch.Tensor,
             if t.get_device() != device:
                 raise ValueError(_capi.DEVICE_ERROR)
         strides.append(stride)
-    _capi.check_device(device)
+    stream = _capi.launch_stream(device)
     if key is None:
         key = torch.empty_strided(shape, dense, dtype=torch.float16, device=codes.device)
     if value is None:
@@ -195,7 +195,7 @@ def dequantize_pages(codes: torch.Tensor, scales: torch.Tensor,
     if tokens:
         _capi.call("pg_int4_dequantize_pages", codes_at, scales_at, pool, ids_at, key_center_at,
                    value_center_at, key.data_ptr(), strides[0], value.data_ptr(), strides[1], tokens,
-                   heads, _capi.current_stream())
+                   heads, stream)
     return key, value
 
 
@@ -238,7 +238,7 @@ def rope_append(rotary: RotaryEmbedding, query: torch.Tensor, key: torch.Tensor,
     if query.get_device() != device or value.get_device() != device \
             or rotary.turns.get_device() != device:
         raise ValueError(_capi.DEVICE_ERROR)
-    _capi.check_device(device)
+    stream = _capi.launch_stream(device)
     if batch == 0:
         return
     exact_pages = min(exact_pages, count)
@@ -248,7 +248,7 @@ def rope_append(rotary: RotaryEmbedding, query: torch.Tensor, key: torch.Tensor,
                key_stride, value_stride, positions_at, rotary.turns.data_ptr(), rotary.amplitude,
                rotary.rotary_dim, int(rotary.interleaved), exact_ids_at, code_ids_at, key_center_at,
                value_center_at, rotated_at, exact_key_at, exact_value_at, exact_pages, codes_at,
-               scales_at, pool, batch, query.shape[1], heads, _capi.current_stream())
+               scales_at, pool, batch, query.shape[1], heads, stream)
 
 
 def plan_work_items(indptr, tail_indptr=None, num_qo_heads: int = 32, num_kv_heads: int = 8,
@@ -372,10 +372,10 @@ class Int4PagedDecode:
                                    "lse must be contiguous float32 [B,Hq]")
         if self._device != device:
             raise ValueError(_capi.DEVICE_ERROR)
-        _capi.check_device(device)
+        stream = _capi.launch_stream(device)
         indices, last, tail_indices, tail_last = self._table_ptrs
         _capi.call("pg_int4_decode_run", self._plan_ref, q.data_ptr(), q.stride(0), codes_at, scales_at,
                    indices, last, exact_k_at, exact_v_at, tail_indices, tail_last, center_at, hkv * DIM,
                    out_at, lse_at, float(self._sm_scale if sm_scale is None else sm_scale),
-                   self.workspace.data_ptr(), _capi.current_stream())
+                   self.workspace.data_ptr(), stream)
         return (out, lse) if return_lse else out

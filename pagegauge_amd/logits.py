@@ -112,7 +112,7 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
         if allowed.get_device() != device:
             raise ValueError(_capi.DEVICE_ERROR)
         allowed_at, allowed_row = allowed.data_ptr(), allowed.stride(0)
-    _capi.check_device(device)
+    stream = _capi.launch_stream(device)
     if batch == 0 or vocab == 0:
         return out
     if capacity == 0:       # a history of no tokens has no address
@@ -122,5 +122,5 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
     _capi.call("pg_shape_logits", at, row, out.data_ptr(), out.stride(0), dtype, batch, vocab,
                history_at, history_row, capacity, lengths_at, prompts_at, repetition_at, frequency_at,
                presence_at, tokens_at, values_at, biases, token_bytes, allowed_at, allowed_row,
-               _capi.current_stream())
+               stream)
     return out

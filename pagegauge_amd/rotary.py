@@ -115,12 +115,17 @@ class RotaryEmbedding:
             out_key, key_args, key_in_place = self._rows(key, out_key, tokens, query.dtype)
             if in_place != key_in_place:
                 raise ValueError("query and key are rotated in place together or not at all")
-        _capi.require_current_device(self.turns, positions, query, out_query, key, out_key)
+        device = query.get_device()
+        if positions.get_device() != device or self.turns.get_device() != device \
+                or out_query.get_device() != device \
+                or key is not None and (key.get_device() != device or out_key.get_device() != device):
+            raise ValueError(_capi.DEVICE_ERROR)
+        stream = _capi.launch_stream(device)
         if tokens and query_args[3] + key_args[3]:
             _capi.call("pg_rotate", *query_args[:4], *key_args[:4], *query_args[4:], *key_args[4:],
                        positions.data_ptr(), positions.element_size(), self.turns.data_ptr(),
                        self.amplitude, tokens, self.head_dim, self.rotary_dim,
-                       int(self.interleaved), dtype, _capi.current_stream())
+                       int(self.interleaved), dtype, stream)
         return out_query, out_key
 
     def _rows(self, x: torch.Tensor, out: Optional[torch.Tensor], tokens: int, dtype):
