@@ -12,11 +12,12 @@
 // One wave takes one K or V part of a block and holds it in registers in the
 // lane order of the packed layout, so that codes leave as one 1 KiB store of 16
 // bytes per lane.  All kernels are bound by HBM once they fill the chip, by a trip
-// or two to it before.  16384 tokens of 8 heads: quantized (85 MB with 16 exact
-// pages) in 19.7 to 20.5 us and read back (84 MB) in 16.0 to 16.6, a copy of as
-// many bytes taking 16.4.  The quantizer's arithmetic is what is left of its
-// distance: 32.5 us with a division per code, 25.3 with clamps and selects.  1000
-// tokens: 4.5 and 4.8 us.
+// or two to it before.  16384 tokens of 8 heads: quantized (84 MB) in 21.3 us and read
+// back in 21.1, rows from and to HBM, where a copy of as many bytes takes 17.4 (19.4
+// and 16.2 where the Infinity Cache holds the rows); 1000 tokens 4.3 us each.  The
+// quantizer's arithmetic is what is left of its distance: 32.5 us with a division per
+// code, 25.3 with clamps and selects.  Reading back took 23.8 with conversions of
+// integers and half lines per store.
 #include "pg_int4.h"
 #include "pg_rotary.h"
 
@@ -62,6 +63,7 @@ __device__ __forceinline__ uint32_t put_code(uint32_t word, int code, int nibble
 }
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
 // Value e of eight minus center e, rounded to float32: one mixed-precision
 // operation (``one`` is 1, where the compiler does not see it).
@@ -215,10 +217,11 @@ __device__ __forceinline__ void quantize_part(const QuantizeArgs& a, int64_t pag
 // blockIdx.z.
 template <bool kWide>
 __global__ __launch_bounds__(kWave * kWavesPerBlock) void int4_quantize_kernel(QuantizeArgs a) {
-  const int64_t page = blockIdx.x;
-  const int head = blockIdx.y * (blockDim.x / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int waves = blockDim.x / kWave, per_page = (a.heads + waves - 1) / waves;
+  const int64_t page = blockIdx.x / per_page;
+  const int head = blockIdx.x % per_page * waves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   if (head >= a.heads) return;
-  if (blockIdx.z == 0)
+  if (blockIdx.y == 0)
     quantize_part<kWide, false>(a, page, head, threadIdx.x % kWave);
   else
     quantize_part<kWide, true>(a, page, head, threadIdx.x % kWave);
@@ -235,41 +238,97 @@ struct DequantizeArgs {
   int heads;
 };
 
+// Lane n's word from lane n ^ 8 of the same 16.
+__device__ __forceinline__ uint32_t across8(uint32_t x) {
+  return __builtin_amdgcn_update_dpp(0, x, 0x128 /* row_ror:8 */, 0xf, 0xf, false);
+}
+
+// Codes in nibbles i and i + 4 of a word: a masked nibble is the FP16 subnormal
+// u * 2^-24, or 16 u * 2^-24 one nibble further up, and less 8 of the same it is the
+// code, exactly.
+__device__ __forceinline__ v2h code_pair(uint32_t word, int i) {
+  const uint32_t shifted = i & 2 ? word >> 8 : word;
+  const uint32_t bits = shifted & (i & 1 ? 0x00f000f0u : 0x000f000fu);
+  return __builtin_bit_cast(v2h, bits) - __builtin_bit_cast(v2h, i & 1 ? 0x00800080u : 0x00080008u);
+}
+
+// Rounded to float32, then to FP16, as the formula is.
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+  return __half_as_ushort(__float2half_rn(a)) | static_cast<uint32_t>(__half_as_ushort(__float2half_rn(b))) << 16;
+}
+
 template <bool kWide, bool kValue>
 __device__ __forceinline__ void dequantize_part(const DequantizeArgs& a, int64_t page, int head, int lane) {
   const int64_t code_page = a.page_ids ? a.page_ids[page] : page;
   const int64_t visible = a.tokens - page * kPageSize;
   const bool held = code_page >= 0 && code_page < a.num_code_pages;
   const int64_t block = (held ? code_page : 0) * a.heads + head;
-  const v4u word = *reinterpret_cast<const v4u*>(a.codes + block * kInt4BlockBytes +
-                                                 kValue * kInt4PartBytes + 16 * lane);
-  const uint16_t* center = a.center[kValue];
-  uint16_t* out = a.out[kValue] + page * kPageSize * a.token_stride[kValue] + head * kHeadDim;
+  const uint16_t* scales = a.scales + block * kInt4BlockScales;
+  v4u word = *reinterpret_cast<const v4u*>(a.codes + block * kInt4BlockBytes +
+                                           kValue * kInt4PartBytes + 16 * lane);
+  const bool upper = lane & 8;
+  // row and dim of store g: V's are those of the lane; K's lanes n and n + 8 trade
+  // words, so that a store writes whole lines: words 2 j and 2 j + 1 of lane n become
+  // dims 64 j + 32 (n / 8) .. of tokens n % 8 and n % 8 + 8 (half lines of 16 tokens
+  // per store took 23.2 us where this took 21.8)
+  auto row_of = [&](int g) { return kValue ? part_row<true>(g, lane) : (lane & 7) + 8 * (g & 1); };
+  auto dim_of = [&](int g) {
+    return kValue ? part_dim<true>(g, lane) : 64 * (g >> 1) + 32 * upper + 8 * (lane >> 4);
+  };
+  if (!kValue) {
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      const uint32_t other = across8(upper ? word[j] : word[j + 1]);
+      word[j] = upper ? other : word[j];
+      word[j + 1] = upper ? word[j + 1] : other;
+    }
+  }
+  float scale[4];
+  v8h center[4];
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const int row = part_row<kValue>(g, lane);
-    const float scale = half_bits_to_float(a.scales[block * kInt4BlockScales + int4_scale_index(kValue, row)]);
+    scale[g] = held ? half_bits_to_float(scales[int4_scale_index(kValue, row_of(g))]) : 0.0f;
     v4u c = {0u, 0u, 0u, 0u};
-    if (center) c = load8<kWide>(center + head * kHeadDim + part_dim<kValue>(g, lane));
-    v4u packed = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t w = kValue ? word[e >> 1] : word[g];
-      const int nibble = kValue ? (g >> 1) + 2 * (e & 1) + 4 * (g & 1) : (e >> 1) + 4 * (e & 1);
-      const int code = static_cast<int>(w >> (4 * nibble) & 15u) - 8;
-      const float value = held ? static_cast<float>(code) * scale + half_at(c, e) : 0.0f;
-      packed[e >> 1] |= static_cast<uint32_t>(__half_as_ushort(__float2half_rn(value))) << (16 * (e & 1));
-    }
-    if (row < visible) store8<kWide>(out + row * a.token_stride[kValue] + part_dim<kValue>(g, lane), packed);
+    if (a.center[kValue] && held) c = load8<kWide>(a.center[kValue] + head * kHeadDim + dim_of(g));
+    center[g] = __builtin_bit_cast(v8h, c);
   }
+  auto value = [&](v2h codes, int half, int i, int g, int e) {
+    return fmaf(static_cast<float>(codes[half]), scale[g] * (i & 1 ? 0x1p20f : 0x1p24f),
+                static_cast<float>(center[g][e]));
+  };
+  v4u out[4];
+  if (!kValue) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {      // dims 2 i and 2 i + 1
+        const v2h codes = code_pair(word[g], i);
+        out[g][i] = half_pair(value(codes, 0, i, g, 2 * i), value(codes, 1, i, g, 2 * i + 1));
+      }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int t = 0; t < 4; t += 2) {   // tokens t and t + 1, channels 2 j and 2 j + 1
+        const int i = t >> 1;
+        const v2h even = code_pair(word[j], i), odd = code_pair(word[j], i + 2);
+        out[t][j] = half_pair(value(even, 0, i, t, 2 * j), value(odd, 0, i, t, 2 * j + 1));
+        out[t + 1][j] = half_pair(value(even, 1, i, t + 1, 2 * j), value(odd, 1, i, t + 1, 2 * j + 1));
+      }
+  }
+  uint16_t* rows = a.out[kValue] + page * kPageSize * a.token_stride[kValue] + head * kHeadDim;
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    if (row_of(g) < visible) store8<kWide>(rows + row_of(g) * a.token_stride[kValue] + dim_of(g), out[g]);
 }
 
 template <bool kWide>
 __global__ __launch_bounds__(kWave * kWavesPerBlock) void int4_dequantize_kernel(DequantizeArgs a) {
-  const int64_t page = blockIdx.x;
-  const int head = blockIdx.y * (blockDim.x / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int waves = blockDim.x / kWave, per_page = (a.heads + waves - 1) / waves;
+  const int64_t page = blockIdx.x / per_page;
+  const int head = blockIdx.x % per_page * waves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   if (head >= a.heads) return;
-  if (blockIdx.z == 0)
+  if (blockIdx.y == 0)
     dequantize_part<kWide, false>(a, page, head, threadIdx.x % kWave);
   else
     dequantize_part<kWide, true>(a, page, head, threadIdx.x % kWave);
@@ -438,7 +497,7 @@ extern "C" int32_t pg_int4_quantize_pages(const void* key, int64_t key_token_str
                         static_cast<const void*>(exact_key_pages), static_cast<const void*>(exact_value_pages)})
     wide = wide && aligned16(p);
   const int waves = std::min(heads, kWavesPerBlock);
-  const dim3 grid(static_cast<uint32_t>(a.pages), (heads + waves - 1) / waves, 2);
+  const dim3 grid(static_cast<uint32_t>(a.pages * ((heads + waves - 1) / waves)), 2);
   if (wide)
     hipLaunchKernelGGL(int4_quantize_kernel<true>, grid, dim3(kWave * waves), 0, as_stream(stream), a);
   else
@@ -479,7 +538,7 @@ extern "C" int32_t pg_int4_dequantize_pages(const void* codes, const void* scale
   for (const void* p : {key_center, value_center, static_cast<const void*>(key), static_cast<const void*>(value)})
     wide = wide && aligned16(p);
   const int waves = std::min(heads, kWavesPerBlock);
-  const dim3 grid(static_cast<uint32_t>(a.pages), (heads + waves - 1) / waves, 2);
+  const dim3 grid(static_cast<uint32_t>(a.pages * ((heads + waves - 1) / waves)), 2);
   if (wide)
     hipLaunchKernelGGL(int4_dequantize_kernel<true>, grid, dim3(kWave * waves), 0, as_stream(stream), a);
   else
