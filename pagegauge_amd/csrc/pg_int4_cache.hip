@@ -29,7 +29,7 @@ namespace {
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr int kWavesPerBlock = 4;
-constexpr int64_t kMaxBlocks = UINT32_MAX / (kWave * kWavesPerBlock);   // of a launch, a dimension
+constexpr int64_t kMaxBlocks = UINT32_MAX / (kWave * kWavesPerBlock);   // of a launch's first dimension
 
 __device__ __forceinline__ uint16_t int4_scale_bits(float maximum) {
   return __half_as_ushort(__float2half_rn(fmaxf(maximum * (1.0f / 7.0f), 0x1p-20f)));
@@ -213,8 +213,8 @@ __device__ __forceinline__ void quantize_part(const QuantizeArgs& a, int64_t pag
                     a.scales + block * kInt4BlockScales, lane);
 }
 
-// Grid (pages, blocks of up to 4 heads, 2): a wave per (page, head), K and V by
-// blockIdx.z.
+// A wave per (page, head), in the order of memory: blocks of up to 4 heads of page
+// after page by blockIdx.x, K and V by blockIdx.y.
 template <bool kWide>
 __global__ __launch_bounds__(kWave * kWavesPerBlock) void int4_quantize_kernel(QuantizeArgs a) {
   const int waves = blockDim.x / kWave, per_page = (a.heads + waves - 1) / waves;
@@ -491,13 +491,13 @@ extern "C" int32_t pg_int4_quantize_pages(const void* key, int64_t key_token_str
   a.num_code_pages = num_code_pages;
   a.num_exact_pages = exact_page_ids ? num_exact_pages : 0;
   a.heads = heads;
-  if (a.pages > kMaxBlocks) return fail(PG_ERROR_UNSUPPORTED, "too many pages for one call");
   bool wide = key_token_stride % 8 == 0 && value_token_stride % 8 == 0;
   for (const void* p : {key, value, key_center, value_center,
                         static_cast<const void*>(exact_key_pages), static_cast<const void*>(exact_value_pages)})
     wide = wide && aligned16(p);
-  const int waves = std::min(heads, kWavesPerBlock);
-  const dim3 grid(static_cast<uint32_t>(a.pages * ((heads + waves - 1) / waves)), 2);
+  const int waves = std::min(heads, kWavesPerBlock), per_page = (heads + waves - 1) / waves;
+  if (a.pages > kMaxBlocks / per_page) return fail(PG_ERROR_UNSUPPORTED, "too many pages for one call");
+  const dim3 grid(static_cast<uint32_t>(a.pages * per_page), 2);
   if (wide)
     hipLaunchKernelGGL(int4_quantize_kernel<true>, grid, dim3(kWave * waves), 0, as_stream(stream), a);
   else
@@ -533,12 +533,12 @@ extern "C" int32_t pg_int4_dequantize_pages(const void* codes, const void* scale
   a.pages = (tokens - 1) / kPageSize + 1;
   a.num_code_pages = num_code_pages;
   a.heads = heads;
-  if (a.pages > kMaxBlocks) return fail(PG_ERROR_UNSUPPORTED, "too many pages for one call");
   bool wide = key_token_stride % 8 == 0 && value_token_stride % 8 == 0;
   for (const void* p : {key_center, value_center, static_cast<const void*>(key), static_cast<const void*>(value)})
     wide = wide && aligned16(p);
-  const int waves = std::min(heads, kWavesPerBlock);
-  const dim3 grid(static_cast<uint32_t>(a.pages * ((heads + waves - 1) / waves)), 2);
+  const int waves = std::min(heads, kWavesPerBlock), per_page = (heads + waves - 1) / waves;
+  if (a.pages > kMaxBlocks / per_page) return fail(PG_ERROR_UNSUPPORTED, "too many pages for one call");
+  const dim3 grid(static_cast<uint32_t>(a.pages * per_page), 2);
   if (wide)
     hipLaunchKernelGGL(int4_dequantize_kernel<true>, grid, dim3(kWave * waves), 0, as_stream(stream), a);
   else

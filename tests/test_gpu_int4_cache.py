@@ -178,6 +178,26 @@ def test_rope_append(cuda, batch, q_heads, kv_heads, layout, part, scaling):
     assert torch.equal(codes[others], codes_before[others]) and not scales[others].any()
 
 
+@pytest.mark.parametrize("layout,part", [("half", 128), ("interleaved", 128), ("half", 66)])
+def test_append_turns_as_rotate_does(cuda, layout, part):
+    """The same bits of a query or key, whichever kernel turned it."""
+    from pagegauge_amd import int4, rotary
+
+    emb = rotary.RotaryEmbedding(128, part, layout=layout)
+    batch, q_heads, kv_heads = 640, 8, 2
+    q, k = _rows(batch, q_heads, 7).to(cuda), _rows(batch, kv_heads, 8).to(cuda)
+    positions = (torch.arange(batch, dtype=torch.int32) * 7919 % 131072).to(cuda)
+    want_q, want_k = emb.rotate(q, k, positions)
+    ids = torch.arange(batch, dtype=torch.int32, device=cuda)
+    none = torch.full_like(ids, -1)
+    zeros = torch.zeros(batch, kv_heads, 128, dtype=torch.float16, device=cuda)
+    rotated, (codes, scales) = torch.empty_like(q), int4.allocate_pages(1, kv_heads, cuda)
+    ring = [torch.zeros(batch, 16, kv_heads, 128, dtype=torch.float16, device=cuda) for _ in range(2)]
+    int4.rope_append(emb, q, k, k, positions, ids, none, zeros, zeros, rotated, *ring, codes, scales)
+    assert torch.equal(rotated, want_q)
+    assert torch.equal(ring[0][ids.long(), positions.long() % 16], want_k)
+
+
 def test_append_skips_ids_outside_the_pools(cuda):
     from pagegauge_amd import int4, rotary
 

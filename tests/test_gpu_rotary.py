@@ -83,6 +83,26 @@ def test_rotation(cuda, dim, part, layout, dtype):
     assert torch.equal(q2, oq) and torch.equal(k2, ok)
 
 
+# tokens and heads of one workgroup, of several, of a last one that is not full;
+# sines of one token that fill the LDS; a vector of copied dims per head
+@pytest.mark.parametrize("tokens,q_heads,kv_heads,dim,part", [
+    (1, 1, 0, 2, 2), (3, 70, 3, 128, 128), (130, 290, 10, 256, 256), (2, 3, 1, 16384, 16384),
+    (2, 3, 1, 16384, 2), (5001, 13, 1, 64, 32), (2, 9000, 1, 4, 2), (70001, 1, 1, 16, 16)])
+def test_rows_of_any_count(cuda, tokens, q_heads, kv_heads, dim, part):
+    from pagegauge_amd import rotary
+
+    print(f"rotary tokens={tokens} heads={q_heads}/{kv_heads} dim={dim} part={part}", flush=True)
+    emb = rotary.RotaryEmbedding(dim, part, 1.0e4, "interleaved" if tokens % 2 else "half")
+    f = rotary.frequencies(part, 1.0e4)
+    positions = torch.arange(tokens, device=cuda, dtype=torch.int64) * 101
+    q = _rows(cuda, torch.float16, tokens, q_heads, dim, 3)
+    k = _rows(cuda, torch.float16, tokens, kv_heads, dim, 4) if kv_heads else None
+    oq, ok = emb.rotate(q, k, positions)
+    _check(emb, f, q, positions, oq)
+    if kv_heads:
+        _check(emb, f, k, positions, ok)
+
+
 @pytest.mark.parametrize("scaling,factor", [("linear", 8.0), ("ntk", 4.0), ("by_parts", 16.0)])
 def test_scalings(cuda, scaling, factor):
     from pagegauge_amd import rotary

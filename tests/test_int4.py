@@ -182,6 +182,11 @@ def test_decode_refuses_memory_of_the_host():
                                 16, 1, None), 1, "exact page ids"),
     ("pg_int4_quantize_pages", (4096, 1, 4096, 1, None, None, 4096, 4096, 1, None, None, None, None, 0,
                                 1 << 50, 8, None), 3, "too many pages"),
+    # fewer pages than a launch has workgroups, but not times two blocks of heads
+    ("pg_int4_quantize_pages", (4096, 1, 4096, 1, None, None, 4096, 4096, 1, None, None, None, None, 0,
+                                16 * 10 ** 7, 8, None), 3, "too many pages"),
+    ("pg_int4_dequantize_pages", (4096, 4096, 1, None, None, None, 4096, 1, 4096, 1, 16 * 10 ** 7, 8, None),
+     3, "too many pages"),
     ("pg_int4_dequantize_pages", (4096, 4096, 0, None, None, None, 4096, 1, 4096, 1, 16, 1, None), 1,
      "no pages"),
     ("pg_int4_dequantize_pages", (4096, 4096, 1, None, None, None, 4096, 1, 4096, 1, -1, 1, None), 1,

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from pagegauge_amd import rotary
+from pagegauge_amd import _capi, rotary
 
 
 def test_frequencies():
@@ -76,3 +76,18 @@ def test_in_place_is_all_or_nothing():
     q = torch.zeros(3, 4, 128, dtype=torch.float16)
     with pytest.raises(ValueError, match="together"):
         _call(query=q, out_query=q)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="host-only checks of the C entry point")
+@pytest.mark.parametrize("over,code,message", [
+    (dict(head_dim=16386, rotary_dim=128), 3, "16384 dims"), (dict(query_heads=65536), 3, "65535 heads"),
+    (dict(query_heads=0), 1, "with a head"), (dict(rotary_dim=130), 1, "even number"),
+    (dict(position_bytes=2), 1, "int32 or int64"), (dict(dtype=3), 1, "FP16, BF16 or FP32"),
+    (dict(out_query=None), 1, "null tensor"), (dict(tokens=1 << 50), 3, "too many rows")])
+def test_c_entry_point_refuses(over, code, message):
+    a = dict(query=4096, query_token=512, query_head=128, query_heads=4, key=None, key_token=0, key_head=0,
+             key_heads=0, out_query=4096, out_query_token=512, out_query_head=128, out_key=None,
+             out_key_token=0, out_key_head=0, positions=4096, position_bytes=4, turns=4096,
+             amplitude=1.0, tokens=3, head_dim=128, rotary_dim=128, interleaved=0, dtype=0, stream=None)
+    a.update(over)
+    assert _capi.library().pg_rotate(*a.values()) == code and message in _capi.last_error()
