@@ -632,7 +632,8 @@ int32_t pg_argmax_f32(const float* x, int32_t rows, int32_t n, int64_t row_strid
  * in elements; key_heads may be 0 (then its pointers are not used).  Outputs
  * may be the inputs themselves, query and key alike.  positions is int32 or
  * int64 (position_bytes 4 or 8), turns float64 [rotary_dim/2].  Angles are
- * reduced in 64 bits, the rotation is float32, rounded once. */
+ * reduced in 64 bits, the rotation is float32, rounded once.  At most 65535
+ * query and 65535 key heads of 16384 dims. */
 int32_t pg_rotate(const void* query, int64_t query_token_stride, int64_t query_head_stride,
                   int32_t query_heads, const void* key, int64_t key_token_stride,
                   int64_t key_head_stride, int32_t key_heads, void* out_query,
