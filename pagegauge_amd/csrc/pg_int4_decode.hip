@@ -6,17 +6,18 @@
 // over codes k, v in [-7, 7] and one scale per token, head and part.  The key
 // center shifts all of a request's scores alike and is left out.
 //
-// A workgroup takes one KV head, up to 8 of its query heads and a range of
-// pages; its 4 waves take groups of 4 pages in turn and meet in LDS once, at the
-// end.  Everything else stays in registers, with hardly an exchange between
-// lanes:
+// A workgroup takes one KV head with its query heads and a range of pages; its 4
+// waves take groups of 4 pages in turn and meet in LDS once, at the end.
+// Everything else stays in registers, with hardly an exchange between lanes:
 //  * QK as K Q^T: tokens are the MFMA's rows, heads its columns, so lane (kg, n)
-//    gets the scores of tokens 4 kg .. 4 kg + 3 for head n % 8.
+//    gets the scores of tokens 4 kg .. 4 kg + 3 for head n % 8, or n where the KV
+//    head has more than 8 (kWide).
 //  * These are, pair of pages by pair, exactly the k slots that the lane feeds
 //    as the A operand of P V: probabilities never leave their lane.  Columns
 //    n < 8 hand over the FP16 part of a probability and columns n >= 8 (the same
 //    heads again) its remainder, so rows r and r + 8 of the product add up to
-//    one of about 22 bits.
+//    one of about 22 bits.  With kWide the two parts are a product each (16 heads
+//    per KV head, 256 requests: 185 us, as two workgroups of 8 heads 268).
 //  * A nibble u = code + 8 masked out of its dword is the FP16 subnormal
 //    u * 2^-24, or 16 u * 2^-24 one nibble further up, and MFMAs multiply
 //    subnormals exactly: 5 operations make 8 operands of V.  Its offset of 8 comes
@@ -59,7 +60,7 @@ typedef uint16_t v2s __attribute__((ext_vector_type(2)));
 
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr int kThreads = kWave * kInt4Waves;
-constexpr int kHeads = kInt4HeadsPerWave;
+constexpr int kNarrowHeads = 8;    // query heads whose probabilities' parts share a product
 
 struct Int4Args {
   const uint16_t* query;
@@ -81,7 +82,7 @@ struct Int4Args {
   uint16_t* out;
   float* lse;
   float sm_scale_log2;
-  int num_qo_heads, num_kv_heads, group, subs;
+  int num_qo_heads, num_kv_heads, group;
 };
 
 __device__ __forceinline__ v2h as_half2(uint32_t bits) { return __builtin_bit_cast(v2h, bits); }
@@ -112,7 +113,7 @@ __device__ __forceinline__ float times_half(float x, uint32_t pair, int which) {
 
 constexpr float kSlack = 4.0f;     // how far (base 2) a score may pass the base
 
-// Running state of one wave.  Lane (kg, n) has head n % 8's: base (before the
+// Running state of one wave.  Lane (kg, n) has head n % 8's (kWide: n's): base (before the
 // softmax scale), limit past which it moves, and offset, the exponent of the sums
 // minus the scaled base; l0 and l1 sum the lane's own tokens 4 kg, 4 kg + 1 and, in
 // sixteenths, 4 kg + 2, 4 kg + 3.  acc[nb][r] is row 4 kg + r of the product,
@@ -135,12 +136,13 @@ __device__ __forceinline__ void scale_sums(State& st, const float (&f)[4]) {
 // Softmax step over kPages pages: s are the lane's scores, masked ones -inf,
 // v_scale pairs of V's scales (FP16; 0 where masked), ``scale`` the softmax scale
 // in base 2, ``exponent`` that of the sums.  p: the lane's rows of the A operand
-// of P V, tokens 4 kg + 2, 4 kg + 3 in sixteenths with kCodes.
-template <int kPages, bool kCodes>
+// of P V, tokens 4 kg + 2, 4 kg + 3 in sixteenths with kCodes; rows of the FP16 part
+// and of the remainder in one, or with kWide in one after the other.
+template <int kPages, bool kCodes, bool kWide>
 __device__ __forceinline__ void softmax_step(State& st, const float (&s)[kPages][4],
                                              const uint32_t (&v_scale)[kPages][2], float scale,
                                              float exponent, float low_part, int lane,
-                                             v8h (&p)[kPages / 2]) {
+                                             v8h (&p)[1 + kWide][kPages / 2]) {
   float top = kNegInf;
 #pragma unroll
   for (int i = 0; i < kPages; ++i)
@@ -160,13 +162,13 @@ __device__ __forceinline__ void softmax_step(State& st, const float (&s)[kPages]
     const int kg = lane >> 4;
     float f[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) f[r] = __shfl(alpha, (4 * kg + r) & 7, kWave);
+    for (int r = 0; r < 4; ++r) f[r] = __shfl(alpha, (4 * kg + r) & (kWide ? 15 : 7), kWave);
     scale_sums(st, f);
   }
   const float offset1 = kCodes ? st.offset - 4.0f : st.offset;
 #pragma unroll
   for (int j = 0; j < kPages / 2; ++j) {
-    uint32_t words[4];
+    uint32_t words[1 + kWide][4];
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
       const int page = 2 * j + (h >> 1), r = 2 * (h & 1);
@@ -178,10 +180,13 @@ __device__ __forceinline__ void softmax_step(State& st, const float (&s)[kPages]
       const float w1 = kCodes ? times_half(x1, v_scale[page][h & 1], 1) : x1;
       // the FP16 part, or what it leaves (rounding down costs the second 2^-21)
       const v2h high = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(w0, w1));
-      words[h] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(
+      if (kWide) words[0][h] = __builtin_bit_cast(uint32_t, high);
+      words[kWide][h] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(
           fmaf(-low_part, static_cast<float>(high.x), w0), fmaf(-low_part, static_cast<float>(high.y), w1)));
     }
-    p[j] = operand(words[0], words[1], words[2], words[3]);
+#pragma unroll
+    for (int part = 0; part < 1 + kWide; ++part)
+      p[part][j] = operand(words[part][0], words[part][1], words[part][2], words[part][3]);
   }
 }
 
@@ -202,7 +207,9 @@ struct Group {
   v4u k[kInt4GroupPages], v[kInt4GroupPages], s[kInt4GroupPages];
 };
 
+template <bool kWide>
 __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
+  constexpr int kHeads = kWide ? 16 : kNarrowHeads;
   __shared__ float part_o[kInt4Waves][kHeads][kHeadDim];
   __shared__ float part_m[kInt4Waves][kHeads];
   __shared__ float part_l[kInt4Waves][kHeads];
@@ -210,17 +217,15 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
   const int lane = threadIdx.x % kWave;
   const int n = lane & 15, kg = lane >> 4;
   const Int4Item it = a.items[blockIdx.x];
-  const int kv = blockIdx.y / a.subs;
-  const int first_head = (blockIdx.y % a.subs) * kHeads;     // within the KV head's group
-  const int heads = min(kHeads, a.group - first_head);
+  const int kv = blockIdx.y, heads = a.group;
   const int hkv = a.num_kv_heads;
 
-  // query: B operand, column n = head n % 8, dims 32 w + 8 kg ..; columns past
+  // query: B operand, column n = head n % kHeads, dims 32 w + 8 kg ..; columns past
   // the heads repeat the first one and are dropped at the end
   v8h q[4];
   {
     const uint16_t* row = a.query + it.request * a.query_batch_stride +
-                          static_cast<int64_t>(kv * a.group + first_head + ((n & 7) < heads ? n & 7 : 0)) * kHeadDim;
+                          static_cast<int64_t>(kv * a.group + (n % kHeads < heads ? n % kHeads : 0)) * kHeadDim;
 #pragma unroll
     for (int w = 0; w < 4; ++w) q[w] = *reinterpret_cast<const v8h*>(row + 32 * w + 8 * kg);
   }
@@ -228,7 +233,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) consume_point(q[w]);
   };
-  const float low_part = n < 8 ? 0.0f : 1.0f;
+  const float low_part = kWide || n >= kHeads ? 1.0f : 0.0f;
 
   State st;
   st.base = st.limit = kNegInf;
@@ -346,21 +351,28 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
           }
         }
       }
-      v8h p[kInt4GroupPages / 2];
-      softmax_step<kInt4GroupPages, true>(st, s, v_scale, scale, exponent, low_part, lane, p);
+      v8h p[1 + kWide][kInt4GroupPages / 2];
+      softmax_step<kInt4GroupPages, true, kWide>(st, s, v_scale, scale, exponent, low_part, lane, p);
 #pragma unroll
       for (int i = 0; i < kInt4GroupPages; ++i) consume_point(cur.v[i]);
+      auto product = [&](const v8h (&rows)[1 + kWide], v8h columns, v4f sum) {
+#pragma unroll
+        for (int part = 0; part < 1 + kWide; ++part)
+          sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(rows[part], columns, sum, 0, 0, 0);
+        return sum;
+      };
 #pragma unroll
       for (int j = 0; j < kInt4GroupPages / 2; ++j) {
-        st.eights = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-            p[j], operand(kEvenEights, kOddEights, kEvenEights, kOddEights), st.eights, 0, 0, 0);
+        v8h rows[1 + kWide];
+#pragma unroll
+        for (int part = 0; part < 1 + kWide; ++part) rows[part] = p[part][j];
+        st.eights = product(rows, operand(kEvenEights, kOddEights, kEvenEights, kOddEights), st.eights);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const uint32_t x = cur.v[2 * j][w], y = cur.v[2 * j + 1][w];
-          st.acc[2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              p[j], operand(even(x), odd(x), even(y), odd(y)), st.acc[2 * w], 0, 0, 0);
-          st.acc[2 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              p[j], operand(even(x >> 8), odd(x >> 8), even(y >> 8), odd(y >> 8)), st.acc[2 * w + 1], 0, 0, 0);
+          st.acc[2 * w] = product(rows, operand(even(x), odd(x), even(y), odd(y)), st.acc[2 * w]);
+          st.acc[2 * w + 1] = product(rows, operand(even(x >> 8), odd(x >> 8), even(y >> 8), odd(y >> 8)),
+                                      st.acc[2 * w + 1]);
         }
       }
     };
@@ -432,9 +444,9 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
           if (r >= limit[i]) v[i][r] = v4u{0u, 0u, 0u, 0u};
         }
       }
-      v8h p[1];
+      v8h p[1 + kWide][1];
       const uint32_t unscaled[2][2] = {};
-      softmax_step<2, false>(st, s, unscaled, a.sm_scale_log2, exponent, low_part, lane, p);
+      softmax_step<2, false, kWide>(st, s, unscaled, a.sm_scale_log2, exponent, low_part, lane, p);
 #pragma unroll
       for (int nb = 0; nb < 8; ++nb) {
         v4u cols;
@@ -443,12 +455,14 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
           cols[2 * i] = pick(v[i][0][nb >> 1], v[i][1][nb >> 1], nb & 1);
           cols[2 * i + 1] = pick(v[i][2][nb >> 1], v[i][3][nb >> 1], nb & 1);
         }
-        st.acc[nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[0], __builtin_bit_cast(v8h, cols), st.acc[nb], 0, 0, 0);
+#pragma unroll
+        for (int part = 0; part < 1 + kWide; ++part)
+          st.acc[nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[part][0], __builtin_bit_cast(v8h, cols), st.acc[nb], 0, 0, 0);
       }
     }
   }
 
-  // ---- the waves meet: rows r and r + 8 of the product, then 4 partial states
+  // ---- the waves meet: parts of the product's rows, then 4 partial states
   float l_sum = st.l0 + st.l1;
   l_sum += __shfl_xor(l_sum, 16, kWave);
   l_sum += __shfl_xor(l_sum, 32, kWave);
@@ -457,10 +471,19 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
     part_m[wave][n] = st.base * a.sm_scale_log2;
     part_l[wave][n] = l_sum * __builtin_amdgcn_exp2f(-exponent);
   }
-  // a swap of two registers' halves adds rows r and r + 8 of two channels at
-  // once: lanes below 32 end with channel 8 n + 2 p, the others with the next
+  // part_o[..][64 b + c]: dim 2 c + b.  A swap of two registers' halves adds rows r
+  // and r + 8 of two channels at once: lanes below 32 end with channel 8 n + 2 p, the
+  // others with the next; with kWide rows are whole.
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
+    if (kWide) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        *reinterpret_cast<float4*>(&part_o[wave][(4 * kg + r) % kHeads][64 * b + 4 * n]) =
+            make_float4(st.acc[b][r] * scale, st.acc[2 + b][r] * scale, st.acc[4 + b][r] * scale,
+                        st.acc[6 + b][r] * scale);
+      continue;
+    }
     float o[4];
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
@@ -468,7 +491,6 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
                                                      __float_as_uint(st.acc[2 * p + 1][r]), false, false);
       o[p] = (__uint_as_float(x.x) + __uint_as_float(x.y)) * scale;
     }
-    // part_o[..][64 b + c]: dim 2 c + b
     *reinterpret_cast<float4*>(&part_o[wave][4 * (kg & 1) + r][64 * (lane >> 5) + 4 * n]) =
         make_float4(o[0], o[1], o[2], o[3]);
   }
@@ -489,7 +511,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
       o.x += f * x.x;
       o.y += f * x.y;
     }
-    const int head = kv * a.group + first_head + h;
+    const int head = kv * a.group + h;
     if (it.items_in_request > 1) {
       const int64_t row = static_cast<int64_t>(blockIdx.x) * a.num_qo_heads + head;
       *reinterpret_cast<float2*>(a.partial_o + row * kHeadDim + 2 * lane) = o;
@@ -706,9 +728,11 @@ extern "C" int32_t pg_int4_decode_run(const pg_int4_plan_t* plan, const void* qu
   a.num_qo_heads = plan->num_qo_heads;
   a.num_kv_heads = plan->num_kv_heads;
   a.group = plan->num_qo_heads / plan->num_kv_heads;
-  a.subs = (a.group + kHeads - 1) / kHeads;
-  hipLaunchKernelGGL(int4_decode_kernel, dim3(plan->num_items, plan->num_kv_heads * a.subs),
-                     dim3(kThreads), 0, as_stream(stream), a);
+  const dim3 grid(plan->num_items, plan->num_kv_heads);
+  if (a.group <= kNarrowHeads)
+    hipLaunchKernelGGL(int4_decode_kernel<false>, grid, dim3(kThreads), 0, as_stream(stream), a);
+  else
+    hipLaunchKernelGGL(int4_decode_kernel<true>, grid, dim3(kThreads), 0, as_stream(stream), a);
   if (int32_t rc = check_launch("int4_decode")) return rc;
   if (plan->max_items_per_request <= 1) return PG_OK;
   Int4CombineArgs c{};

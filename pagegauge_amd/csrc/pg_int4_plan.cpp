@@ -54,8 +54,6 @@ int32_t build_int4_plan(const int32_t* host_indptr, const int32_t* host_tail_ind
   // their pages (49K tokens: 32 items 16.6 us, 64 items 18.1; 64K 18.9 and 20.8),
   // and two where they cannot (128K tokens: 33 items, an uneven round, 46.8 us, 64
   // items 33.6; 16 requests of 8K 38.3 and 34.4).
-  const int64_t groups = static_cast<int64_t>(num_kv_heads) *
-                         ceil_div(num_qo_heads / num_kv_heads, kInt4HeadsPerWave);
   const int64_t cus = num_cus > 0 ? num_cus : 256;
   auto balanced = [&](int64_t target) {
     int64_t low = kInt4Waves * kInt4GroupPages, high = std::max(low, total);
@@ -67,8 +65,8 @@ int32_t build_int4_plan(const int32_t* host_indptr, const int32_t* host_tail_ind
     }
     return high;
   };
-  int64_t cap = balanced(std::max<int64_t>(batch_size, cus / groups));
-  if (cap > kInt4MaxItemPages) cap = balanced(std::max<int64_t>(batch_size, 2 * cus / groups));
+  int64_t cap = balanced(std::max<int64_t>(batch_size, cus / num_kv_heads));
+  if (cap > kInt4MaxItemPages) cap = balanced(std::max<int64_t>(batch_size, 2 * cus / num_kv_heads));
   items.clear();
   item_ptr.assign(batch_size + 1, 0);
   int64_t most = 0;

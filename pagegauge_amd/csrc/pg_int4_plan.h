@@ -13,12 +13,10 @@ namespace pg {
 constexpr int kInt4Waves = 4;           // waves of a workgroup, sharing one item's pages
 constexpr int kInt4GroupPages = 4;      // consecutive pages a wave takes at a time
 constexpr int kInt4MaxItemPages = kInt4Waves * 64;   // a wave holds its page ids one per lane
-constexpr int kInt4HeadsPerWave = 8;    // query heads of a KV head that one wave takes
 constexpr int kInt4MaxItemsPerRequest = 4096;
 constexpr int kInt4TailWeight = 4;      // an FP16 page's bytes in 4-bit pages
 
-// One workgroup's share of a request, for one KV head and up to 8 of its query
-// heads: history pages [page_begin, page_end) of the page table and exact
+// One workgroup's share of a request, for one KV head: history pages [page_begin, page_end) of the page table and exact
 // pages [tail_begin, tail_end) of the tail's, either perhaps empty.
 struct Int4Item {
   int32_t request;

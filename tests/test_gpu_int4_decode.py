@@ -78,13 +78,18 @@ class Case:
                 assert np.isneginf(lse[b]).all()
 
 
+# up to 8 query heads per KV head, and more
+both_forms = pytest.mark.parametrize("kv_heads,group", [(8, 4), (2, 16)])
+
+
 # one token, inside a page, whole groups of pages, several items, past an item's pages
 @pytest.mark.parametrize("history,tail", [
     ([1], [0]), ([0], [1]), ([17], [15]), ([64], [33]), ([512], [256]), ([4000], [256]),
     ([9001], [16]), ([0, 1, 300, 0, 65, 2048], [0, 0, 256, 40, 17, 250])])
-def test_lengths(cuda, history, tail):
-    print(f"attention history={history} tail={tail}", flush=True)
-    c = Case(cuda, history, tail, 8, 4)
+@both_forms
+def test_lengths(cuda, history, tail, kv_heads, group):
+    print(f"attention history={history} tail={tail} heads={kv_heads}x{group}", flush=True)
+    c = Case(cuda, history, tail, kv_heads, group)
     c.check(*c.run())
 
 
@@ -119,30 +124,33 @@ def test_no_center_given_outputs_and_strides(cuda):
 
 
 @pytest.mark.parametrize("scale", [2.0 ** -14, 2000.0])
-def test_scales_of_any_size(cuda, scale):
+@both_forms
+def test_scales_of_any_size(cuda, scale, kv_heads, group):
     """Values far below and above 1 beside exact ones near 1."""
-    c = Case(cuda, [500, 20], [30, 0], 4, 4, scale=scale)
+    c = Case(cuda, [500, 20], [30, 0], kv_heads, group, scale=scale)
     c.scales[..., 0, :] = 0.1           # K's
     c.check(*c.run())
 
 
-def test_scores_far_apart(cuda):
+@both_forms
+def test_scores_far_apart(cuda, kv_heads, group):
     """One token outweighs all others by any factor; all tokens alike."""
-    c = Case(cuda, [900], [60], 2, 4)
+    c = Case(cuda, [900], [60], kv_heads, group)
     c.q *= 30.0
     c.check(*c.run())
     c.q.zero_()
     c.check(*c.run())
 
 
-def test_what_lies_behind_the_last_token_is_not_read(cuda):
+@both_forms
+def test_what_lies_behind_the_last_token_is_not_read(cuda, kv_heads, group):
     """NaN and infinities in the masked rows of both kinds of pages."""
-    c = Case(cuda, [37, 530], [21, 5], 4, 4)
+    c = Case(cuda, [37, 530], [21, 5], kv_heads, group)
     want = c.run()
     for b in range(2):
         page = int(c.tables[0][1][int(c.tables[0][0][b + 1]) - 1])
         used = (c.history[b] - 1) % 16 + 1
-        rows = c.scales[page].view(4, 4, 2, 4)
+        rows = c.scales[page].view(kv_heads, 4, 2, 4)
         for t in range(used, 16):
             rows[:, t // 4, :, t % 4] = float("nan") if t % 2 else float("inf")
         page = int(c.tables[1][1][int(c.tables[1][0][b + 1]) - 1])
@@ -167,9 +175,10 @@ def test_lengths_are_read_on_the_device(cuda):
     assert torch.equal(out, lone.center.repeat_interleave(4, dim=1)) and torch.isneginf(lse).all()
 
 
-def test_infinite_scores(cuda):
+@pytest.mark.parametrize("group", [4, 16])
+def test_infinite_scores(cuda, group):
     """Scores of -inf leave the others; a NaN score makes its head NaN."""
-    c = Case(cuda, [0], [40], 1, 4)
+    c = Case(cuda, [0], [40], 1, group)
     c.q[:] = 1.0
     c.exact[0].fill_(0.25)
     first = int(c.tables[1][1][0])
@@ -181,7 +190,7 @@ def test_infinite_scores(cuda):
     c.exact[0][first, :, 0, 0] = 0.25
     c.q[0, 2, 0] = float("nan")
     out, lse = c.run()
-    assert out[0, 2].isnan().all() and out[0, [0, 1, 3]].isfinite().all()
+    assert out[0, 2].isnan().all() and out[0, [h for h in range(group) if h != 2]].isfinite().all()
 
 
 def test_pool_past_4_gib(cuda):
