@@ -177,16 +177,13 @@ int32_t dispatch(RotaryArgs a, int vec, int head_dim, bool interleaved, void* st
   const int units = a.turned_units + (copies ? (head_dim - a.rotary_dim) / (2 * vec) : 0);
   const int heads = a.rows[0].heads + a.rows[1].heads;
   const int64_t per_token = static_cast<int64_t>(heads) * units;
-  // many units: 640 per workgroup, of whole tokens; few: about one per thread, a
-  // token's heads over several workgroups (8 tokens of 40 heads 2.9 us, in whole
-  // tokens 3.4; 1024 5.6 and 6.2; but 4096 16.4 and 15.0)
-  a.tokens_per_block = 1;
-  a.heads_per_slice = heads;
-  if (a.tokens * per_token >= kFull)
-    a.tokens_per_block = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(
-        kBlockUnits / per_token, kMaxPairs / (a.rotary_dim / 2))));
-  else
-    a.heads_per_slice = std::min(heads, std::max(1, kThreads / units));
+  // Whole tokens of 640 units per workgroup, where there are many, and of one per
+  // thread otherwise; a token of more than that is cut at its heads (8 tokens of 40
+  // heads 2.9 us, whole 3.4; 1024 5.6 and 6.2; but 4096 16.4 and 15.0).
+  const bool many = a.tokens * per_token >= kFull;
+  const int64_t fit = (many ? kBlockUnits : kThreads) / per_token;
+  a.tokens_per_block = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(fit, kMaxPairs / (a.rotary_dim / 2))));
+  a.heads_per_slice = many ? heads : std::min(heads, std::max(1, kThreads / units));
   // numbers and divisors of place() stay below 2^16
   a.heads_per_slice = std::min(a.heads_per_slice, std::max(1, kMaxUnits / units));
   a.pairs = Divisor::by(a.rotary_dim / 2);
