@@ -48,25 +48,41 @@ int32_t build_int4_plan(const int32_t* host_indptr, const int32_t* host_tail_ind
     history += r.pages;
     exact_pages += r.tail;
   }
-  // The smallest largest share (``cap``, in weighted pages) with which the batch
-  // takes no more workgroups than ``target``, but at least one group of pages per
-  // wave.  One workgroup per CU is the better plan as long as its waves can hold
-  // their pages (49K tokens: 32 items 16.6 us, 64 items 18.1; 64K 18.9 and 20.8),
-  // and two where they cannot (128K tokens: 33 items, an uneven round, 46.8 us, 64
-  // items 33.6; 16 requests of 8K 38.3 and 34.4).
+  // ``balanced``: the smallest largest share (``cap``, in weighted pages) with which the
+  // batch takes no more workgroups than ``target``, but at least one group of pages
+  // per wave.
   const int64_t cus = num_cus > 0 ? num_cus : 256;
+  auto items_of = [&](int64_t cap) {
+    int64_t n = 0;
+    for (const Request& r : requests) n += r.cuts(cap);
+    return n;
+  };
   auto balanced = [&](int64_t target) {
     int64_t low = kInt4Waves * kInt4GroupPages, high = std::max(low, total);
     while (low < high) {
       const int64_t cap = low + (high - low) / 2;
-      int64_t n = 0;
-      for (const Request& r : requests) n += r.cuts(cap);
-      if (n <= target) high = cap; else low = cap + 1;
+      if (items_of(cap) <= target) high = cap; else low = cap + 1;
     }
     return high;
   };
-  int64_t cap = balanced(std::max<int64_t>(batch_size, cus / num_kv_heads));
-  if (cap > kInt4MaxItemPages) cap = balanced(std::max<int64_t>(batch_size, 2 * cus / num_kv_heads));
+  // One workgroup per CU is the better plan (49K tokens: 32 items 16.6 us, 64 items
+  // 18.1; 64K 18.9 and 20.8) unless its waves cannot hold their pages (128K tokens: 33
+  // items, an uneven round, 46.8 us, 64 items 33.6; 16 requests of 8K 38.3 and 34.4)
+  // or requests do not divide over so few (17 requests of 3.3K: 32 items, of a whole
+  // request the largest, 27.6, 64 items 24.0): then it is two.
+  const int64_t one = std::max<int64_t>(1, cus / num_kv_heads);
+  const int64_t two = std::max<int64_t>(1, 2 * cus / num_kv_heads);
+  int64_t cap = balanced(std::max<int64_t>(batch_size, one));
+  const int64_t cap2 = balanced(std::max<int64_t>(batch_size, two));
+  if (cap > kInt4MaxItemPages || 10 * cap > 24 * cap2) {
+    // More than two per CU are brought to whole rounds (6 requests of 13K to 70K: 66
+    // items 73.4 us, 128 items 60.5; 84 of 468 to 4391 tokens 77.2 and 71; 90 of 500
+    // to 8000: 141 items 105, 192 items 99), unless there are more than two rounds
+    // and no request is cut yet (130 of 512 to 4000: 93.6, 192 items 101.3).
+    cap = cap2;
+    const int64_t n = items_of(cap), rounds = ceil_div(n, two);
+    if (rounds == 2 || (rounds > 2 && rounds <= 4 && n > batch_size)) cap = balanced(rounds * two);
+  }
   items.clear();
   item_ptr.assign(batch_size + 1, 0);
   int64_t most = 0;
