@@ -73,12 +73,14 @@ struct alignas(sizeof(T) * kVec) Vec {
 
 // Grid (rows, tiles), so that the tiles of a row are a multiple of the batch apart
 // and, in batches of whole eights, share an XCD's L2 for the row's history (64 rows
-// 17.2 us, tiles first 17.8); kVec 1 for rows that are not 16-byte aligned.
+// 17.2 us, tiles first 17.8).  With kVec 1 a value at a time; kShifted for rows that do
+// not all start with a vector: a tile's index 0 does, and a row starts ``pad`` values
+// into its first tile (51 rows of 103354 12.1 us, a value at a time 16.2).
 //
 // The tile's logits and the first tokens of the history are requested before
 // anything else, so that the trips to memory overlap (64 x 131072 with
 // histories of 4096: 20.5 us one after the other).
-template <typename T, typename Token, int kVec>
+template <typename T, typename Token, int kVec, bool kShifted>
 __global__ __launch_bounds__(kThreads) void shape_logits_kernel(LogitsArgs a) {
   constexpr int kSteps = kVec > 1 ? kMaxTile / (kThreads * kVec) : 1;
   constexpr int kBatch = 4;                                    // tokens of a thread in flight
@@ -86,23 +88,47 @@ __global__ __launch_bounds__(kThreads) void shape_logits_kernel(LogitsArgs a) {
   uint32_t* counts = lds;
   int* bias_at = reinterpret_cast<int*>(lds) + a.tile;         // of the tokens that have a bias
   const int row = blockIdx.x;
-  const int base = blockIdx.y * a.tile;
-  const int size = min(a.tile, a.vocab - base);
   const int tid = threadIdx.x;
-  const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride + base;
-  // the mask's bits of a vector: tiles and vectors are aligned to its words
-  const int32_t* allowed = a.allowed ? a.allowed + row * a.allowed_stride + (base >> 5) : nullptr;
-  auto bits = [&](int i) { return allowed ? static_cast<uint32_t>(allowed[i >> 5]) >> (i & 31) : ~0u; };
+  const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
+  T* out = static_cast<T*>(a.out) + row * a.out_stride;
+  const int pad = kShifted ? reinterpret_cast<uintptr_t>(in) / sizeof(T) % kVec : 0;
+  const int base = static_cast<int>(blockIdx.y) * a.tile - pad;      // token at index 0
+  const int low = kShifted && base < 0 ? pad : 0, size = min(a.tile, a.vocab - base);   // the tile's tokens
+  in += base;
+  out += base;
+  if (kShifted && low >= size) return;       // the last tile of a row that needs none
+  const int32_t* allowed = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+  // the mask's bits of the tokens from index i on, of the kVec of a vector with ``both``
+  auto bits = [&](int i, bool both) {
+    if (!allowed) return ~0u;
+    const int token = base + i;
+    const uint32_t word = allowed[token >> 5];
+    if (!kShifted || !both) return word >> (token & 31);
+    const uint64_t next = static_cast<uint32_t>(allowed[(token + kVec - 1) >> 5]);
+    return static_cast<uint32_t>((next << 32 | word) >> (token & 31));
+  };
+  // whole vectors [whole, rest), and a thread for each value before and behind them;
+  // with kVec 1 a thread for each of the first kThreads
+  const int whole = (low + kVec - 1) / kVec * kVec, rest = max(whole, size / kVec * kVec);
+  const int edge = kVec == 1 || tid < kVec ? low + tid : rest + tid - kVec;
+  const bool has_edge = kVec == 1 ? edge < size
+                                  : tid < 2 * kVec && edge < (tid < kVec ? min(whole, size) : size);
   Vec<T, kVec> held[kSteps];
   uint32_t words[kSteps];
-  if (kVec > 1 && size >= kVec) {
+  if (kVec > 1 && whole < rest) {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      // a vector past the row's end is read from its start, and not used
-      const int i = (tid + s * kThreads) * kVec, at = i + kVec <= size ? i : 0;
+      // where there is no whole vector, the first one is read and not used
+      const int i = (tid + s * kThreads) * kVec, at = i >= whole && i < rest ? i : whole;
       held[s] = *reinterpret_cast<const Vec<T, kVec>*>(in + at);
-      words[s] = bits(at);
+      words[s] = bits(at, true);
     }
+  }
+  T edge_value{};
+  uint32_t edge_bits = 0;
+  if (has_edge) {
+    edge_value = in[edge];
+    edge_bits = bits(edge, false);
   }
   const float repetition = a.repetition ? a.repetition[row] : 1.0f;
   const float frequency = a.frequency ? a.frequency[row] : 0.0f;
@@ -128,7 +154,7 @@ __global__ __launch_bounds__(kThreads) void shape_logits_kernel(LogitsArgs a) {
     for (int i = tid; i < a.tile / 4; i += kThreads) reinterpret_cast<uint4*>(counts)[i] = uint4{0u, 0u, 0u, 0u};
     for (int i = tid; i < a.biases; i += kThreads) {
       const int64_t at = static_cast<int64_t>(bias_tokens[i]) - base;
-      if (at >= 0 && at < size) bias_at[at] = -1;
+      if (at >= low && at < size) bias_at[at] = -1;
     }
     __syncthreads();
     for (int64_t first = 0; first < length; first += kBatch * kThreads) {
@@ -137,13 +163,13 @@ __global__ __launch_bounds__(kThreads) void shape_logits_kernel(LogitsArgs a) {
       for (int k = 0; k < kBatch; ++k) {
         const int64_t i = first + tid + k * kThreads;
         const int64_t at = static_cast<int64_t>(batch[k]) - base;
-        if (i >= length || at < 0 || at >= size) continue;
+        if (i >= length || at < low || at >= size) continue;
         if (i >= prompt) atomicAdd(&counts[at], 1u); else atomicOr(&counts[at], kSeen);
       }
     }
     for (int i = tid; i < a.biases; i += kThreads) {
       const int64_t at = static_cast<int64_t>(bias_tokens[i]) - base;
-      if (at < 0 || at >= size) continue;
+      if (at < low || at >= size) continue;
       atomicMax(&bias_at[at], i);
       atomicOr(&counts[at], kBiased);
     }
@@ -159,22 +185,19 @@ __global__ __launch_bounds__(kThreads) void shape_logits_kernel(LogitsArgs a) {
     if (c & kBiased) x += bias_values[bias_at[at]];
     return x;
   };
-  T* out = static_cast<T*>(a.out) + row * a.out_stride + base;
-  auto one = [&](int i, uint32_t bit) {
-    out[i] = bit & 1u ? from_float<T>(shape(to_float(in[i]), counted ? counts[i] : 0u, i)) : from_float<T>(kNegInf);
+  auto one = [&](T x, uint32_t bit, int i) {
+    out[i] = from_float<T>(bit & 1u ? shape(to_float(x), counted ? counts[i] : 0u, i) : kNegInf);
   };
+  if (has_edge) one(edge_value, edge_bits, edge);
   if (kVec == 1) {
-    for (int i = tid; i < size; i += kThreads) one(i, bits(i));
+    for (int i = tid + kThreads; i < size; i += kThreads) one(in[i], bits(i, false), i);
     return;
   }
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
     const int i = (tid + s * kThreads) * kVec;
-    if (i >= size) break;
-    if (i + kVec > size) {
-      for (int e = 0; i + e < size; ++e) one(i + e, bits(i + e));
-      break;
-    }
+    if (i >= rest) break;
+    if (kShifted && i < whole) continue;
     const uint32_t word = words[s];
     uint32_t c[kVec];
 #pragma unroll
@@ -193,22 +216,32 @@ __global__ __launch_bounds__(kThreads) void shape_logits_kernel(LogitsArgs a) {
   }
 }
 
+// How rows lie in vectors of 16 bytes; kSingle: taken value by value.
+enum class Rows { kAligned, kShifted, kSingle };
+
 template <typename T, typename Token>
-int32_t launch(const LogitsArgs& a, int batch, bool wide, void* stream) {
+int32_t launch(const LogitsArgs& a, int batch, Rows rows, void* stream) {
   constexpr int kWide = 16 / sizeof(T);
-  const dim3 grid(batch, (a.vocab + a.tile - 1) / a.tile);
+  const int most = a.vocab + (rows == Rows::kShifted ? kWide - 1 : 0);
+  const dim3 grid(batch, (most + a.tile - 1) / a.tile);
   const size_t lds = sizeof(uint32_t) * a.tile * (a.biases ? 2 : a.history ? 1 : 0);
-  if (wide)
-    hipLaunchKernelGGL((shape_logits_kernel<T, Token, kWide>), grid, dim3(kThreads), lds, as_stream(stream), a);
-  else
-    hipLaunchKernelGGL((shape_logits_kernel<T, Token, 1>), grid, dim3(kThreads), lds, as_stream(stream), a);
+  switch (rows) {
+    case Rows::kAligned:
+      hipLaunchKernelGGL((shape_logits_kernel<T, Token, kWide, false>), grid, dim3(kThreads), lds, as_stream(stream), a);
+      break;
+    case Rows::kShifted:
+      hipLaunchKernelGGL((shape_logits_kernel<T, Token, kWide, true>), grid, dim3(kThreads), lds, as_stream(stream), a);
+      break;
+    default:
+      hipLaunchKernelGGL((shape_logits_kernel<T, Token, 1, false>), grid, dim3(kThreads), lds, as_stream(stream), a);
+  }
   return check_launch("shape_logits");
 }
 
 template <typename T>
-int32_t dispatch(const LogitsArgs& a, int batch, int token_bytes, bool wide, void* stream) {
-  return token_bytes == 8 ? launch<T, int64_t>(a, batch, wide, stream)
-                          : launch<T, int32_t>(a, batch, wide, stream);
+int32_t dispatch(const LogitsArgs& a, int batch, int token_bytes, Rows rows, void* stream) {
+  return token_bytes == 8 ? launch<T, int64_t>(a, batch, rows, stream)
+                          : launch<T, int32_t>(a, batch, rows, stream);
 }
 
 }  // namespace
@@ -267,11 +300,21 @@ extern "C" int32_t pg_shape_logits(const void* logits, int64_t logits_stride, vo
   a.allowed = allowed;
   a.allowed_stride = allowed_stride;
   const int64_t size = dtype == PG_DTYPE_FP32 ? 4 : 2;
-  const bool wide = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
-                    (logits_stride * size) % 16 == 0 && (out_stride * size) % 16 == 0;
+  const uintptr_t first = reinterpret_cast<uintptr_t>(logits), out_first = reinterpret_cast<uintptr_t>(out);
+  const bool strided = batch > 1;
+  // tiles of a value per thread need no vectors, whose threads would be few (4 rows of
+  // 32768 4.1 us, with vectors 4.7)
+  Rows rows = Rows::kSingle;
+  if (a.tile > kThreads) {
+    if (first % 16 == 0 && out_first % 16 == 0 &&
+        !(strided && (logits_stride * size % 16 || out_stride * size % 16)))
+      rows = Rows::kAligned;
+    else if ((first - out_first) % 16 == 0 && !(strided && (logits_stride - out_stride) * size % 16))
+      rows = Rows::kShifted;
+  }
   switch (dtype) {
-    case PG_DTYPE_FP16: return dispatch<__half>(a, batch, token_bytes, wide, stream);
-    case PG_DTYPE_BF16: return dispatch<__hip_bfloat16>(a, batch, token_bytes, wide, stream);
-    default: return dispatch<float>(a, batch, token_bytes, wide, stream);
+    case PG_DTYPE_FP16: return dispatch<__half>(a, batch, token_bytes, rows, stream);
+    case PG_DTYPE_BF16: return dispatch<__hip_bfloat16>(a, batch, token_bytes, rows, stream);
+    default: return dispatch<float>(a, batch, token_bytes, rows, stream);
   }
 }

@@ -23,10 +23,13 @@ def _want(logits, history, lengths, prompts, repetition, frequency, presence, bi
             r = 1.0 if repetition is None else float(repetition[b])
             x[b, t] = x[b, t] / r if x[b, t] > 0 else x[b, t] * r
             c = made.count(t)
-            less = (0.0 if frequency is None else float(frequency[b])) * c
-            less += 0.0 if presence is None or not c else float(presence[b])
-            x[b, t] -= less
-            size[b, t] = max(size[b, t], size[b, t] * r, size[b, t] / r) + abs(less)
+            often = (0.0 if frequency is None else float(frequency[b])) * c
+            once = 0.0 if presence is None or not c else float(presence[b])
+            x[b, t] -= often + once
+            # the two are taken off one after the other: x r - often, which is
+            # rounded, may be as large as both though often + once is small
+            # (0.1 - 0.12), so that each term counts by its own size
+            size[b, t] = max(size[b, t], size[b, t] * r, size[b, t] / r) + abs(often) + abs(once)
         if bias_tokens is not None:
             for t, v in {int(t): float(v) for t, v in zip(bias_tokens[b], bias_values[b])}.items():
                 if 0 <= t < vocab:
@@ -78,9 +81,12 @@ def _run(logits, a, out=None):
                         allowed=a["allowed"])
 
 
-# tiles of every size, vocabularies that end inside a vector, a word and a tile
+# tiles of every size, vocabularies that end inside a vector, a word and a tile; rows
+# that start anywhere in a vector, and past the end of their last whole tile for it
 @pytest.mark.parametrize("batch,vocab,capacity", [(1, 1, 1), (2, 31, 9), (3, 1000, 50), (1, 32768, 5000),
-                                                  (5, 8197, 2), (130, 8192, 40)])
+                                                  (5, 8197, 2), (130, 8192, 40), (9, 2047, 20),
+                                                  (9, 50001, 700), (300, 3, 4), (300, 2047, 20),
+                                                  (257, 8191, 3), (90, 10241, 30)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("token_type", [torch.int32, torch.int64])
 def test_all_parts(cuda, batch, vocab, capacity, dtype, token_type):
@@ -132,6 +138,22 @@ def test_strides_alignment_and_padding(cuda):
         _run(view, b, view)
         _check(view, *want)
         assert (wide[:, :begin] == 5.0).all() and (wide[:, begin + 777:] == 5.0).all()
+    # as many rows as make larger tiles, in rows of another buffer, whose ends are kept
+    logits, a = _case(cuda, 270, 777, 30, 3, torch.float16, torch.int32)
+    want = _want(logits, **a)
+    for width, begin in ((784, 0), (789, 5)):
+        wide = torch.full((270, width), 5.0, device=cuda, dtype=torch.float16)
+        wide[:, begin:begin + 777] = logits
+        view = wide[:, begin:begin + 777]
+        _run(view, a, view)
+        _check(view, *want)
+        assert (wide[:, :begin] == 5.0).all() and (wide[:, begin + 777:] == 5.0).all()
+    # an output whose rows lie otherwise than the logits'
+    logits, a = _case(cuda, 260, 777, 30, 3, torch.float32, torch.int32)
+    want = _want(logits, **a)
+    other = torch.full((260, 779), 5.0, device=cuda)
+    _check(_run(logits, a, other[:, 1:778]), *want)
+    assert (other[:, 0] == 5.0).all() and (other[:, 778] == 5.0).all()
 
 
 def test_extreme_logits(cuda):
