@@ -363,13 +363,16 @@ class Int4PagedDecode:
             out = torch.empty_like(q)
             if not out.is_contiguous():
                 out = torch.empty(q.shape, device=q.device, dtype=torch.float16)
-        out_at = _capi.pointer(out, torch.float16, q.shape, device,
-                               "out must be contiguous float16, shaped like q")
-        if lse is None and return_lse:
-            lse = torch.empty_strided((batch, hq), (hq, 1), dtype=torch.float32, device=q.device)
+            out_at = out.data_ptr()
+        else:
+            out_at = _capi.pointer(out, torch.float16, q.shape, device,
+                                   "out must be contiguous float16, shaped like q")
         if lse is not None:
             lse_at = _capi.pointer(lse, torch.float32, (batch, hq), device,
                                    "lse must be contiguous float32 [B,Hq]")
+        elif return_lse:
+            lse = torch.empty_strided((batch, hq), (hq, 1), dtype=torch.float32, device=q.device)
+            lse_at = lse.data_ptr()
         if self._device != device:
             raise ValueError(_capi.DEVICE_ERROR)
         stream = _capi.launch_stream(device)
