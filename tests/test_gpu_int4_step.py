@@ -184,3 +184,70 @@ def test_captured_steps_equal_eager_ones(cuda):
     for name in ("tokens", "history", "codes", "scales", "out", "lse", "shaped"):
         assert torch.equal(getattr(eager, name), getattr(graphed, name)), name
     assert all(torch.equal(a, b) for a, b in zip(eager.exact, graphed.exact))
+
+
+def test_serving_tables(cuda):
+    """The tables of ``serving.decode_tables`` drive the step: exact sink, suffix
+    and ring pages, history in 4 bits, pages that a step completed read back."""
+    from pagegauge_amd import int4, rotary, serving as sv
+
+    gen = torch.Generator().manual_seed(11)
+    half = lambda *s: torch.randn(*s, generator=gen).half().to(cuda)  # noqa: E731
+    pol = sv.Policy(prefix_pages=1, suffix_pages=2, tail_pages=2)
+    ledger, rope = sv.Ledger(2, pol), rotary.RotaryEmbedding(128)
+    codes, scales = int4.allocate_pages(64, HKV, cuda)
+    exact = [half(2 * pol.storage_pages, 16, HKV, 128) for _ in range(2)]
+    centers = [torch.zeros(2, HKV, 128, device=cuda, dtype=torch.float16) for _ in range(2)]
+    free = torch.randperm(64, generator=gen).tolist()
+    leases, tables = [], []
+    for prompt in (200, 133):
+        count = -(-prompt // 16)
+        tables.append([free.pop() for _ in range(count)])
+        lease = ledger.admit(f"request {prompt}", prompt, tables[-1], ready=True)
+        leases.append(lease)
+        key, value = half(prompt, HKV, 128), half(prompt, HKV, 128)
+        for c, x in zip(centers, (key, value)):
+            c[lease.slot] = x.float().mean(0).half()
+        pages = sv.partition(prompt, prompt, pol)["exact"]
+        slots = [sv.exact_slot(p, prompt, lease.slot, pol) if p in pages else -1 for p in range(count)]
+        int4.quantize_pages(key, value, codes, scales,
+                            page_ids=torch.tensor(tables[-1], device=cuda, dtype=torch.int32),
+                            key_center=centers[0][lease.slot], value_center=centers[1][lease.slot],
+                            exact_page_ids=torch.tensor(slots, device=cuda, dtype=torch.int32),
+                            exact_key=exact[0], exact_value=exact[1])
+    decode = int4.Int4PagedDecode(torch.empty(16 << 20, device=cuda, dtype=torch.uint8))
+    completed, read_back = set(), set()
+    for _ in range(70):
+        scheduled = []
+        for lease, table in zip(leases, tables):
+            at = ledger.view(lease).current_tokens
+            if at % 16 == 0:
+                table.append(free.pop())
+            scheduled.append((lease, at, table))
+        batch = ledger.stage_decode(scheduled)
+        t = sv.decode_tables(batch, pol, device=cuda)
+        read_back |= completed & set(t.old_indices.tolist())
+        completed |= {table[at // 16] for _, at, table in scheduled if at % 16 == 15}
+        kc, vc = (c[t.request_slots.long()].contiguous() for c in centers)
+        rotated = torch.empty(2, HQ, 128, device=cuda, dtype=torch.float16)
+        int4.rope_append(rope, half(2, HQ, 128), half(2, HKV, 128), half(2, HKV, 128), t.positions,
+                         t.exact_page_ids, t.code_page_ids, kc, vc, rotated, *exact, codes, scales)
+        decode.plan(t.old_indptr, t.old_indices, t.old_last_page_len, t.exact_indptr,
+                    t.exact_indices, t.exact_last_page_len, num_qo_heads=HQ, num_kv_heads=HKV)
+        out = decode.run(rotated, codes, scales, exact, value_center=vc)
+        (kq, ks), (vq, vs) = unpack(codes, scales)
+        pools = [(kq * ks.astype(np.float64)[..., None], vq * vs.astype(np.float64)[..., None]),
+                 tuple(x.double().cpu().numpy() for x in exact)]
+        for b, (_, at, _) in enumerate(scheduled):
+            old = t.old_indices[t.old_indptr[b]:t.old_indptr[b + 1]].cpu().numpy()
+            new = t.exact_indices[t.exact_indptr[b]:t.exact_indptr[b + 1]].cpu().numpy()
+            k, v = (np.concatenate([pools[0][i][old], pools[1][i][new]]).reshape(-1, HKV, 128)
+                    for i in range(2))
+            used = at + 1
+            assert -(-used // 16) * 16 == len(k)
+            want, _, bound, _ = attention(rotated[b].cpu().numpy(), k[:used], v[:used],
+                                          vc[b].cpu().numpy(), 128 ** -0.5)
+            allowed = (np.abs(want) + bound[:, None]) * 2.0 ** -11 + bound[:, None] + 2.0 ** -24
+            assert (np.abs(out[b].double().cpu().numpy() - want) <= allowed).all()
+        ledger.commit_decode(batch)
+    assert len(read_back) >= 4
