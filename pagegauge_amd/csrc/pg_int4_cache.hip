@@ -352,38 +352,66 @@ struct AppendArgs {
   int query_heads, kv_heads;
 };
 
-// One wave per row of a request (query heads, then K, then V heads): lane p
-// holds pair p of the rotated part, or two dims past it.  What the row needs is
+constexpr int kQueryRows = 4;      // query heads of a wave
+
+// One wave per 4 query heads of a request, then per K and per V head: lane p
+// holds pair p of the rotated part, or two dims past it.  What the rows need is
 // requested at once, the rows of a page that closes included: the kernel's time
 // is that of its trips to memory, one for the request's position and ids and one
-// for everything else (as a chain of five, 256 requests took 10.4 us; now 7.0 to
-// 7.5, 4.4 for 8 requests that all close a page).
+// for everything else (as a chain of five, 256 requests took 10.4 us in place of
+// 6.9).  With a wave per query head, more than the chip holds at once, 256 requests
+// of 32 query and 8 KV heads took 6.9 us and 1024 took 15.0; now 6.3 and 11.2, and 3.7
+// for 8 requests that all close a page.
 __global__ __launch_bounds__(kWave * kWavesPerBlock) void int4_rope_append_kernel(AppendArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t own[kWavesPerBlock][kHeadDim];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int row = blockIdx.y * kWavesPerBlock + wave;
-  if (row >= a.query_heads + 2 * a.kv_heads) return;   // whole waves; no barrier below
+  const int query_waves = (a.query_heads + kQueryRows - 1) / kQueryRows;
+  if (row >= query_waves + 2 * a.kv_heads) return;     // whole waves; no barrier below
   const int request = blockIdx.x;
-  const int kind = row < a.query_heads ? 0 : row < a.query_heads + a.kv_heads ? 1 : 2;
-  const int head = kind == 0 ? row : kind == 1 ? row - a.query_heads : row - a.query_heads - a.kv_heads;
-  const uint16_t* in = a.rows[kind] + request * a.batch_stride[kind] + head * kHeadDim;
   const bool turned = lane < a.rotary_dim / 2;
   const int first = turned && !a.interleaved ? lane : 2 * lane;
   const int second = turned && !a.interleaved ? lane + a.rotary_dim / 2 : 2 * lane + 1;
+  if (row < query_waves) {
+    const int head = row * kQueryRows, heads = min(kQueryRows, a.query_heads - head);
+    const uint16_t* in = a.rows[0] + request * a.batch_stride[0] + head * kHeadDim;
+    uint16_t x_bits[kQueryRows], y_bits[kQueryRows];
+#pragma unroll
+    for (int k = 0; k < kQueryRows; ++k) {
+      x_bits[k] = in[min(k, heads - 1) * kHeadDim + first];
+      y_bits[k] = in[min(k, heads - 1) * kHeadDim + second];
+    }
+    const double turns = a.turns[turned ? lane : 0];
+    const int32_t position = a.positions[request];
+    if (position < 0) return;
+    const float2 cos_sin = rotary_cos_sin(position, turns, a.amplitude);
+    uint16_t* out = a.rotated_query + (static_cast<int64_t>(request) * a.query_heads + head) * kHeadDim;
+#pragma unroll
+    for (int k = 0; k < kQueryRows; ++k) {
+      if (k >= heads) break;
+      const float2 pair = rotate_pair(half_bits_to_float(x_bits[k]), half_bits_to_float(y_bits[k]), cos_sin);
+      out[k * kHeadDim + first] = turned ? __half_as_ushort(__float2half_rn(pair.x)) : x_bits[k];
+      out[k * kHeadDim + second] = turned ? __half_as_ushort(__float2half_rn(pair.y)) : y_bits[k];
+    }
+    return;
+  }
+  const int kind = row < query_waves + a.kv_heads ? 1 : 2;
+  const int head = row - query_waves - (kind == 1 ? 0 : a.kv_heads);
+  const uint16_t* in = a.rows[kind] + request * a.batch_stride[kind] + head * kHeadDim;
   const int32_t position = a.positions[request];
   const int64_t exact_page = a.exact_ids[request], code_page = a.code_ids[request];
   const uint16_t x_bits = in[first], y_bits = in[second];
   const double turns = a.turns[turned ? lane : 0];
   if (position < 0) return;
   const int offset = position % kPageSize;
-  const bool stored = kind > 0 && exact_page >= 0 && exact_page < a.num_exact_pages;
-  const bool closes = stored && offset == kPageSize - 1 && code_page >= 0 && code_page < a.num_code_pages;
+  if (exact_page < 0 || exact_page >= a.num_exact_pages) return;
+  const bool closes = offset == kPageSize - 1 && code_page >= 0 && code_page < a.num_code_pages;
 
   // rows of the page in the packed order; row 15 is this token's own and comes
   // from LDS, row 14 is read in its place
   v4u held[4];
   const int64_t row_stride = static_cast<int64_t>(a.kv_heads) * kHeadDim;
-  uint16_t* page = stored ? a.exact[kind - 1] + exact_page * kPageSize * row_stride + head * kHeadDim : nullptr;
+  uint16_t* page = a.exact[kind - 1] + exact_page * kPageSize * row_stride + head * kHeadDim;
   if (closes) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -392,25 +420,14 @@ __global__ __launch_bounds__(kWave * kWavesPerBlock) void int4_rope_append_kerne
       held[g] = *reinterpret_cast<const v4u*>(page + min(r, kPageSize - 2) * row_stride + dim);
     }
   }
-  float cx = 0.0f, cy = 0.0f;
-  if (stored) {
-    const uint16_t* center = a.center[kind - 1] + (static_cast<int64_t>(request) * a.kv_heads + head) * kHeadDim;
-    cx = half_bits_to_float(center[first]);
-    cy = half_bits_to_float(center[second]);
-  }
+  const uint16_t* center = a.center[kind - 1] + (static_cast<int64_t>(request) * a.kv_heads + head) * kHeadDim;
+  const float cx = half_bits_to_float(center[first]), cy = half_bits_to_float(center[second]);
   float x = half_bits_to_float(x_bits), y = half_bits_to_float(y_bits);
-  if (kind < 2 && turned) {
+  if (kind == 1 && turned) {
     const float2 pair = rotate_pair(x, y, rotary_cos_sin(position, turns, a.amplitude));
     x = pair.x;
     y = pair.y;
   }
-  if (kind == 0) {
-    uint16_t* out = a.rotated_query + (static_cast<int64_t>(request) * a.query_heads + head) * kHeadDim;
-    out[first] = __half_as_ushort(__float2half_rn(x));
-    out[second] = __half_as_ushort(__float2half_rn(y));
-    return;
-  }
-  if (!stored) return;
   const uint16_t xb = __half_as_ushort(__float2half_rn(x - cx));
   const uint16_t yb = __half_as_ushort(__float2half_rn(y - cy));
   page[offset * row_stride + first] = xb;
@@ -565,7 +582,8 @@ extern "C" int32_t pg_int4_rope_append(
     return fail(PG_ERROR_INVALID_ARGUMENT, "batch, head and page counts must be positive");
   if (rotary_dim <= 0 || rotary_dim % 2 || rotary_dim > kHeadDim)
     return fail(PG_ERROR_INVALID_ARGUMENT, "the rotated part must be an even number of a head's dims");
-  const int64_t row_blocks = (static_cast<int64_t>(query_heads) + 2 * kv_heads + kWavesPerBlock - 1) / kWavesPerBlock;
+  const int64_t query_waves = (static_cast<int64_t>(query_heads) + kQueryRows - 1) / kQueryRows;
+  const int64_t row_blocks = (query_waves + 2 * kv_heads + kWavesPerBlock - 1) / kWavesPerBlock;
   if (row_blocks > 65535) return fail(PG_ERROR_UNSUPPORTED, "too many heads for one call");
   if (batch_size > kMaxBlocks) return fail(PG_ERROR_UNSUPPORTED, "too many requests for one call");
   if (batch_size == 0) return PG_OK;
