@@ -16,27 +16,28 @@
 //    as the A operand of P V: probabilities never leave their lane.  Columns
 //    n < 8 hand over the FP16 part of a probability and columns n >= 8 (the same
 //    heads again) its remainder, so rows r and r + 8 of the product add up to
-//    one of about 22 bits.  With kWide the two parts are a product each (16 heads
-//    per KV head, 256 requests: 185 us, as two workgroups of 8 heads 268).
-//  * A nibble u = code + 8 masked out of its dword is the FP16 subnormal
-//    u * 2^-24, or 16 u * 2^-24 one nibble further up, and MFMAs multiply
-//    subnormals exactly: 5 operations make 8 operands of V.  Its offset of 8 comes
-//    off the product, as one more column against 8s.  K's comes off the operands,
-//    4 operations more: off its product it costs the scores two bits (lse 1e-6 off
-//    instead of 3e-7, for 15.5 us against 16.6 at 49K tokens).  The scales
-//    multiply scores and probabilities in float32.
+//    one of about 23 bits.  With kWide the two parts are a product each (16 heads
+//    per KV head, 256 requests: 188 us, as two workgroups of 8 heads 268).
+//  * Codes are exact FP16 operands, normal ones: a nibble u = code + 8 is masked out
+//    under an exponent and 1024 + 8 or 64 + 8 taken off, 2.5 operations per pair.  Masked
+//    nibbles as they are, FP16 subnormals, would save one of these and cost the result:
+//    the sums of an MFMA are cut at a width that counts from an operand's nominal
+//    exponent, and subnormal ones lose the bits that they lack (6 to 7 % of the outputs
+//    a step from the nearest FP16 value and lse 4e-6 to 5e-6 off, now 0.04 % at most and
+//    6e-7); with V's offset of 8 also left to the product it was 15 to 18 %.  The
+//    scales multiply scores and probabilities in float32.
 //  * The softmax's base follows the running maximum lazily: it moves when a
 //    score passes it by 2^4, so most groups of pages need no exchange at all.
 //
 // Probabilities times V's scales are carried relative to a power of two that
 // puts the largest of the wave's scales near 2^10 (2^14 with the base's slack), so
-// that two FP16 parts hold them to 2^-34 of the largest.
+// that two FP16 parts hold them to 2^-23 of themselves or 2^-35 of the largest.
 //
 // Bound by HBM once a wave has several groups, by a chain of trips to memory
 // (work item, page ids, pages, partial rows) before.  Kernel times on MI355X, and
-// of the same walk without its arithmetic: 256 requests (829 MB) 168 and 165 us,
-// 8 requests of 4K to 32K (164 MB) 34 and 32, one of 49K tokens (53 MB) 14.4 and
-// 12.3, of 4K (5 MB) 5.4 and 4.6; a join adds 2.4 to 4.6 us.  Measured and not
+// of the same walk without its arithmetic: 256 requests (829 MB) 170 and 165 us,
+// 8 requests of 4K to 32K (164 MB) 34 and 32, one of 49K tokens (53 MB) 14.9 and
+// 12.3, of 4K (5 MB) 5.5 and 4.6; a join adds 2.4 to 4.6 us.  Measured and not
 // taken: 8 waves a workgroup (one fits a CU, and nothing covers its start and
 // end: 256 requests 191 us), and a join by the workgroup that ends last (49K
 // tokens 18.7 us a call against 17.2 with the second launch, before the last
@@ -53,6 +54,7 @@ namespace {
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
@@ -93,17 +95,24 @@ __device__ __forceinline__ v8h operand(uint32_t a, uint32_t b, uint32_t c, uint3
   return __builtin_bit_cast(v8h, v4u{a, b, c, d});
 }
 
-// Nibbles 0 and 4 of a dword as FP16 u * 2^-24, and 1 and 5 as 16 u * 2^-24.
-__device__ __forceinline__ uint32_t even(uint32_t word) { return word & 0x000f000fu; }
-__device__ __forceinline__ uint32_t odd(uint32_t word) { return word & 0x00f000f0u; }
-constexpr uint32_t kEvenEights = 0x00080008u, kOddEights = 0x00800080u;     // u = 8
+// Codes of a dword in FP16, as 8 MFMA operands in their order: a nibble u = code + 8
+// put under the exponent of 1024 (nibbles 0 and 4), or one nibble further up of 64 (1
+// and 5), is 1024 + u or 64 + u, and less 1032 or 72 it is the code, exactly.  The
+// exponents are held in registers: masking and putting is one operation that takes
+// but one constant of another kind.
+struct Exponents {
+  uint32_t even = 0x64006400u, odd = 0x54005400u;
+  __device__ __forceinline__ Exponents() { asm("" : "+v"(even), "+v"(odd)); }
+  __device__ __forceinline__ uint32_t even_codes(uint32_t word) const {
+    return __builtin_bit_cast(uint32_t, as_half2((word & 0x000f000fu) | even) - as_half2(0x64086408u));
+  }
+  __device__ __forceinline__ uint32_t odd_codes(uint32_t word) const {
+    return __builtin_bit_cast(uint32_t, as_half2((word & 0x00f000f0u) | odd) - as_half2(0x54805480u));
+  }
+};
 
-// The same of codes, u - 8: exact, as all of it is a multiple of 2^-24.
-__device__ __forceinline__ uint32_t even_codes(uint32_t word) {
-  return __builtin_bit_cast(uint32_t, as_half2(even(word)) - as_half2(kEvenEights));
-}
-__device__ __forceinline__ uint32_t odd_codes(uint32_t word) {
-  return __builtin_bit_cast(uint32_t, as_half2(odd(word)) - as_half2(kOddEights));
+__device__ __forceinline__ v2h to_half2(float x, float y) {
+  return __builtin_convertvector((v2f{x, y}), v2h);
 }
 
 // x times one half of ``pair``: one mixed-precision operation, no conversion.
@@ -115,29 +124,26 @@ constexpr float kSlack = 4.0f;     // how far (base 2) a score may pass the base
 
 // Running state of one wave.  Lane (kg, n) has head n % 8's (kWide: n's): base (before the
 // softmax scale), limit past which it moves, and offset, the exponent of the sums
-// minus the scaled base; l0 and l1 sum the lane's own tokens 4 kg, 4 kg + 1 and, in
-// sixteenths, 4 kg + 2, 4 kg + 3.  acc[nb][r] is row 4 kg + r of the product,
-// channel 8 n + nb, and eights[r] that row's sum of weights times 8.
+// minus the scaled base; l sums the lane's own tokens.  acc[nb][r] is row 4 kg + r of
+// the product, channel 8 n + nb.
 struct State {
   float base, limit, offset;
-  float l0, l1;
-  v4f acc[8], eights;
+  float l[2];                      // of tokens 4 kg, 4 kg + 1 and of the other two
+  v4f acc[8];
 };
 
 __device__ __forceinline__ void scale_sums(State& st, const float (&f)[4]) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    st.eights[r] *= f[r];
+  for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int nb = 0; nb < 8; ++nb) st.acc[nb][r] *= f[r];
-  }
 }
 
 // Softmax step over kPages pages: s are the lane's scores, masked ones -inf,
 // v_scale pairs of V's scales (FP16; 0 where masked), ``scale`` the softmax scale
 // in base 2, ``exponent`` that of the sums.  p: the lane's rows of the A operand
-// of P V, tokens 4 kg + 2, 4 kg + 3 in sixteenths with kCodes; rows of the FP16 part
-// and of the remainder in one, or with kWide in one after the other.
+// of P V, with kCodes times V's scales; rows of the FP16 part and of the remainder in
+// one, or with kWide in one after the other.
 template <int kPages, bool kCodes, bool kWide>
 __device__ __forceinline__ void softmax_step(State& st, const float (&s)[kPages][4],
                                              const uint32_t (&v_scale)[kPages][2], float scale,
@@ -157,31 +163,29 @@ __device__ __forceinline__ void softmax_step(State& st, const float (&s)[kPages]
     st.base = base;
     st.limit = base + kSlack / scale;
     st.offset = base == kNegInf ? exponent : fmaf(-base, scale, exponent);
-    st.l0 *= alpha;
-    st.l1 *= alpha;
+    st.l[0] *= alpha;
+    st.l[1] *= alpha;
     const int kg = lane >> 4;
     float f[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) f[r] = __shfl(alpha, (4 * kg + r) & (kWide ? 15 : 7), kWave);
     scale_sums(st, f);
   }
-  const float offset1 = kCodes ? st.offset - 4.0f : st.offset;
 #pragma unroll
   for (int j = 0; j < kPages / 2; ++j) {
     uint32_t words[1 + kWide][4];
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
       const int page = 2 * j + (h >> 1), r = 2 * (h & 1);
-      const float offset = h & 1 ? offset1 : st.offset;
-      const float x0 = __builtin_amdgcn_exp2f(fmaf(s[page][r], scale, offset));
-      const float x1 = __builtin_amdgcn_exp2f(fmaf(s[page][r + 1], scale, offset));
-      if (h & 1) st.l1 += x0 + x1; else st.l0 += x0 + x1;
+      const float x0 = __builtin_amdgcn_exp2f(fmaf(s[page][r], scale, st.offset));
+      const float x1 = __builtin_amdgcn_exp2f(fmaf(s[page][r + 1], scale, st.offset));
+      st.l[h & 1] += x0 + x1;
       const float w0 = kCodes ? times_half(x0, v_scale[page][h & 1], 0) : x0;
       const float w1 = kCodes ? times_half(x1, v_scale[page][h & 1], 1) : x1;
-      // the FP16 part, or what it leaves (rounding down costs the second 2^-21)
-      const v2h high = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(w0, w1));
+      // the FP16 part, or what it leaves, each to nearest: together within 2^-23
+      const v2h high = to_half2(w0, w1);
       if (kWide) words[0][h] = __builtin_bit_cast(uint32_t, high);
-      words[kWide][h] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(
+      words[kWide][h] = __builtin_bit_cast(uint32_t, to_half2(
           fmaf(-low_part, static_cast<float>(high.x), w0), fmaf(-low_part, static_cast<float>(high.y), w1)));
     }
 #pragma unroll
@@ -237,11 +241,10 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
 
   State st;
   st.base = st.limit = kNegInf;
-  st.offset = st.l0 = st.l1 = 0.0f;
-  st.eights = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  st.offset = st.l[0] = st.l[1] = 0.0f;
 #pragma unroll
   for (int nb = 0; nb < 8; ++nb) st.acc[nb] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  float exponent = 0.0f, acc_exponent = 0.0f;    // of the sums l and acc
+  float exponent = 0.0f;           // of the sums l and acc
 
   // ---- history: groups wave, wave + 4, ... of the item's pages
   const int count = it.page_end - it.page_begin;
@@ -283,14 +286,6 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
     for (int g = 0; g < 4; ++g)
       raw[g] = *reinterpret_cast<const v2u*>(scale_bytes + (my_block >> 5) + 16 * g + 8);
     take_query();
-    // q against the even and the odd nibbles of two dwords
-    v8h q_even[2], q_odd[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const v4u x = __builtin_bit_cast(v4u, q[2 * h]), y = __builtin_bit_cast(v4u, q[2 * h + 1]);
-      q_even[h] = operand(x[0], x[2], y[0], y[2]);
-      q_odd[h] = operand(x[1], x[3], y[1], y[3]);
-    }
     {
       // positive FP16 values order as their bits do
       if (whole < count) {
@@ -310,8 +305,8 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
       if (largest > 0.0f) frexpf(largest, &e);
       exponent = st.offset = static_cast<float>(10 - e);
     }
-    const float scale = a.sm_scale_log2 * 0x1p20f;       // the products are dots times 2^-20
 
+    const Exponents at;
     auto compute = [&](int g, Group& cur) {
       const int first = kInt4GroupPages * (kInt4Waves * g + wave);
       float s[kInt4GroupPages][4];
@@ -319,19 +314,15 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
       for (int i = 0; i < kInt4GroupPages; ++i) {
         consume_point(cur.k[i]);
         consume_point(cur.s[i]);
-        v4f dot_even = {0.0f, 0.0f, 0.0f, 0.0f};
-        v4f dot_odd = {0.0f, 0.0f, 0.0f, 0.0f};
+        v4f dot = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t x = cur.k[i][2 * h], y = cur.k[i][2 * h + 1];
-          dot_even = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              operand(even_codes(x), even_codes(x >> 8), even_codes(y), even_codes(y >> 8)), q_even[h], dot_even, 0, 0, 0);
-          dot_odd = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              operand(odd_codes(x), odd_codes(x >> 8), odd_codes(y), odd_codes(y >> 8)), q_odd[h], dot_odd, 0, 0, 0);
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t x = cur.k[i][w];
+          dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              operand(at.even_codes(x), at.odd_codes(x), at.even_codes(x >> 8), at.odd_codes(x >> 8)), q[w], dot, 0, 0, 0);
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          s[i][r] = times_half(fmaf(dot_even[r], 16.0f, dot_odd[r]), cur.s[i][r >> 1], r & 1);
+        for (int r = 0; r < 4; ++r) s[i][r] = times_half(dot[r], cur.s[i][r >> 1], r & 1);
       }
       uint32_t v_scale[kInt4GroupPages][2];
 #pragma unroll
@@ -352,7 +343,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
         }
       }
       v8h p[1 + kWide][kInt4GroupPages / 2];
-      softmax_step<kInt4GroupPages, true, kWide>(st, s, v_scale, scale, exponent, low_part, lane, p);
+      softmax_step<kInt4GroupPages, true, kWide>(st, s, v_scale, a.sm_scale_log2, exponent, low_part, lane, p);
 #pragma unroll
       for (int i = 0; i < kInt4GroupPages; ++i) consume_point(cur.v[i]);
       auto product = [&](const v8h (&rows)[1 + kWide], v8h columns, v4f sum) {
@@ -366,13 +357,14 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
         v8h rows[1 + kWide];
 #pragma unroll
         for (int part = 0; part < 1 + kWide; ++part) rows[part] = p[part][j];
-        st.eights = product(rows, operand(kEvenEights, kOddEights, kEvenEights, kOddEights), st.eights);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const uint32_t x = cur.v[2 * j][w], y = cur.v[2 * j + 1][w];
-          st.acc[2 * w] = product(rows, operand(even(x), odd(x), even(y), odd(y)), st.acc[2 * w]);
-          st.acc[2 * w + 1] = product(rows, operand(even(x >> 8), odd(x >> 8), even(y >> 8), odd(y >> 8)),
-                                      st.acc[2 * w + 1]);
+          st.acc[2 * w] = product(
+              rows, operand(at.even_codes(x), at.odd_codes(x), at.even_codes(y), at.odd_codes(y)), st.acc[2 * w]);
+          st.acc[2 * w + 1] = product(
+              rows, operand(at.even_codes(x >> 8), at.odd_codes(x >> 8), at.even_codes(y >> 8), at.odd_codes(y >> 8)),
+              st.acc[2 * w + 1]);
         }
       }
     };
@@ -391,13 +383,6 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
     } else {
       compute(g, buf[0]);
     }
-#pragma unroll
-    for (int nb = 0; nb < 8; ++nb) st.acc[nb] -= st.eights;
-    st.l0 = fmaf(st.l1, 16.0f, st.l0);
-    st.l1 = 0.0f;
-    st.base *= 0x1p20f;            // as the dots themselves
-    st.limit *= 0x1p20f;
-    acc_exponent = exponent - 24.0f;
   } else {
     take_query();
   }
@@ -406,13 +391,13 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
   const int tail_count = it.tail_end - it.tail_begin;
   if (2 * wave < tail_count) {
     // probabilities alone: their largest is 1, or 2^4 with the base's slack
-    const float change_l = __builtin_amdgcn_exp2f(10.0f - exponent);
-    const float change = __builtin_amdgcn_exp2f(10.0f - acc_exponent);
-    st.l0 *= change_l;
+    const float change = __builtin_amdgcn_exp2f(10.0f - exponent);
+    st.l[0] *= change;
+    st.l[1] *= change;
     st.offset += 10.0f - exponent;
     const float f[4] = {change, change, change, change};
     scale_sums(st, f);
-    exponent = acc_exponent = 10.0f;
+    exponent = 10.0f;
     const int64_t row_stride = static_cast<int64_t>(hkv) * kHeadDim;
     const int last_len = min(a.tail_last_len[it.request], kPageSize);
     for (int page = 2 * wave; page < tail_count; page += 2 * kInt4Waves) {
@@ -463,13 +448,13 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
   }
 
   // ---- the waves meet: parts of the product's rows, then 4 partial states
-  float l_sum = st.l0 + st.l1;
+  float l_sum = st.l[0] + st.l[1];
   l_sum += __shfl_xor(l_sum, 16, kWave);
   l_sum += __shfl_xor(l_sum, 32, kWave);
-  const float scale = __builtin_amdgcn_exp2f(-acc_exponent);
+  const float scale = __builtin_amdgcn_exp2f(-exponent);
   if (kg == 0 && n < kHeads) {
     part_m[wave][n] = st.base * a.sm_scale_log2;
-    part_l[wave][n] = l_sum * __builtin_amdgcn_exp2f(-exponent);
+    part_l[wave][n] = l_sum * scale;
   }
   // part_o[..][64 b + c]: dim 2 c + b.  A swap of two registers' halves adds rows r
   // and r + 8 of two channels at once: lanes below 32 end with channel 8 n + 2 p, the
@@ -690,7 +675,7 @@ extern "C" int32_t pg_int4_decode_run(const pg_int4_plan_t* plan, const void* qu
     return fail(PG_ERROR_INVALID_ARGUMENT, "history segment tensors missing");
   if (plan->has_tail && (!tail_k || !tail_v || !tail_indices || !tail_last_len))
     return fail(PG_ERROR_INVALID_ARGUMENT, "tail segment tensors missing");
-  // the kernel multiplies it by 2^20 log2(e)
+  // the kernel multiplies it by log2(e), and scores of any FP16 values by that
   if (!(sm_scale > 0.0f) || !(sm_scale < 0x1p100f))
     return fail(PG_ERROR_INVALID_ARGUMENT, "sm_scale must be positive and below 2^100");
   for (const void* p : {query, codes, scales, tail_k, tail_v})

@@ -14,7 +14,7 @@ import numpy as np
 import pytest
 import torch
 
-from int4_helpers import attention, random_pool, unpack
+from int4_helpers import attention, nibble_maps, random_pool, unpack
 
 pytestmark = pytest.mark.gpu
 
@@ -236,3 +236,76 @@ def test_graphs_sharing_a_workspace_and_streams(cuda):
         got = c.run()
     stream.synchronize()
     assert torch.equal(got[0], want[0][0])
+
+
+def _set_nibbles(c, part, codes):
+    """Puts ``codes`` [tokens, Hkv, 128] into the history's pages as K (0) or V (1)."""
+    where = nibble_maps()[part]
+    ids = c.tables[0][1].cpu().numpy()
+    nibbles = np.full((c.codes.shape[0], c.hkv, 2048), 8, np.uint8)
+    rows = codes.reshape(len(ids), 16, c.hkv, 128).transpose(0, 2, 1, 3)
+    nibbles[ids] = (rows[:, :, where[:, 0], where[:, 1]] + 8).astype(np.uint8)
+    c.codes[:, :, part] = torch.from_numpy(nibbles[..., ::2] | nibbles[..., 1::2] << 4).to(c.codes.device)
+
+
+@both_forms
+def test_a_value_among_zeros_keeps_its_bits(cuda, kv_heads, group):
+    """Values of code 0 add nothing, however many: 4096 tokens of one item weigh alike,
+    and each channel has one value that is not 0, of code 1 or -1 and its token's
+    scale.  The output is scale / 4096 but for the rounding of the probabilities' sum,
+    a chain of fewer than 700 additions of 2^-24 each (below 2^-14), of a probability,
+    its product with the scale, the join of 4 waves and the quotient (below 2^-18
+    together), and FP16's 2^-11."""
+    tokens = 4096
+    c = Case(cuda, [tokens], [0], kv_heads, group, with_tail=False)
+    c.decode.plan(*c.tables[0], num_qo_heads=kv_heads * group, num_kv_heads=kv_heads, num_cus=1)
+    assert c.decode.num_work_items == 1
+    c.q.zero_()
+    gen = torch.Generator().manual_seed(8)
+    # scales of 11 bits from 1 to 128: exact products, outputs that are no subnormals
+    c.scales.copy_(torch.randint(1024, 2048, c.scales.shape, generator=gen)
+                   * 2.0 ** -torch.randint(4, 11, c.scales.shape, generator=gen))
+    at = torch.randint(0, tokens, (kv_heads, 128), generator=gen).numpy()
+    sign = (torch.randint(0, 2, (kv_heads, 128), generator=gen) * 2 - 1).numpy()
+    codes = np.zeros((tokens, kv_heads, 128), np.int64)
+    for h in range(kv_heads):
+        codes[at[h], h, np.arange(128)] = sign[h]
+    _set_nibbles(c, 1, codes)
+    out, _ = c.run(value_center=None)
+    scales = unpack(c.codes, c.scales)[1][1].astype(np.float64)                # [pages, 16, Hkv]
+    pages = c.tables[0][1].cpu().numpy()
+    want = np.repeat([sign[h] * scales[pages[at[h] // 16], at[h] % 16, h] / tokens
+                      for h in range(kv_heads)], group, axis=0)
+    got = out[0].double().cpu().numpy()
+    assert (np.abs(got - want) <= np.abs(want) * (2.0 ** -11 + 2.0 ** -14 + 2.0 ** -17)).all()
+
+
+@both_forms
+def test_small_products_beside_large_ones(cuda, kv_heads, group):
+    """Requests of one token whose key has two codes of 1 or -1 that meet query values of
+    1 to 2 and of 2^-10 to 2^-9: the dot has 22 bits, so no order of float32 sums
+    rounds it.  lse is that dot times the scale, the softmax scale and log2(e): each
+    product rounds once, their base twice more and its weight's exponent once, 2^-24
+    of the score each and below 2^-21 together, and log2 of a weight near 1 is good to
+    2^-20."""
+    batch = 40
+    c = Case(cuda, [1] * batch, [0] * batch, kv_heads, group, with_tail=False)
+    gen = torch.Generator().manual_seed(9)
+    q = torch.randn(batch, kv_heads * group, 128, generator=gen)
+    codes = np.zeros((batch * 16, kv_heads, 128), np.int64)
+    for b in range(batch):
+        for h in range(kv_heads):
+            large, small = torch.randperm(128, generator=gen)[:2].tolist()
+            codes[16 * b, h, [large, small]] = (torch.randint(0, 2, (2,), generator=gen) * 2 - 1).numpy()
+            rows = slice(h * group, (h + 1) * group)
+            q[b, rows, large] = 1.0 + torch.rand(group, generator=gen)
+            q[b, rows, small] = 2.0 ** -10 * (1.0 + torch.rand(group, generator=gen))
+    c.q.copy_(q)
+    _set_nibbles(c, 0, codes)
+    out, lse = c.run(sm_scale=4.0)
+    ids = c.tables[0][1].cpu().numpy()
+    scales = unpack(c.codes, c.scales)[0][1].astype(np.float64)[ids, 0]            # [B, Hkv]
+    dots = np.einsum("bhgd,bhd->bhg", c.q.double().cpu().numpy().reshape(batch, kv_heads, group, 128),
+                     codes[::16].astype(np.float64))
+    want = (dots * scales[..., None] * 4.0 * np.log2(np.e)).reshape(batch, -1)
+    assert (np.abs(lse.double().cpu().numpy() - want) <= np.abs(want) * 2.0 ** -21 + 2.0 ** -20).all()
