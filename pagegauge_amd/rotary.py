@@ -13,7 +13,8 @@ was trained on:
 * ``"by_parts"``: pairs that turn more than ``beta_fast`` times within
   ``original_context`` keep their frequency, those that turn less than
   ``beta_slow`` times are divided by ``factor``, with a linear ramp over the
-  pairs between, and both rows scaled by ``0.1 ln(factor) + 1`` (unless
+  pairs between (its ends rounded outwards to whole pairs, within 0 and
+  ``rotary_dim - 1``), and both rows scaled by ``0.1 ln(factor) + 1`` (unless
   ``attention_factor`` is given).
 
 The angles are worked out in the kernel, so nothing grows with the context; they
@@ -54,8 +55,10 @@ def frequencies(rotary_dim: int, theta: float, scaling: str = "none", factor: fl
     def pair(turns: float) -> float:     # the pair that turns so many times
         return r * math.log(original_context / (turns * 2.0 * math.pi)) / (2.0 * math.log(theta))
 
+    # the ramp may end past the last of the r / 2 pairs, whose frequencies it then does not
+    # stretch by the whole factor
     low = max(math.floor(pair(beta_fast)), 0)
-    high = min(math.ceil(pair(beta_slow)), r // 2 - 1)
+    high = min(math.ceil(pair(beta_slow)), r - 1)
     ramp = ((torch.arange(r // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
     return f * (1.0 - ramp) + f / factor * ramp
 

@@ -91,3 +91,22 @@ def test_c_entry_point_refuses(over, code, message):
              amplitude=1.0, tokens=3, head_dim=128, rotary_dim=128, interleaved=0, dtype=0, stream=None)
     a.update(over)
     assert _capi.library().pg_rotate(*a.values()) == code and message in _capi.last_error()
+
+
+@pytest.mark.parametrize("r,theta,context,factor", [
+    (64, 1.0e4, 65536, 4.0), (32, 1.0e4, 65536, 8.0), (128, 1.0e4, 131072, 2.0), (8, 100.0, 8192, 4.0)])
+def test_by_parts_where_the_slowest_pair_turns_more_than_once(r, theta, context, factor):
+    """A ramp that ends past the last pair keeps its slope: no pair is stretched by the
+    whole factor, and each by its place between the pairs that turn 32 times and once."""
+    f = rotary.frequencies(r, theta)
+    turns = f * context / (2 * math.pi)
+    assert turns[-1] > 1.0
+    got = rotary.frequencies(r, theta, "by_parts", factor, context)
+    assert bool((got * factor > f * 1.01).all())
+    # from one pair to the next, turns fall by theta^(2 / r)
+    ends = [r / 2 * math.log(context / (2 * math.pi * n), theta) for n in (32.0, 1.0)]
+    low, high = max(0, math.floor(ends[0])), min(r - 1, math.ceil(ends[1]))
+    assert high > r // 2 - 1
+    for i in range(r // 2):
+        share = min(1.0, max(0.0, (i - low) / (high - low)))
+        assert math.isclose(float(got[i]), float(f[i]) * (1 - share + share / factor), rel_tol=1e-12)
