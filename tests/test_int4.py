@@ -232,3 +232,45 @@ def test_last_lengths_are_checked_where_there_are_pages():
     for bad in ([0, 1, 1], [17, 1, 1], [1, 1, -1]):
         with pytest.raises(ValueError, match="last must lie"):
             int4._check_last(indptr, torch.tensor(bad), "last")
+
+
+def _weights(pages, tail, hq, hkv, cus):
+    tables = [np.concatenate(([0], np.cumsum(n))).tolist() for n in (pages, tail)]
+    _, items, _ = int4.plan_work_items(*tables, hq, hkv, cus)
+    return [(i[2] - i[1]) + 4 * (i[5] - i[4]) for i in items.tolist()]
+
+
+def _check_shares(pages, tail, hkv, cus):
+    """No item outweighs both two full ones and twice an even share (and the tail page
+    that a cut falls into)."""
+    share = -(-(sum(pages) + 4 * sum(tail)) // max(len(pages), cus // hkv, 1))
+    assert max(_weights(pages, tail, 4 * hkv, hkv, cus)) <= max(2 * 256, 2 * share) + 4
+
+
+@pytest.mark.parametrize("pages,tail", [
+    # a long exact tail beside a history that needs more items than there are CUs
+    ([100000, 0], [0, 4000]), ([100000, 200], [16, 4000]),
+    # and beside so many requests that each would be one item
+    ([40] * 299 + [0], [0] * 299 + [3000]), ([240] * 256 + [16], [16] * 256 + [1000])])
+def test_long_tails_are_shared_out(pages, tail):
+    _check_shares(pages, tail, 8, 256)
+
+
+def test_shares_of_drawn_batches():
+    rng = random.Random(12)
+    for _ in range(200):
+        n = rng.choice([1, 2, 7, rng.randint(1, 400)])
+        pages = [rng.choice([0, rng.randint(0, 256), rng.randint(0, 20000)]) for _ in range(n)]
+        tail = [rng.choice([0, 16, rng.randint(0, 200), rng.randint(0, 5000)]) for _ in range(n)]
+        _check_shares(pages, tail, rng.choice([1, 2, 8, 16]), rng.choice([64, 256, 304]))
+
+
+@pytest.mark.parametrize("pages,tail,items", [
+    # one item per CU: 49K and 64K tokens; two where its waves cannot hold its pages
+    # (128K tokens and a ring) or requests do not divide over so few (17 of 3.3K)
+    ([3056], [16], 32), ([4080], [16], 32), ([8192], [16], 64), ([192] * 17, [16] * 17, 51),
+    ([512] * 16, [0] * 16, 32),
+    # whole requests, one item each
+    ([144] * 256, [16] * 256, 256)])
+def test_plans_take_the_items_that_the_rules_say(pages, tail, items):
+    assert len(_weights(pages, tail, 32, 8, 256)) == items
