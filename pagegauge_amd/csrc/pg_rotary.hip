@@ -26,8 +26,13 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlockUnits = 640;          // of a workgroup, where there are many
-constexpr int kMaxPairs = 4096;           // of a workgroup, 32 KiB of LDS
+constexpr int kMaxPairs = 4096;           // of tokens that share a workgroup, 32 KiB of LDS
 constexpr int kMaxUnits = 60000;          // of a workgroup
+// A token by itself may have more pairs; its sines fill at most the LDS that a launch
+// gets without asking for more, and its head is one slice.
+constexpr int kMaxHeadDim = 16384;
+static_assert(sizeof(float2) * (kMaxHeadDim / 2) <= 64 * 1024 && kMaxPairs <= kMaxHeadDim / 2, "LDS of a workgroup");
+static_assert(kMaxHeadDim / 2 <= kMaxUnits, "units of a head");
 constexpr int64_t kFull = 2048 * kThreads;     // units of a call
 
 struct RotaryRows {
@@ -221,7 +226,7 @@ extern "C" int32_t pg_rotate(const void* query, int64_t query_token_stride,
   clear_error();
   if (query_heads < 0 || key_heads < 0 || tokens < 0 || query_heads + static_cast<int64_t>(key_heads) <= 0)
     return fail(PG_ERROR_INVALID_ARGUMENT, "token and head counts must be nonnegative, with a head");
-  if (query_heads > 65535 || key_heads > 65535 || head_dim > 16384)
+  if (query_heads > 65535 || key_heads > 65535 || head_dim > kMaxHeadDim)
     return fail(PG_ERROR_UNSUPPORTED, "at most 65535 heads of 16384 dims");
   if (!positions || !turns || (query_heads && (!query || !out_query)) || (key_heads && (!key || !out_key)))
     return fail(PG_ERROR_INVALID_ARGUMENT, "null tensor pointer");
