@@ -263,6 +263,16 @@ def require_current_device(*tensors) -> None:
         launch_stream(device)
 
 
+def refuse_gradients(*tensors) -> None:
+    """ValueError where autograd would follow one of the tensors (None aside): the
+    kernels have no backward pass, and the result would silently have no history."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("no gradient is computed here: call it under torch.no_grad() "
+                                 "or on detached tensors")
+
+
 def pointer(t: torch.Tensor, dtype, shape: tuple, device: int, what: str) -> int:
     """Address of a contiguous tensor of this type, shape and device; ``what``
     is the ValueError of another one."""

@@ -339,11 +339,13 @@ class Int4PagedDecode:
         [B, Hq, 128], with ``return_lse`` also the base-2 lse float32 [B, Hq].
         ``exact_cache`` is the (K, V) pages of the tail, ``value_center``
         [B, Hkv, 128].  A request without tokens gives its center (or zeros)
-        and an lse of -inf."""
+        and an lse of -inf.  Queries, pages and centers that autograd follows are
+        refused: there is no backward pass."""
         if not self._planned:
             raise RuntimeError("plan() must be called before run()")
         hkv, hq, batch = self._num_kv_heads, self._num_qo_heads, self._batch
         _check_query(q, batch, hq)
+        _capi.refuse_gradients(q, value_center)
         device = q.get_device()
         pool, codes_at, scales_at = _pool(codes, scales, hkv, device)
         exact_k_at = exact_v_at = center_at = lse_at = None
@@ -351,6 +353,7 @@ class Int4PagedDecode:
             if exact_cache is None:
                 raise ValueError("a plan with a tail needs the exact pages")
             exact_k, exact_v = exact_cache
+            _capi.refuse_gradients(exact_k, exact_v)
             pages, exact_k_at = _exact(exact_k, hkv, device, _EXACT_KEY)
             count, exact_v_at = _exact(exact_v, hkv, device, _EXACT_VALUE)
             if self._id_ranges[1] is not None:

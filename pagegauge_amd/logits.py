@@ -50,7 +50,8 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
     ``history`` is int32 or int64 [B, capacity], each row's tokens first;
     lengths are int32 [B], the penalties and biases float32.  Tokens outside
     the vocabulary (padding) are ignored.  Computed in float32; ``out`` may be
-    ``logits``, but not otherwise overlap them.  Returns ``out``."""
+    ``logits``, but not otherwise overlap them.  Logits, penalties and biases that
+    autograd follows are refused: there is no backward pass.  Returns ``out``."""
     dtype = _DTYPES.get(logits.dtype)
     if dtype is None or logits.dim() != 2:
         raise ValueError("logits must be FP16, BF16 or float32 [B, V] rows")
@@ -70,6 +71,7 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
         raise ValueError("logits shaped in place must keep their strides")
     elif out.get_device() != device:
         raise ValueError(_capi.DEVICE_ERROR)
+    _capi.refuse_gradients(logits, repetition, frequency, presence, bias_values)
     rows = (batch,)
     token_bytes = capacity = history_row = 0
     history_at = lengths_at = prompts_at = None

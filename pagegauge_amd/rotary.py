@@ -105,7 +105,8 @@ class RotaryEmbedding:
         """(rotated query, rotated key) of rows [T, H, head_dim] at ``positions``
         [T] (int32 or int64): FP16, BF16 or FP32, any token and head strides
         (slices of a fused projection).  ``key`` may be None.  The outputs may
-        be the inputs themselves, but not otherwise overlap them."""
+        be the inputs themselves, but not otherwise overlap them.  Rows that
+        autograd follows are refused: there is no backward pass."""
         dtype = _DTYPES.get(query.dtype)
         if dtype is None:
             raise ValueError("rotary rows must be FP16, BF16 or FP32")
@@ -118,6 +119,7 @@ class RotaryEmbedding:
             out_key, key_args, key_in_place = self._rows(key, out_key, tokens, query.dtype)
             if in_place != key_in_place:
                 raise ValueError("query and key are rotated in place together or not at all")
+        _capi.refuse_gradients(query, key)
         device = query.get_device()
         if positions.get_device() != device or self.turns.get_device() != device \
                 or out_query.get_device() != device \

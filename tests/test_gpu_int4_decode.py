@@ -309,3 +309,17 @@ def test_small_products_beside_large_ones(cuda, kv_heads, group):
                      codes[::16].astype(np.float64))
     want = (dots * scales[..., None] * 4.0 * np.log2(np.e)).reshape(batch, -1)
     assert (np.abs(lse.double().cpu().numpy() - want) <= np.abs(want) * 2.0 ** -21 + 2.0 ** -20).all()
+
+
+def test_gradients_are_refused(cuda):
+    """The result would have no history: it is not computed, but for no_grad()."""
+    c = Case(cuda, [40], [20], 2, 4)
+    want = c.run()
+    wanted = dict(q=c.q, value_center=c.center, exact_cache=c.exact)
+    for name, t in wanted.items():
+        t = ([x.clone().requires_grad_() for x in t] if name == "exact_cache"
+             else t.clone().requires_grad_())
+        with pytest.raises(ValueError, match="no gradient"):
+            c.run(**{name: t})
+        with torch.no_grad():
+            assert torch.equal(c.run(**{name: t})[0], want[0])

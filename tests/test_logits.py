@@ -54,3 +54,13 @@ def test_c_entry_point_refuses(over, code, message):
              allowed=None, allowed_stride=0, stream=None)
     a.update(over)
     assert _capi.library().pg_shape_logits(*a.values()) == code and message in _capi.last_error()
+
+
+@pytest.mark.parametrize("name", ["logits", "repetition", "frequency", "presence", "bias_values"])
+def test_gradients_are_refused(name):
+    """The result would have no history: it is not computed, but for no_grad()."""
+    a = dict(logits=torch.zeros(2, 40), history=_H, history_lengths=_N, repetition=_F, frequency=_F,
+             presence=_F, bias_tokens=_H, bias_values=torch.zeros(2, 5))
+    a[name] = a[name].clone().requires_grad_()
+    with pytest.raises(ValueError, match="no gradient"):
+        shape_logits(a.pop("logits"), **a)

@@ -110,3 +110,15 @@ def test_by_parts_where_the_slowest_pair_turns_more_than_once(r, theta, context,
     for i in range(r // 2):
         share = min(1.0, max(0.0, (i - low) / (high - low)))
         assert math.isclose(float(got[i]), float(f[i]) * (1 - share + share / factor), rel_tol=1e-12)
+
+
+@pytest.mark.parametrize("name", ["query", "key"])
+def test_rows_with_a_gradient_are_refused(name):
+    """The result would have no history: it is not computed, but for no_grad()."""
+    heads = {"query": 4, "key": 2}[name]
+    rows = torch.zeros(3, heads, 128, dtype=torch.float16, requires_grad=True)
+    for x in (rows, rows * 2.0):
+        with pytest.raises(ValueError, match="no gradient"):
+            _call(**{name: x})
+    with torch.no_grad(), pytest.raises(ValueError, match="current CUDA device"):
+        _call(**{name: rows})
