@@ -251,3 +251,42 @@ def test_serving_tables(cuda):
             assert (np.abs(out[b].double().cpu().numpy() - want) <= allowed).all()
         ledger.commit_decode(batch)
     assert len(read_back) >= 4
+
+
+def test_captured_steps_close_pages(cuda):
+    """The steps of one page window to its last token: the replay that fills the page
+    holds it in 4 bits, from rows that earlier replays stored."""
+    from int4_helpers import held
+
+    eager, graphed = (Served(cuda, [16, 160], 16) for _ in range(2))
+    for _ in range(16):
+        eager.prepare()
+        eager.step()
+        eager.advance()
+    graphed.prepare()
+    keep = [t.clone() for t in (graphed.tokens, *graphed.exact, graphed.codes, graphed.scales)]
+    graphed.step()                                      # warm-up
+    for t, was in zip((graphed.tokens, *graphed.exact, graphed.codes, graphed.scales), keep):
+        t.copy_(was)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        graphed.step()
+    pages = graphed.code_ids.long()
+    for i in range(16):
+        assert not graphed.prepare()
+        before = graphed.codes[pages].clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        graphed.check()
+        closed = ~(graphed.codes[pages] == before).flatten(1).all(1)
+        assert closed.tolist() == [i == 15] * 2
+        graphed.advance()
+    assert graphed.length == [32, 176]
+    for (codes, scales), ring in zip(unpack(graphed.codes, graphed.scales), graphed.exact):
+        for b in range(2):
+            want_codes, want_scales = held(ring[int(graphed.exact_ids[b])].float().cpu().numpy())
+            np.testing.assert_array_equal(codes[int(pages[b])], want_codes)
+            np.testing.assert_array_equal(scales[int(pages[b])], want_scales)
+    for name in ("tokens", "history", "codes", "scales", "out", "lse", "shaped"):
+        assert torch.equal(getattr(eager, name), getattr(graphed, name)), name
+    assert all(torch.equal(a, b) for a, b in zip(eager.exact, graphed.exact))
