@@ -21,9 +21,7 @@
 // to 1.  One row of 32768 takes 5.6 us.  Measured and not taken at 64 rows: 512
 // threads with tiles of 4096 or 8192 (19.5, 20.5 us), 256 with 4096 (22.3), and
 // two tiles per workgroup with the tokens kept in registers (21.2).
-#include "pg_common.h"
-
-#include <hip/hip_bf16.h>
+#include "pg_types.h"
 
 #include <algorithm>
 
@@ -54,21 +52,6 @@ struct LogitsArgs {
   int biases;
   const int32_t* allowed;
   int64_t allowed_stride;
-};
-
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__hip_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_float(float v) { return v; }
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __hip_bfloat16 from_float<__hip_bfloat16>(float v) {
-  return __float2bfloat16(v);
-}
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-
-template <typename T, int kVec>
-struct alignas(sizeof(T) * kVec) Vec {
-  T v[kVec];
 };
 
 // Grid (rows, tiles), so that the tiles of a row are a multiple of the batch apart

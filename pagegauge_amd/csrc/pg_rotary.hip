@@ -16,8 +16,7 @@
 // units with 2 or 4 in flight per thread 65.9 and 69, and longer ones (1280, 2560)
 // 64.3 and 69.
 #include "pg_rotary.h"
-
-#include <hip/hip_bf16.h>
+#include "pg_types.h"
 
 #include <algorithm>
 
@@ -62,21 +61,6 @@ struct RotaryArgs {
   int tokens_per_block;
   int wide_positions;
   Divisor pairs, units, slice; // rotary_dim / 2, units of a head, heads_per_slice
-};
-
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__hip_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_float(float v) { return v; }
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __hip_bfloat16 from_float<__hip_bfloat16>(float v) {
-  return __float2bfloat16(v);
-}
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-
-template <typename T, int kVec>
-struct alignas(sizeof(T) * kVec) Vec {
-  T v[kVec];
 };
 
 // A workgroup takes the heads of a slice of a few tokens: their sines once, into
