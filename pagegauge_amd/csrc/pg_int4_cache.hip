@@ -360,8 +360,10 @@ constexpr int kQueryRows = 4;      // query heads of a wave
 // is that of its trips to memory, one for the request's position and ids and one
 // for everything else (as a chain of five, 256 requests took 10.4 us in place of
 // 6.9).  With a wave per query head, more than the chip holds at once, 256 requests
-// of 32 query and 8 KV heads took 6.9 us and 1024 took 15.0; now 6.3 and 11.2, and 3.7
-// for 8 requests that all close a page.
+// of 32 query and 8 KV heads took 6.9 us and 1024 took 15.0; now 6.3 to 7.4 and 11.2, and
+// 3.7 to 4.4 for 8 requests that all close a page.  Large batches are bound by its accesses
+// of 2 bytes per lane and the sines that 16 waves of a request work out alike: at a copy's
+// rate their bytes take 1.7 and 6.7 us (5.5 and 22 where all close a page, now 8.7 and 23.8).
 __global__ __launch_bounds__(kWave * kWavesPerBlock) void int4_rope_append_kernel(AppendArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t own[kWavesPerBlock][kHeadDim];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;

@@ -37,7 +37,7 @@
 // (work item, page ids, pages, partial rows) before.  Kernel times on MI355X, and
 // of the same walk without its arithmetic: 256 requests (829 MB) 170 and 165 us,
 // 8 requests of 4K to 32K (164 MB) 34 and 32, one of 49K tokens (53 MB) 14.9 and
-// 12.3, of 4K (5 MB) 5.5 and 4.6; a join adds 2.4 to 4.6 us.  Measured and not
+// 12.4, of 4K (5 MB) 5.5 and 4.7; a join adds 2.4 to 4.6 us.  Measured and not
 // taken: 8 waves a workgroup (one fits a CU, and nothing covers its start and
 // end: 256 requests 191 us), and a join by the workgroup that ends last (49K
 // tokens 18.7 us a call against 17.2 with the second launch, before the last

@@ -11,7 +11,7 @@ apart, of rows centered on the request's channel means:
 * ``quantize_pages`` -- a prompt's token-major K and V into pages, with the
   centered FP16 copies of its exact pages (the 4-bit ``update.prefill_page_gauge``);
 * ``dequantize_pages`` -- back to FP16, for a prompt that continues a cached
-  prefix;
+  prefix (its attention is the caller's: ``decoder.prefill`` takes whole prompts);
 * ``rope_append`` -- one token per request: rotation, centered append to the
   exact pages, and the page that a token completed held in 4 bits (the 4-bit
   ``rope_append_page_gauge_slots``, with ``rotary.RotaryEmbedding``);
