@@ -54,21 +54,22 @@ int32_t build_int4_plan(const int32_t* host_indptr, const int32_t* host_tail_ind
   // long exact tails would be left whole where these take the target up alone (100000
   // history pages beside 4000 exact ones: 1393 us, now 393) or as many requests do (299 of
   // 41 pages beside one of 3000 exact ones: 881 us, now 133): no share exceeds two full
-  // items' and twice an even one.
+  // items' and twice an even one, unless a request would have too many items.
   const int64_t cus = num_cus > 0 ? num_cus : 256;
   auto items_of = [&](int64_t cap) {
     int64_t n = 0;
     for (const Request& r : requests) n += r.cuts(cap);
     return n;
   };
+  const int64_t full = std::max<int64_t>(2 * kInt4MaxItemPages, ceil_div(total, kInt4MaxItemsPerRequest));
   auto balanced = [&](int64_t target) {
     int64_t low = kInt4Waves * kInt4GroupPages, high = std::max(low, total);
-    if (items_of(high) > target) return std::min<int64_t>(high, 2 * kInt4MaxItemPages);
+    if (items_of(high) > target) return std::min(high, full);
     while (low < high) {
       const int64_t cap = low + (high - low) / 2;
       if (items_of(cap) <= target) high = cap; else low = cap + 1;
     }
-    return std::min(high, std::max<int64_t>(2 * kInt4MaxItemPages, 2 * ceil_div(total, target)));
+    return std::min(high, std::max(full, 2 * ceil_div(total, target)));
   };
   // One workgroup per CU is the better plan (49K tokens: 32 items 16.6 us, 64 items
   // 18.1; 64K 18.9 and 20.8) unless its waves cannot hold their pages (128K tokens: 33

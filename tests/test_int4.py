@@ -274,3 +274,12 @@ def test_shares_of_drawn_batches():
     ([144] * 256, [16] * 256, 256)])
 def test_plans_take_the_items_that_the_rules_say(pages, tail, items):
     assert len(_weights(pages, tail, 32, 8, 256)) == items
+
+
+@pytest.mark.parametrize("pages,tail", [([100000, 0], [0, 600000]), ([0] * 10000, [3000000] + [0] * 9999)])
+def test_long_tails_keep_to_the_items_of_a_request(pages, tail):
+    """Tails of millions of tokens are shared out among as many items as a request may have."""
+    tables = [np.concatenate(([0], np.cumsum(n))).tolist() for n in (pages, tail)]
+    plan, items, _ = int4.plan_work_items(*tables)
+    assert 2048 < plan.max_items_per_request <= 4096
+    assert int(items[:, 5].max()) == sum(tail)
