@@ -163,7 +163,8 @@ def dequantize_pages(codes: torch.Tensor, scales: torch.Tensor,
     """(K, V) rows [tokens, Hkv, 128] in FP16 that pages ``page_ids`` (device
     int32; None: the whole pool in order) stand for, ``code * scale + center``.
     ``tokens`` defaults to whole pages.  Ids outside the pool give zeros.
-    ``key`` and ``value`` may be given (token rows may be strided)."""
+    ``key`` and ``value`` may be given (token rows may be strided).  Scales and
+    centers that autograd follows are refused: there is no backward pass."""
     if codes.dim() != 4 or codes.shape[1] == 0:
         raise ValueError(_CODES)
     heads, device = codes.shape[1], codes.get_device()
@@ -173,6 +174,7 @@ def dequantize_pages(codes: torch.Tensor, scales: torch.Tensor,
     tokens = pages * PAGE if tokens is None else int(tokens)
     if not 0 <= tokens <= pages * PAGE:
         raise ValueError(f"{pages} pages hold at most {pages * PAGE} tokens, asked for {tokens}")
+    _capi.refuse_gradients(scales, key_center, value_center)
     key_center_at, value_center_at = _centers(key_center, value_center, (heads, DIM), device)
     shape, dense = (tokens, heads, DIM), (heads * DIM, DIM, 1)
     strides = []

@@ -283,3 +283,15 @@ def test_long_tails_keep_to_the_items_of_a_request(pages, tail):
     plan, items, _ = int4.plan_work_items(*tables)
     assert 2048 < plan.max_items_per_request <= 4096
     assert int(items[:, 5].max()) == sum(tail)
+
+
+@pytest.mark.parametrize("name", ["scales", "key_center", "value_center"])
+def test_dequantize_refuses_gradients(name):
+    """The result would have no history: it is not computed, but for no_grad()."""
+    codes, scales = int4.allocate_pages(2, 2, "cpu")
+    a = dict(scales=scales, key_center=_half(2, 128), value_center=_half(2, 128))
+    a[name].requires_grad_()
+    with pytest.raises(ValueError, match="no gradient"):
+        int4.dequantize_pages(codes, **a)
+    with torch.no_grad(), pytest.raises(ValueError, match="current CUDA device"):
+        int4.dequantize_pages(codes, **a)
