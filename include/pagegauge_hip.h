@@ -7,8 +7,8 @@
  * void* (NULL = the null stream).  Every function returns PG_OK (0) or an
  * error code; pg_last_error() then gives the message of the failing call on
  * the calling thread.  No entry point allocates device memory, synchronises
- * the stream or returns data to the host except pg_decode_plan (which copies
- * a work list into the caller's workspace and waits for that copy).
+ * the stream or returns data to the host except the plans (which copy a
+ * work list into the caller's workspace and wait for that copy).
  *
  * Layouts (reference conventions, tests/page_gauge_append_extension.cu:1-40):
  *   query / key / value rows   fp16 [B, H, 128] with contiguous head rows,
@@ -781,6 +781,161 @@ int32_t pg_shape_logits(const void* logits, int64_t logits_stride, void* out, in
                         const void* bias_tokens, const float* bias_values, int32_t biases,
                         int32_t token_bytes, const int32_t* allowed, int64_t allowed_stride,
                         void* stream);
+
+/* ------------------------------------------------------------------------
+ * Pages of a pool: copied, counted, handed out, moved together.
+ * ---------------------------------------------------------------------- */
+
+/* One plane of a pool: ``rows`` (layers, or 1) of pages page_stride bytes apart,
+ * page_bytes of each used, rows row_stride bytes apart. */
+typedef struct pg_page_plane {
+  void* base;
+  int64_t page_bytes;
+  int64_t page_stride;
+  int64_t rows;
+  int64_t row_stride;
+} pg_page_plane_t;
+
+/* Copies page source[i] to page target[i], i < moves, in every plane and row.  Ids
+ * outside [0, pages) skip their copy.  Targets must differ from each other and be no
+ * call's sources; a source may go to several targets.  host_planes is read by the call. */
+int32_t pg_copy_pages(const pg_page_plane_t* host_planes, int32_t planes, int64_t pages,
+                      const int32_t* source, const int32_t* target, int64_t moves, void* stream);
+
+/* Users per page: refs int32 [pages], 16-byte aligned.  Adds ``by`` to refs[ids[i]]
+ * for each i < count, by < 0 to no less than 0.  Ids may repeat; those outside
+ * [0, pages) are skipped. */
+int32_t pg_pool_adjust(int32_t* refs, int64_t pages, const int32_t* ids, int64_t count, int32_t by,
+                       void* stream);
+
+/* The ``count`` lowest pages without users, ascending, into out, -1 where there are no
+ * more; their counts become 1. */
+int32_t pg_pool_take(int32_t* refs, int64_t pages, int32_t* out, int64_t count, void* stream);
+
+/* The fewest moves that bring the pages in use, live[0] of them, to the front: the
+ * i-th lowest one at or past live[0] (source[i]) to the i-th lowest free one below it
+ * (target[i]); -1 in the rest of the pages / 2 entries.  remap[p] is where page p is
+ * afterwards, -1 for a free one.  refs is only read. */
+int32_t pg_pool_stage_compaction(const int32_t* refs, int64_t pages, int32_t* source, int32_t* target,
+                                 int32_t* remap, int32_t* live, void* stream);
+
+/* Moves the counts along: refs[target[i]] = refs[source[i]], refs[source[i]] = 0. */
+int32_t pg_pool_commit_compaction(int32_t* refs, int64_t pages, const int32_t* source,
+                                  const int32_t* target, int64_t moves, void* stream);
+
+/* out[i] = remap[ids[i]], i < count; ids outside [0, pages) stay.  out may be ids. */
+int32_t pg_rewrite_ids(const int32_t* ids, const int32_t* remap, int64_t pages, int64_t count,
+                       int32_t* out, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention over shared prefixes, and over selected pages.
+ * ---------------------------------------------------------------------- */
+
+/* Plan of either (opaque to the caller; copied by value).  Offsets lie in the
+ * workspace. */
+typedef struct pg_segment_plan {
+  int32_t batch_size;
+  int32_t num_qo_heads;
+  int32_t num_kv_heads;
+  int32_t kind;
+  int32_t has_prefix;
+  int32_t has_history;
+  int32_t has_tail;
+  int32_t num_items;
+  int32_t max_slots;
+  int32_t slot_base_count;
+  int32_t selected_pages;
+  int32_t first_pages;
+  int32_t last_pages;
+  int32_t max_pages;
+  int64_t items_offset;
+  int64_t slot_ptr_offset;
+  int64_t slot_base_offset;
+  int64_t indptr_offset;
+  int64_t scores_offset;
+  int64_t partial_offset;
+  int64_t partial_rows;
+  int64_t workspace_bytes;
+} pg_segment_plan_t;
+
+/* Cuts a batch into work items.  Prefix s, pages host_prefix_indptr[s] .. [s + 1] of
+ * the prefixes' table, is shared by requests host_prefix_requests[2 s] ..
+ * [2 s + 1]; a request may have none, or several.  Its own pages are host_indptr[b] ..
+ * [b + 1], its exact ones host_tail_indptr[b] .. [b + 1] (NULL: none).  kind is
+ * PG_KV_INT8 or PG_KV_FP16, of prefixes' and own pages; 1 to 16 query heads per KV
+ * head.  The work list is copied into the workspace, and the copy waited for. */
+int32_t pg_prefix_plan(const int32_t* host_prefix_requests, const int32_t* host_prefix_indptr,
+                       int32_t segments, const int32_t* host_indptr, const int32_t* host_tail_indptr,
+                       int32_t batch_size, int32_t num_qo_heads, int32_t num_kv_heads, int32_t kind,
+                       int32_t num_cus, void* workspace, int64_t workspace_bytes,
+                       pg_segment_plan_t* plan, void* stream);
+
+/* The same on the host alone, and with selected_pages > 0 (and no prefixes) that of
+ * pg_sparse_plan: items_out (NULL, or room for items_capacity items of 16 int32: first
+ * request, first row, rows, prefix or -1, first and end page, the last one, first and end
+ * tail page, the last one, place in slot_base or -1, split, the request's first page and
+ * pages, two zeros), slot_ptr_out [B + 1] and slot_base_out, either NULL. */
+int32_t pg_segment_plan_host(const int32_t* host_prefix_requests, const int32_t* host_prefix_indptr,
+                             int32_t segments, const int32_t* host_indptr,
+                             const int32_t* host_tail_indptr, int32_t batch_size,
+                             int32_t num_qo_heads, int32_t num_kv_heads, int32_t kind,
+                             int32_t selected_pages, int32_t num_cus, pg_segment_plan_t* plan,
+                             int32_t* items_out, int64_t items_capacity, int32_t* slot_ptr_out,
+                             int32_t* slot_base_out, int64_t slot_base_capacity);
+
+/* Attention of query rows [B, Hq, 128] (fp16, dense heads) over the prefixes of each
+ * request, its own pages and its exact pages, plus the value center [B, Hkv, 128] (or
+ * NULL).  key and value: pages [*, 16, Hkv, 128], with PG_KV_INT8 codes whose scales are
+ * key_scale and value_scale [*, Hkv].  The last page of a prefix holds prefix_last_len[s]
+ * tokens, of a request's own ones last_page_len[b], of the tail tail_last_len[b], all
+ * read on the device.  The keys that a request sees must be centered alike.  out fp16
+ * [B, Hq, 128]; lse float32 [B, Hq] base 2, or NULL.  A request without tokens gives its
+ * center and an lse of -inf.  Runs that share a workspace must not overlap. */
+int32_t pg_prefix_run(const pg_segment_plan_t* plan, const void* query, int64_t query_batch_stride,
+                      const void* key, const void* value, const void* key_scale,
+                      const void* value_scale, const int32_t* prefix_indices,
+                      const int32_t* prefix_last_len, const int32_t* indices,
+                      const int32_t* last_page_len, const void* tail_k, const void* tail_v,
+                      const int32_t* tail_indices, const int32_t* tail_last_len,
+                      const void* value_center, void* out, float* lse, float sm_scale,
+                      void* workspace, void* stream);
+
+/* bounds int8 [pool_pages, Hkv, 2, 128]: the least and the largest code of each channel
+ * of pages page_ids[i], i < count (NULL: page i), over their first lengths[i] tokens
+ * (NULL: 16; 127 and -128 where that is 0).  Ids outside the pool are skipped. */
+int32_t pg_sparse_key_bounds(const void* key_codes, void* bounds, int64_t pool_pages,
+                             const int32_t* page_ids, const int32_t* lengths, int64_t count,
+                             int32_t kv_heads, void* stream);
+
+/* Plan of the attention over selected_pages INT8 pages of each request and KV head, among
+ * them its first first_pages and last last_pages; at most 65535 requests. */
+int32_t pg_sparse_plan(const int32_t* host_indptr, const int32_t* host_tail_indptr, int32_t batch_size,
+                       int32_t num_qo_heads, int32_t num_kv_heads, int32_t selected_pages,
+                       int32_t first_pages, int32_t last_pages, int32_t num_cus, void* workspace,
+                       int64_t workspace_bytes, pg_segment_plan_t* plan, void* stream);
+
+/* selected int32 [B, Hkv, selected_pages]: positions in each request's table, ascending,
+ * -1 past the last.  With q' the row of a query head in steps of 2^(x - 7), rounded half
+ * to even, at most 127 of them, where its largest magnitude is f 2^x with f in [0.5, 1),
+ * a page scores
+ *   max over the KV head's query heads of
+ *     f32(sum_d max(q'_d lo_d, q'_d hi_d) * key_scale) * 2^(x - 7),
+ * -inf for a row with an infinity or NaN and where the score is NaN.  The highest
+ * scores are taken, among equal ones the lowest positions. */
+int32_t pg_sparse_select(const pg_segment_plan_t* plan, const void* query, int64_t query_batch_stride,
+                         const void* bounds, const void* key_scale, const int32_t* indices,
+                         int32_t* selected, void* workspace, void* stream);
+
+/* pg_prefix_run without prefixes, over the own pages at the positions ``selected``
+ * [B, Hkv, selected_pages] alone (those outside a request's table are not read; of a
+ * request with fewer pages only that many entries are). */
+int32_t pg_sparse_run(const pg_segment_plan_t* plan, const void* query, int64_t query_batch_stride,
+                      const void* key, const void* value, const void* key_scale,
+                      const void* value_scale, const int32_t* indices, const int32_t* last_page_len,
+                      const int32_t* selected, const void* tail_k, const void* tail_v,
+                      const int32_t* tail_indices, const int32_t* tail_last_len,
+                      const void* value_center, void* out, float* lse, float sm_scale,
+                      void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

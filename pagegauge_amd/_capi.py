@@ -80,6 +80,42 @@ class Int4Plan(ctypes.Structure):
     ]
 
 
+class PagePlane(ctypes.Structure):
+    """Mirror of ``pg_page_plane_t``."""
+
+    _fields_ = [("base", _p), ("page_bytes", _i64), ("page_stride", _i64), ("rows", _i64),
+                ("row_stride", _i64)]
+
+
+class SegmentPlan(ctypes.Structure):
+    """Mirror of ``pg_segment_plan_t``."""
+
+    _fields_ = [
+        ("batch_size", _i32),
+        ("num_qo_heads", _i32),
+        ("num_kv_heads", _i32),
+        ("kind", _i32),
+        ("has_prefix", _i32),
+        ("has_history", _i32),
+        ("has_tail", _i32),
+        ("num_items", _i32),
+        ("max_slots", _i32),
+        ("slot_base_count", _i32),
+        ("selected_pages", _i32),
+        ("first_pages", _i32),
+        ("last_pages", _i32),
+        ("max_pages", _i32),
+        ("items_offset", _i64),
+        ("slot_ptr_offset", _i64),
+        ("slot_base_offset", _i64),
+        ("indptr_offset", _i64),
+        ("scores_offset", _i64),
+        ("partial_offset", _i64),
+        ("partial_rows", _i64),
+        ("workspace_bytes", _i64),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/pagegauge_hip.h
 PROTOTYPES = {
     "pg_last_error": (ctypes.c_char_p, []),
@@ -159,6 +195,24 @@ PROTOTYPES = {
                                  _p]),
     "pg_int4_decode_run": (_i32, [ctypes.POINTER(Int4Plan), _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p,
                                   _p, _i64, _p, _p, _f32, _p, _p]),
+    "pg_copy_pages": (_i32, [ctypes.POINTER(PagePlane), _i32, _i64, _p, _p, _i64, _p]),
+    "pg_pool_adjust": (_i32, [_p, _i64, _p, _i64, _i32, _p]),
+    "pg_pool_take": (_i32, [_p, _i64, _p, _i64, _p]),
+    "pg_pool_stage_compaction": (_i32, [_p, _i64, _p, _p, _p, _p, _p]),
+    "pg_pool_commit_compaction": (_i32, [_p, _i64, _p, _p, _i64, _p]),
+    "pg_rewrite_ids": (_i32, [_p, _p, _i64, _i64, _p, _p]),
+    "pg_prefix_plan": (_i32, [_p, _p, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32, _p, _i64,
+                              ctypes.POINTER(SegmentPlan), _p]),
+    "pg_segment_plan_host": (_i32, [_p, _p, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32,
+                                    ctypes.POINTER(SegmentPlan), _p, _i64, _p, _p, _i64]),
+    "pg_prefix_run": (_i32, [ctypes.POINTER(SegmentPlan), _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p,
+                             _p, _p, _p, _p, _p, _p, _p, _f32, _p, _p]),
+    "pg_sparse_key_bounds": (_i32, [_p, _p, _i64, _p, _p, _i64, _i32, _p]),
+    "pg_sparse_plan": (_i32, [_p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p, _i64,
+                              ctypes.POINTER(SegmentPlan), _p]),
+    "pg_sparse_select": (_i32, [ctypes.POINTER(SegmentPlan), _p, _i64, _p, _p, _p, _p, _p, _p]),
+    "pg_sparse_run": (_i32, [ctypes.POINTER(SegmentPlan), _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p,
+                             _p, _p, _p, _p, _p, _p, _f32, _p, _p]),
     "pg_shape_logits": (_i32, [_p, _i64, _p, _i64, _i32, _i32, _i32, _p, _i64, _i64, _p, _p, _p, _p,
                                _p, _p, _p, _i32, _i32, _p, _i64, _p]),
     "pg_argmax_f32": (_i32, [_p, _i32, _i32, _i64, _p, _p]),

@@ -73,6 +73,10 @@ SOURCES = {
     "pg_int4_cache.hip": ["-ffp-contract=off"],
     "pg_int4_decode.hip": [],
     "pg_logits.hip": [],
+    "pg_pages.hip": [],
+    "pg_segment_plan.cpp": [],
+    "pg_prefix.hip": [],
+    "pg_sparse.hip": [],
 }
 
 BENCH_SOURCES = {

@@ -1,0 +1,250 @@
+"""Attention of single tokens where requests share the beginnings of their contexts.
+
+Requests that fork from one prompt, or that follow one long document or
+instruction, hold the same pages at the front of their tables.
+``SharedPrefixDecode`` reads each shared page once for all of them: the prefix's
+keys and values meet the query rows of every request that has it in one product,
+and the partial softmax states join with those of a request's own pages and its
+exact FP16 tail.  Prefixes may nest (a common instruction, then a document, then
+the forks of one answer).
+
+Pages are INT8 (``decode.PageGaugeSegmentedDecode``'s: codes, and a scale per page
+and KV head) or FP16 (``decode.BatchDecodeWithPagedKVCacheWrapper``'s), with 1 to
+16 query heads per KV head.  Keys that one request sees must be centered alike:
+requests keep the key center of the prompt that they share (forks do).  The value
+center is one too: codes of shared values hold what that center left.
+
+Everything runs on the current stream and nothing but ``plan`` synchronises.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from . import _capi
+from .decode import (_check_cache, _check_index, _check_page_ids, _check_query, _check_scale, _host_i32,
+                     _host_tables, _num_cus, _page_id_range)
+
+DIM = 128
+PAGE = 16
+
+_KINDS = {torch.int8: _capi.PG_KV_INT8, torch.float16: _capi.PG_KV_FP16}
+_CENTERS = "centers must be contiguous float16 [B,Hkv,128]"
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _check_last(indptr: torch.Tensor, last: torch.Tensor, what: str) -> None:
+    """The last length of every table with pages lies in [1, 16] (host tensors)."""
+    if bool(((indptr[1:] > indptr[:-1]) & ((last < 1) | (last > PAGE))).any()):
+        raise ValueError(f"{what} must lie in [1, {PAGE}]")
+
+
+def _tables(indptr, indices, last, what: str = ""):
+    """Host indptr of a checked CSR page table, and the range of its page ids."""
+    name = f"{what}_" if what else ""
+    _check_index(indices, f"{name}indices")
+    _check_index(last, f"{name}last_page_len")
+    host, host_last = _host_tables(indptr, last, indices, what)
+    _check_last(host, host_last, f"{name}last_page_len")
+    return host, _page_id_range(indices, host)
+
+
+def _prefix_ranges(prefix_requests) -> torch.Tensor:
+    """Host int32 [S, 2] of the prefixes' requests."""
+    ranges = prefix_requests if isinstance(prefix_requests, torch.Tensor) else \
+        torch.tensor([tuple(r) for r in prefix_requests], dtype=torch.int32).reshape(-1, 2)
+    if ranges.dim() != 2 or ranges.shape[1] != 2:
+        raise ValueError("prefix_requests must be (first, end) of each prefix's requests, [S, 2]")
+    return _host_i32(ranges)
+
+
+def plan_work_items(indptr, tail_indptr=None, prefix_requests=(), prefix_indptr=(0,), num_qo_heads: int = 32,
+                    num_kv_heads: int = 8, kv_data_type=torch.int8, selected_pages: int = 0,
+                    num_cus: int = 256):
+    """Run the planner on the host only: ``(plan, items [n, 16], slot_ptr [B + 1],
+    slot_base)``, as ``pg_segment_plan_host`` gives them."""
+    lib = _capi.library()
+    host, ranges, shared = _host_i32(indptr), _prefix_ranges(prefix_requests), _host_i32(prefix_indptr)
+    tail = None if tail_indptr is None else _host_i32(tail_indptr)
+    if host.dim() != 1 or host.numel() < 2 or tail is not None and tail.shape != host.shape:
+        raise ValueError("indptr must be a 1-D tensor of batch_size + 1 >= 2 entries")
+    if shared.shape != (len(ranges) + 1,):
+        raise ValueError("prefix_indptr must have one entry per prefix and one more")
+    if kv_data_type not in _KINDS:
+        raise ValueError("pages must be int8 or float16")
+    batch, plan = host.numel() - 1, _capi.SegmentPlan()
+    args = (ranges.data_ptr(), shared.data_ptr(), len(ranges), host.data_ptr(), _ptr(tail), batch, num_qo_heads,
+            num_kv_heads, _KINDS[kv_data_type], selected_pages, num_cus, ctypes.byref(plan))
+    _capi.check(lib.pg_segment_plan_host(*args, None, 0, None, None, 0), "decode plan")
+    items = torch.empty(plan.num_items, 16, dtype=torch.int32)
+    slot_ptr = torch.empty(batch + 1, dtype=torch.int32)
+    slot_base = torch.empty(plan.slot_base_count, dtype=torch.int32)
+    _capi.check(lib.pg_segment_plan_host(*args, items.data_ptr(), items.shape[0], slot_ptr.data_ptr(),
+                                         slot_base.data_ptr(), slot_base.numel()), "decode plan")
+    return plan, items, slot_ptr, slot_base
+
+
+class _SegmentDecode:
+    """What attention over shared prefixes and over selected pages have in common:
+    the workspace with its plan, and the checks of a run."""
+
+    def __init__(self, workspace: torch.Tensor) -> None:
+        if not workspace.is_cuda or workspace.dtype != torch.uint8 or not workspace.is_contiguous() \
+                or workspace.data_ptr() % 256:
+            raise ValueError("workspace must be a contiguous CUDA uint8 tensor, 256-byte aligned")
+        self.workspace = workspace
+        self._device = workspace.get_device()
+        self._plan = _capi.SegmentPlan()
+        self._plan_ref = ctypes.byref(self._plan)
+        self._planned = False
+
+    @property
+    def num_work_items(self) -> int:
+        return int(self._plan.num_items)
+
+    @property
+    def workspace_bytes(self) -> int:
+        """Bytes of the workspace that the plan uses."""
+        return int(self._plan.workspace_bytes)
+
+    def _plan_tail(self, host, tail_indptr, tail_indices, tail_last_page_len):
+        if (tail_indptr is None) != (tail_indices is None) or (tail_indptr is None) != (
+                tail_last_page_len is None):
+            raise ValueError("tail indptr, indices and last_page_len go together")
+        if tail_indptr is None:
+            return None, None
+        tail, tail_range = _tables(tail_indptr, tail_indices, tail_last_page_len, "tail")
+        if tail.numel() != host.numel():
+            raise ValueError("history and tail page tables must cover the same batch")
+        return tail, tail_range
+
+    def _keep_plan(self, batch, num_qo_heads, num_kv_heads, kv_data_type, sm_scale, tables, ranges, tail_range):
+        self._planned = True
+        self._batch, self._num_qo_heads, self._num_kv_heads = batch, num_qo_heads, num_kv_heads
+        self._kv_dtype = kv_data_type
+        self._sm_scale = sm_scale if sm_scale is not None else 1.0 / math.sqrt(DIM)
+        self._tables = tables                       # alive, and where the kernels read
+        self._table_ptrs = tuple(_ptr(t) for t in tables)
+        self._ranges, self._tail_range = ranges, tail_range
+
+    def _run_args(self, q, kv_cache, k_page_scale, v_page_scale, exact_cache, value_center, out, lse, return_lse):
+        """Checked pointers of a run, and its outputs."""
+        hkv, hq, batch = self._num_kv_heads, self._num_qo_heads, self._batch
+        _check_query(q, batch, hq)
+        k_cache, v_cache = kv_cache
+        _capi.refuse_gradients(q, value_center, k_cache, v_cache, k_page_scale, v_page_scale)
+        device = q.get_device()
+        for name, cache in (("k_cache", k_cache), ("v_cache", v_cache)):
+            _check_cache(cache, name, self._kv_dtype, hkv)
+        pages = min(k_cache.shape[0], v_cache.shape[0])
+        if self._kv_dtype is torch.int8:
+            if k_page_scale is None or v_page_scale is None:
+                raise ValueError("INT8 pages need k_page_scale and v_page_scale")
+            _check_scale(k_page_scale, "k_page_scale", k_cache.shape[0], hkv)
+            _check_scale(v_page_scale, "v_page_scale", v_cache.shape[0], hkv)
+        elif k_page_scale is not None or v_page_scale is not None:
+            raise ValueError("FP16 pages have no scales")
+        for id_range in self._ranges:
+            _check_page_ids(id_range, pages, "KV")
+        exact_k = exact_v = None
+        if self._tables[-1] is not None:
+            if exact_cache is None:
+                raise ValueError("a plan with a tail needs the exact pages")
+            exact_k, exact_v = exact_cache
+            _capi.refuse_gradients(exact_k, exact_v)
+            _check_cache(exact_k, "exact_key", torch.float16, hkv)
+            _check_cache(exact_v, "exact_value", torch.float16, hkv)
+            _check_page_ids(self._tail_range, min(exact_k.shape[0], exact_v.shape[0]), "exact tail")
+        center_at = None
+        if value_center is not None:
+            center_at = _capi.pointer(value_center, torch.float16, (batch, hkv, DIM), device, _CENTERS)
+        for t in (k_cache, v_cache, k_page_scale, v_page_scale, exact_k, exact_v):
+            if t is not None and t.get_device() != device:
+                raise ValueError(_capi.DEVICE_ERROR)
+        out_at = lse_at = None
+        if out is not None:
+            out_at = _capi.pointer(out, torch.float16, q.shape, device,
+                                   "out must be contiguous float16, shaped like q")
+        if lse is not None:
+            lse_at = _capi.pointer(lse, torch.float32, (batch, hq), device,
+                                   "lse must be contiguous float32 [B,Hq]")
+        if self._device != device:
+            raise ValueError(_capi.DEVICE_ERROR)
+        stream = _capi.launch_stream(device)
+        if out is None:
+            out = torch.empty(q.shape, device=q.device, dtype=torch.float16)
+            out_at = out.data_ptr()
+        if lse is None and return_lse:
+            lse = torch.empty((batch, hq), dtype=torch.float32, device=q.device)
+            lse_at = lse.data_ptr()
+        cache_at = (k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_page_scale), _ptr(v_page_scale))
+        return cache_at, (_ptr(exact_k), _ptr(exact_v)), center_at, out, lse, out_at, lse_at, stream
+
+
+class SharedPrefixDecode(_SegmentDecode):
+    """Attention of one token per request over shared prefixes, a request's own pages,
+    an exact FP16 tail and the value center (``plan`` / ``run`` as
+    ``decode.PageGaugeSegmentedDecode``).  Runs of one object share its workspace and
+    must not overlap on different streams; it belongs to this object alone."""
+
+    def plan(self, prefix_requests, prefix_indptr, prefix_indices: torch.Tensor,
+             prefix_last_page_len: torch.Tensor, indptr, indices: torch.Tensor,
+             last_page_len: torch.Tensor, tail_indptr=None, tail_indices: Optional[torch.Tensor] = None,
+             tail_last_page_len: Optional[torch.Tensor] = None, num_qo_heads: int = 32,
+             num_kv_heads: int = 8, sm_scale: Optional[float] = None, kv_data_type=torch.int8,
+             num_cus: Optional[int] = None) -> None:
+        """``prefix_requests``: (first, end) of the neighbouring requests that have
+        each prefix, [S, 2], in any order, nested or overlapping.  CSR page tables of
+        the prefixes, of the requests' own pages and, with ``tail_indptr``, of the
+        exact pages; any of them may be empty, of a request or as a whole.
+        ``indices`` and the last lengths (device int32) must stay alive until the next
+        ``plan`` and are re-read by every run (lengths within [0, 16] may move), so a
+        captured run stays valid until the next ``plan``.  Waits for the GPU."""
+        if kv_data_type not in _KINDS:
+            raise ValueError("pages must be int8 or float16")
+        ranges = _prefix_ranges(prefix_requests)
+        host, own_range = _tables(indptr, indices, last_page_len)
+        tail, tail_range = self._plan_tail(host, tail_indptr, tail_indices, tail_last_page_len)
+        shared, shared_range = _host_i32(prefix_indptr), None
+        if shared.shape != (len(ranges) + 1,):
+            raise ValueError("prefix_indptr must have one entry per prefix and one more")
+        if len(ranges):
+            shared, shared_range = _tables(prefix_indptr, prefix_indices, prefix_last_page_len, "prefix")
+        else:
+            _check_index(prefix_indices, "prefix_indices")
+            _check_index(prefix_last_page_len, "prefix_last_page_len")
+        tables = (prefix_indices, prefix_last_page_len, indices, last_page_len, tail_indices, tail_last_page_len)
+        _capi.require_current_device(self.workspace, *tables)
+        batch = host.numel() - 1
+        _capi.call("pg_prefix_plan", ranges.data_ptr(), shared.data_ptr(), len(ranges), host.data_ptr(), _ptr(tail),
+                   batch, num_qo_heads, num_kv_heads, _KINDS[kv_data_type], int(num_cus or _num_cus(indices.device)),
+                   self.workspace.data_ptr(), self.workspace.numel(), self._plan_ref, _capi.current_stream())
+        self._keep_plan(batch, num_qo_heads, num_kv_heads, kv_data_type, sm_scale, tables,
+                        (own_range, shared_range), tail_range)
+
+    def run(self, q: torch.Tensor, kv_cache, k_page_scale: Optional[torch.Tensor] = None,
+            v_page_scale: Optional[torch.Tensor] = None, exact_cache=None,
+            value_center: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None,
+            out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, return_lse: bool = False):
+        """Attention of ``q`` [B, Hq, 128] (FP16, dense heads): ``out`` FP16 [B, Hq, 128],
+        with ``return_lse`` also the base-2 lse float32 [B, Hq].  ``kv_cache`` is the
+        (K, V) pages of prefixes and own tables, with INT8 pages their scales
+        [pages, Hkv]; ``exact_cache`` the (K, V) pages of the tail, ``value_center``
+        [B, Hkv, 128].  A request without tokens gives its center (or zeros) and an lse
+        of -inf.  Tensors that autograd follows are refused: there is no backward pass."""
+        if not self._planned:
+            raise RuntimeError("plan() must be called before run()")
+        cache_at, exact_at, center_at, out, lse, out_at, lse_at, stream = self._run_args(
+            q, kv_cache, k_page_scale, v_page_scale, exact_cache, value_center, out, lse, return_lse)
+        prefix_ids, prefix_last, indices, last, tail_indices, tail_last = self._table_ptrs
+        _capi.call("pg_prefix_run", self._plan_ref, q.data_ptr(), q.stride(0), *cache_at, prefix_ids, prefix_last,
+                   indices, last, *exact_at, tail_indices, tail_last, center_at, out_at, lse_at,
+                   float(self._sm_scale if sm_scale is None else sm_scale), self.workspace.data_ptr(), stream)
+        return (out, lse) if return_lse else out
