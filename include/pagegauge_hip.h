@@ -874,7 +874,8 @@ int32_t pg_prefix_plan(const int32_t* host_prefix_requests, const int32_t* host_
  * pg_sparse_plan: items_out (NULL, or room for items_capacity items of 16 int32: first
  * request, first row, rows, prefix or -1, first and end page, the last one, first and end
  * tail page, the last one, place in slot_base or -1, split, the request's first page and
- * pages, two zeros), slot_ptr_out [B + 1] and slot_base_out, either NULL. */
+ * pages, rows that its workgroup is made for, a zero), slot_ptr_out [B + 1] and
+ * slot_base_out, either NULL. */
 int32_t pg_segment_plan_host(const int32_t* host_prefix_requests, const int32_t* host_prefix_indptr,
                              int32_t segments, const int32_t* host_indptr,
                              const int32_t* host_tail_indptr, int32_t batch_size,

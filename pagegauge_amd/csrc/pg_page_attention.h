@@ -39,7 +39,6 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 constexpr int kAttentionThreads = kWave * kSegmentWaves;
-constexpr int kNarrowRows = 8;       // query rows whose probabilities' parts share a product
 constexpr float kSlack = 4.0f;       // how far (base 2) a score may pass the base
 constexpr float kExactExponent = 10.0f;   // of the sums over exact pages
 
@@ -296,19 +295,26 @@ __device__ __forceinline__ void exact_pages(RowState& st, const v8h (&q)[4], con
   pipelined(groups, buf, issue, compute);
 }
 
+// What the waves of a workgroup meet in.
+template <bool kWide>
+struct NarrowMeeting {
+  static constexpr int kRows = kWide ? 16 : kNarrowRows;
+  float o[kSegmentWaves][kRows][kHeadDim];
+  float m[kSegmentWaves][kRows];
+  float l[kSegmentWaves][kRows];
+};
+
 template <bool kCodes, bool kSelected, bool kWide>
-__global__ __launch_bounds__(kAttentionThreads, 2) void page_attention_kernel(PageAttentionArgs a) {
-  constexpr int kRows = kWide ? 16 : kNarrowRows;
-  __shared__ float part_o[kSegmentWaves][kRows][kHeadDim];
-  __shared__ float part_m[kSegmentWaves][kRows];
-  __shared__ float part_l[kSegmentWaves][kRows];
+__device__ __forceinline__ void page_attention(const PageAttentionArgs& a, const SegmentItem& it, int kv,
+                                               NarrowMeeting<kWide>& meet) {
+  constexpr int kRows = NarrowMeeting<kWide>::kRows;
+  auto& part_o = meet.o;
+  auto& part_m = meet.m;
+  auto& part_l = meet.l;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const int n = lane & 15, kg = lane >> 4;
   const int hkv = a.num_kv_heads;
-  // KV heads vary fastest: with 8 of them each XCD reads one head's lines
-  const int kv = blockIdx.x % hkv;
-  const SegmentItem it = a.items[blockIdx.x / hkv];
 
   // query rows: B operand, column n = row n % kRows, dims in the order of K's loads;
   // columns past the rows repeat the first one and are dropped at the end

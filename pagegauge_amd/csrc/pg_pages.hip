@@ -11,6 +11,10 @@
 namespace pg {
 namespace {
 
+// plain vectors: structs of them, not yet loaded, would go through LDS
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
 constexpr int kThreads = 256;
 constexpr int kPlanesPerLaunch = 32;
 
@@ -40,27 +44,25 @@ constexpr uint32_t kCopyBlock = kThreads * kCopyInFlight;
 
 template <typename T>
 __device__ __forceinline__ void copy_block(const CopyArgs& a, const CopyPlane& p, uint8_t* row, uint32_t first) {
-  const T* from[kCopyInFlight];
-  T* to[kCopyInFlight];
   T value[kCopyInFlight];
+  int64_t to[kCopyInFlight];
 #pragma unroll
   for (int i = 0; i < kCopyInFlight; ++i) {
     const uint64_t at = static_cast<uint64_t>(first) * kCopyBlock + i * kThreads + threadIdx.x;
     const uint64_t move = p.shift >= 0 ? at >> p.shift : at / p.page_units;
-    to[i] = nullptr;
-    if (move >= a.moves) continue;
-    const uint32_t unit = static_cast<uint32_t>(at - move * p.page_units);
-    const int32_t source = a.source[move], target = a.target[move];
-    if (source < 0 || source >= a.pages || target < 0 || target >= a.pages) continue;
-    from[i] = reinterpret_cast<const T*>(row + source * p.page_stride) + unit;
-    to[i] = reinterpret_cast<T*>(row + target * p.page_stride) + unit;
+    to[i] = -1;
+    if (move < a.moves) {
+      const int64_t unit = static_cast<int64_t>(at - move * p.page_units) * sizeof(T);
+      const int32_t source = a.source[move], target = a.target[move];
+      if (source >= 0 && source < a.pages && target >= 0 && target < a.pages) {
+        to[i] = target * p.page_stride + unit;
+        value[i] = *reinterpret_cast<const T*>(row + source * p.page_stride + unit);
+      }
+    }
   }
 #pragma unroll
   for (int i = 0; i < kCopyInFlight; ++i)
-    if (to[i]) value[i] = *from[i];
-#pragma unroll
-  for (int i = 0; i < kCopyInFlight; ++i)
-    if (to[i]) *to[i] = value[i];
+    if (to[i] >= 0) *reinterpret_cast<T*>(row + to[i]) = value[i];
 }
 
 // A plane's row (one layer) is copied as one sequence of the moves' pages, in blocks of
@@ -73,8 +75,8 @@ __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyArgs a) {
   const uint32_t row_index = block / p.row_blocks, first = block % p.row_blocks;
   uint8_t* row = p.base + row_index * p.row_stride;
   switch (p.log_bytes) {
-    case 4: return copy_block<uint4>(a, p, row, first);
-    case 3: return copy_block<uint2>(a, p, row, first);
+    case 4: return copy_block<v4u>(a, p, row, first);
+    case 3: return copy_block<v2u>(a, p, row, first);
     case 2: return copy_block<uint32_t>(a, p, row, first);
     case 1: return copy_block<uint16_t>(a, p, row, first);
     default: return copy_block<uint8_t>(a, p, row, first);

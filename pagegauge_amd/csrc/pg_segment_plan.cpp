@@ -15,9 +15,22 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct Unit {
   int32_t segment, request;               // segment -1: the request's own pages
   int64_t rows, pages, tail, tail_weight;
-  int64_t blocks() const { return ceil_div(rows, kSegmentRows); }
+  bool shared() const { return rows > kSegmentRows; }
+  // rows of one workgroup, and the partial rows that it makes of each
+  int64_t block_rows() const {
+    if (!shared()) return rows > kNarrowRows ? kSegmentRows : kNarrowRows;
+    return rows > 2 * kSharedRows ? 4 * kSharedRows : 2 * kSharedRows;
+  }
+  int64_t parts() const { return block_rows() == 2 * kSharedRows ? 2 : 1; }
+  int64_t blocks() const { return ceil_div(rows, block_rows()); }
+  // rows of each block, evenly, in whole waves over shared tiles
+  int64_t step() const {
+    return !shared() ? block_rows() : ceil_div(ceil_div(rows, blocks()), kSharedRows) * kSharedRows;
+  }
   int64_t weight() const { return pages + tail_weight * tail; }
-  int64_t cuts(int64_t cap) const { return std::max<int64_t>(1, ceil_div(weight(), cap)); }
+  int64_t cuts(int64_t cap) const {
+    return std::max<int64_t>(1, ceil_div(weight(), shared() ? cap : std::min<int64_t>(cap, kSegmentMaxPages)));
+  }
 };
 
 int32_t check_indptr(const int32_t* indptr, int32_t count) {
@@ -81,7 +94,7 @@ int32_t build_segment_plan(const SegmentBatch& b, SegmentWork& work, pg_segment_
     for (const Unit& u : units) n += u.cuts(cap) * u.blocks();
     return n;
   };
-  int64_t low = kSegmentWaves * kSegmentGroupPages, high = kSegmentMaxPages;
+  int64_t low = kSegmentWaves * kSegmentGroupPages, high = kSharedMaxPages;
   while (low < high) {
     const int64_t cap = low + (high - low) / 2;
     if (items_of(cap) <= target) high = cap; else low = cap + 1;
@@ -89,7 +102,7 @@ int32_t build_segment_plan(const SegmentBatch& b, SegmentWork& work, pg_segment_
   const int64_t cap = high;
   const int64_t count = items_of(cap);
   for (const Unit& u : units)
-    if (u.cuts(cap) > kSegmentMaxSlots) return fail(PG_ERROR_UNSUPPORTED, "too many pages in one request");
+    if (u.cuts(cap) * u.parts() > kSegmentMaxSlots) return fail(PG_ERROR_UNSUPPORTED, "too many pages in one request");
   if (count > static_cast<int64_t>(UINT32_MAX) / (kSegmentWaves * 64) / b.num_kv_heads)
     return fail(PG_ERROR_UNSUPPORTED, "too many work items");
 
@@ -106,7 +119,7 @@ int32_t build_segment_plan(const SegmentBatch& b, SegmentWork& work, pg_segment_
       if (work.slot_base.size() + requests > INT32_MAX) return fail(PG_ERROR_UNSUPPORTED, "too many work items");
       for (int32_t r = u.request; r < u.request + requests; ++r) {
         work.slot_base.push_back(static_cast<int32_t>(slots[r]));      // from the request's first one, so far
-        slots[r] += cuts;
+        slots[r] += cuts * u.parts();
         if (slots[r] > kSegmentMaxSlots) return fail(PG_ERROR_UNSUPPORTED, "too many pages in one request");
       }
     }
@@ -120,11 +133,11 @@ int32_t build_segment_plan(const SegmentBatch& b, SegmentWork& work, pg_segment_
       int64_t page_end = std::min(u.pages, w);
       int64_t exact_end = w <= u.pages ? 0 : (w - u.pages) / tail_weight;
       if (i + 1 == cuts) { page_end = u.pages; exact_end = u.tail; }
-      for (int64_t row = 0; row < u.rows; row += kSegmentRows) {
+      for (int64_t row = 0; row < u.rows; row += u.step()) {
         SegmentItem it{};
         it.request = u.request;
         it.row_first = static_cast<int32_t>(row);
-        it.rows = static_cast<int32_t>(std::min<int64_t>(kSegmentRows, u.rows - row));
+        it.rows = static_cast<int32_t>(std::min<int64_t>(u.step(), u.rows - row));
         it.segment = u.segment;
         it.page_begin = static_cast<int32_t>(begin + page);
         it.page_end = static_cast<int32_t>(begin + page_end);
@@ -133,7 +146,8 @@ int32_t build_segment_plan(const SegmentBatch& b, SegmentWork& work, pg_segment_
         it.tail_end = static_cast<int32_t>(tail_begin + exact_end);
         it.last_tail = static_cast<int32_t>(tail_begin + u.tail - 1);
         it.slot_at = slot_at;
-        it.split = static_cast<int32_t>(i);
+        it.block_rows = static_cast<int32_t>(u.block_rows());
+        it.split = static_cast<int32_t>(i * u.parts());
         if (own) {
           it.table_begin = b.indptr[u.request];
           it.table_pages = b.indptr[u.request + 1] - b.indptr[u.request];

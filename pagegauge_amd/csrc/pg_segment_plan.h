@@ -13,13 +13,17 @@ namespace pg {
 constexpr int kSegmentWaves = 4;          // waves of a workgroup
 constexpr int kSegmentGroupPages = 4;     // consecutive pages a wave takes at a time
 constexpr int kSegmentMaxPages = kSegmentWaves * 64;   // a wave holds its page ids one per lane
-constexpr int kSegmentRows = 16;          // query rows of an item
+constexpr int kSegmentRows = 16;          // query rows of an item without shared tiles
+constexpr int kNarrowRows = 8;            // or, with both parts of a probability in one product
+constexpr int kSharedRows = 32;           // of a wave over shared tiles: items of 2 or 4 waves' rows
+constexpr int kSharedMaxPages = 512;      // of an item over shared tiles, held in LDS
 constexpr int kSegmentMaxSlots = 1 << 16; // partial rows of one request
 
 // One workgroup's share, for one KV head: ``rows`` query rows over pages [page_begin,
 // page_end) of a page table and exact pages [tail_begin, tail_end), either perhaps empty.
 // Row i is row R = row_first + i of the segment's: query head R % group (of the KV head's)
-// of request ``request`` + R / group.
+// of request ``request`` + R / group.  Over shared tiles of 2 waves' rows each row has two
+// partial rows, in slots one after the other.
 struct SegmentItem {
   int32_t request, row_first, rows;
   int32_t segment;                        // of the prefix tables, or -1: the request's own table
@@ -28,7 +32,8 @@ struct SegmentItem {
   int32_t slot_at;                        // the requests' first slots: slot_base[slot_at + R / group]; -1: the output
   int32_t split;                          // added to these
   int32_t table_begin, table_pages;       // of the request, where pages are selected
-  int32_t reserved[2];
+  int32_t block_rows;                     // kNarrowRows, kSegmentRows, or 2 or 4 times kSharedRows: shared tiles
+  int32_t reserved;
 };
 static_assert(sizeof(SegmentItem) == 64, "work item layout");
 

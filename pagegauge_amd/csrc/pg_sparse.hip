@@ -48,7 +48,8 @@ __global__ __launch_bounds__(kBoundsThreads) void key_bounds_kernel(BoundsArgs a
   const uint8_t* from = a.codes + static_cast<int64_t>(page) * kPageSize * row_bytes + piece * 16;
   v4u x[kPageSize];
 #pragma unroll
-  for (int t = 0; t < kPageSize; ++t) x[t] = *reinterpret_cast<const v4u*>(from + t * row_bytes);
+  for (int t = 0; t < kPageSize; ++t)    // rows past the page's tokens are its last one again
+    x[t] = *reinterpret_cast<const v4u*>(from + min(t, max(length - 1, 0)) * row_bytes);
   v2i16 low[8], high[8];
 #pragma unroll
   for (int d = 0; d < 8; ++d) {
@@ -57,7 +58,6 @@ __global__ __launch_bounds__(kBoundsThreads) void key_bounds_kernel(BoundsArgs a
   }
 #pragma unroll
   for (int t = 0; t < kPageSize; ++t) {
-    if (t >= length) break;
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
       const v2i16 odd = as_pair(x[t][d]);
@@ -74,6 +74,10 @@ __global__ __launch_bounds__(kBoundsThreads) void key_bounds_kernel(BoundsArgs a
     // bytes 1 and 3 of the odd halves, and of the even ones, back in order
     least[d] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, low[d]), __builtin_bit_cast(uint32_t, low[4 + d]), 0x07030501u);
     most[d] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, high[d]), __builtin_bit_cast(uint32_t, high[4 + d]), 0x07030501u);
+  }
+  if (length == 0) {
+    least = v4u{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+    most = v4u{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
   }
   uint8_t* to = a.bounds + (static_cast<int64_t>(page) * a.heads + piece / kPieces) * 2 * kHeadDim + piece % kPieces * 16;
   *reinterpret_cast<v4u*>(to) = least;
@@ -278,6 +282,14 @@ __global__ __launch_bounds__(kPickThreads) void pick_pages_kernel(SelectArgs a) 
   }
 }
 
+template <bool kWide>
+__global__ __launch_bounds__(kAttentionThreads, 2) void selected_attention_kernel(PageAttentionArgs a) {
+  __shared__ NarrowMeeting<kWide> meet;
+  // KV heads vary fastest: with 8 of them each XCD reads one head's lines
+  const SegmentItem it = a.items[blockIdx.x / a.num_kv_heads];
+  page_attention<true, true, kWide>(a, it, blockIdx.x % a.num_kv_heads, meet);
+}
+
 }  // namespace
 }  // namespace pg
 
@@ -406,9 +418,9 @@ extern "C" int32_t pg_sparse_run(const pg_segment_plan_t* plan, const void* quer
   const dim3 grid(static_cast<unsigned>(plan->num_items) * plan->num_kv_heads);
   hipStream_t s = as_stream(stream);
   if (a.group > kNarrowRows)
-    hipLaunchKernelGGL((page_attention_kernel<true, true, true>), grid, dim3(kAttentionThreads), 0, s, a);
+    hipLaunchKernelGGL(selected_attention_kernel<true>, grid, dim3(kAttentionThreads), 0, s, a);
   else
-    hipLaunchKernelGGL((page_attention_kernel<true, true, false>), grid, dim3(kAttentionThreads), 0, s, a);
+    hipLaunchKernelGGL(selected_attention_kernel<false>, grid, dim3(kAttentionThreads), 0, s, a);
   if (int32_t rc = check_launch("selected_attention")) return rc;
   return launch_combine(*plan, a, workspace, s);
 }

@@ -16,7 +16,7 @@ from pagegauge_amd import _capi, pages, prefix, sparse
 
 ROOT = Path(__file__).resolve().parents[1]
 FIELDS = ("request", "row_first", "rows", "segment", "page_begin", "page_end", "last_page", "tail_begin",
-          "tail_end", "last_tail", "slot_at", "split", "table_begin", "table_pages", "reserved0", "reserved1")
+          "tail_end", "last_tail", "slot_at", "split", "table_begin", "table_pages", "block_rows", "reserved")
 
 
 def _check_plan(segments, own, tail, hq, hkv, cus, kind=torch.int8, selected=0):
@@ -33,7 +33,12 @@ def _check_plan(segments, own, tail, hq, hkv, cus, kind=torch.int8, selected=0):
     seen = {}                                    # (request, head, segment or None, "page" / "tail") -> ranges
     used, slots_of = set(), {}
     for it in items:
-        assert 0 < it["rows"] and it["page_end"] - it["page_begin"] <= 256 and it["tail_end"] - it["tail_begin"] <= 256
+        most = 256 if it["block_rows"] <= 16 else 512       # page ids of a wave's lanes, or in LDS
+        assert it["block_rows"] in (8, 16, 64, 128) and 0 < it["rows"] <= it["block_rows"]
+        assert it["page_end"] - it["page_begin"] <= most and it["tail_end"] - it["tail_begin"] <= 256
+        if it["block_rows"] > 16:
+            assert it["segment"] >= 0 and it["page_begin"] < it["page_end"] and it["slot_at"] >= 0
+        parts = 2 if it["block_rows"] == 64 else 1
         for row in range(it["row_first"], it["row_first"] + it["rows"]):
             request, head = it["request"] + row // group, row % group
             s = it["segment"]
@@ -50,13 +55,14 @@ def _check_plan(segments, own, tail, hq, hkv, cus, kind=torch.int8, selected=0):
             seen.setdefault((request, head, s, "page"), []).append((it["page_begin"], it["page_end"]))
             if it["slot_at"] < 0:
                 assert slot_ptr[request] == slot_ptr[request + 1]
-                slot = None
+                slots = [None]
             else:
                 slot = slot_base[it["slot_at"] + row // group] + it["split"]
-                assert slot_ptr[request] <= slot < slot_ptr[request + 1]
-            assert (request, head, slot) not in used
-            used.add((request, head, slot))
-            slots_of.setdefault((request, head), []).append(slot)
+                slots = list(range(slot, slot + parts))
+                assert slot_ptr[request] <= slot and slots[-1] < slot_ptr[request + 1]
+            assert not used & {(request, head, slot) for slot in slots}
+            used |= {(request, head, slot) for slot in slots}
+            slots_of.setdefault((request, head), []).extend(slots)
     for r in range(len(own)):
         for h in range(group):
             parts = [(s, "page", shared[s], shared[s + 1]) for s, (a, b, _) in enumerate(segments) if a <= r < b]
