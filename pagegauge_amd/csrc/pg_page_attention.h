@@ -600,6 +600,60 @@ inline void place_work(const pg_segment_plan_t& plan, void* workspace, float sm_
   a.group = plan.num_qo_heads / plan.num_kv_heads;
 }
 
+// Joins few partial rows: a wave per (request, query head), two dims a lane, 4 rows
+// requested at once.
+constexpr int kFewRows = 4;
+constexpr int kFewSlots = 16;
+
+__global__ __launch_bounds__(kCombineThreads) void combine_few_kernel(CombineArgs a, int64_t pairs) {
+  const int64_t pair = static_cast<int64_t>(blockIdx.x) * (kCombineThreads / kWave) +
+                       __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  if (pair >= pairs) return;
+  const int lane = threadIdx.x % kWave;
+  const int64_t request = pair / a.num_qo_heads;
+  const int head = static_cast<int>(pair - request * a.num_qo_heads);
+  const int begin = a.item_ptr[request], end = a.item_ptr[request + 1];
+  if (begin == end) return;          // its only workgroup wrote the output
+  float m = kNoScore, l = 0.0f;
+  float2 o = make_float2(0.0f, 0.0f);
+  for (int first = begin; first < end; first += kFewRows) {
+    float mi[kFewRows], li[kFewRows];
+    float2 x[kFewRows];
+#pragma unroll
+    for (int k = 0; k < kFewRows; ++k) {
+      const int64_t at = static_cast<int64_t>(min(first + k, end - 1)) * a.num_qo_heads + head;
+      mi[k] = first + k < end ? a.partial_m[at] : kNoScore;
+      li[k] = a.partial_l[at];
+      x[k] = *reinterpret_cast<const float2*>(a.partial_o + at * kHeadDim + 2 * lane);
+    }
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < kFewRows; ++k) top = fmaxf(top, mi[k]);
+    const float base = top == kNoScore ? 0.0f : top;
+    const float f = __builtin_amdgcn_exp2f(m - base);
+    l *= f;
+    o = make_float2(o.x * f, o.y * f);
+#pragma unroll
+    for (int k = 0; k < kFewRows; ++k) {
+      if (first + k >= end) break;
+      const float g = __builtin_amdgcn_exp2f(mi[k] - base);
+      l = fmaf(g, li[k], l);
+      o.x = fmaf(g, x[k].x, o.x);
+      o.y = fmaf(g, x[k].y, o.y);
+    }
+    m = top;
+  }
+  float2 c = make_float2(0.0f, 0.0f);
+  if (a.value_center) {
+    const uint32_t bits = *reinterpret_cast<const uint32_t*>(
+        a.value_center + request * a.center_batch_stride + (head / a.group) * kHeadDim + 2 * lane);
+    c = make_float2(half_bits_to_float(static_cast<uint16_t>(bits)), half_bits_to_float(static_cast<uint16_t>(bits >> 16)));
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  *reinterpret_cast<__half2*>(a.out + pair * kHeadDim + 2 * lane) = __floats2half2_rn(o.x * inv + c.x, o.y * inv + c.y);
+  if (lane == 0 && a.lse) a.lse[pair] = l == 0.0f ? kNoScore : log2f(l) + m;
+}
+
 // Joins the requests that have partial rows; the others' workgroups wrote the output.
 inline int32_t launch_combine(const pg_segment_plan_t& plan, const PageAttentionArgs& a, const void* workspace,
                               hipStream_t stream) {
@@ -617,8 +671,17 @@ inline int32_t launch_combine(const pg_segment_plan_t& plan, const PageAttention
   c.group = a.group;
   c.single = plan.batch_size == 1 ? plan.max_slots : 0;
   c.written = 0;
-  hipLaunchKernelGGL(combine_kernel, dim3(plan.batch_size, plan.num_qo_heads, kHeadDim / 64),
-                     dim3(kCombineThreads), 0, stream, c);
+  const int64_t pairs = static_cast<int64_t>(plan.batch_size) * plan.num_qo_heads;
+  if (plan.max_slots <= kFewSlots) {
+    constexpr int kPairs = kCombineThreads / kWave;
+    if (pairs > static_cast<int64_t>(UINT32_MAX) / kWave - kPairs)
+      return fail(PG_ERROR_UNSUPPORTED, "too many requests for one launch");
+    hipLaunchKernelGGL(combine_few_kernel, dim3(static_cast<unsigned>((pairs + kPairs - 1) / kPairs)),
+                       dim3(kCombineThreads), 0, stream, c, pairs);
+  } else {
+    hipLaunchKernelGGL(combine_kernel, dim3(plan.batch_size, plan.num_qo_heads, kHeadDim / 64),
+                       dim3(kCombineThreads), 0, stream, c);
+  }
   return check_launch("combine");
 }
 

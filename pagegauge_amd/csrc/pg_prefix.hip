@@ -26,6 +26,7 @@ struct SharedTiles {
   float k_scale[kSharedMaxPages];
   float v_scale[kSharedMaxPages];
   float largest[kSegmentWaves];
+  int32_t plain[kSegmentWaves];                          // no K scale below 0
 };
 
 // A prefix's pages with 17 query rows and more: kRowWaves waves of 32 query rows share
@@ -58,7 +59,6 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
   const int hkv = a.num_kv_heads;
   const int part = wave / kRowWaves;
   const int row_wave = 32 * (wave % kRowWaves);
-  const bool active = row_wave < it.rows;
   const int count = it.page_end - it.page_begin;
   const int tiles = (count + kTilePages - 1) / kTilePages;
 
@@ -66,13 +66,16 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
   {
     const int32_t* table = a.prefix_indices + it.page_begin;
     float largest = 0.0f;
+    bool plain = true;
     for (int i = threadIdx.x; i < tiles * kTilePages; i += kAttentionThreads) {
       const int32_t id = table[min(i, count - 1)];
       lds.ids[i] = id;
       if (kCodes) {
         const int64_t at = static_cast<int64_t>(id) * hkv + kv;
         const float v = i < count ? half_bits_to_float(a.value_scale[at]) : 0.0f;
-        lds.k_scale[i] = half_bits_to_float(a.key_scale[at]) * a.sm_scale_log2;
+        const float k = half_bits_to_float(a.key_scale[at]) * a.sm_scale_log2;
+        plain &= k >= 0.0f;
+        lds.k_scale[i] = k;
         lds.v_scale[i] = v;
         if (fabsf(v) < -kNoScore) largest = fmaxf(largest, fabsf(v));
       }
@@ -80,6 +83,8 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
     if (kCodes) {
       largest = wave_max(largest);
       if (lane == 0) lds.largest[wave] = largest;
+      const bool all = !__builtin_amdgcn_ballot_w64(!plain);
+      if (lane == 0) lds.plain[wave] = all;
     }
   }
   const int row = it.row_first + min(row_wave + column, it.rows - 1);
@@ -95,7 +100,9 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
   const int visible = (count - 1) * kPageSize + last_len;
   __syncthreads();
   float v_unit = 1.0f, v_back = 1.0f;                    // 2^-e and 2^e of V's scales
+  bool plain = true;
   if (kCodes) {
+    plain = __builtin_amdgcn_readfirstlane(lds.plain[0] & lds.plain[1] & lds.plain[2] & lds.plain[3]);
     float largest = lds.largest[0];
 #pragma unroll
     for (int w = 1; w < kSegmentWaves; ++w) largest = fmaxf(largest, lds.largest[w]);
@@ -196,23 +203,8 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
       vf[p] = kCodes ? lds.v_scale[kTilePages * tile + 2 * part + p] * v_unit : 1.0f;
     }
   };
-  // scores times their factors in place, which are then 1
-  auto scale_scores = [&](v16f (&s)[kBlocks], float (&kf)[kSteps]) {
-#pragma unroll
-    for (int p = 0; p < kSteps; ++p) {
-#pragma unroll
-      for (int r = 0; r < 8; ++r) s[p / 2][8 * (p % 2) + r] *= kf[p];
-      kf[p] = 1.0f;
-    }
-  };
-  auto softmax = [&](v16f (&s)[kBlocks], float (&kf)[kSteps], const float (&vf)[kSteps], v8h (&pr)[kSteps]) {
-    if (kCodes) {
-      // the largest score is that of the largest product, unless a scale is negative
-      bool negative = false;
-#pragma unroll
-      for (int p = 0; p < kSteps; ++p) negative |= !(kf[p] >= 0.0f);
-      if (__builtin_amdgcn_ballot_w64(negative)) scale_scores(s, kf);
-    }
+  // the largest of the scores, once per row
+  auto maximum = [&](const v16f (&s)[kBlocks], const float (&kf)[kSteps]) {
     float mx = kNoScore;
 #pragma unroll
     for (int p = 0; p < kSteps; ++p) {
@@ -221,10 +213,10 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
       for (int r = 1; r < 8; ++r) top = fmaxf(top, s[p / 2][8 * (p % 2) + r]);
       mx = fmaxf(mx, top * kf[p]);
     }
-    {
-      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-      mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-    }
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+    return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  };
+  auto raise = [&](float mx) {
     if (__builtin_amdgcn_ballot_w64(mx > m + kRescaleLimit)) {
       const float m_new = fmaxf(m, mx);
       const float alpha = __builtin_amdgcn_exp2f(m - m_new);
@@ -236,61 +228,75 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
     }
+  };
+  // probabilities page by page, each followed by its product
+  auto attend = [&](int buffer, const v16f (&s)[kBlocks], const float (&kf)[kSteps], const float (&vf)[kSteps]) {
 #pragma unroll
-    for (int p = 0; p < kSteps; ++p)
+    for (int p = 0; p < kSteps; ++p) {
+      v8h pr;
 #pragma unroll
       for (int r = 0; r < 8; r += 2) {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[p / 2][8 * (p % 2) + r], kf[p], -m));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(s[p / 2][8 * (p % 2) + r + 1], kf[p], -m));
         l0 += p0;
         l1 += p1;
-        pr[p][r] = static_cast<_Float16>(kCodes ? p0 * vf[p] : p0);
-        pr[p][r + 1] = static_cast<_Float16>(kCodes ? p1 * vf[p] : p1);
+        pr[r] = static_cast<_Float16>(kCodes ? p0 * vf[p] : p0);
+        pr[r + 1] = static_cast<_Float16>(kCodes ? p1 * vf[p] : p1);
       }
-  };
-  auto pv = [&](int buffer, const v8h (&pr)[kSteps]) {
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k)
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        const uint8_t* at = lds.tiles + v_at[d] + buffer * kTileBytes + k * 4096;
+        const uint8_t* at = lds.tiles + v_at[d] + buffer * kTileBytes + p * 4096;
         const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((PG_LDS v4s*)at);
         const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((PG_LDS v4s*)(at + 2048));
-        const v8h vf = __builtin_shufflevector(__builtin_bit_cast(v4h, lo), __builtin_bit_cast(v4h, hi),
-                                               0, 1, 2, 3, 4, 5, 6, 7);
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pr[k], o[d], 0, 0, 0);
+        const v8h columns = __builtin_shufflevector(__builtin_bit_cast(v4h, lo), __builtin_bit_cast(v4h, hi),
+                                                    0, 1, 2, 3, 4, 5, 6, 7);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(columns, pr, o[d], 0, 0, 0);
       }
+    }
   };
   // iteration j: tile j is in LDS, tile j + 1 on its way to registers
   v16f s[kBlocks];
-  auto body = [&](int j, int buffer, bool last) {
+  auto stage_next = [&](int j, int buffer) {
+    store_k(buffer ^ 1);
+    store_v(j + 1, buffer ^ 1);
+    // past the end the last tile comes again, and is not used
+    const int next = min(j + 2, tiles - 1);
+    load_k(next);
+    load_v(next);
+  };
+  // tiles without a masked token
+  auto body = [&](int j, int buffer) {
     __syncthreads();
-    if (!last) {
-      store_k(buffer ^ 1);
-      store_v(j + 1, buffer ^ 1);
-      if (j + 2 < tiles) {
-        load_k(j + 2);
-        load_v(j + 2);
-      }
-    }
-    if (active) {
-      float kf[kSteps], vf[kSteps];
-      v8h pr[kSteps];
-      factors(j, kf, vf);
-      qk(buffer, s);
-      if (last) {
-        scale_scores(s, kf);
+    float kf[kSteps], vf[kSteps];
+    factors(j, kf, vf);
+    __builtin_amdgcn_s_setprio(1);
+    qk(buffer, s);
+    __builtin_amdgcn_s_setprio(0);
+    stage_next(j, buffer);
+    const float mx = maximum(s, kf);
+    raise(mx);
+    __builtin_amdgcn_s_setprio(1);
+    attend(buffer, s, kf, vf);
+    __builtin_amdgcn_s_setprio(0);
+  };
+  auto masked_body = [&](int j, int buffer) {
+    __syncthreads();
+    if (j + 1 < tiles) stage_next(j, buffer);
+    float kf[kSteps], vf[kSteps];
+    factors(j, kf, vf);
+    qk(buffer, s);
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b)
+    for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int token = kTileTokens * j + 32 * (part + b) + 8 * (r / 4) + 4 * half + r % 4;
-            s[b][r] = token < visible ? s[b][r] : kNoScore;
-          }
+      for (int r = 0; r < 16; ++r) {
+        const int token = kTileTokens * j + 32 * (part + b) + 8 * (r / 4) + 4 * half + r % 4;
+        s[b][r] = token < visible ? s[b][r] * kf[2 * b + r / 8] : kNoScore;
       }
-      softmax(s, kf, vf, pr);
-      pv(buffer, pr);
-    }
+#pragma unroll
+    for (int p = 0; p < kSteps; ++p) kf[p] = 1.0f;
+    const float mx = maximum(s, kf);
+    raise(mx);
+    attend(buffer, s, kf, vf);
   };
 
   load_k(0);
@@ -301,8 +307,11 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
     load_k(1);
     load_v(1);
   }
-  for (int j = 0; j + 1 < tiles; ++j) body(j, j & 1, false);
-  body(tiles - 1, (tiles - 1) & 1, true);
+  // the largest score of a page is that of its largest product, unless a scale is negative
+  int j = 0;
+  if (plain)
+    for (; j + 1 < tiles; ++j) body(j, j & 1);
+  for (; j < tiles; ++j) masked_body(j, j & 1);
 
   if (row_wave + column >= it.rows) return;
   float l = l0 + l1;

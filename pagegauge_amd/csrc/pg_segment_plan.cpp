@@ -11,6 +11,9 @@ namespace {
 int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Pages that a workgroup is worth, where there are more workgroups than fit at once.
+constexpr int64_t kSmallestShare = 64;
+
 // Pages that are read together, by ``blocks`` workgroups of query rows.
 struct Unit {
   int32_t segment, request;               // segment -1: the request's own pages
@@ -28,9 +31,7 @@ struct Unit {
     return !shared() ? block_rows() : ceil_div(ceil_div(rows, blocks()), kSharedRows) * kSharedRows;
   }
   int64_t weight() const { return pages + tail_weight * tail; }
-  int64_t cuts(int64_t cap) const {
-    return std::max<int64_t>(1, ceil_div(weight(), shared() ? cap : std::min<int64_t>(cap, kSegmentMaxPages)));
-  }
+  int64_t cuts(int64_t cap) const { return std::max<int64_t>(1, ceil_div(weight(), cap)); }
 };
 
 int32_t check_indptr(const int32_t* indptr, int32_t count) {
@@ -85,24 +86,40 @@ int32_t build_segment_plan(const SegmentBatch& b, SegmentWork& work, pg_segment_
     if (pages || tail || !covered[r]) units.push_back({-1, r, group, pages, tail, tail_weight});
   }
 
-  // ---- the smallest largest share with which the batch takes no more than two
-  // workgroups per CU, from one group of pages per wave to what a wave's lanes can hold
+  // ---- the largest shares, of shared tiles and of the others apart: the smallest with which
+  // they take their part of two workgroups per CU; where they are more requests or
+  // prefixes than that, half of an even share, since the longest go first and the short
+  // ones fill in behind them.  Shared tiles keep the matrix cores busy with one
+  // workgroup per CU, and the other then reads requests' own pages beside it; they take
+  // both where there is little to read.
   const int64_t cus = b.num_cus > 0 ? b.num_cus : 256;
-  const int64_t target = std::max<int64_t>(1, 2 * cus / b.num_kv_heads);
-  auto items_of = [&](int64_t cap) {
+  const int64_t slots_at_once = std::max<int64_t>(2, 2 * cus / b.num_kv_heads);
+  auto items_of = [&](bool shared, int64_t cap) {
     int64_t n = 0;
-    for (const Unit& u : units) n += u.cuts(cap) * u.blocks();
+    for (const Unit& u : units) n += u.shared() == shared ? u.cuts(cap) * u.blocks() : 0;
     return n;
   };
-  int64_t low = kSegmentWaves * kSegmentGroupPages, high = kSharedMaxPages;
-  while (low < high) {
-    const int64_t cap = low + (high - low) / 2;
-    if (items_of(cap) <= target) high = cap; else low = cap + 1;
-  }
-  const int64_t cap = high;
-  const int64_t count = items_of(cap);
+  int64_t weights[2] = {0, 0};
+  for (const Unit& u : units) weights[u.shared()] += u.weight() * u.blocks();
+  auto largest_share = [&](bool shared, int64_t target) {
+    int64_t cap = shared ? kSharedMaxPages : kSegmentMaxPages;
+    if (items_of(shared, cap) > target)
+      return std::min(cap, std::max(weights[shared] / (2 * target), kSmallestShare));
+    int64_t low = kSegmentWaves * kSegmentGroupPages;
+    while (low < cap) {
+      const int64_t middle = low + (cap - low) / 2;
+      if (items_of(shared, middle) <= target) cap = middle; else low = middle + 1;
+    }
+    return cap;
+  };
+  const int64_t shared_target = weights[0] > weights[1] / 2 ? slots_at_once / 2 : slots_at_once;
+  const int64_t shared_cap = largest_share(true, shared_target);
+  const int64_t shared_items = items_of(true, shared_cap);
+  const int64_t own_cap = largest_share(false, std::max(slots_at_once - shared_items, slots_at_once / 2));
+  auto cuts_of = [&](const Unit& u) { return u.cuts(u.shared() ? shared_cap : own_cap); };
+  const int64_t count = shared_items + items_of(false, own_cap);
   for (const Unit& u : units)
-    if (u.cuts(cap) * u.parts() > kSegmentMaxSlots) return fail(PG_ERROR_UNSUPPORTED, "too many pages in one request");
+    if (cuts_of(u) * u.parts() > kSegmentMaxSlots) return fail(PG_ERROR_UNSUPPORTED, "too many pages in one request");
   if (count > static_cast<int64_t>(UINT32_MAX) / (kSegmentWaves * 64) / b.num_kv_heads)
     return fail(PG_ERROR_UNSUPPORTED, "too many work items");
 
@@ -111,7 +128,7 @@ int32_t build_segment_plan(const SegmentBatch& b, SegmentWork& work, pg_segment_
   work = SegmentWork{};
   work.items.reserve(count);
   for (const Unit& u : units) {
-    const int64_t cuts = u.cuts(cap);
+    const int64_t cuts = cuts_of(u);
     const bool direct = u.segment < 0 && cuts == 1 && !covered[u.request];
     const int32_t slot_at = direct ? -1 : static_cast<int32_t>(work.slot_base.size());
     const int32_t requests = static_cast<int32_t>(u.rows / group);
@@ -176,7 +193,7 @@ int32_t build_segment_plan(const SegmentBatch& b, SegmentWork& work, pg_segment_
   // slots of an item's requests count from the batch's first one
   size_t at = 0;
   for (const Unit& u : units) {
-    if (u.segment < 0 && !covered[u.request] && u.cuts(cap) == 1) continue;
+    if (u.segment < 0 && !covered[u.request] && cuts_of(u) == 1) continue;
     for (int32_t r = u.request; r < u.request + u.rows / group; ++r) work.slot_base[at++] += work.slot_ptr[r];
   }
 
