@@ -814,8 +814,8 @@ int32_t pg_pool_take(int32_t* refs, int64_t pages, int32_t* out, int64_t count, 
 
 /* The fewest moves that bring the pages in use, live[0] of them, to the front: the
  * i-th lowest one at or past live[0] (source[i]) to the i-th lowest free one below it
- * (target[i]); -1 in the rest of the pages / 2 entries.  remap[p] is where page p is
- * afterwards, -1 for a free one.  refs is only read. */
+ * (target[i]); -1 in the rest of the pages / 2 entries.  remap[p] (16-byte aligned) is
+ * where page p is afterwards, -1 for a free one.  refs is only read. */
 int32_t pg_pool_stage_compaction(const int32_t* refs, int64_t pages, int32_t* source, int32_t* target,
                                  int32_t* remap, int32_t* live, void* stream);
 
@@ -921,8 +921,9 @@ int32_t pg_sparse_plan(const int32_t* host_indptr, const int32_t* host_tail_indp
  * a page scores
  *   max over the KV head's query heads of
  *     f32(sum_d max(q'_d lo_d, q'_d hi_d) * key_scale) * 2^(x - 7),
- * -inf for a row with an infinity or NaN and where the score is NaN.  The highest
- * scores are taken, among equal ones the lowest positions. */
+ * -inf for a row with an infinity or NaN and where the score is NaN.  Taken are the
+ * first and last pages, and of the others those with the highest scores, among
+ * equal ones the lowest positions. */
 int32_t pg_sparse_select(const pg_segment_plan_t* plan, const void* query, int64_t query_batch_stride,
                          const void* bounds, const void* key_scale, const int32_t* indices,
                          int32_t* selected, void* workspace, void* stream);

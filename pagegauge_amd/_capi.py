@@ -195,7 +195,7 @@ PROTOTYPES = {
                                  _p]),
     "pg_int4_decode_run": (_i32, [ctypes.POINTER(Int4Plan), _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p,
                                   _p, _i64, _p, _p, _f32, _p, _p]),
-    "pg_copy_pages": (_i32, [ctypes.POINTER(PagePlane), _i32, _i64, _p, _p, _i64, _p]),
+    "pg_copy_pages": (_i32, [_p, _i32, _i64, _p, _p, _i64, _p]),
     "pg_pool_adjust": (_i32, [_p, _i64, _p, _i64, _i32, _p]),
     "pg_pool_take": (_i32, [_p, _i64, _p, _i64, _p]),
     "pg_pool_stage_compaction": (_i32, [_p, _i64, _p, _p, _p, _p, _p]),

@@ -188,25 +188,37 @@ __global__ __launch_bounds__(kScanThreads) void stage_kernel(const int32_t* refs
                                                              int32_t* target, int32_t* remap, int32_t* live_out) {
   __shared__ int wave_sums[kScanThreads / kWave];
   int live = 0, before;
-  for (int64_t stretch = 0; stretch < pages; stretch += kStretch)
-    live += block_scan(__popc(live_bits(refs, stretch + threadIdx.x * kScanPages, pages)), before, wave_sums);
+  uint32_t used = 0;
+  for (int64_t stretch = 0; stretch < pages; stretch += kStretch) {
+    used = live_bits(refs, stretch + threadIdx.x * kScanPages, pages);
+    live += block_scan(__popc(used), before, wave_sums);
+  }
   if (threadIdx.x == 0) *live_out = live;
   int holes = 0, movers = 0;
   for (int64_t stretch = 0; stretch < pages; stretch += kStretch) {
     const int64_t first = stretch + threadIdx.x * kScanPages;
-    const int held = static_cast<int>(max(min(pages - first, static_cast<int64_t>(kScanPages)), int64_t{0}));
-    const int below = static_cast<int>(max(min(live - first, static_cast<int64_t>(held)), int64_t{0}));
-    const uint32_t used = live_bits(refs, first, pages);
+    const int below = static_cast<int>(max(min(live - first, static_cast<int64_t>(kScanPages)), int64_t{0}));
+    if (pages > kStretch) used = live_bits(refs, first, pages);       // of one stretch they are in hand
     uint32_t hole = ~used & ((1u << below) - 1);
     uint32_t mover = used & ~((1u << below) - 1);
-    const int all_holes = block_scan(__popc(hole), before, wave_sums);
-    for (int at = holes + before; hole; ++at, hole &= hole - 1) target[at] = static_cast<int32_t>(first + __ffs(hole) - 1);
-    const int all_movers = block_scan(__popc(mover), before, wave_sums);
-    for (int at = movers + before; mover; ++at, mover &= mover - 1) source[at] = static_cast<int32_t>(first + __ffs(mover) - 1);
-    for (int i = 0; i < held; ++i)       // movers' entries follow below
-      if (i < below || !(used >> i & 1)) remap[first + i] = used >> i & 1 ? static_cast<int32_t>(first + i) : -1;
-    holes += all_holes;
-    movers += all_movers;
+    // both counts of a stretch fit 16 bits; pages below ``live`` are pages of the pool
+    const int all = block_scan(__popc(hole) << 16 | __popc(mover), before, wave_sums);
+    for (int at = holes + (before >> 16); hole; ++at, hole &= hole - 1)
+      target[at] = static_cast<int32_t>(first + __ffs(hole) - 1);
+    for (int at = movers + (before & 0xffff), left = mover; left; ++at, left &= left - 1)
+      source[at] = static_cast<int32_t>(first + __ffs(left) - 1);
+    // movers' entries follow below
+    const uint32_t stays = used & ~mover;
+    auto entry = [&](int i) { return stays >> i & 1 ? static_cast<int32_t>(first + i) : -1; };
+    if (first + kScanPages <= pages) {
+#pragma unroll
+      for (int i = 0; i < kScanPages; i += 4)
+        *reinterpret_cast<int4*>(remap + first + i) = make_int4(entry(i), entry(i + 1), entry(i + 2), entry(i + 3));
+    } else {
+      for (int i = 0; first + i < pages; ++i) remap[first + i] = entry(i);
+    }
+    holes += all >> 16;
+    movers += all & 0xffff;
   }
   __syncthreads();
   const int half = pages / 2;
@@ -334,6 +346,7 @@ extern "C" int32_t pg_pool_stage_compaction(const int32_t* refs, int64_t pages, 
                                             int32_t* remap, int32_t* live, void* stream) {
   clear_error();
   if (int32_t rc = check_pool(refs, pages)) return rc;
+  if (reinterpret_cast<uintptr_t>(remap) % 16) return fail(PG_ERROR_INVALID_ARGUMENT, "remap must be 16-byte aligned");
   if (!live || (pages && !remap) || (pages > 1 && (!source || !target)))
     return fail(PG_ERROR_INVALID_ARGUMENT, "null output of a compaction");
   hipLaunchKernelGGL(stage_kernel, dim3(1), dim3(kScanThreads), 0, as_stream(stream), refs,

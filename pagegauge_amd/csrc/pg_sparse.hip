@@ -101,6 +101,7 @@ struct SelectArgs {
 
 constexpr int kScoreThreads = 256;
 constexpr int kScorePages = 16;      // rows of an MFMA
+constexpr int kMostGroups = 8;       // of so many pages, per wave: two page ids a lane
 
 // Sixteen pages at a time are the rows of v_mfma_i32_16x16x64_i8 and the KV head's query
 // heads its columns; 4 products take the 128 lower bounds and the 128 upper ones.
@@ -160,16 +161,21 @@ __global__ __launch_bounds__(kScoreThreads) void page_scores_kernel(SelectArgs a
       }
   }
 
-  float* scores = a.scores + (static_cast<int64_t>(request) * hkv + kv) * a.max_pages;
-  for (int g = 0; g < a.wave_groups; ++g) {
-    const int at = first + g * kScorePages;
-    if (at >= pages) break;
-    const int page = a.indices[begin + min(at + n, pages - 1)];
-    const uint8_t* from = a.bounds + (static_cast<int64_t>(page) * hkv + kv) * 2 * kHeadDim + 16 * kg;
-    v4i x[4];
+  // lane l has the page ids and scales of the wave's pages l and 64 + l
+  const int last = min(first + a.wave_groups * kScorePages, pages) - 1;
+  int ids[2];
+  float scales[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) ids[i] = a.indices[begin + min(first + 64 * i + lane, last)];
+  const uint8_t* bounds = a.bounds + kv * 2 * kHeadDim + 16 * kg;
+  auto load = [&](int g, v4i (&x)[4]) {
+    const int64_t page = __shfl(g < 4 ? ids[0] : ids[1], kScorePages * (g & 3) + n, kWave);
+    const uint8_t* from = bounds + page * hkv * 2 * kHeadDim;
 #pragma unroll
     for (int w = 0; w < 4; ++w) x[w] = *reinterpret_cast<const v4i*>(from + 64 * w);
-    const float my_scale = half_bits_to_float(a.key_scale[static_cast<int64_t>(page) * hkv + kv]);
+  };
+  float* scores = a.scores + (static_cast<int64_t>(request) * hkv + kv) * a.max_pages;
+  auto compute = [&](int g, const v4i (&x)[4]) {
     v4i sum = {0, 0, 0, 0};
     sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[0], below[0], sum, 0, 0, 0);
     sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[1], below[1], sum, 0, 0, 0);
@@ -179,15 +185,23 @@ __global__ __launch_bounds__(kScoreThreads) void page_scores_kernel(SelectArgs a
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       // |sum| < 2^21: one rounding, of its product with the FP16 scale
-      const float scaled = static_cast<float>(sum[r]) * __shfl(my_scale, 4 * kg + r, kWave);
-      best[r] = row16_max(fmaxf(scaled * unit, kNoScore));
+      const float scale = __shfl(g < 4 ? scales[0] : scales[1], kScorePages * (g & 3) + 4 * kg + r, kWave);
+      best[r] = row16_max(fmaxf(static_cast<float>(sum[r]) * scale * unit, kNoScore));
     }
-    if (n < 4) {
-      const int position = at + 4 * kg + n;
-      float score = n == 0 ? best[0] : n == 1 ? best[1] : n == 2 ? best[2] : best[3];
-      if (position < a.first || position >= pages - a.last) score = -kNoScore;
-      if (position < pages) scores[position] = score;
-    }
+    const int position = first + g * kScorePages + 4 * kg + n;
+    if (n < 4 && position <= last) scores[position] = n == 0 ? best[0] : n == 1 ? best[1] : n == 2 ? best[2] : best[3];
+  };
+  const int groups = (last - first) / kScorePages + 1;
+  v4i x[2][4];
+  load(0, x[0]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) scales[i] = half_bits_to_float(a.key_scale[static_cast<int64_t>(ids[i]) * hkv + kv]);
+  for (int g = 0; g < groups; g += 2) {
+    if (g + 1 < groups) load(g + 1, x[1]);
+    compute(g, x[0]);
+    if (g + 1 >= groups) break;
+    if (g + 2 < groups) load(g + 2, x[0]);
+    compute(g + 1, x[1]);
   }
 }
 
@@ -195,20 +209,32 @@ __global__ __launch_bounds__(kScoreThreads) void page_scores_kernel(SelectArgs a
 
 constexpr int kPickThreads = 1024;
 constexpr int kPickWaves = kPickThreads / kWave;
-constexpr int kBins = 2048;          // 11 bits of a key, then 11, then 10
+constexpr int kBins = 2 * kPickThreads;
+constexpr int kListed = 1024;        // scores near the last one taken that are compared one by one
 
-// Whole numbers in the order of the scores: -0 as 0, NaN never gets here.
+// Whole numbers in the order of the scores, -0 as 0 (NaN never gets here); none is 0.
 __device__ __forceinline__ uint32_t order_key(float score) {
   const uint32_t bits = __float_as_uint(score == 0.0f ? 0.0f : score);
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-// One workgroup per (KV head, request): the key of the take-th largest score bit group by
-// bit group from histograms, then everything above it and the lowest positions at it.
+__device__ __forceinline__ float score_of(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+// One workgroup per (KV head, request): the key of the last score that is taken, then
+// everything above it and the lowest positions at it, in order.  A histogram over 2048
+// equal parts of the scores' range leaves a few to be ranked one by one, or where very many
+// are alike, to further histograms over the bits of their keys.  Up to kHeld keys stay in a
+// thread's registers; with kHeld = 0 the scores are read again each time.
+template <int kHeld>
 __global__ __launch_bounds__(kPickThreads) void pick_pages_kernel(SelectArgs a) {
   __shared__ uint32_t bins[kBins];
+  __shared__ uint32_t list[kListed];
+  __shared__ uint32_t counts[kHeld > 0 ? kHeld * kPickWaves : kPickWaves];
   __shared__ uint32_t wave_sums[kPickWaves];
-  __shared__ uint32_t found[2];
+  __shared__ float wave_low[kPickWaves], wave_high[kPickWaves];
+  __shared__ uint32_t found[3], listed;
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
   const int kv = blockIdx.x, request = blockIdx.y;
   const int pages = a.indptr[request + 1] - a.indptr[request];
@@ -218,23 +244,28 @@ __global__ __launch_bounds__(kPickThreads) void pick_pages_kernel(SelectArgs a) 
     return;
   }
   const float* scores = a.scores + (static_cast<int64_t>(request) * a.num_kv_heads + kv) * a.max_pages;
-
-  uint32_t prefix = 0;               // bits of the wanted key found so far
-  uint32_t wanted = a.take;          // its rank among the keys with these bits, from the top, 1-based
-  int shift = 32;
-#pragma unroll 1
-  for (int step = 0; step < 3; ++step) {
-    const int width = step < 2 ? 11 : 10;
-    const int before = shift;
-    shift -= width;
-    for (int i = tid; i < kBins; i += kPickThreads) bins[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < pages; i += kPickThreads) {
-      const uint32_t key = order_key(scores[i]);
-      if (before == 32 || key >> before == prefix >> before) atomicAdd(&bins[key >> shift & ((1u << width) - 1)], 1u);
+  // 0 for the pages that are taken anyway
+  auto key_at = [&](int i) { return i < a.first || i >= pages - a.last ? 0u : order_key(scores[i]); };
+  uint32_t held[kHeld > 0 ? kHeld : 1];
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) {
+    const int i = tid + j * kPickThreads;
+    held[j] = i < pages ? key_at(i) : 0;
+  }
+  auto each_key = [&](auto&& body) {
+    if constexpr (kHeld > 0) {
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j)
+        if (held[j]) body(held[j]);
+    } else {
+      for (int i = tid; i < pages; i += kPickThreads)
+        if (const uint32_t key = key_at(i)) body(key);
     }
-    __syncthreads();
-    // keys in higher bins than this thread's pair, from the top
+  };
+
+  // the bin of ``bins`` in which the wanted-th largest key falls, its rank there, and how
+  // many keys the bin has
+  auto find_bin = [&](uint32_t wanted) {
     const int top = kBins - 2 - 2 * tid;
     const uint32_t upper = bins[top + 1], lower = bins[top];
     uint32_t x = upper + lower;
@@ -251,34 +282,163 @@ __global__ __launch_bounds__(kPickThreads) void pick_pages_kernel(SelectArgs a) 
       const bool in_upper = wanted <= above + upper;
       found[0] = in_upper ? top + 1 : top;
       found[1] = wanted - (in_upper ? above : above + upper);
+      found[2] = in_upper ? upper : lower;
     }
     __syncthreads();
-    prefix |= found[0] << shift;
+  };
+  auto clear_bins = [&]() {
+    bins[tid] = 0;
+    bins[tid + kPickThreads] = 0;
+  };
+
+  uint32_t wanted = a.take - a.first - a.last;       // rank of the last key taken, from the top
+  uint32_t last_key = ~0u;                           // none
+  if (wanted > 0) {
+    float low = -kNoScore, high = kNoScore;
+    each_key([&](uint32_t key) {
+      const float s = score_of(key);
+      if (fabsf(s) < -kNoScore) {
+        low = fminf(low, s);
+        high = fmaxf(high, s);
+      }
+    });
+    low = -wave_max(-low);
+    high = wave_max(high);
+    if (lane == 0) {
+      wave_low[wave] = low;
+      wave_high[wave] = high;
+    }
+    clear_bins();
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    low = -row16_max(-wave_low[lane % kPickWaves]);
+    high = row16_max(wave_high[lane % kPickWaves]);
+    // rounded alike for all, and never falling as the score rises
+    const float per_bin = (kBins - 1) / fmaxf(high - low, 0x1p-100f);
+    auto bin_of = [&](uint32_t key) {
+      return static_cast<uint32_t>(fminf(fmaxf((score_of(key) - low) * per_bin, 0.0f), static_cast<float>(kBins - 1)));
+    };
+    each_key([&](uint32_t key) { atomicAdd(&bins[bin_of(key)], 1u); });
+    __syncthreads();
+    find_bin(wanted);
+    const uint32_t bin = found[0];
     wanted = found[1];
+    if (found[2] <= kListed) {
+      each_key([&](uint32_t key) {
+        if (bin_of(key) == bin) list[atomicAdd(&listed, 1u)] = key;
+      });
+      __syncthreads();
+      const uint32_t count = listed;
+      if (static_cast<uint32_t>(tid) < count) {
+        const uint32_t mine = list[tid];
+        uint32_t larger = 0, equal = 0;
+        for (uint32_t i = 0; i < count; ++i) {
+          larger += list[i] > mine;
+          equal += list[i] == mine;
+        }
+        if (larger < wanted && wanted <= larger + equal) {
+          found[0] = mine;
+          found[1] = wanted - larger;
+        }
+      }
+      __syncthreads();
+      last_key = found[0];
+      wanted = found[1];
+    } else {
+      last_key = 0;
+      int shift = 32;
+#pragma unroll 1
+      for (int step = 0; step < 3; ++step) {         // 11 bits, then 11, then 10
+        const int width = step < 2 ? 11 : 10, before = shift;
+        shift -= width;
+        __syncthreads();
+        clear_bins();
+        __syncthreads();
+        each_key([&](uint32_t key) {
+          if (bin_of(key) == bin && (before == 32 || key >> before == last_key >> before))
+            atomicAdd(&bins[key >> shift & ((1u << width) - 1)], 1u);
+        });
+        __syncthreads();
+        find_bin(wanted);
+        last_key |= found[0] << shift;
+        wanted = found[1];
+      }
+    }
   }
 
-  // ``prefix`` is the take-th largest key; of those equal to it the first ``wanted``
-  uint32_t larger = 0, equal = 0;    // taken and seen in the stretches so far
-  for (int first = 0; first < pages; first += kPickThreads) {
-    const int i = first + tid;
-    const uint32_t key = i < pages ? order_key(scores[i]) : 0;
-    const bool is_larger = i < pages && key > prefix, is_equal = i < pages && key == prefix;
-    const uint64_t larger_mask = __builtin_amdgcn_ballot_w64(is_larger), equal_mask = __builtin_amdgcn_ballot_w64(is_equal);
-    if (lane == 0)
-      wave_sums[wave] = static_cast<uint32_t>(__popcll(larger_mask)) | static_cast<uint32_t>(__popcll(equal_mask)) << 16;
-    __syncthreads();
-    uint32_t front = 0, all = 0;
-    for (int w = 0; w < kPickWaves; ++w) {
-      if (w < wave) front += wave_sums[w];
-      all += wave_sums[w];
+  // larger keys and the pages taken anyway, and of the equal keys the first ``wanted``
+  auto classes = [&](int i, uint32_t key, uint64_t& larger, uint64_t& equal) {
+    larger = __builtin_amdgcn_ballot_w64(i < pages && (key == 0 || key > last_key));
+    equal = __builtin_amdgcn_ballot_w64(i < pages && key == last_key);
+  };
+  const uint64_t lanes_below = (1ull << lane) - 1;
+  auto write = [&](int i, uint64_t larger, uint64_t equal, uint32_t larger_before, uint32_t equal_before) {
+    larger_before += __popcll(larger & lanes_below);
+    equal_before += __popcll(equal & lanes_below);
+    if ((larger >> lane & 1) || ((equal >> lane & 1) && equal_before < wanted))
+      out[larger_before + min(equal_before, wanted)] = i;
+  };
+  if constexpr (kHeld > 0) {
+    // counts of (stretch, wave) in the order of positions, 16 bits each
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      uint64_t larger, equal;
+      classes(tid + j * kPickThreads, held[j], larger, equal);
+      if (lane == 0)
+        counts[j * kPickWaves + wave] = static_cast<uint32_t>(__popcll(larger)) | static_cast<uint32_t>(__popcll(equal)) << 16;
     }
-    const uint64_t lanes_below = (1ull << lane) - 1;
-    const uint32_t larger_before = larger + (front & 0xffff) + __popcll(larger_mask & lanes_below);
-    const uint32_t equal_before = equal + (front >> 16) + __popcll(equal_mask & lanes_below);
-    if (is_larger || (is_equal && equal_before < wanted)) out[larger_before + min(equal_before, wanted)] = i;
-    larger += all & 0xffff;
-    equal += all >> 16;
     __syncthreads();
+    constexpr int kCounts = kHeld * kPickWaves;
+    constexpr int kEach = (kCounts + kWave - 1) / kWave;
+    if (wave == 0) {
+      uint32_t mine[kEach], sum = 0;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int at = lane * kEach + e;
+        mine[e] = at < kCounts ? counts[at] : 0;
+        sum += mine[e];
+      }
+      uint32_t x = sum;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) {
+        const uint32_t y = __shfl_up(x, d, kWave);
+        if (lane >= d) x += y;
+      }
+      x -= sum;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int at = lane * kEach + e;
+        if (at < kCounts) counts[at] = x;
+        x += mine[e];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      uint64_t larger, equal;
+      classes(tid + j * kPickThreads, held[j], larger, equal);
+      const uint32_t front = counts[j * kPickWaves + wave];
+      write(tid + j * kPickThreads, larger, equal, front & 0xffff, front >> 16);
+    }
+  } else {
+    uint32_t larger_so_far = 0, equal_so_far = 0;
+    for (int first = 0; first < pages; first += kPickThreads) {
+      const int i = first + tid;
+      uint64_t larger, equal;
+      classes(i, i < pages ? key_at(i) : 0, larger, equal);
+      if (lane == 0)
+        wave_sums[wave] = static_cast<uint32_t>(__popcll(larger)) | static_cast<uint32_t>(__popcll(equal)) << 16;
+      __syncthreads();
+      uint32_t front = 0, all = 0;
+      for (int w = 0; w < kPickWaves; ++w) {
+        if (w < wave) front += wave_sums[w];
+        all += wave_sums[w];
+      }
+      write(i, larger, equal, larger_so_far + (front & 0xffff), equal_so_far + (front >> 16));
+      larger_so_far += all & 0xffff;
+      equal_so_far += all >> 16;
+      __syncthreads();
+    }
   }
 }
 
@@ -372,7 +532,7 @@ extern "C" int32_t pg_sparse_select(const pg_segment_plan_t* plan, const void* q
   if (plan->max_pages > plan->selected_pages) {
     const int64_t groups = (plan->max_pages + kScorePages - 1) / kScorePages;
     const int64_t waves = groups * plan->num_kv_heads * plan->batch_size;
-    a.wave_groups = static_cast<int>(std::min<int64_t>(8, std::max<int64_t>(1, waves / 4096)));
+    a.wave_groups = static_cast<int>(std::min<int64_t>(kMostGroups, std::max<int64_t>(1, waves / 4096)));
     const int64_t block_groups = static_cast<int64_t>(a.wave_groups) * (kScoreThreads / kWave);
     hipLaunchKernelGGL(page_scores_kernel,
                        dim3(static_cast<unsigned>((groups + block_groups - 1) / block_groups), plan->num_kv_heads,
@@ -380,7 +540,15 @@ extern "C" int32_t pg_sparse_select(const pg_segment_plan_t* plan, const void* q
                        dim3(kScoreThreads), 0, s, a);
     if (int32_t rc = check_launch("page_scores")) return rc;
   }
-  hipLaunchKernelGGL(pick_pages_kernel, dim3(plan->num_kv_heads, plan->batch_size), dim3(kPickThreads), 0, s, a);
+  const dim3 grid(plan->num_kv_heads, plan->batch_size), threads(kPickThreads);
+  if (plan->max_pages <= 2 * kPickThreads)
+    hipLaunchKernelGGL(pick_pages_kernel<2>, grid, threads, 0, s, a);
+  else if (plan->max_pages <= 8 * kPickThreads)
+    hipLaunchKernelGGL(pick_pages_kernel<8>, grid, threads, 0, s, a);
+  else if (plan->max_pages <= 32 * kPickThreads)
+    hipLaunchKernelGGL(pick_pages_kernel<32>, grid, threads, 0, s, a);
+  else
+    hipLaunchKernelGGL(pick_pages_kernel<0>, grid, threads, 0, s, a);
   return check_launch("pick_pages");
 }
 

@@ -21,6 +21,8 @@ Calls that change a pool or its pages must follow each other on one stream.
 
 from __future__ import annotations
 
+import ctypes
+import functools
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -36,9 +38,9 @@ def _ids(ids: torch.Tensor, device: int, what: str) -> int:
     return _capi.pointer(ids, torch.int32, ids.shape, device, f"{what} must be contiguous int32 [n]")
 
 
-def _plane(plane: torch.Tensor, page_dim: int) -> tuple[int, int, int, int]:
-    """(page bytes, page stride, rows, row stride), in bytes, of a plane."""
-    shape, strides, size = plane.shape, plane.stride(), plane.element_size()
+@functools.lru_cache(maxsize=1024)
+def _plane(shape: tuple, strides: tuple, size: int, page_dim: int) -> tuple[int, tuple]:
+    """(pages, (page bytes, page stride, rows, row stride), in bytes) of a plane."""
     if len(shape) <= page_dim:
         raise ValueError(f"planes must have their pages in dimension {page_dim}")
     dense = 1
@@ -55,7 +57,7 @@ def _plane(plane: torch.Tensor, page_dim: int) -> tuple[int, int, int, int]:
     by_pages = row_stride >= page_bytes and page_stride >= (rows - 1) * row_stride + page_bytes
     if page_stride < page_bytes or (rows > 1 and not by_rows and not by_pages):
         raise ValueError("pages of a plane must not overlap")
-    return page_bytes, page_stride, rows, row_stride
+    return pages, (page_bytes, page_stride, rows, row_stride)
 
 
 def copy_pages(planes: Sequence[torch.Tensor], source: torch.Tensor, target: torch.Tensor, *,
@@ -74,22 +76,22 @@ def copy_pages(planes: Sequence[torch.Tensor], source: torch.Tensor, target: tor
     _capi.refuse_gradients(*planes)
     device, pages = source.get_device(), None
     source_at, target_at = _ids(source, device, "source"), _ids(target, device, "target")
-    entries = (_capi.PagePlane * len(planes))()
-    count = 0
+    entries = []                                    # pg_page_plane_t: five 64-bit fields
     for plane in planes:
         if plane.get_device() != device:
             raise ValueError(_capi.DEVICE_ERROR)
-        page_bytes, page_stride, rows, row_stride = _plane(plane, page_dim)
+        here, place = _plane(plane.shape, plane.stride(), plane.element_size(), page_dim)
         if pages is None:
-            pages = plane.shape[page_dim]
-        if plane.shape[page_dim] != pages:
+            pages = here
+        if here != pages:
             raise ValueError("planes must have the same number of pages")
-        if page_bytes and rows and pages:
-            entries[count] = _capi.PagePlane(plane.data_ptr(), page_bytes, page_stride, rows, row_stride)
-            count += 1
+        if place[0] and place[2] and pages:
+            entries += (plane.data_ptr(), *place)
     stream = _capi.launch_stream(device)
-    if count and source.numel():
-        _capi.call("pg_copy_pages", entries, count, pages, source_at, target_at, source.numel(), stream)
+    moves = source.shape[0]
+    if entries and moves:
+        _capi.call("pg_copy_pages", (ctypes.c_int64 * len(entries))(*entries), len(entries) // 5, pages, source_at,
+                   target_at, moves, stream)
 
 
 def rewrite_ids(ids: torch.Tensor, remap: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -175,13 +177,19 @@ class PagePool:
         for the counts, on the same stream, before anything else changes the pool.
         ``out`` may hold an earlier call's tensors."""
         pages, device = self.pages, self._device
-        shapes = ((pages // 2,), (pages // 2,), (pages,), (1,))
-        if out is None:
-            stream = _capi.launch_stream(device)
-            out = Moves(*(torch.empty(shape, dtype=torch.int32, device=self.refs.device) for shape in shapes))
-        at = [_capi.pointer(t, torch.int32, shape, device, "out must be the tensors of a compaction of this pool")
-              for t, shape in zip(out, shapes)]
+        half = pages // 2
+        what = "out must be the tensors of a compaction of this pool"
         stream = _capi.launch_stream(device)
+        if out is None:
+            # one allocation, remap (16-byte aligned) in front
+            whole = torch.empty(pages + 2 * half + 1, dtype=torch.int32, device=self.refs.device)
+            remap, source, target, live = whole.split_with_sizes((pages, half, half, 1))
+            out = Moves(source, target, remap, live)
+            remap_at = whole.data_ptr()
+            source_at = remap_at + 4 * pages
+            at = source_at, source_at + 4 * half, remap_at, source_at + 8 * half
+        else:
+            at = [_capi.pointer(t, torch.int32, (n,), device, what) for t, n in zip(out, (half, half, pages, 1))]
         _capi.call("pg_pool_stage_compaction", self.refs.data_ptr(), pages, *at, stream)
         return out
 

@@ -26,14 +26,20 @@ from typing import Optional
 import torch
 
 from . import _capi
-from .decode import (_check_cache, _check_index, _check_page_ids, _check_query, _check_scale, _host_i32,
-                     _host_tables, _num_cus, _page_id_range)
+from .decode import (_check_index, _check_page_ids, _check_query, _host_i32, _host_tables, _num_cus,
+                     _page_id_range)
 
 DIM = 128
 PAGE = 16
 
 _KINDS = {torch.int8: _capi.PG_KV_INT8, torch.float16: _capi.PG_KV_FP16}
+
+# what the checks below say
 _CENTERS = "centers must be contiguous float16 [B,Hkv,128]"
+_CACHE = {dtype: f"k_cache and v_cache must be contiguous {name} [pages,16,Hkv,128], as planned"
+          for dtype, name in ((torch.int8, "int8"), (torch.float16, "float16"))}
+_SCALES = "k_page_scale and v_page_scale must be contiguous float16 [pages,Hkv]"
+_EXACT = "exact_key and exact_value must be contiguous float16 [pages,16,Hkv,128]"
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -139,36 +145,39 @@ class _SegmentDecode:
         hkv, hq, batch = self._num_kv_heads, self._num_qo_heads, self._batch
         _check_query(q, batch, hq)
         k_cache, v_cache = kv_cache
+        device, dtype = q.get_device(), self._kv_dtype
         _capi.refuse_gradients(q, value_center, k_cache, v_cache, k_page_scale, v_page_scale)
-        device = q.get_device()
-        for name, cache in (("k_cache", k_cache), ("v_cache", v_cache)):
-            _check_cache(cache, name, self._kv_dtype, hkv)
-        pages = min(k_cache.shape[0], v_cache.shape[0])
-        if self._kv_dtype is torch.int8:
+        if k_cache.dim() != 4 or v_cache.dim() != 4:
+            raise ValueError(_CACHE[dtype])
+        k_pages, v_pages = k_cache.shape[0], v_cache.shape[0]
+        cache_at = [_capi.pointer(k_cache, dtype, (k_pages, PAGE, hkv, DIM), device, _CACHE[dtype]),
+                    _capi.pointer(v_cache, dtype, (v_pages, PAGE, hkv, DIM), device, _CACHE[dtype]), None, None]
+        if dtype is torch.int8:
             if k_page_scale is None or v_page_scale is None:
                 raise ValueError("INT8 pages need k_page_scale and v_page_scale")
-            _check_scale(k_page_scale, "k_page_scale", k_cache.shape[0], hkv)
-            _check_scale(v_page_scale, "v_page_scale", v_cache.shape[0], hkv)
+            cache_at[2] = _capi.pointer(k_page_scale, torch.float16, (k_pages, hkv), device, _SCALES)
+            cache_at[3] = _capi.pointer(v_page_scale, torch.float16, (v_pages, hkv), device, _SCALES)
         elif k_page_scale is not None or v_page_scale is not None:
             raise ValueError("FP16 pages have no scales")
         for id_range in self._ranges:
-            _check_page_ids(id_range, pages, "KV")
-        exact_k = exact_v = None
+            if id_range is not None:
+                _check_page_ids(id_range, min(k_pages, v_pages), "KV")
+        exact_at = (None, None)
         if self._tables[-1] is not None:
             if exact_cache is None:
                 raise ValueError("a plan with a tail needs the exact pages")
             exact_k, exact_v = exact_cache
             _capi.refuse_gradients(exact_k, exact_v)
-            _check_cache(exact_k, "exact_key", torch.float16, hkv)
-            _check_cache(exact_v, "exact_value", torch.float16, hkv)
-            _check_page_ids(self._tail_range, min(exact_k.shape[0], exact_v.shape[0]), "exact tail")
-        center_at = None
+            if exact_k.dim() != 4 or exact_v.dim() != 4:
+                raise ValueError(_EXACT)
+            k_pages, v_pages = exact_k.shape[0], exact_v.shape[0]
+            exact_at = (_capi.pointer(exact_k, torch.float16, (k_pages, PAGE, hkv, DIM), device, _EXACT),
+                        _capi.pointer(exact_v, torch.float16, (v_pages, PAGE, hkv, DIM), device, _EXACT))
+            if self._tail_range is not None:
+                _check_page_ids(self._tail_range, min(k_pages, v_pages), "exact tail")
+        center_at = lse_at = None
         if value_center is not None:
             center_at = _capi.pointer(value_center, torch.float16, (batch, hkv, DIM), device, _CENTERS)
-        for t in (k_cache, v_cache, k_page_scale, v_page_scale, exact_k, exact_v):
-            if t is not None and t.get_device() != device:
-                raise ValueError(_capi.DEVICE_ERROR)
-        out_at = lse_at = None
         if out is not None:
             out_at = _capi.pointer(out, torch.float16, q.shape, device,
                                    "out must be contiguous float16, shaped like q")
@@ -179,13 +188,12 @@ class _SegmentDecode:
             raise ValueError(_capi.DEVICE_ERROR)
         stream = _capi.launch_stream(device)
         if out is None:
-            out = torch.empty(q.shape, device=q.device, dtype=torch.float16)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
             out_at = out.data_ptr()
         if lse is None and return_lse:
             lse = torch.empty((batch, hq), dtype=torch.float32, device=q.device)
             lse_at = lse.data_ptr()
-        cache_at = (k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_page_scale), _ptr(v_page_scale))
-        return cache_at, (_ptr(exact_k), _ptr(exact_v)), center_at, out, lse, out_at, lse_at, stream
+        return cache_at, exact_at, center_at, out, lse, out_at, lse_at, stream
 
 
 class SharedPrefixDecode(_SegmentDecode):
