@@ -600,10 +600,14 @@ inline void place_work(const pg_segment_plan_t& plan, void* workspace, float sm_
   a.group = plan.num_qo_heads / plan.num_kv_heads;
 }
 
-// Joins few partial rows: a wave per (request, query head), two dims a lane, 4 rows
-// requested at once.
+// Joins few partial rows of many requests: a wave per (request, query head), two dims a lane,
+// 4 rows requested at once.  Workgroups of combine_kernel, which take two dims' halves of a
+// pair and 64 rows at once, are too many and too empty then (8192 pairs of 7 rows: 15.4 us,
+// 9.6 so); with few pairs they join in one trip to memory (32 pairs of 8 rows: 3.3 us, 4.3 so;
+// 128 pairs of 9 rows 3.3 and 5.7).
 constexpr int kFewRows = 4;
 constexpr int kFewSlots = 16;
+constexpr int64_t kManyPairs = 1024;
 
 __global__ __launch_bounds__(kCombineThreads) void combine_few_kernel(CombineArgs a, int64_t pairs) {
   const int64_t pair = static_cast<int64_t>(blockIdx.x) * (kCombineThreads / kWave) +
@@ -672,7 +676,7 @@ inline int32_t launch_combine(const pg_segment_plan_t& plan, const PageAttention
   c.single = plan.batch_size == 1 ? plan.max_slots : 0;
   c.written = 0;
   const int64_t pairs = static_cast<int64_t>(plan.batch_size) * plan.num_qo_heads;
-  if (plan.max_slots <= kFewSlots) {
+  if (plan.max_slots <= kFewSlots && pairs >= kManyPairs) {
     constexpr int kPairs = kCombineThreads / kWave;
     if (pairs > static_cast<int64_t>(UINT32_MAX) / kWave - kPairs)
       return fail(PG_ERROR_UNSUPPORTED, "too many requests for one launch");

@@ -115,6 +115,13 @@ __global__ __launch_bounds__(kScoreThreads) void page_scores_kernel(SelectArgs a
   const int first = (blockIdx.x * (kScoreThreads / kWave) + wave) * a.wave_groups * kScorePages;
   if (first >= pages) return;
 
+  // lane l has the page ids and scales of the wave's pages l and 64 + l
+  const int last = min(first + a.wave_groups * kScorePages, pages) - 1;
+  int ids[2];
+  float scales[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) ids[i] = a.indices[begin + min(first + 64 * i + lane, last)];
+
   // the head's query in steps of a power of two, at most 127 of them
   v4i below[2], above[2];
   float unit;
@@ -161,12 +168,6 @@ __global__ __launch_bounds__(kScoreThreads) void page_scores_kernel(SelectArgs a
       }
   }
 
-  // lane l has the page ids and scales of the wave's pages l and 64 + l
-  const int last = min(first + a.wave_groups * kScorePages, pages) - 1;
-  int ids[2];
-  float scales[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) ids[i] = a.indices[begin + min(first + 64 * i + lane, last)];
   const uint8_t* bounds = a.bounds + kv * 2 * kHeadDim + 16 * kg;
   auto load = [&](int g, v4i (&x)[4]) {
     const int64_t page = __shfl(g < 4 ? ids[0] : ids[1], kScorePages * (g & 3) + n, kWave);
@@ -532,7 +533,11 @@ extern "C" int32_t pg_sparse_select(const pg_segment_plan_t* plan, const void* q
   if (plan->max_pages > plan->selected_pages) {
     const int64_t groups = (plan->max_pages + kScorePages - 1) / kScorePages;
     const int64_t waves = groups * plan->num_kv_heads * plan->batch_size;
-    a.wave_groups = static_cast<int>(std::min<int64_t>(kMostGroups, std::max<int64_t>(1, waves / 4096)));
+    // more pages per wave, which has its query to prepare first, once there are waves
+    // enough to keep every CU reading (45 uneven requests, 43000 pages of 4 heads: 12.5 us so,
+    // 14.2 with twice the groups and 15.4 with half; 8 requests of 8192 pages, 134 MB of
+    // bounds: 25.7, 25.6 and 28.4)
+    a.wave_groups = static_cast<int>(std::min<int64_t>(kMostGroups, std::max<int64_t>(1, waves / 8192)));
     const int64_t block_groups = static_cast<int64_t>(a.wave_groups) * (kScoreThreads / kWave);
     hipLaunchKernelGGL(page_scores_kernel,
                        dim3(static_cast<unsigned>((groups + block_groups - 1) / block_groups), plan->num_kv_heads,
