@@ -15,6 +15,9 @@ constexpr int kTileTokens = 64;
 constexpr int kTilePages = kTileTokens / kPageSize;
 constexpr int kTileBytes = kTileTokens * kHeadDim * 2;   // 16 KiB of FP16
 constexpr float kRescaleLimit = 8.0f;                    // log2
+// Probabilities are 2^7 times what the running maximum makes them, so at most 2^15 where it
+// lags: as far up in FP16's range as goes, for the small ones' sake.
+constexpr float kProbabilityExponent = 7.0f;
 // The running maximum before the first score.  Finite, so that a tile of -inf scores adds
 // probabilities of 0 and not exp2(-inf + inf).
 constexpr float kLowest = -__FLT_MAX__;
@@ -41,10 +44,10 @@ struct SharedTiles {
 //
 // INT8 codes become FP16 once, on their way into LDS, for all rows; K's scales multiply
 // scores and V's the probabilities, a page (16 tokens) being one step of the product over
-// tokens.  Probabilities times V's scales go in as one FP16 value, off by 2^-11 of itself at
-// most, less than the output's own rounding in the mean over many tokens; V's scales are
-// taken relative to the power of two at the item's largest, and probabilities do not exceed
-// 2^8 (the running maximum is raised when a score passes it by that).
+// tokens.  Probabilities times V's scales go in as one FP16 value: off by 2^-11 of itself at
+// most, which in the mean over tokens comes to less than the output's own rounding (errors
+// against 64 bits 2.1e-4 of the outputs, as with float32 throughout), or by 2^-32 of what the
+// largest scale could weigh (V's scales count from the power of two at the item's largest).
 //
 // Tiles go from memory to registers a whole iteration before they are put in LDS.
 template <bool kCodes, int kRowWaves>
@@ -96,7 +99,7 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
     for (int k = 0; k < 8; ++k) qf[k] = *reinterpret_cast<const v8h*>(qp + 16 * k);
   }
   // tokens of the item that are visible: all but those past the prefix's last one
-  const int last_len = it.page_end - 1 == it.last_page ? min(a.prefix_last[it.segment], kPageSize) : kPageSize;
+  const int last_len = it.page_end - 1 == it.last_page ? max(min(a.prefix_last[it.segment], kPageSize), 0) : kPageSize;
   const int visible = (count - 1) * kPageSize + last_len;
   __syncthreads();
   float v_unit = 1.0f, v_back = 1.0f;                    // 2^-e and 2^e of V's scales
@@ -231,13 +234,14 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
   };
   // probabilities page by page, each followed by its product
   auto attend = [&](int buffer, const v16f (&s)[kBlocks], const float (&kf)[kSteps], const float (&vf)[kSteps]) {
+    const float offset = kProbabilityExponent - m;
 #pragma unroll
     for (int p = 0; p < kSteps; ++p) {
       v8h pr;
 #pragma unroll
       for (int r = 0; r < 8; r += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[p / 2][8 * (p % 2) + r], kf[p], -m));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[p / 2][8 * (p % 2) + r + 1], kf[p], -m));
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[p / 2][8 * (p % 2) + r], kf[p], offset));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[p / 2][8 * (p % 2) + r + 1], kf[p], offset));
         l0 += p0;
         l1 += p1;
         pr[r] = static_cast<_Float16>(kCodes ? p0 * vf[p] : p0);
@@ -322,7 +326,7 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
   const int64_t slot = a.slot_base[it.slot_at + in_segment] + it.split + part;
   const int64_t to = slot * a.num_qo_heads + head;
   if (half == 0) {
-    a.partial_m[to] = l == 0.0f ? kNoScore : m;
+    a.partial_m[to] = l == 0.0f ? kNoScore : m - kProbabilityExponent;
     a.partial_l[to] = l;
   }
   float* out = a.partial_o + to * kHeadDim + 4 * half;

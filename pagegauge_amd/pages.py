@@ -124,23 +124,27 @@ class Moves(NamedTuple):
 
 class PagePool:
     """Users per page of a pool: ``refs`` (device int32 [pages], zero: free), which may
-    be read, or set as a whole, like any tensor."""
+    be read, or written in place, like any tensor."""
 
     def __init__(self, pages: int, device="cuda") -> None:
         if not 0 <= pages < 2 ** 31:
             raise ValueError("a pool holds 0 to 2^31 - 1 pages")
-        self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
-        self._device = self.refs.get_device()
+        self._refs = torch.zeros(pages, dtype=torch.int32, device=device)
+        self._device = self._refs.get_device()
+
+    @property
+    def refs(self) -> torch.Tensor:
+        return self._refs
 
     @property
     def pages(self) -> int:
-        return self.refs.numel()
+        return self._refs.shape[0]
 
     def _adjust(self, ids: torch.Tensor, by: int) -> None:
         ids_at = _ids(ids, self._device, "page ids")
         stream = _capi.launch_stream(self._device)
         if ids.numel():
-            _capi.call("pg_pool_adjust", self.refs.data_ptr(), self.pages, ids_at, ids.numel(), by, stream)
+            _capi.call("pg_pool_adjust", self._refs.data_ptr(), self.pages, ids_at, ids.numel(), by, stream)
 
     def share(self, ids: torch.Tensor, users: int = 1) -> None:
         """``users`` more users of each of the pages ``ids`` (device int32 [n]).  Ids may
@@ -164,10 +168,10 @@ class PagePool:
                                                         "out must be contiguous int32 [count]")
         stream = _capi.launch_stream(self._device)
         if out is None:
-            out = torch.empty(count, dtype=torch.int32, device=self.refs.device)
+            out = torch.empty(count, dtype=torch.int32, device=self._refs.device)
             out_at = out.data_ptr()
         if count:
-            _capi.call("pg_pool_take", self.refs.data_ptr(), self.pages, out_at, count, stream)
+            _capi.call("pg_pool_take", self._refs.data_ptr(), self.pages, out_at, count, stream)
         return out
 
     def stage_compaction(self, out: Optional[Moves] = None) -> Moves:
@@ -182,7 +186,7 @@ class PagePool:
         stream = _capi.launch_stream(device)
         if out is None:
             # one allocation, remap (16-byte aligned) in front
-            whole = torch.empty(pages + 2 * half + 1, dtype=torch.int32, device=self.refs.device)
+            whole = torch.empty(pages + 2 * half + 1, dtype=torch.int32, device=self._refs.device)
             remap, source, target, live = whole.split_with_sizes((pages, half, half, 1))
             out = Moves(source, target, remap, live)
             remap_at = whole.data_ptr()
@@ -190,7 +194,7 @@ class PagePool:
             at = source_at, source_at + 4 * half, remap_at, source_at + 8 * half
         else:
             at = [_capi.pointer(t, torch.int32, (n,), device, what) for t, n in zip(out, (half, half, pages, 1))]
-        _capi.call("pg_pool_stage_compaction", self.refs.data_ptr(), pages, *at, stream)
+        _capi.call("pg_pool_stage_compaction", self._refs.data_ptr(), pages, *at, stream)
         return out
 
     def commit_compaction(self, moves: Moves) -> None:
@@ -200,5 +204,5 @@ class PagePool:
                                   "source and target must have one id per move")
         stream = _capi.launch_stream(self._device)
         if moves.source.numel():
-            _capi.call("pg_pool_commit_compaction", self.refs.data_ptr(), self.pages, source_at, target_at,
+            _capi.call("pg_pool_commit_compaction", self._refs.data_ptr(), self.pages, source_at, target_at,
                        moves.source.numel(), stream)

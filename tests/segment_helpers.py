@@ -6,7 +6,7 @@ numbers, summed in float32 (128 additions, 8 more roundings for scales): its err
 base 2 is at most 136 * 2^-24 of sum |q||k| sm log2(e), and a weight is off by ln 2 times
 that.  exp2, the two-part FP16 probability and its product with V's scale add 2^-20; a
 kernel that takes the probability as one FP16 value adds half a step of it, 2^-11, or
-where it is subnormal 2^-25 of the largest.  Sums of T tokens take at most T / 16 + 64
+where it is subnormal 2^-32 of the largest.  Sums of T tokens take at most T / 16 + 64
 float32 additions, each off by 2^-24 of the sum.  An output is a weighted mean, off by at
 most the weights' error times the largest |v| (twice where the sum of weights is off as
 well), then rounded to FP16 (2^-11).  lse is off by the score's error and a few float32
@@ -63,7 +63,7 @@ def check_head(out, lse, q, k, v, center, sm_scale, single_part):
         score = 136 * 2.0 ** -24 * spread
         weight = 2 * (np.log(2.0) * score + 2.0 ** -20 + (len(k) / 16 + 64) * 2.0 ** -24)
         if single_part:
-            weight += 2.0 ** -11 + len(k) * 2.0 ** -25
+            weight += 2.0 ** -11 + len(k) * 2.0 ** -32
         bound = (weight * np.abs(v).max())[:, None]
         assert (np.abs(lse - want_lse) <= score + 2.0 ** -20 + 2.0 ** -22 * np.abs(want_lse)
                 + (len(k) / 16 + 64) * 2.0 ** -24).all(), np.abs(lse - want_lse).max()

@@ -135,6 +135,53 @@ def test_scales_that_differ_from_page_to_page(cuda):
     b.check(*run(planned(b, cuda), b))
 
 
+@pytest.mark.parametrize("requests", [1, 3, 10, 30])
+def test_small_values_beside_large_ones_without_weight(cuda, requests):
+    """V's scales are of 2^-20, but for one page that no query attends to (its keys are far
+    from all): the small values keep FP16's precision in every form.  A probability
+    times its scale is 2^20 below what the largest scale could make it and 2^12 above the
+    least FP16 value where that is put at 2^15: half a step is 2^-11 of it at most."""
+    b = Batch(cuda, [(0, requests, 960)], [0] * requests, [0] * requests, 1, 4)
+    b.q.abs_()
+    b.q += 0.25
+    b.scales[1].fill_(2.0 ** -20)
+    far = int(b.prefix_ids[30])
+    b.cache[0][far] = -128
+    b.scales[0][far] = 4.0                       # scores of -128 * 4 * sum |q| sm: below -2000
+    b.scales[1][far] = 1.0
+    out, lse = run(planned(b, cuda), b, value_center=None)
+    pools = [c[b.prefix_ids.long()].double().cpu() * s[b.prefix_ids.long()].double().cpu()[:, None, :, None]
+             for c, s in zip(b.cache, b.scales)]
+    k, v = (p.reshape(960, 128) for p in pools)
+    scores = b.q.double().cpu() @ k.T * 128 ** -0.5
+    weights = torch.softmax(scores, -1)
+    want = weights @ v
+    size = weights @ v.abs()                     # what the roundings of the terms are relative to
+    # terms 2^-11 each, sums and exponents as in segment_helpers (scores below 2^6 here, but for
+    # the far page's), then the output's half step: a subnormal's is 2^-25
+    bound = size * (2.0 ** -11 + 2.0 ** -13) + 2.0 ** -25 + want.abs() * 2.0 ** -11
+    assert bool(((out.double().cpu() - want).abs() <= bound).all())
+
+
+@both_kinds
+@pytest.mark.parametrize("requests", [1, 4, 30])
+def test_infinite_scores(cuda, kind, requests):
+    """Scores of -inf leave the others."""
+    b = Batch(cuda, [(0, requests, 300)], [0] * requests, [20] * requests, 1, 4, kind)
+    b.q.abs_()
+    first = int(b.prefix_ids[0])
+    decode = planned(b, cuda)
+    if kind is torch.float16:
+        b.cache[0][first, :, 0, 7] = float("-inf")
+    else:
+        b.cache[0][first] = -128
+        b.scales[0][first] = float("inf")        # -128 * inf: -inf, for any q above 0
+        b.q += 0.25
+    out, lse = run(decode, b)
+    b.prefix_ids, b.prefix_ptr[1] = b.prefix_ids[1:], int(b.prefix_ptr[1]) - 1     # as without that page
+    b.check(out, lse)
+
+
 @both_kinds
 def test_scores_that_climb(cuda, kind):
     """The largest score is the last one, far above the others: every base moves."""
@@ -214,6 +261,40 @@ def test_captured_runs_follow_their_inputs(cuda):
             torch.cuda.synchronize()
             want, want_lse = run(decode, b)
             assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+def test_graphs_that_share_a_workspace(cuda):
+    """Two captured runs of one object replayed in turn beside eager work."""
+    b = Batch(cuda, [(0, 40, 700)], spread(40, 0, 60), spread(40, 0, 20), 2, 4)
+    decode = planned(b, cuda)
+    queries = [b.q, b.q.flip(0).contiguous()]
+    want = [run(decode, b, q=q) for q in queries]
+    outs = [(torch.empty_like(o), torch.empty_like(l)) for o, l in want]
+    graphs = []
+    for q, (out, lse) in zip(queries, outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            run(decode, b, q=q, out=out, lse=lse)
+    for _ in range(3):
+        for graph, got, wanted in zip(graphs, outs, want):
+            got[0].zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got[0], wanted[0]) and torch.equal(got[1], wanted[1])
+        assert torch.equal(run(decode, b)[0], want[0][0])
+
+
+def test_gradients_are_refused(cuda):
+    b = Batch(cuda, [(0, 2, 40)], [20, 3], [5, 5], 2, 4)
+    decode = planned(b, cuda)
+    want = run(decode, b)
+    follow = lambda t: t.clone().requires_grad_()  # noqa: E731
+    for over in (dict(q=follow(b.q)), dict(value_center=follow(b.center)), dict(k_page_scale=follow(b.scales[0])),
+                 dict(v_page_scale=follow(b.scales[1])), dict(exact_cache=(b.exact[0], follow(b.exact[1])))):
+        with pytest.raises(ValueError, match="no gradient"):
+            run(decode, b, **over)
+        with torch.no_grad():
+            assert torch.equal(run(decode, b, **over)[0], want[0])
 
 
 def test_same_as_the_segmented_decode_over_whole_tables(cuda):
