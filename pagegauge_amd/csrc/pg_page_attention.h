@@ -601,11 +601,12 @@ inline void place_work(const pg_segment_plan_t& plan, void* workspace, float sm_
 }
 
 // Joins few partial rows of many requests: a wave per (request, query head), two dims a lane,
-// 4 rows requested at once.  Workgroups of combine_kernel, which take two dims' halves of a
-// pair and 64 rows at once, are too many and too empty then (8192 pairs of 7 rows: 15.4 us,
-// 9.6 so); with few pairs they join in one trip to memory (32 pairs of 8 rows: 3.3 us, 4.3 so;
-// 128 pairs of 9 rows 3.3 and 5.7).
-constexpr int kFewRows = 4;
+// 8 rows requested at once.  Workgroups of combine_kernel, which take half a pair's dims and
+// 64 rows at once, are too many and too empty then (8192 pairs of 5 rows: 14.4 us, 7.9 so; 1952
+// pairs of up to 15: 6.6 and 4.9); of few pairs those are the shorter trip (32 pairs of 8 rows:
+// 3.3 us, 4.3 with 4 rows at once here).  With more rows per pair neither is the faster (2048
+// pairs of 18).
+constexpr int kFewRows = 8;
 constexpr int kFewSlots = 16;
 constexpr int64_t kManyPairs = 1024;
 
@@ -625,8 +626,10 @@ __global__ __launch_bounds__(kCombineThreads) void combine_few_kernel(CombineArg
     float2 x[kFewRows];
 #pragma unroll
     for (int k = 0; k < kFewRows; ++k) {
-      const int64_t at = static_cast<int64_t>(min(first + k, end - 1)) * a.num_qo_heads + head;
-      mi[k] = first + k < end ? a.partial_m[at] : kNoScore;
+      mi[k] = kNoScore;
+      if (first + k >= end) continue;
+      const int64_t at = static_cast<int64_t>(first + k) * a.num_qo_heads + head;
+      mi[k] = a.partial_m[at];
       li[k] = a.partial_l[at];
       x[k] = *reinterpret_cast<const float2*>(a.partial_o + at * kHeadDim + 2 * lane);
     }

@@ -86,36 +86,45 @@ int32_t build_segment_plan(const SegmentBatch& b, SegmentWork& work, pg_segment_
     if (pages || tail || !covered[r]) units.push_back({-1, r, group, pages, tail, tail_weight});
   }
 
-  // ---- the largest shares, of shared tiles and of the others apart: the smallest with which
-  // they take their part of two workgroups per CU; where they are more requests or
-  // prefixes than that, half of an even share, since the longest go first and the short
-  // ones fill in behind them.  Shared tiles keep the matrix cores busy with one
-  // workgroup per CU, and the other then reads requests' own pages beside it; they take
-  // both where there is little to read.
+  // ---- the largest share: the smallest with which everything runs at once, two
+  // workgroups per CU (61 requests of 7 prefixes: 33.5 us; with shares of shared tiles
+  // and of own pages apart, as below, 39.4).  Where requests and prefixes are more than
+  // that, shared tiles get one workgroup per CU, which is what the matrix cores need, and
+  // own pages, in half of even shares, are read beside them: the longest go first and the
+  // short ones fill in behind them (256 requests on 1024 pages: shared tiles in 4 parts
+  // 175 us, in 2 parts 250, in 6 parts 196, in 8 parts 215); with little of their own to
+  // read shared tiles get both (the same with one exact page each: 108 us, 118 with one).
   const int64_t cus = b.num_cus > 0 ? b.num_cus : 256;
-  const int64_t slots_at_once = std::max<int64_t>(2, 2 * cus / b.num_kv_heads);
+  const int64_t at_once = std::max<int64_t>(2, 2 * cus / b.num_kv_heads);
   auto items_of = [&](bool shared, int64_t cap) {
     int64_t n = 0;
     for (const Unit& u : units) n += u.shared() == shared ? u.cuts(cap) * u.blocks() : 0;
     return n;
   };
-  int64_t weights[2] = {0, 0};
-  for (const Unit& u : units) weights[u.shared()] += u.weight() * u.blocks();
-  auto largest_share = [&](bool shared, int64_t target) {
-    int64_t cap = shared ? kSharedMaxPages : kSegmentMaxPages;
-    if (items_of(shared, cap) > target)
-      return std::min(cap, std::max(weights[shared] / (2 * target), kSmallestShare));
+  // the smallest share in [one group of pages per wave, high] that ``fits``, or 0
+  auto smallest = [](int64_t high, auto&& fits) -> int64_t {
+    if (!fits(high)) return 0;
     int64_t low = kSegmentWaves * kSegmentGroupPages;
-    while (low < cap) {
-      const int64_t middle = low + (cap - low) / 2;
-      if (items_of(shared, middle) <= target) cap = middle; else low = middle + 1;
+    while (low < high) {
+      const int64_t middle = low + (high - low) / 2;
+      if (fits(middle)) high = middle; else low = middle + 1;
     }
-    return cap;
+    return high;
   };
-  const int64_t shared_target = weights[0] > weights[1] / 2 ? slots_at_once / 2 : slots_at_once;
-  const int64_t shared_cap = largest_share(true, shared_target);
+  int64_t shared_cap = smallest(kSharedMaxPages, [&](int64_t cap) {
+    return items_of(true, cap) + items_of(false, std::min<int64_t>(cap, kSegmentMaxPages)) <= at_once;
+  });
+  int64_t own_cap = std::min<int64_t>(shared_cap, kSegmentMaxPages);
+  if (!shared_cap) {
+    int64_t weights[2] = {0, 0};
+    for (const Unit& u : units) weights[u.shared()] += u.weight() * u.blocks();
+    auto half_share = [&](bool shared) { return std::max(weights[shared] / at_once, kSmallestShare); };
+    const int64_t shared_target = weights[0] > weights[1] / 2 ? at_once / 2 : at_once;
+    shared_cap = smallest(kSharedMaxPages, [&](int64_t cap) { return items_of(true, cap) <= shared_target; });
+    if (!shared_cap) shared_cap = std::min<int64_t>(kSharedMaxPages, half_share(true));
+    own_cap = std::min<int64_t>(kSegmentMaxPages, half_share(false));
+  }
   const int64_t shared_items = items_of(true, shared_cap);
-  const int64_t own_cap = largest_share(false, std::max(slots_at_once - shared_items, slots_at_once / 2));
   auto cuts_of = [&](const Unit& u) { return u.cuts(u.shared() ? shared_cap : own_cap); };
   const int64_t count = shared_items + items_of(false, own_cap);
   for (const Unit& u : units)
