@@ -66,7 +66,10 @@ __device__ __forceinline__ void copy_block(const CopyArgs& a, const CopyPlane& p
 }
 
 // A plane's row (one layer) is copied as one sequence of the moves' pages, in blocks of
-// 1024 vectors of 16 bytes (or what the page's size and place allow).
+// 1024 vectors of 16 bytes (or what the page's size and place allow).  Bound by HBM: 540
+// exact pages of K and V in 8 layers, 566 MB read and written, 95 to 101 us (5.6 to 6.0 TB/s;
+// a copy of 1 GiB reaches 5.1), 8 pages 3.8 us; a list with empty entries costs their
+// workgroups (4096 moves of an INT8 pool in 8192 entries, 268 MB, 59 us: 4.5 TB/s).
 __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyArgs a) {
   int plane = 0;
   while (plane + 1 < a.planes_used && blockIdx.x >= a.planes[plane + 1].first_block) ++plane;
@@ -183,7 +186,9 @@ __global__ __launch_bounds__(kScanThreads) void take_kernel(int32_t* refs, int32
 
 // The pages in use, ``live`` of them, are to fill the pool's front: the i-th lowest page
 // at or past ``live`` that is in use goes to the i-th lowest free one below it, the
-// fewest moves there are.  No page is both a source and a target.
+// fewest moves there are.  No page is both a source and a target.  Bound by the trips of one
+// workgroup: 16384 pages 9.8 us, 1021 pages 5.8 (with a scan for each list and entries of remap
+// stored one by one 14.4 and 7.2).
 __global__ __launch_bounds__(kScanThreads) void stage_kernel(const int32_t* refs, int32_t pages, int32_t* source,
                                                              int32_t* target, int32_t* remap, int32_t* live_out) {
   __shared__ int wave_sums[kScanThreads / kWave];

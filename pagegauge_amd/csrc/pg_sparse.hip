@@ -34,7 +34,8 @@ __device__ __forceinline__ v2i16 as_pair(uint32_t x) { return __builtin_bit_cast
 // A thread takes 16 channels of a page's 16 tokens, all requested at once; neighbouring
 // threads take neighbouring channels and heads, so a wave reads whole token rows.  Signed
 // bytes are compared as the high bytes of 16-bit halves: the odd ones where they are, the
-// even ones a byte further up.
+// even ones a byte further up.  Bound by the reads: 8191 pages of 8 heads, 151 MB, in 22.8 us
+// where they are still in the Infinity Cache and 32 where not (4.6 TB/s); 32 pages 3.3 us.
 __global__ __launch_bounds__(kBoundsThreads) void key_bounds_kernel(BoundsArgs a) {
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * kBoundsThreads + threadIdx.x;
   if (unit >= a.units) return;
@@ -104,7 +105,9 @@ constexpr int kScorePages = 16;      // rows of an MFMA
 constexpr int kMostGroups = 8;       // of so many pages, per wave: two page ids a lane
 
 // Sixteen pages at a time are the rows of v_mfma_i32_16x16x64_i8 and the KV head's query
-// heads its columns; 4 products take the 128 lower bounds and the 128 upper ones.
+// heads its columns; 4 products take the 128 lower bounds and the 128 upper ones.  Page ids
+// and scales are requested once per wave, a group's bounds while the one before is scored.
+// Bound by the reads of bounds: 65536 pages of 8 heads, 134 MB, 26 to 28 us (4.8 to 5.2 TB/s).
 __global__ __launch_bounds__(kScoreThreads) void page_scores_kernel(SelectArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
@@ -213,7 +216,7 @@ constexpr int kPickWaves = kPickThreads / kWave;
 constexpr int kBins = 2 * kPickThreads;
 constexpr int kListed = 1024;        // scores near the last one taken that are compared one by one
 
-// Whole numbers in the order of the scores, -0 as 0 (NaN never gets here); none is 0.
+// Whole numbers in the order of the scores, -0 as 0.
 __device__ __forceinline__ uint32_t order_key(float score) {
   const uint32_t bits = __float_as_uint(score == 0.0f ? 0.0f : score);
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
@@ -223,19 +226,26 @@ __device__ __forceinline__ float score_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// One workgroup per (KV head, request): the key of the last score that is taken, then
-// everything above it and the lowest positions at it, in order.  A histogram over 2048
-// equal parts of the scores' range leaves a few to be ranked one by one, or where very many
-// are alike, to further histograms over the bits of their keys.  Up to kHeld keys stay in a
-// thread's registers; with kHeld = 0 the scores are read again each time.
+// One workgroup per (KV head, request): the last score that is taken, then everything above
+// it and the lowest positions at it, in order.  A histogram over 2048 equal parts of the
+// scores' range leaves a few to be ranked one by one, or where very many are alike, to
+// further histograms over their bits.  Up to kHeld scores stay in a thread's registers;
+// with kHeld = 0 they are read again each time.  Scores are no NaN; here NaN stands for a
+// page that is taken anyway.
+//
+// Bound by its chain of steps between barriers: 8 workgroups of 2048 pages 5.9 us, 64 of 8192
+// 9.2 (with scores as ordered whole numbers throughout 11.1, as three histograms over their
+// bits, read from memory each time, 17.4: scores share their leading bits, and additions
+// to one bin wait for each other).
 template <int kHeld>
 __global__ __launch_bounds__(kPickThreads) void pick_pages_kernel(SelectArgs a) {
   __shared__ uint32_t bins[kBins];
-  __shared__ uint32_t list[kListed];
+  __shared__ float list[kListed];
   __shared__ uint32_t counts[kHeld > 0 ? kHeld * kPickWaves : kPickWaves];
   __shared__ uint32_t wave_sums[kPickWaves];
   __shared__ float wave_low[kPickWaves], wave_high[kPickWaves];
   __shared__ uint32_t found[3], listed;
+  __shared__ float found_score;
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
   const int kv = blockIdx.x, request = blockIdx.y;
   const int pages = a.indptr[request + 1] - a.indptr[request];
@@ -245,22 +255,24 @@ __global__ __launch_bounds__(kPickThreads) void pick_pages_kernel(SelectArgs a) 
     return;
   }
   const float* scores = a.scores + (static_cast<int64_t>(request) * a.num_kv_heads + kv) * a.max_pages;
-  // 0 for the pages that are taken anyway
-  auto key_at = [&](int i) { return i < a.first || i >= pages - a.last ? 0u : order_key(scores[i]); };
-  uint32_t held[kHeld > 0 ? kHeld : 1];
+  const float anyway = __uint_as_float(0x7fc00000u);
+  auto score_at = [&](int i) { return i < a.first || i >= pages - a.last ? anyway : scores[i]; };
+  float held[kHeld > 0 ? kHeld : 1];
 #pragma unroll
   for (int j = 0; j < kHeld; ++j) {
     const int i = tid + j * kPickThreads;
-    held[j] = i < pages ? key_at(i) : 0;
+    held[j] = i < pages ? score_at(i) : anyway;
   }
-  auto each_key = [&](auto&& body) {
+  auto each_score = [&](auto&& body) {
     if constexpr (kHeld > 0) {
 #pragma unroll
       for (int j = 0; j < kHeld; ++j)
-        if (held[j]) body(held[j]);
+        if (held[j] == held[j]) body(held[j]);
     } else {
-      for (int i = tid; i < pages; i += kPickThreads)
-        if (const uint32_t key = key_at(i)) body(key);
+      for (int i = tid; i < pages; i += kPickThreads) {
+        const float s = score_at(i);
+        if (s == s) body(s);
+      }
     }
   };
 
@@ -292,12 +304,11 @@ __global__ __launch_bounds__(kPickThreads) void pick_pages_kernel(SelectArgs a) 
     bins[tid + kPickThreads] = 0;
   };
 
-  uint32_t wanted = a.take - a.first - a.last;       // rank of the last key taken, from the top
-  uint32_t last_key = ~0u;                           // none
+  uint32_t wanted = a.take - a.first - a.last;       // rank of the last score taken, from the top
+  float last_score = anyway;                         // none
   if (wanted > 0) {
     float low = -kNoScore, high = kNoScore;
-    each_key([&](uint32_t key) {
-      const float s = score_of(key);
+    each_score([&](float s) {
       if (fabsf(s) < -kNoScore) {
         low = fminf(low, s);
         high = fmaxf(high, s);
@@ -316,37 +327,37 @@ __global__ __launch_bounds__(kPickThreads) void pick_pages_kernel(SelectArgs a) 
     high = row16_max(wave_high[lane % kPickWaves]);
     // rounded alike for all, and never falling as the score rises
     const float per_bin = (kBins - 1) / fmaxf(high - low, 0x1p-100f);
-    auto bin_of = [&](uint32_t key) {
-      return static_cast<uint32_t>(fminf(fmaxf((score_of(key) - low) * per_bin, 0.0f), static_cast<float>(kBins - 1)));
+    auto bin_of = [&](float s) {
+      return static_cast<uint32_t>(fminf(fmaxf((s - low) * per_bin, 0.0f), static_cast<float>(kBins - 1)));
     };
-    each_key([&](uint32_t key) { atomicAdd(&bins[bin_of(key)], 1u); });
+    each_score([&](float s) { atomicAdd(&bins[bin_of(s)], 1u); });
     __syncthreads();
     find_bin(wanted);
     const uint32_t bin = found[0];
     wanted = found[1];
     if (found[2] <= kListed) {
-      each_key([&](uint32_t key) {
-        if (bin_of(key) == bin) list[atomicAdd(&listed, 1u)] = key;
+      each_score([&](float s) {
+        if (bin_of(s) == bin) list[atomicAdd(&listed, 1u)] = s;
       });
       __syncthreads();
       const uint32_t count = listed;
       if (static_cast<uint32_t>(tid) < count) {
-        const uint32_t mine = list[tid];
+        const float mine = list[tid];
         uint32_t larger = 0, equal = 0;
         for (uint32_t i = 0; i < count; ++i) {
           larger += list[i] > mine;
           equal += list[i] == mine;
         }
         if (larger < wanted && wanted <= larger + equal) {
-          found[0] = mine;
+          found_score = mine;
           found[1] = wanted - larger;
         }
       }
       __syncthreads();
-      last_key = found[0];
+      last_score = found_score;
       wanted = found[1];
     } else {
-      last_key = 0;
+      uint32_t key = 0;
       int shift = 32;
 #pragma unroll 1
       for (int step = 0; step < 3; ++step) {         // 11 bits, then 11, then 10
@@ -355,22 +366,24 @@ __global__ __launch_bounds__(kPickThreads) void pick_pages_kernel(SelectArgs a) 
         __syncthreads();
         clear_bins();
         __syncthreads();
-        each_key([&](uint32_t key) {
-          if (bin_of(key) == bin && (before == 32 || key >> before == last_key >> before))
-            atomicAdd(&bins[key >> shift & ((1u << width) - 1)], 1u);
+        each_score([&](float s) {
+          const uint32_t at = order_key(s);
+          if (bin_of(s) == bin && (before == 32 || at >> before == key >> before))
+            atomicAdd(&bins[at >> shift & ((1u << width) - 1)], 1u);
         });
         __syncthreads();
         find_bin(wanted);
-        last_key |= found[0] << shift;
+        key |= found[0] << shift;
         wanted = found[1];
       }
+      last_score = score_of(key);
     }
   }
 
-  // larger keys and the pages taken anyway, and of the equal keys the first ``wanted``
-  auto classes = [&](int i, uint32_t key, uint64_t& larger, uint64_t& equal) {
-    larger = __builtin_amdgcn_ballot_w64(i < pages && (key == 0 || key > last_key));
-    equal = __builtin_amdgcn_ballot_w64(i < pages && key == last_key);
+  // larger scores and the pages taken anyway, and of the equal ones the first ``wanted``
+  auto classes = [&](int i, float s, uint64_t& larger, uint64_t& equal) {
+    larger = __builtin_amdgcn_ballot_w64(i < pages && (s != s || s > last_score));
+    equal = __builtin_amdgcn_ballot_w64(i < pages && s == last_score);
   };
   const uint64_t lanes_below = (1ull << lane) - 1;
   auto write = [&](int i, uint64_t larger, uint64_t equal, uint32_t larger_before, uint32_t equal_before) {
@@ -426,7 +439,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_pages_kernel(SelectArgs a) 
     for (int first = 0; first < pages; first += kPickThreads) {
       const int i = first + tid;
       uint64_t larger, equal;
-      classes(i, i < pages ? key_at(i) : 0, larger, equal);
+      classes(i, i < pages ? score_at(i) : anyway, larger, equal);
       if (lane == 0)
         wave_sums[wave] = static_cast<uint32_t>(__popcll(larger)) | static_cast<uint32_t>(__popcll(equal)) << 16;
       __syncthreads();
