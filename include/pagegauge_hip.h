@@ -819,7 +819,8 @@ int32_t pg_pool_take(int32_t* refs, int64_t pages, int32_t* out, int64_t count, 
 int32_t pg_pool_stage_compaction(const int32_t* refs, int64_t pages, int32_t* source, int32_t* target,
                                  int32_t* remap, int32_t* live, void* stream);
 
-/* Moves the counts along: refs[target[i]] = refs[source[i]], refs[source[i]] = 0. */
+/* Moves the counts along: refs[target[i]] = refs[source[i]], refs[source[i]] = 0, where
+ * the source still has users. */
 int32_t pg_pool_commit_compaction(int32_t* refs, int64_t pages, const int32_t* source,
                                   const int32_t* target, int64_t moves, void* stream);
 

@@ -16,6 +16,10 @@ call signatures:
   head, frequencies scaled for long contexts;
 * ``int4`` -- the cache held in 4 bits: prompt writer, reader-back, append with
   the rotation on the way, attention;
+* ``pages`` -- pages of a pool that requests share: counted, handed out, copied, compacted;
+* ``prefix`` -- attention that reads prefixes shared by requests once;
+* ``sparse`` -- bounds of pages' keys, the choice of pages that matter to a token, attention
+  over them;
 * ``logits`` -- penalties, biases and masks before a token is picked;
 * ``page_table`` -- the page-table algebra of the decoder harness;
 * ``decoder`` -- the Mistral-shaped decoder over these kernels;
@@ -24,5 +28,5 @@ call signatures:
 * ``workloads`` -- the seeded benchmark configurations.
 """
 
-__all__ = ["runtime", "decode", "update", "rotary", "int4", "logits", "page_table", "decoder",
-           "serving", "serving_bridge", "workloads"]
+__all__ = ["runtime", "decode", "update", "rotary", "int4", "pages", "prefix", "sparse", "logits",
+           "page_table", "decoder", "serving", "serving_bridge", "workloads"]

@@ -243,6 +243,7 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(int32_t* refs, int32_t
   if (i >= moves) return;
   const int32_t from = source[i], to = target[i];
   if (from < 0 || from >= pages || to < 0 || to >= pages) return;
+  if (refs[from] <= 0) return;       // moved already, or given back since
   refs[to] = refs[from];
   refs[from] = 0;
 }

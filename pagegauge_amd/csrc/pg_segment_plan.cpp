@@ -65,7 +65,7 @@ int32_t build_segment_plan(const SegmentBatch& b, SegmentWork& work, pg_segment_
   const int64_t tail_weight = b.kind == PG_KV_INT8 ? 2 : 1;      // of an FP16 page, by bytes
   std::vector<Unit> units;
   std::vector<bool> covered(b.batch_size, false);
-  int64_t prefix_pages = 0, history = 0, tails = 0, max_pages = 0;
+  int64_t prefix_pages = 0, history = 0, tails = 0, max_pages = 0, all_pages = 0;
   for (int32_t s = 0; s < b.segments; ++s) {
     const int32_t begin = b.prefix_requests[2 * s], end = b.prefix_requests[2 * s + 1];
     if (begin < 0 || end < begin || end > b.batch_size)
@@ -81,6 +81,7 @@ int32_t build_segment_plan(const SegmentBatch& b, SegmentWork& work, pg_segment_
     const int64_t pages = b.selected > 0 ? std::min<int64_t>(all, b.selected) : all;
     const int64_t tail = b.tail_indptr ? b.tail_indptr[r + 1] - b.tail_indptr[r] : 0;
     max_pages = std::max(max_pages, all);
+    all_pages += all;
     history += pages;
     tails += tail;
     if (pages || tail || !covered[r]) units.push_back({-1, r, group, pages, tail, tail_weight});
@@ -229,7 +230,7 @@ int32_t build_segment_plan(const SegmentBatch& b, SegmentWork& work, pg_segment_
   p.slot_ptr_offset = place((static_cast<int64_t>(b.batch_size) + 1) * 4);
   p.slot_base_offset = place(static_cast<int64_t>(work.slot_base.size()) * 4);
   p.indptr_offset = place(b.selected > 0 ? (static_cast<int64_t>(b.batch_size) + 1) * 4 : 0);
-  p.scores_offset = place(b.selected > 0 ? 4 * max_pages * b.batch_size * b.num_kv_heads : 0);
+  p.scores_offset = place(b.selected > 0 ? 4 * all_pages * b.num_kv_heads : 0);
   p.partial_offset = place(rows * b.num_qo_heads * (kHeadDim + 2) * 4);
   p.partial_rows = rows;
   p.workspace_bytes = offset;

@@ -94,9 +94,9 @@ struct SelectArgs {
   const uint16_t* key_scale;       // [pages, Hkv]
   const int32_t* indices;
   const int32_t* indptr;           // [B + 1]
-  float* scores;                   // [B, Hkv, max_pages]
+  float* scores;                   // [Hkv, pages] of each request, one after the other
   int32_t* selected;               // [B, Hkv, take]
-  int max_pages, take, first, last;
+  int take, first, last;
   int num_kv_heads, group, wave_groups;
 };
 
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(kScoreThreads) void page_scores_kernel(SelectArgs a
 #pragma unroll
     for (int w = 0; w < 4; ++w) x[w] = *reinterpret_cast<const v4i*>(from + 64 * w);
   };
-  float* scores = a.scores + (static_cast<int64_t>(request) * hkv + kv) * a.max_pages;
+  float* scores = a.scores + static_cast<int64_t>(begin - a.indptr[0]) * hkv + static_cast<int64_t>(kv) * pages;
   auto compute = [&](int g, const v4i (&x)[4]) {
     v4i sum = {0, 0, 0, 0};
     sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[0], below[0], sum, 0, 0, 0);
@@ -248,13 +248,14 @@ __global__ __launch_bounds__(kPickThreads) void pick_pages_kernel(SelectArgs a) 
   __shared__ float found_score;
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
   const int kv = blockIdx.x, request = blockIdx.y;
-  const int pages = a.indptr[request + 1] - a.indptr[request];
+  const int begin = a.indptr[request], pages = a.indptr[request + 1] - begin;
   int32_t* out = a.selected + (static_cast<int64_t>(request) * a.num_kv_heads + kv) * a.take;
   if (pages <= a.take) {
     for (int i = tid; i < a.take; i += kPickThreads) out[i] = i < pages ? i : -1;
     return;
   }
-  const float* scores = a.scores + (static_cast<int64_t>(request) * a.num_kv_heads + kv) * a.max_pages;
+  const float* scores = a.scores + static_cast<int64_t>(begin - a.indptr[0]) * a.num_kv_heads +
+                        static_cast<int64_t>(kv) * pages;
   const float anyway = __uint_as_float(0x7fc00000u);
   auto score_at = [&](int i) { return i < a.first || i >= pages - a.last ? anyway : scores[i]; };
   float held[kHeld > 0 ? kHeld : 1];
@@ -536,7 +537,6 @@ extern "C" int32_t pg_sparse_select(const pg_segment_plan_t* plan, const void* q
   a.indptr = reinterpret_cast<const int32_t*>(ws + plan->indptr_offset);
   a.scores = reinterpret_cast<float*>(ws + plan->scores_offset);
   a.selected = selected;
-  a.max_pages = plan->max_pages;
   a.take = plan->selected_pages;
   a.first = plan->first_pages;
   a.last = plan->last_pages;

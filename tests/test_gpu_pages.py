@@ -173,6 +173,8 @@ def test_compaction(cuda, pages_in_pool):
         for p in used:
             want[remap[p]] = refs[p]
         assert pool.refs.tolist() == want
+        pool.commit_compaction(moves)                              # once more: nothing is left to move
+        assert pool.refs.tolist() == want
 
 
 def test_captured_calls_follow_the_pool(cuda):

@@ -135,6 +135,15 @@ def test_scales_that_differ_from_page_to_page(cuda):
     b.check(*run(planned(b, cuda), b))
 
 
+@pytest.mark.parametrize("requests", [2, 10, 40])
+def test_scales_of_either_sign(cuda, requests):
+    """No writer makes them, but what they stand for is plain: code times scale."""
+    b = Batch(cuda, [(0, requests, 900)], spread(requests, 0, 30), [0] * requests, 1, 4)
+    sign = 1 - 2 * (torch.arange(len(b.scales[0]), device=cuda) % 3 == 1).half()[:, None]
+    b.scales = [b.scales[0] * sign, b.scales[1] * sign.flip(0)]
+    b.check(*run(planned(b, cuda), b))
+
+
 @pytest.mark.parametrize("requests", [1, 3, 10, 30])
 def test_small_values_beside_large_ones_without_weight(cuda, requests):
     """V's scales are of 2^-20, but for one page that no query attends to (its keys are far
