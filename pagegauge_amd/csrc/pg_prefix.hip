@@ -56,8 +56,11 @@ struct SharedTiles {
 // LDS 35 %, and the two waves of a SIMD hide little of one behind the other.  69 GFLOP, 8
 // parts: 91 us over INT8 pages (753 TFLOP/s), 84 over FP16 ones (818; a library product of 8192
 // cubed reaches 1194); 32 query rows per KV head 15 us.  Measured and not taken: the scores of
-// tile j + 1 beside the softmax of tile j (registers spill; 95.7 us), interleaving orders for
-// the scheduler (97 to 104), no wave priority (93.8), tiles of 16 rows throughout (341).
+// tile j + 1 beside the softmax of tile j (one wave's 256 registers just hold it: 102 us),
+// orders of instructions for the scheduler (97 to 104), no wave priority (93.8), priority to
+// one of a CU's workgroups (96), V's scales in the exponents (the same with an eighth fewer
+// vector operations), another swizzle without V's conflicts on the way into LDS (the same),
+// tiles of 16 rows throughout (341).
 template <bool kCodes, int kRowWaves>
 __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, const SegmentItem& it, int kv,
                                                  SharedTiles& lds) {

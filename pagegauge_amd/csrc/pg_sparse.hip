@@ -107,7 +107,8 @@ constexpr int kMostGroups = 8;       // of so many pages, per wave: two page ids
 // Sixteen pages at a time are the rows of v_mfma_i32_16x16x64_i8 and the KV head's query
 // heads its columns; 4 products take the 128 lower bounds and the 128 upper ones.  Page ids
 // and scales are requested once per wave, a group's bounds while the one before is scored.
-// Bound by the reads of bounds: 65536 pages of 8 heads, 134 MB, 26 to 28 us (4.8 to 5.2 TB/s).
+// Bound by the reads of bounds: 65536 pages of 8 heads, 134 MB, 26 to 28 us where the Infinity
+// Cache still has some, 34 where not (3.9 TB/s; the same with a page's heads side by side).
 __global__ __launch_bounds__(kScoreThreads) void page_scores_kernel(SelectArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
