@@ -71,6 +71,9 @@ def copy_pages(planes: Sequence[torch.Tensor], source: torch.Tensor, target: tor
         raise ValueError("page_dim must be 0 or 1")
     if source.shape != target.shape:
         raise ValueError("source and target must have one id per copy")
+    if isinstance(planes, torch.Tensor):
+        raise ValueError("planes must be a sequence of tensors")
+    planes = tuple(planes)
     if not planes:
         raise ValueError("no planes to copy")
     _capi.refuse_gradients(*planes)

@@ -83,6 +83,9 @@ def test_copies_of_nothing(cuda):
     pages.copy_pages([torch.ones(0, 8, device=cuda)], ints([0], cuda), ints([1], cuda))
     pages.copy_pages([torch.ones(4, 0, device=cuda), plane], ints([-1], cuda), ints([1], cuda))
     assert bool((plane == 1).all())
+    plane[2] = 5
+    pages.copy_pages((p for p in (plane,)), ints([2], cuda), ints([0], cuda))      # any iterable
+    assert bool((plane[0] == 5).all())
 
 
 def test_counts(cuda):
@@ -218,7 +221,7 @@ def test_refuses(cuda):
     plane, one = torch.zeros(4, 8, device=cuda), ints([1], cuda)
     for planes, source, target, over, message in (
             ([plane], one.long(), one.long(), {}, "int32"), ([plane], one, ints([1, 2], cuda), {}, "one id per copy"),
-            ([], one, one, {}, "no planes"), ([plane, plane[:3]], one, one, {}, "same number of pages"),
+            ([], one, one, {}, "no planes"), (plane, one, one, {}, "sequence of tensors"), ([plane, plane[:3]], one, one, {}, "same number of pages"),
             ([plane[:, ::2]], one, one, {}, "contiguous"), ([plane[:1].expand(4, 8)], one, one, {}, "overlap"),
             ([plane[None].expand(2, 4, 8)], one, one, dict(page_dim=1), "overlap"),
             ([plane], one, one, dict(page_dim=2), "page_dim"), ([plane.cpu()], one, one, {}, "device"),
