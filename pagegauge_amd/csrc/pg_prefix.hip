@@ -32,7 +32,7 @@ struct SharedTiles {
   int32_t plain[kSegmentWaves];                          // no K scale below 0
 };
 
-// A prefix's pages with 17 query rows and more: kRowWaves waves of 32 query rows share
+// A prefix's pages with more than 32 query rows: kRowWaves waves of 32 query rows share
 // every tile of 64 tokens through LDS, as FP16.
 //
 // A wave keeps its query rows as the B operand of v_mfma_f32_32x32x16_f16 and computes
@@ -55,7 +55,7 @@ struct SharedTiles {
 // rows per KV head) over 16384 tokens MFMA takes 32 %, the VALU 49 % (35 % over FP16 pages),
 // LDS 35 %, and the two waves of a SIMD hide little of one behind the other.  69 GFLOP, 8
 // parts: 91 us over INT8 pages (753 TFLOP/s), 84 over FP16 ones (818; a library product of 8192
-// cubed reaches 1194); 32 query rows per KV head 15 us.  Measured and not taken: the scores of
+// cubed reaches 1194); 48 query rows per KV head 19 us.  Measured and not taken: the scores of
 // tile j + 1 beside the softmax of tile j (one wave's 256 registers just hold it: 102 us),
 // orders of instructions for the scheduler (97 to 104), no wave priority (93.8), priority to
 // one of a CU's workgroups (96), V's scales in the exponents (the same with an eighth fewer

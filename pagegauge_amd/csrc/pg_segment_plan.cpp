@@ -18,7 +18,11 @@ constexpr int64_t kSmallestShare = 64;
 struct Unit {
   int32_t segment, request;               // segment -1: the request's own pages
   int64_t rows, pages, tail, tail_weight;
-  bool shared() const { return rows > kSegmentRows; }
+  // Two blocks of 16 rows that read the pages each are still the faster, mostly (8 requests of 4
+  // heads on 16384 tokens, with the join: INT8 19.7 and 21.7 us, FP16 20.4 and 23.7; on 60000
+  // 41.8 and 39.0, 47.3 and 51.0); of three the tiles are (12 requests on 16384: 25.5 and 24.9;
+  // on 60000 55.3 and 41.7).
+  bool shared() const { return rows > 2 * kSegmentRows; }
   // rows of one workgroup, and the partial rows that it makes of each
   int64_t block_rows() const {
     if (!shared()) return rows > kNarrowRows ? kSegmentRows : kNarrowRows;
