@@ -35,6 +35,8 @@
 #include "pg_combine.h"
 #include "pg_segment_plan.h"
 
+#include <cstring>
+
 namespace pg {
 namespace {
 
@@ -710,14 +712,16 @@ inline int32_t plan_into(const SegmentBatch& batch, void* workspace, int64_t wor
     if (p.workspace_bytes > workspace_bytes)
       return fail(PG_ERROR_WORKSPACE, "decode workspace too small: need " + std::to_string(p.workspace_bytes) +
                                           " bytes, have " + std::to_string(workspace_bytes));
-    uint8_t* ws = static_cast<uint8_t*>(workspace);
-    auto copy = [&](int64_t offset, const void* from, size_t bytes) {
-      return !bytes || hipMemcpyAsync(ws + offset, from, bytes, hipMemcpyHostToDevice, stream) == hipSuccess;
+    // the tables lie in front of the workspace, one after the other: one copy
+    std::vector<uint8_t> tables(p.scores_offset);
+    auto put = [&](int64_t offset, const void* from, size_t bytes) {
+      if (bytes) std::memcpy(tables.data() + offset, from, bytes);
     };
-    if (!copy(p.items_offset, work.items.data(), work.items.size() * sizeof(SegmentItem)) ||
-        !copy(p.slot_ptr_offset, work.slot_ptr.data(), work.slot_ptr.size() * sizeof(int32_t)) ||
-        !copy(p.slot_base_offset, work.slot_base.data(), work.slot_base.size() * sizeof(int32_t)) ||
-        !copy(p.indptr_offset, batch.indptr, batch.selected > 0 ? work.slot_ptr.size() * sizeof(int32_t) : 0) ||
+    put(p.items_offset, work.items.data(), work.items.size() * sizeof(SegmentItem));
+    put(p.slot_ptr_offset, work.slot_ptr.data(), work.slot_ptr.size() * sizeof(int32_t));
+    put(p.slot_base_offset, work.slot_base.data(), work.slot_base.size() * sizeof(int32_t));
+    put(p.indptr_offset, batch.indptr, batch.selected > 0 ? work.slot_ptr.size() * sizeof(int32_t) : 0);
+    if (hipMemcpyAsync(workspace, tables.data(), tables.size(), hipMemcpyHostToDevice, stream) != hipSuccess ||
         hipStreamSynchronize(stream) != hipSuccess)
       return fail(PG_ERROR_LAUNCH, "plan copy failed");
     *plan = p;
