@@ -71,6 +71,39 @@ def test_large_groups_and_long_prefixes(cuda, kind):
     b.check(out, lse, requests=[0, 1, 19, 20, 21, 77, 146, 147, 149])
 
 
+@pytest.mark.parametrize("longest,few", [(1000, True), (4000, False)])
+@both_kinds
+def test_many_requests(cuda, kind, longest, few):
+    """More than 1024 (request, head) pairs, some without a join: with up to 16 partial rows
+    joined a wave each, with more as few requests are."""
+    own = spread(300, 0, 40)
+    own[7], own[290] = longest, 0
+    b = Batch(cuda, [(0, 280, 300), (100, 103, 77), (200, 260, 1200)], own, spread(300, 0, 18), 1, 4, kind)
+    decode = planned(b, cuda)
+    assert (decode._plan.max_slots <= 16) == few
+    out, lse = run(decode, b)
+    b.check(out, lse)
+    again = run(decode, b, value_center=None)
+    b.check(*again, center=False, requests=[0, 7, 101, 279, 280, 299])
+
+
+def test_two_objects_on_two_streams(cuda):
+    """Each with its own workspace, at the same time."""
+    batches = [Batch(cuda, [(0, 40, 3000)], spread(40, 0, 200), spread(40, 0, 30), 2, 4, seed=s) for s in (1, 2)]
+    decodes = [planned(b, cuda) for b in batches]
+    want = [run(d, b) for d, b in zip(decodes, batches)]
+    streams = [torch.cuda.Stream() for _ in batches]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (d, b) in enumerate(zip(decodes, batches)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(d, b))
+    torch.cuda.synchronize()
+    for results, (out, lse) in zip(got, want):
+        assert all(torch.equal(o, out) and torch.equal(l, lse) for o, l in results)
+
+
 @both_kinds
 def test_requests_without_any_prefix(cuda, kind):
     b = Batch(cuda, [], [5000, 0, 33], [100, 0, 16], 2, 4, kind)

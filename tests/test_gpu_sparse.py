@@ -116,16 +116,21 @@ def test_choice_of_many(cuda, pages):
     assert np.array_equal(got.cpu().numpy(), expected_selection(b, bounds, pages, first, 1))
 
 
-def test_choice_among_a_hundred_thousand_pages(cuda):
-    """Bounds alone: a long context, with equal scores throughout."""
+@pytest.mark.parametrize("pages", [2047, 5003, 20_011, 100_003])
+@pytest.mark.parametrize("alike", [True, False])
+def test_choice_among_many_pages(cuda, pages, alike):
+    """Bounds alone, of long contexts, with equal scores throughout or hardly any."""
     from pagegauge_amd import sparse
 
+    print(f"choice among {pages} {alike}", flush=True)
     gen = torch.Generator().manual_seed(9)
-    pages = 100_003
     bounds = torch.randint(-2, 3, (pages, 1, 2, 128), generator=gen).to(torch.int8).to(cuda)
     bounds[:, :, 1] += 4
-    bounds[:, :, :, 4:] = 0
+    if alike:
+        bounds[:, :, :, 4:] = 0
     scale = torch.ones(pages, 1, dtype=torch.float16, device=cuda)
+    if not alike:
+        scale = (torch.rand(pages, 1, generator=gen) + 0.5).half().to(cuda)
     q = torch.zeros(1, 2, 128, dtype=torch.float16, device=cuda)
     q[0, 0, :4], q[0, 1, 1:3] = 1.0, -0.5
     ids = torch.randperm(pages, generator=gen).int().to(cuda)
@@ -133,9 +138,9 @@ def test_choice_among_a_hundred_thousand_pages(cuda):
     decode.plan([0, pages], ids, torch.tensor([16], dtype=torch.int32, device=cuda), pages=777, num_qo_heads=2,
                 num_kv_heads=1)
     got = decode.select(q, bounds, scale).cpu().numpy()
-    s = expected_scores(q[0], bounds[ids.long()], scale, 2)
+    s = expected_scores(q[0], bounds[ids.long()], scale[ids.long()], 2)
     s[0, 0] = s[0, -1] = np.inf
-    assert len(np.unique(s)) < 60
+    assert (len(np.unique(s)) < 60) == alike
     assert np.array_equal(got[0, 0], sorted(np.argsort(-s[0], kind="stable")[:777]))
 
 
@@ -172,6 +177,19 @@ def test_attention_over_the_choice(cuda, kv_heads, group, pages):
     out, lse = run(without, b, selected, exact_cache=None, value_center=None)
     b.tail_ptr.zero_()
     b.check(out, lse, selected=selected.cpu().numpy(), center=False, single_part=False)
+
+
+def test_many_requests(cuda):
+    """More than 1024 (request, head) pairs, ragged, some without a page."""
+    gen = torch.Generator().manual_seed(4)
+    own = torch.randint(0, 900, (150,), generator=gen).tolist()
+    own[3] = own[149] = 0
+    b = Batch(cuda, [], own, torch.randint(0, 40, (150,), generator=gen).tolist(), 2, 4)
+    bounds = bounds_of(b, cuda)
+    decode = planned(b, cuda, 20, 2, 1)
+    selected = decode.select(b.q, bounds, b.scales[0])
+    assert np.array_equal(selected.cpu().numpy(), expected_selection(b, bounds, 20, 2, 1))
+    b.check(*run(decode, b, selected), selected=selected.cpu().numpy(), single_part=False)
 
 
 def test_attention_over_a_callers_choice(cuda):
