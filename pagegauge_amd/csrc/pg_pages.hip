@@ -188,7 +188,8 @@ __global__ __launch_bounds__(kScanThreads) void take_kernel(int32_t* refs, int32
 // at or past ``live`` that is in use goes to the i-th lowest free one below it, the
 // fewest moves there are.  No page is both a source and a target.  Bound by the trips of one
 // workgroup: 16384 pages 9.8 us, 1021 pages 5.8 (with a scan for each list and entries of remap
-// stored one by one 14.4 and 7.2).
+// stored one by one 14.4 and 7.2; over masks of 64 neighbouring pages, more than the scalar
+// registers hold, 18.2 and 9.8 to 12.2).
 __global__ __launch_bounds__(kScanThreads) void stage_kernel(const int32_t* refs, int32_t pages, int32_t* source,
                                                              int32_t* target, int32_t* remap, int32_t* live_out) {
   __shared__ int wave_sums[kScanThreads / kWave];
