@@ -189,6 +189,9 @@ int32_t build_segment_plan(const SegmentBatch& b, SegmentWork& work, pg_segment_
       exact = exact_end;
     }
   }
+  // The longest first, which also puts the shared tiles of a full batch one to a CU and own
+  // pages beside them: a CU of an XCD gets every 32nd workgroup (taken in turns, two shared ones
+  // met on a CU and the batch above took 254 us instead of 200 on the same card).
   auto weight_of = [&](const SegmentItem& it) {
     return it.page_end - it.page_begin + tail_weight * (it.tail_end - it.tail_begin);
   };
