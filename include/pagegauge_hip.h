@@ -904,7 +904,8 @@ int32_t pg_prefix_run(const pg_segment_plan_t* plan, const void* query, int64_t 
 
 /* bounds int8 [pool_pages, Hkv, 2, 128]: the least and the largest code of each channel
  * of pages page_ids[i], i < count (NULL: page i), over their first lengths[i] tokens
- * (NULL: 16; 127 and -128 where that is 0).  Ids outside the pool are skipped. */
+ * (NULL: 16; 127 and -128 where that is 0).  Ids outside the pool are skipped, the
+ * others must differ from each other. */
 int32_t pg_sparse_key_bounds(const void* key_codes, void* bounds, int64_t pool_pages,
                              const int32_t* page_ids, const int32_t* lengths, int64_t count,
                              int32_t kv_heads, void* stream);

@@ -41,7 +41,7 @@ def key_bounds(key_codes: torch.Tensor, bounds: torch.Tensor, *, page_ids: Optio
     of ``key_codes`` int8 [pages, 16, Hkv, 128] into ``bounds`` [pages, Hkv, 2, 128].
     ``lengths`` (device int32 [n]) is the tokens that each page holds, 16 if not given;
     a page without tokens gets 127 and -128, the lowest of all scores.  Ids outside the
-    pool (-1) are skipped."""
+    pool (-1) are skipped; the others must differ from each other."""
     if key_codes.dim() != 4 or key_codes.shape[2] == 0:
         raise ValueError("key_codes must be contiguous int8 [pages,16,Hkv,128]")
     pages, _, heads, _ = key_codes.shape
