@@ -76,7 +76,11 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
   const int count = it.page_end - it.page_begin;
   const int tiles = (count + kTilePages - 1) / kTilePages;
 
-  // the item's pages; missing ones of the last tile repeat its last page, masked below
+  // tokens of the item that are visible: all but those past the prefix's last one
+  const int last_len = it.page_end - 1 == it.last_page ? max(min(a.prefix_last[it.segment], kPageSize), 0) : kPageSize;
+  const int visible = (count - 1) * kPageSize + last_len;
+  // the item's pages; missing ones of the last tile repeat its last page, masked below, and a
+  // page without a visible token counts with scales of 0, whatever its own are
   {
     const int32_t* table = a.prefix_indices + it.page_begin;
     float largest = 0.0f;
@@ -86,8 +90,9 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
       lds.ids[i] = id;
       if (kCodes) {
         const int64_t at = static_cast<int64_t>(id) * hkv + kv;
-        const float v = i < count ? half_bits_to_float(a.value_scale[at]) : 0.0f;
-        const float k = half_bits_to_float(a.key_scale[at]) * a.sm_scale_log2;
+        const bool seen = i * kPageSize < visible;
+        const float v = seen ? half_bits_to_float(a.value_scale[at]) : 0.0f;
+        const float k = seen ? half_bits_to_float(a.key_scale[at]) * a.sm_scale_log2 : 0.0f;
         plain &= k >= 0.0f;
         lds.k_scale[i] = k;
         lds.v_scale[i] = v;
@@ -109,9 +114,6 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
 #pragma unroll
     for (int k = 0; k < 8; ++k) qf[k] = *reinterpret_cast<const v8h*>(qp + 16 * k);
   }
-  // tokens of the item that are visible: all but those past the prefix's last one
-  const int last_len = it.page_end - 1 == it.last_page ? max(min(a.prefix_last[it.segment], kPageSize), 0) : kPageSize;
-  const int visible = (count - 1) * kPageSize + last_len;
   __syncthreads();
   float v_unit = 1.0f, v_back = 1.0f;                    // 2^-e and 2^e of V's scales
   bool plain = true;
