@@ -824,7 +824,9 @@ int32_t pg_pool_stage_compaction(const int32_t* refs, int64_t pages, int32_t* so
 int32_t pg_pool_commit_compaction(int32_t* refs, int64_t pages, const int32_t* source,
                                   const int32_t* target, int64_t moves, void* stream);
 
-/* out[i] = remap[ids[i]], i < count; ids outside [0, pages) stay.  out may be ids. */
+/* out[i] = remap[ids[i]], i < count; ids outside [0, pages) stay.  out may be ids.
+ * Ids of free pages become -1, which pg_prefix_run, pg_sparse_select and pg_sparse_run
+ * leave out of a table and other attention calls do not take. */
 int32_t pg_rewrite_ids(const int32_t* ids, const int32_t* remap, int64_t pages, int64_t count,
                        int32_t* out, void* stream);
 
@@ -890,9 +892,10 @@ int32_t pg_segment_plan_host(const int32_t* host_prefix_requests, const int32_t*
  * NULL).  key and value: pages [*, 16, Hkv, 128], with PG_KV_INT8 codes whose scales are
  * key_scale and value_scale [*, Hkv].  The last page of a prefix holds prefix_last_len[s]
  * tokens, of a request's own ones last_page_len[b], of the tail tail_last_len[b], all
- * read on the device.  The keys that a request sees must be centered alike.  out fp16
- * [B, Hq, 128]; lse float32 [B, Hq] base 2, or NULL.  A request without tokens gives its
- * center and an lse of -inf.  Runs that share a workspace must not overlap. */
+ * read on the device.  Page ids below 0 are no pages and are left out.  The keys that a
+ * request sees must be centered alike.  out fp16 [B, Hq, 128]; lse float32 [B, Hq] base 2,
+ * or NULL.  A request without tokens gives its center and an lse of -inf.  Runs that share
+ * a workspace must not overlap. */
 int32_t pg_prefix_run(const pg_segment_plan_t* plan, const void* query, int64_t query_batch_stride,
                       const void* key, const void* value, const void* key_scale,
                       const void* value_scale, const int32_t* prefix_indices,
@@ -923,9 +926,9 @@ int32_t pg_sparse_plan(const int32_t* host_indptr, const int32_t* host_tail_indp
  * a page scores
  *   max over the KV head's query heads of
  *     f32(sum_d max(q'_d lo_d, q'_d hi_d) * key_scale) * 2^(x - 7),
- * -inf for a row with an infinity or NaN and where the score is NaN.  Taken are the
- * first and last pages, and of the others those with the highest scores, among
- * equal ones the lowest positions. */
+ * -inf for a row with an infinity or NaN, where the score is NaN, and for a page id below
+ * 0.  Taken are the first and last pages, and of the others those with the highest
+ * scores, among equal ones the lowest positions. */
 int32_t pg_sparse_select(const pg_segment_plan_t* plan, const void* query, int64_t query_batch_stride,
                          const void* bounds, const void* key_scale, const int32_t* indices,
                          int32_t* selected, void* workspace, void* stream);

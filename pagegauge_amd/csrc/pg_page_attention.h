@@ -363,7 +363,9 @@ __device__ __forceinline__ void page_attention(const PageAttentionArgs& a, const
       my_page = (it.segment >= 0 ? a.prefix_indices : a.indices)[listed];
       my_visible = listed == it.last_page ? last_len : kPageSize;
     }
-    if (at >= count) my_visible = 0;
+    // an entry below 0 is no page: the pool's first one is read in its place, and weighs nothing
+    if (at >= count || my_page < 0) my_visible = 0;
+    my_page = max(my_page, 0);
     if constexpr (!kCodes) {
       exponent = st.offset = kExactExponent;
       exact_pages<kWide>(st, q, static_cast<const uint16_t*>(a.key), static_cast<const uint16_t*>(a.value), count,
@@ -483,8 +485,8 @@ __device__ __forceinline__ void page_attention(const PageAttentionArgs& a, const
     const int listed = it.tail_begin + min(at, tail_count - 1);
     const int my_page = a.tail_indices[listed];
     int my_visible = listed == it.last_tail ? min(a.tail_last[it.request], kPageSize) : kPageSize;
-    if (at >= tail_count) my_visible = 0;
-    exact_pages<kWide>(st, q, a.tail_k, a.tail_v, tail_count, my_page, my_visible, kv, hkv, a.sm_scale_log2,
+    if (at >= tail_count || my_page < 0) my_visible = 0;
+    exact_pages<kWide>(st, q, a.tail_k, a.tail_v, tail_count, max(my_page, 0), my_visible, kv, hkv, a.sm_scale_log2,
                        low_part, wave, lane);
   }
 

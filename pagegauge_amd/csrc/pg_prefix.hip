@@ -25,11 +25,11 @@ constexpr float kLowest = -__FLT_MAX__;
 // LDS of a workgroup over shared rows: K0 K1 V0 V1, and the item's pages.
 struct SharedTiles {
   uint8_t tiles[4 * kTileBytes];
-  int32_t ids[kSharedMaxPages];
+  int32_t ids[kSharedMaxPages];                          // below 0: no page, the pool's first one is read
   float k_scale[kSharedMaxPages];
   float v_scale[kSharedMaxPages];
   float largest[kSegmentWaves];
-  int32_t plain[kSegmentWaves];                          // no K scale below 0
+  int32_t plain[kSegmentWaves];                          // no K scale below 0, no id either
 };
 
 // A prefix's pages with more than 32 query rows: kRowWaves waves of 32 query rows share
@@ -88,9 +88,10 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
     for (int i = threadIdx.x; i < tiles * kTilePages; i += kAttentionThreads) {
       const int32_t id = table[min(i, count - 1)];
       lds.ids[i] = id;
+      plain &= id >= 0;
       if (kCodes) {
-        const int64_t at = static_cast<int64_t>(id) * hkv + kv;
-        const bool seen = i * kPageSize < visible;
+        const int64_t at = static_cast<int64_t>(max(id, 0)) * hkv + kv;
+        const bool seen = i * kPageSize < visible && id >= 0;
         const float v = seen ? half_bits_to_float(a.value_scale[at]) : 0.0f;
         const float k = seen ? half_bits_to_float(a.key_scale[at]) * a.sm_scale_log2 : 0.0f;
         plain &= k >= 0.0f;
@@ -102,9 +103,9 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
     if (kCodes) {
       largest = wave_max(largest);
       if (lane == 0) lds.largest[wave] = largest;
-      const bool all = !__builtin_amdgcn_ballot_w64(!plain);
-      if (lane == 0) lds.plain[wave] = all;
     }
+    const bool all = !__builtin_amdgcn_ballot_w64(!plain);
+    if (lane == 0) lds.plain[wave] = all;
   }
   const int row = it.row_first + min(row_wave + column, it.rows - 1);
   const int in_segment = row / a.group, head = kv * a.group + row % a.group;
@@ -116,9 +117,8 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
   }
   __syncthreads();
   float v_unit = 1.0f, v_back = 1.0f;                    // 2^-e and 2^e of V's scales
-  bool plain = true;
+  const bool plain = __builtin_amdgcn_readfirstlane(lds.plain[0] & lds.plain[1] & lds.plain[2] & lds.plain[3]);
   if (kCodes) {
-    plain = __builtin_amdgcn_readfirstlane(lds.plain[0] & lds.plain[1] & lds.plain[2] & lds.plain[3]);
     float largest = lds.largest[0];
 #pragma unroll
     for (int w = 1; w < kSegmentWaves; ++w) largest = fmaxf(largest, lds.largest[w]);
@@ -144,7 +144,7 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
   auto load = [&](const uint8_t* bytes, int tile, v4u (&r)[kLoads]) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int id = __builtin_amdgcn_readfirstlane(lds.ids[page_at(tile, i)]);
+      const int id = __builtin_amdgcn_readfirstlane(max(lds.ids[page_at(tile, i)], 0));
       r[i] = *reinterpret_cast<const v4u*>(bytes + id * page_bytes + from);
     }
   };
@@ -170,10 +170,11 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
   auto load_v = [&](int tile) { load(v_bytes, tile, vr); };
   auto store_k = [&](int buffer) { store(lds.tiles + buffer * kTileBytes, kr, 15, 1); };
   auto store_v = [&](int tile, int buffer) {
-    if (!kCodes && tile == tiles - 1) {                  // rows not written may hold anything
+    if (!kCodes && (tile == tiles - 1 || !plain)) {      // rows not written may hold anything
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
-        if (kTileTokens * tile + my_row + 16 * i >= visible) vr[i] = v4u{0u, 0u, 0u, 0u};
+        if (kTileTokens * tile + my_row + 16 * i >= visible || lds.ids[page_at(tile, i)] < 0)
+          vr[i] = v4u{0u, 0u, 0u, 0u};
     }
     store(lds.tiles + (2 + buffer) * kTileBytes, vr, 3, 4);
   };
@@ -281,7 +282,7 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
     load_k(next);
     load_v(next);
   };
-  // tiles without a masked token
+  // tiles without a masked token or a missing page
   auto body = [&](int j, int buffer) {
     __syncthreads();
     float kf[kSteps], vf[kSteps];
@@ -302,12 +303,15 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
     float kf[kSteps], vf[kSteps];
     factors(j, kf, vf);
     qk(buffer, s);
+    int end[kSteps];                                     // of what is visible, for the wave's pages
+#pragma unroll
+    for (int p = 0; p < kSteps; ++p) end[p] = lds.ids[kTilePages * j + 2 * part + p] < 0 ? 0 : visible;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int token = kTileTokens * j + 32 * (part + b) + 8 * (r / 4) + 4 * half + r % 4;
-        s[b][r] = token < visible ? s[b][r] * kf[2 * b + r / 8] : kNoScore;
+        s[b][r] = token < end[2 * b + r / 8] ? s[b][r] * kf[2 * b + r / 8] : kNoScore;
       }
 #pragma unroll
     for (int p = 0; p < kSteps; ++p) kf[p] = 1.0f;
@@ -324,7 +328,8 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
     load_k(1);
     load_v(1);
   }
-  // the largest score of a page is that of its largest product, unless a scale is negative
+  // the largest score of a page is that of its largest product, unless a scale is negative;
+  // with a missing page every tile is looked at
   int j = 0;
   if (plain)
     for (; j + 1 < tiles; ++j) body(j, j & 1);

@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kScoreThreads) void page_scores_kernel(SelectArgs a
 
   const uint8_t* bounds = a.bounds + kv * 2 * kHeadDim + 16 * kg;
   auto load = [&](int g, v4i (&x)[4]) {
-    const int64_t page = __shfl(g < 4 ? ids[0] : ids[1], kScorePages * (g & 3) + n, kWave);
+    const int64_t page = max(__shfl(g < 4 ? ids[0] : ids[1], kScorePages * (g & 3) + n, kWave), 0);
     const uint8_t* from = bounds + page * hkv * 2 * kHeadDim;
 #pragma unroll
     for (int w = 0; w < 4; ++w) x[w] = *reinterpret_cast<const v4i*>(from + 64 * w);
@@ -200,7 +200,11 @@ __global__ __launch_bounds__(kScoreThreads) void page_scores_kernel(SelectArgs a
   v4i x[2][4];
   load(0, x[0]);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) scales[i] = half_bits_to_float(a.key_scale[static_cast<int64_t>(ids[i]) * hkv + kv]);
+  for (int i = 0; i < 2; ++i) {
+    // an entry below 0 is no page and has no score: the pool's first one is read in its place
+    const float scale = half_bits_to_float(a.key_scale[static_cast<int64_t>(max(ids[i], 0)) * hkv + kv]);
+    scales[i] = ids[i] < 0 ? __uint_as_float(0x7fc00000u) : scale;
+  }
   for (int g = 0; g < groups; g += 2) {
     if (g + 1 < groups) load(g + 1, x[1]);
     compute(g, x[0]);

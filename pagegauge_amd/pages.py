@@ -99,7 +99,10 @@ def copy_pages(planes: Sequence[torch.Tensor], source: torch.Tensor, target: tor
 
 def rewrite_ids(ids: torch.Tensor, remap: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``remap[ids[i]]`` for a table of page ids (device int32, any shape); ids outside
-    ``remap`` stay as they are.  ``out`` may be ``ids``."""
+    ``remap`` stay as they are.  ``out`` may be ``ids``.  The entry of a page without
+    users becomes -1: calls of ``prefix`` and ``sparse`` planned over the table leave it
+    out, those of ``decode`` and ``int4`` take ids of the pool alone, so a request that
+    has ended leaves their tables first."""
     device = ids.get_device()
     what = "ids and out must be contiguous int32, shaped alike"
     ids_at = _capi.pointer(ids, torch.int32, ids.shape, device, what)

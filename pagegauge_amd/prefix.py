@@ -213,8 +213,10 @@ class SharedPrefixDecode(_SegmentDecode):
         the prefixes, of the requests' own pages and, with ``tail_indptr``, of the
         exact pages; any of them may be empty, of a request or as a whole.
         ``indices`` and the last lengths (device int32) must stay alive until the next
-        ``plan`` and are re-read by every run (lengths within [0, 16] may move), so a
-        captured run stays valid until the next ``plan``.  Waits for the GPU."""
+        ``plan`` and are re-read by every run, so a captured run stays valid until the
+        next ``plan``.  Lengths may move within [0, 16], and ids may be rewritten in
+        place within the pool; an entry below 0 is no page and is left out.  Waits for
+        the GPU."""
         if kv_data_type not in _KINDS:
             raise ValueError("pages must be int8 or float16")
         ranges = _prefix_ranges(prefix_requests)

@@ -73,8 +73,9 @@ class SelectedPagesDecode(_SegmentDecode):
         KV head, all of a request that has no more; the first ``first_pages`` and last
         ``last_pages`` of the table are always among them.  ``indices`` and the last
         lengths (device int32) must stay alive until the next ``plan`` and are re-read
-        by every call (lengths within [0, 16] may move), so captured calls stay valid
-        until the next ``plan``.  Waits for the GPU."""
+        by every call, so captured calls stay valid until the next ``plan``.  Lengths may
+        move within [0, 16], and ids may be rewritten in place within the pool; an entry
+        below 0 is no page, has no score and is left out.  Waits for the GPU."""
         if pages <= 0:
             raise ValueError("at least one page must be selected")
         if first_pages < 0 or last_pages < 0 or first_pages + last_pages > pages:

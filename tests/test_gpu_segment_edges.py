@@ -1,16 +1,19 @@
 """Attention over shared prefixes and selected pages where a call is allowed and rare:
-pages without a token left (tolerances: segment_helpers).
+pages without a token left, tables that lose pages after the plan (tolerances:
+segment_helpers).
 
 A prefix of up to 32 query rows per KV head takes the form without tiles, of up to 64 the
 one with tiles of two waves' rows, of more the one of four."""
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
-from segment_helpers import Batch
-from test_gpu_prefix import planned, run, spread
+import test_gpu_sparse as selecting
+from segment_helpers import Batch, check_head, values
+from test_gpu_prefix import both_kinds, planned, run, spread
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +37,108 @@ def test_a_page_without_tokens_weighs_nothing(cuda, requests, left):
         scale[pages] = left
     got, got_lse = run(decode, b)
     assert torch.equal(got, out) and torch.equal(got_lse, lse)
+
+
+def cleared(ids, every, first):
+    """Ids with some entries below 0."""
+    ids = ids.clone()
+    ids[first::every] = -1
+    ids[first + every::3 * every] = -2 ** 31
+    return ids
+
+
+def with_a_spoiled_first_page(b):
+    """The pools with a page in front that no table names, and holds what must not count."""
+    for pools in (b.cache, b.exact):
+        for i in range(2):
+            bad = torch.full_like(pools[i][:1], 77 if pools[i].dtype is torch.int8 else float("nan"))
+            pools[i] = torch.cat((bad, pools[i]))
+    if b.kind is torch.int8:
+        b.scales = [torch.cat((torch.full_like(s[:1], float("nan")), s)) for s in b.scales]
+    for ids in (b.prefix_ids, b.ids, b.tail_ids):
+        ids += 1
+
+
+def seen_of(b, selected=None):
+    """``f(b, h)``: float64 K and V [T, 128] that KV head h of request b sees, without the
+    entries below 0."""
+    pools = [values(c, s) for c, s in zip(b.cache, b.scales)]
+    exact = [values(c, None) for c in b.exact]
+
+    def rows(pools, ptr, ids, last, i, h, positions=None):
+        table, n = ids[int(ptr[i]):int(ptr[i + 1])].tolist(), int(last[i])
+        return [[p[page, :n if at == len(table) - 1 else 16, h] for p in pools] for at, page in enumerate(table)
+                if page >= 0 and (positions is None or at in positions)]
+
+    def seen(r, h):
+        found = []
+        for i, (first, end, _) in enumerate(b.segments):
+            if first <= r < end:
+                found += rows(pools, b.prefix_ptr, b.prefix_ids, b.prefix_last, i, h)
+        found += rows(pools, b.own_ptr, b.ids, b.last, r, h, None if selected is None else selected[r, h].tolist())
+        found += rows(exact, b.tail_ptr, b.tail_ids, b.tail_last, r, h)
+        return [np.concatenate([x[i] for x in found] + [np.zeros((0, 128))]) for i in range(2)]
+
+    return seen
+
+
+def check(b, out, lse, seen, single_part=True):
+    for r in range(b.batch):
+        for h in range(b.hkv):
+            rows = slice(h * b.group, (h + 1) * b.group)
+            check_head(out[r, rows].double().cpu().numpy(), lse[r, rows].double().cpu().numpy(),
+                       b.q[r, rows].cpu().numpy(), *seen(r, h), b.center[r, h].cpu().numpy(), 128 ** -0.5, single_part)
+
+
+@both_kinds
+@pytest.mark.parametrize("requests", FORMS)
+def test_entries_below_0_are_no_pages(cuda, requests, kind):
+    """Rewritten in place after the plan: some, all of a tile, the last ones, all."""
+    print(f"no pages {requests} {kind}", flush=True)
+    b = Batch(cuda, [(0, requests, 3005), (1, requests, 90)], spread(requests, 1, 300), spread(requests, 0, 60), 2, 4,
+              kind)
+    with_a_spoiled_first_page(b)
+    decode = planned(b, cuda)
+    whole = [t.clone() for t in (b.prefix_ids, b.ids, b.tail_ids)]
+    last = b.prefix_ids.clone()
+    last[int(b.prefix_ptr[1]) - 1] = last[-1] = -1
+    tile = b.prefix_ids.clone()
+    tile[16:25] = -1
+    for prefix_ids, ids, tail_ids in ((cleared(whole[0], 7, 2), cleared(whole[1], 3, 1), cleared(whole[2], 2, 0)),
+                                      (tile, whole[1], whole[2]), (last, cleared(whole[1], 1, 0), whole[2]),
+                                      [torch.full_like(t, -1) for t in whole]):
+        for at, new in zip((b.prefix_ids, b.ids, b.tail_ids), (prefix_ids, ids, tail_ids)):
+            at.copy_(new)
+        out, lse = run(decode, b)
+        check(b, out, lse, seen_of(b))
+    assert bool((lse == -torch.inf).all())
+    again = planned(b, cuda)                                 # and planned with such entries
+    assert torch.equal(run(again, b)[0], out)
+
+
+@pytest.mark.parametrize("group", [4, 16])
+@pytest.mark.parametrize("pages", [9, 200])
+def test_selections_leave_out_entries_below_0(cuda, pages, group):
+    print(f"selected no pages {pages} {group}", flush=True)
+    b = Batch(cuda, [], [3000, 100, 1, 1601], [40, 0, 16, 3], 2, group)
+    with_a_spoiled_first_page(b)
+    bounds = selecting.bounds_of(b, cuda)
+    bounds[0, :, 0], bounds[0, :, 1] = -128, 127
+    decode = selecting.planned(b, cuda, pages, 1, 1)
+    for every, first in ((5, 3), (1, 0)):
+        b.ids.copy_(cleared(b.ids, every, first))
+        b.ids[int(b.own_ptr[1]) - 1] = -1                    # a forced one among them
+        selected = decode.select(b.q, bounds, b.scales[0])
+        want = np.full((4, 2, pages), -1)
+        for r in range(4):
+            at = b.ids[int(b.own_ptr[r]):int(b.own_ptr[r + 1])]
+            s = selecting.expected_scores(b.q[r], bounds[at.clamp(min=0).long()], b.scales[0][at.clamp(min=0).long()],
+                                          group)
+            s[:, at.cpu().numpy() < 0] = -np.inf
+            s[:, 0] = s[:, -1] = np.inf
+            for h in range(2):
+                best = sorted(np.argsort(-s[h], kind="stable")[:pages])
+                want[r, h, :len(best)] = best
+        assert np.array_equal(selected.cpu().numpy(), want)
+        out, lse = selecting.run(decode, b, selected)
+        check(b, out, lse, seen_of(b, selected.cpu().numpy()), single_part=False)
