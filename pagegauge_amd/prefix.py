@@ -14,7 +14,9 @@ and KV head) or FP16 (``decode.BatchDecodeWithPagedKVCacheWrapper``'s), with 1 t
 requests keep the key center of the prompt that they share (forks do).  The value
 center is one too: codes of shared values hold what that center left.
 
-Everything runs on the current stream and nothing but ``plan`` synchronises.
+Everything runs on the current stream and nothing but ``plan`` synchronises.  (Where page
+ids are checked, as ``decode.CHECK_PAGE_IDS`` says, a call with fewer pages than the ids
+asked for when last looked at looks again, which does too.)
 """
 
 from __future__ import annotations
@@ -52,14 +54,41 @@ def _check_last(indptr: torch.Tensor, last: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what} must lie in [1, {PAGE}]")
 
 
+class _PageIds:
+    """The page ids of a planned table, and (where ``decode.CHECK_PAGE_IDS`` is set) between
+    which they lay when last looked at."""
+
+    def __init__(self, indices: torch.Tensor, host_indptr: torch.Tensor) -> None:
+        self._indices, self._indptr = indices, host_indptr
+        self._empty = int(host_indptr[0]) == int(host_indptr[-1])
+        self._look()
+
+    def _look(self) -> None:
+        found = _page_id_range(self._indices, self._indptr)
+        self._range = None if found is None else tuple(max(i, 0) for i in found)
+
+    def check(self, pool_pages: int, what: str) -> None:
+        """All ids are of a pool of so many pages.  Tables may be rewritten in place after the
+        plan: one whose ids were too large is looked at again before it is refused, which waits
+        for the GPU and so is left out while a graph is captured."""
+        # in the place of an entry below 0, which is no page, the first one is read
+        if pool_pages == 0 and not self._empty:
+            raise ValueError(f"{what} page tables with entries, but the pool holds no pages")
+        if self._range is None or self._range[1] < pool_pages:
+            return
+        if not (self._indices.is_cuda and torch.cuda.is_current_stream_capturing()):
+            self._look()
+        _check_page_ids(self._range, pool_pages, what)
+
+
 def _tables(indptr, indices, last, what: str = ""):
-    """Host indptr of a checked CSR page table, and the range of its page ids."""
+    """Host indptr of a checked CSR page table, and its page ids."""
     name = f"{what}_" if what else ""
     _check_index(indices, f"{name}indices")
     _check_index(last, f"{name}last_page_len")
     host, host_last = _host_tables(indptr, last, indices, what)
     _check_last(host, host_last, f"{name}last_page_len")
-    return host, _page_id_range(indices, host)
+    return host, _PageIds(indices, host)
 
 
 def _prefix_ranges(prefix_requests) -> torch.Tensor:
@@ -126,19 +155,19 @@ class _SegmentDecode:
             raise ValueError("tail indptr, indices and last_page_len go together")
         if tail_indptr is None:
             return None, None
-        tail, tail_range = _tables(tail_indptr, tail_indices, tail_last_page_len, "tail")
+        tail, tail_ids = _tables(tail_indptr, tail_indices, tail_last_page_len, "tail")
         if tail.numel() != host.numel():
             raise ValueError("history and tail page tables must cover the same batch")
-        return tail, tail_range
+        return tail, tail_ids
 
-    def _keep_plan(self, batch, num_qo_heads, num_kv_heads, kv_data_type, sm_scale, tables, ranges, tail_range):
+    def _keep_plan(self, batch, num_qo_heads, num_kv_heads, kv_data_type, sm_scale, tables, page_ids, tail_ids):
         self._planned = True
         self._batch, self._num_qo_heads, self._num_kv_heads = batch, num_qo_heads, num_kv_heads
         self._kv_dtype = kv_data_type
         self._sm_scale = sm_scale if sm_scale is not None else 1.0 / math.sqrt(DIM)
         self._tables = tables                       # alive, and where the kernels read
         self._table_ptrs = tuple(_ptr(t) for t in tables)
-        self._ranges, self._tail_range = ranges, tail_range
+        self._page_ids, self._tail_ids = page_ids, tail_ids
 
     def _run_args(self, q, kv_cache, k_page_scale, v_page_scale, exact_cache, value_center, out, lse, return_lse):
         """Checked pointers of a run, and its outputs."""
@@ -159,9 +188,8 @@ class _SegmentDecode:
             cache_at[3] = _capi.pointer(v_page_scale, torch.float16, (v_pages, hkv), device, _SCALES)
         elif k_page_scale is not None or v_page_scale is not None:
             raise ValueError("FP16 pages have no scales")
-        for id_range in self._ranges:
-            if id_range is not None:
-                _check_page_ids(id_range, min(k_pages, v_pages), "KV")
+        for ids in self._page_ids:
+            ids.check(min(k_pages, v_pages), "KV")
         exact_at = (None, None)
         if self._tables[-1] is not None:
             if exact_cache is None:
@@ -173,8 +201,7 @@ class _SegmentDecode:
             k_pages, v_pages = exact_k.shape[0], exact_v.shape[0]
             exact_at = (_capi.pointer(exact_k, torch.float16, (k_pages, PAGE, hkv, DIM), device, _EXACT),
                         _capi.pointer(exact_v, torch.float16, (v_pages, PAGE, hkv, DIM), device, _EXACT))
-            if self._tail_range is not None:
-                _check_page_ids(self._tail_range, min(k_pages, v_pages), "exact tail")
+            self._tail_ids.check(min(k_pages, v_pages), "exact tail")
         center_at = lse_at = None
         if value_center is not None:
             center_at = _capi.pointer(value_center, torch.float16, (batch, hkv, DIM), device, _CENTERS)
@@ -220,13 +247,14 @@ class SharedPrefixDecode(_SegmentDecode):
         if kv_data_type not in _KINDS:
             raise ValueError("pages must be int8 or float16")
         ranges = _prefix_ranges(prefix_requests)
-        host, own_range = _tables(indptr, indices, last_page_len)
-        tail, tail_range = self._plan_tail(host, tail_indptr, tail_indices, tail_last_page_len)
-        shared, shared_range = _host_i32(prefix_indptr), None
+        host, own_ids = _tables(indptr, indices, last_page_len)
+        tail, tail_ids = self._plan_tail(host, tail_indptr, tail_indices, tail_last_page_len)
+        shared, page_ids = _host_i32(prefix_indptr), [own_ids]
         if shared.shape != (len(ranges) + 1,):
             raise ValueError("prefix_indptr must have one entry per prefix and one more")
         if len(ranges):
-            shared, shared_range = _tables(prefix_indptr, prefix_indices, prefix_last_page_len, "prefix")
+            shared, shared_ids = _tables(prefix_indptr, prefix_indices, prefix_last_page_len, "prefix")
+            page_ids.append(shared_ids)
         else:
             _check_index(prefix_indices, "prefix_indices")
             _check_index(prefix_last_page_len, "prefix_last_page_len")
@@ -237,7 +265,7 @@ class SharedPrefixDecode(_SegmentDecode):
                    batch, num_qo_heads, num_kv_heads, _KINDS[kv_data_type], int(num_cus or _num_cus(indices.device)),
                    self.workspace.data_ptr(), self.workspace.numel(), self._plan_ref, _capi.current_stream())
         self._keep_plan(batch, num_qo_heads, num_kv_heads, kv_data_type, sm_scale, tables,
-                        (own_range, shared_range), tail_range)
+                        page_ids, tail_ids)
 
     def run(self, q: torch.Tensor, kv_cache, k_page_scale: Optional[torch.Tensor] = None,
             v_page_scale: Optional[torch.Tensor] = None, exact_cache=None,

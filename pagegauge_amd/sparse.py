@@ -14,7 +14,8 @@ query by a cheap score:
 * ``SelectedPagesDecode.run`` -- attention over the picked pages, an exact FP16 tail
   and the value center.
 
-Everything runs on the current stream and nothing but ``plan`` synchronises.
+Everything runs on the current stream and nothing but ``plan`` synchronises (and checks
+of page ids, as ``prefix`` says).
 """
 
 from __future__ import annotations
@@ -80,8 +81,8 @@ class SelectedPagesDecode(_SegmentDecode):
             raise ValueError("at least one page must be selected")
         if first_pages < 0 or last_pages < 0 or first_pages + last_pages > pages:
             raise ValueError(f"{first_pages} first and {last_pages} last pages do not fit {pages} selected ones")
-        host, own_range = _tables(indptr, indices, last_page_len)
-        tail, tail_range = self._plan_tail(host, tail_indptr, tail_indices, tail_last_page_len)
+        host, own_ids = _tables(indptr, indices, last_page_len)
+        tail, tail_ids = self._plan_tail(host, tail_indptr, tail_indices, tail_last_page_len)
         tables = (indices, last_page_len, tail_indices, tail_last_page_len)
         _capi.require_current_device(self.workspace, *tables)
         batch = host.numel() - 1
@@ -89,7 +90,7 @@ class SelectedPagesDecode(_SegmentDecode):
                    first_pages, last_pages, int(num_cus or _num_cus(indices.device)), self.workspace.data_ptr(),
                    self.workspace.numel(), self._plan_ref, _capi.current_stream())
         self._pages = pages
-        self._keep_plan(batch, num_qo_heads, num_kv_heads, torch.int8, sm_scale, tables, (own_range,), tail_range)
+        self._keep_plan(batch, num_qo_heads, num_kv_heads, torch.int8, sm_scale, tables, (own_ids,), tail_ids)
 
     def _selection(self, selected: torch.Tensor, device: int) -> int:
         return _capi.pointer(selected, torch.int32, (self._batch, self._num_kv_heads, self._pages), device,
@@ -112,9 +113,8 @@ class SelectedPagesDecode(_SegmentDecode):
         _check_scale(k_page_scale, "k_page_scale", pool, self._num_kv_heads)
         if k_page_scale.get_device() != device or self._device != device:
             raise ValueError(_capi.DEVICE_ERROR)
-        for id_range in self._ranges:
-            if id_range is not None and (id_range[0] < 0 or id_range[1] >= pool):
-                raise ValueError(f"page ids span [{id_range[0]}, {id_range[1]}] but bounds are of {pool} pages")
+        for ids in self._page_ids:
+            ids.check(pool, "bounds'")
         out_at = None if out is None else self._selection(out, device)
         stream = _capi.launch_stream(device)
         if out is None:

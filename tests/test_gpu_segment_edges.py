@@ -142,3 +142,47 @@ def test_selections_leave_out_entries_below_0(cuda, pages, group):
         assert np.array_equal(selected.cpu().numpy(), want)
         out, lse = selecting.run(decode, b, selected)
         check(b, out, lse, seen_of(b, selected.cpu().numpy()), single_part=False)
+
+
+def test_ended_requests_and_a_pool_cut_to_its_pages(cuda, monkeypatch):
+    """Requests end, the pool is compacted, tables are rewritten in place and the planes cut to
+    what is in use: the others' attention keeps its bits, and with ids checked, those past a
+    cut are refused."""
+    from pagegauge_amd import decode as checks
+    from pagegauge_amd import pages
+
+    monkeypatch.setattr(checks, "CHECK_PAGE_IDS", True)
+    b = Batch(cuda, [(0, 12, 700)], spread(12, 20, 200), [0] * 12, 2, 4)
+    count = len(b.cache[0])
+    pool = pages.PagePool(count, device=cuda)
+    pool.share(b.prefix_ids)
+    pool.share(b.ids)
+    bounds = selecting.bounds_of(b, cuda)
+    decode, part = planned(b, cuda, with_tail=False), selecting.planned(b, cuda, 5, with_tail=False)
+    out, lse = run(decode, b, exact_cache=None)
+    selected = part.select(b.q, bounds, b.scales[0])
+    part_out = selecting.run(part, b, selected, exact_cache=None)
+    for r in (0, 5):
+        pool.release(b.ids[int(b.own_ptr[r]):int(b.own_ptr[r + 1])].contiguous())
+    moves = pool.stage_compaction()
+    planes = (*b.cache, *b.scales, bounds)
+    pages.copy_pages(planes, moves.source, moves.target)
+    for ids in (b.prefix_ids, b.ids):
+        pages.rewrite_ids(ids, moves.remap, out=ids)
+    pool.commit_compaction(moves)
+    live = int(moves.live)
+    assert live < count and bool((b.ids < 0).any())
+    b.cache, b.scales, bounds = [c[:live].clone() for c in b.cache], [s[:live].clone() for s in b.scales], bounds[:live]
+    got, got_lse = run(decode, b, exact_cache=None)
+    got_selected = part.select(b.q, bounds, b.scales[0])
+    got_part = selecting.run(part, b, got_selected, exact_cache=None)
+    stay = [r for r in range(12) if r not in (0, 5)]
+    for x, y in ((got, out), (got_lse, lse), (got_selected, selected), *zip(got_part, part_out)):
+        assert torch.equal(x[stay], y[stay])
+    check(b, got, got_lse, seen_of(b))
+    for cut, message in ((int(b.ids.max()), "page ids span"), (0, "no pages")):
+        less = dict(kv_cache=[c[:cut] for c in b.cache], k_page_scale=b.scales[0][:cut], v_page_scale=b.scales[1][:cut])
+        with pytest.raises(ValueError, match=message):
+            run(decode, b, exact_cache=None, **less)
+        with pytest.raises(ValueError, match=message):
+            part.select(b.q, bounds[:cut], b.scales[0][:cut])

@@ -205,3 +205,27 @@ def test_cpu_tensors_are_refused():
                  lambda: sparse.SelectedPagesDecode(torch.empty(1024, dtype=torch.uint8))):
         with pytest.raises(ValueError):
             call()
+
+
+def test_page_ids_are_looked_at_again_before_they_are_refused(monkeypatch):
+    """A table rewritten in place after the plan; entries below 0 are no pages."""
+    from pagegauge_amd import decode
+
+    monkeypatch.setattr(decode, "CHECK_PAGE_IDS", True)
+    ids = torch.tensor([9, 3, 7, 12], dtype=torch.int32)
+    planned = prefix._PageIds(ids, torch.tensor([1, 4], dtype=torch.int32))
+    planned.check(13, "KV")
+    with pytest.raises(ValueError, match=r"KV page ids span \[3, 12\] but the pool holds 12 pages"):
+        planned.check(12, "KV")
+    ids.copy_(torch.tensor([99, 2, -1, 5]))
+    planned.check(6, "KV")
+    with pytest.raises(ValueError, match=r"span \[0, 5\]"):
+        planned.check(5, "KV")
+    ids.fill_(-1)                                # page 0 is read in their place
+    planned.check(1, "KV")
+    monkeypatch.setattr(decode, "CHECK_PAGE_IDS", False)
+    for unchecked in (planned, prefix._PageIds(ids, torch.tensor([1, 4], dtype=torch.int32))):
+        with pytest.raises(ValueError, match="no pages"):
+            unchecked.check(0, "KV")
+    empty = prefix._PageIds(ids, torch.tensor([0, 0], dtype=torch.int32))
+    empty.check(0, "KV")
