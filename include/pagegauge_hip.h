@@ -803,8 +803,8 @@ int32_t pg_copy_pages(const pg_page_plane_t* host_planes, int32_t planes, int64_
                       const int32_t* source, const int32_t* target, int64_t moves, void* stream);
 
 /* Users per page: refs int32 [pages], 16-byte aligned.  Adds ``by`` to refs[ids[i]]
- * for each i < count, by < 0 to no less than 0.  Ids may repeat; those outside
- * [0, pages) are skipped. */
+ * for each i < count, by < 0 to no less than 0; a count that reaches 2^31 - 1 stays
+ * there.  Ids may repeat; those outside [0, pages) are skipped. */
 int32_t pg_pool_adjust(int32_t* refs, int64_t pages, const int32_t* ids, int64_t count, int32_t by,
                        void* stream);
 

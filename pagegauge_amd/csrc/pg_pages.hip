@@ -95,12 +95,15 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(int32_t* refs, int32_t
   const int32_t id = ids[i];
   if (id < 0 || id >= pages) return;
   if (by > 0) {
-    atomicAdd(refs + id, by);
+    // Past int32 the count would be that of a free page: it is put to the largest one and
+    // stays there.  The last to touch a count that passed it is one that puts it there: the
+    // first addition after that passes it again.
+    if (atomicAdd(refs + id, by) > INT32_MAX - by) atomicExch(refs + id, INT32_MAX);
     return;
   }
   // never below zero: a page that nobody uses stays free
   int32_t seen = refs[id];
-  while (seen > 0) {
+  while (seen > 0 && seen < INT32_MAX) {
     const int32_t old = atomicCAS(refs + id, seen, max(seen + by, 0));
     if (old == seen) break;
     seen = old;

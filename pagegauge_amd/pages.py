@@ -154,13 +154,15 @@ class PagePool:
 
     def share(self, ids: torch.Tensor, users: int = 1) -> None:
         """``users`` more users of each of the pages ``ids`` (device int32 [n]).  Ids may
-        repeat; those outside the pool (-1) are skipped."""
+        repeat; those outside the pool (-1) are skipped.  A count that reaches 2^31 - 1 stays
+        there: the page is never free again, but by a write to ``refs``."""
         if not 0 < users < 2 ** 31:
             raise ValueError("users must be positive")
         self._adjust(ids, users)
 
     def release(self, ids: torch.Tensor, users: int = 1) -> None:
-        """``users`` fewer users of each of the pages, not below none."""
+        """``users`` fewer users of each of the pages, not below none; a count of 2^31 - 1
+        stays."""
         if not 0 < users < 2 ** 31:
             raise ValueError("users must be positive")
         self._adjust(ids, -users)

@@ -242,3 +242,21 @@ def test_refuses(cuda):
             call()
     with pytest.raises(RuntimeError, match="more moves"):
         pool.commit_compaction(pages.PagePool(20, device=cuda).stage_compaction())
+
+
+@pytest.mark.parametrize("users", [1, 2 ** 20, 2 ** 30, 2 ** 31 - 1])
+def test_counts_stay_at_the_largest(cuda, users):
+    """A count past int32 stays at 2^31 - 1 for good: the page is never handed out."""
+    from pagegauge_amd import pages
+
+    most = 2 ** 31 - 1
+    pool = pages.PagePool(8, device=cuda)
+    pool.refs.copy_(ints([0, most - 1, most, most - users, 5, 1, 1, 1], cuda))
+    ids = [0, 1, 2, 3, 3, -1, 8] + [4] * 5000
+    pool.share(ints(ids, cuda), users)
+    want = [min(users, most), most, most, most, min(5 + 5000 * users, most), 1, 1, 1]
+    assert pool.refs.tolist() == want
+    pool.release(ints([1, 2, 3, 3, 0], cuda), users)
+    want[0] = most if users == most else 0
+    assert pool.refs.tolist() == want
+    assert pool.take(8).tolist() == ([-1] if users == most else [0]) + [-1] * 7
