@@ -18,6 +18,11 @@ constexpr float kRescaleLimit = 8.0f;                    // log2
 // Probabilities are 2^7 times what the running maximum makes them, so at most 2^15 where it
 // lags: as far up in FP16's range as goes, for the small ones' sake.
 constexpr float kProbabilityExponent = 7.0f;
+// A maximum past which scores are scaled before it comes off them: the product that it was
+// rounded from may be further above it than FP16's range allows, from 2^26 on.
+// A row that has seen nothing, or an infinity, has no part in that: other rows keep their bits.
+constexpr float kLargeScore = 0x1p20f;
+constexpr float kNoSuchScore = 0x1p127f;
 // The running maximum before the first score.  Finite, so that a tile of -inf scores adds
 // probabilities of 0 and not exp2(-inf + inf).
 constexpr float kLowest = -__FLT_MAX__;
@@ -282,6 +287,19 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
     load_k(next);
     load_v(next);
   };
+  // the products each by itself, not within the sum with the base
+  auto scale_scores = [&](float (&kf)[kSteps]) {
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float x = s[b][r] * kf[2 * b + r / 8];
+        consume_point(x);
+        s[b][r] = x;
+      }
+#pragma unroll
+    for (int p = 0; p < kSteps; ++p) kf[p] = 1.0f;
+  };
   // tiles without a masked token or a missing page
   auto body = [&](int j, int buffer) {
     __syncthreads();
@@ -293,6 +311,7 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
     stage_next(j, buffer);
     const float mx = maximum(s, kf);
     raise(mx);
+    if (__builtin_amdgcn_ballot_w64(fabsf(m) > kLargeScore && fabsf(m) < kNoSuchScore)) scale_scores(kf);
     __builtin_amdgcn_s_setprio(1);
     attend(buffer, s, kf, vf);
     __builtin_amdgcn_s_setprio(0);
@@ -303,6 +322,7 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
     float kf[kSteps], vf[kSteps];
     factors(j, kf, vf);
     qk(buffer, s);
+    scale_scores(kf);
     int end[kSteps];                                     // of what is visible, for the wave's pages
 #pragma unroll
     for (int p = 0; p < kSteps; ++p) end[p] = lds.ids[kTilePages * j + 2 * part + p] < 0 ? 0 : visible;
@@ -311,10 +331,8 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int token = kTileTokens * j + 32 * (part + b) + 8 * (r / 4) + 4 * half + r % 4;
-        s[b][r] = token < end[2 * b + r / 8] ? s[b][r] * kf[2 * b + r / 8] : kNoScore;
+        s[b][r] = token < end[2 * b + r / 8] ? s[b][r] : kNoScore;
       }
-#pragma unroll
-    for (int p = 0; p < kSteps; ++p) kf[p] = 1.0f;
     const float mx = maximum(s, kf);
     raise(mx);
     attend(buffer, s, kf, vf);

@@ -1,6 +1,6 @@
 """Attention over shared prefixes and selected pages where a call is allowed and rare:
-pages without a token left, tables that lose pages after the plan (tolerances:
-segment_helpers).
+pages without a token left, tables that lose pages after the plan, scores of any size
+(tolerances: segment_helpers).
 
 A prefix of up to 32 query rows per KV head takes the form without tiles, of up to 64 the
 one with tiles of two waves' rows, of more the one of four."""
@@ -12,7 +12,7 @@ import pytest
 import torch
 
 import test_gpu_sparse as selecting
-from segment_helpers import Batch, check_head, values
+from segment_helpers import LOG2E, Batch, check_head, values
 from test_gpu_prefix import both_kinds, planned, run, spread
 
 pytestmark = pytest.mark.gpu
@@ -186,3 +186,72 @@ def test_ended_requests_and_a_pool_cut_to_its_pages(cuda, monkeypatch):
             run(decode, b, exact_cache=None, **less)
         with pytest.raises(ValueError, match=message):
             part.select(b.q, bounds[:cut], b.scales[0][:cut])
+
+
+@both_kinds
+@pytest.mark.parametrize("requests", FORMS)
+@pytest.mark.parametrize("sm_scale", [2.0 ** -60, 128 ** -0.5, 2.0 ** 30, float(np.nextafter(np.float32(2.0 ** 80), 0.0))])
+def test_scores_of_any_size(cuda, requests, kind, sm_scale):
+    """Queries of +-2^15 meet keys that are the same in all dims: every score is exact and they
+    are equal or at least 2^6 apart in base 2, or with the smallest softmax scale within 2^-16
+    of each other.  A row sees the mean of the values at its largest score, or of all."""
+    print(f"scores {requests} {kind} {sm_scale}", flush=True)
+    b = Batch(cuda, [(0, requests, 1000)], spread(requests, 17, 70), spread(requests, 0, 40), 1, 4, kind)
+    gen = torch.Generator().manual_seed(3)
+    b.q = (torch.randint(0, 2, (requests, 4, 1), generator=gen) * 2 - 1).expand(requests, 4, 128).half() * 2.0 ** 15
+    b.q = b.q.contiguous().to(cuda)
+    pool = len(b.cache[0])
+    sign = (torch.randint(0, 5, (pool, 16, 1, 1), generator=gen) == 0).expand(pool, 16, 1, 128).to(cuda)
+    if kind is torch.int8:
+        b.cache[0] = torch.where(sign, 127, -128).to(torch.int8)
+        b.scales[0].fill_(2.0 ** 15)
+    else:
+        b.cache[0] = torch.where(sign, 2.0 ** 15, -2.0 ** 14).half()
+    pages = len(b.exact[0])
+    b.exact[0] = torch.where(sign.repeat(2, 1, 1, 1)[:pages] if pages > pool else sign[:pages], 2.0 ** 15, 2.0 ** 9).half()
+    out, lse = run(planned(b, cuda), b, sm_scale=sm_scale)
+    seen = b.keys_and_values()
+    for r in range(requests):
+        k, v = seen(r, 0)
+        for row in range(4):
+            s = b.q[r, row].double().cpu().numpy() @ k.T * (np.float64(np.float32(sm_scale)) * LOG2E)
+            weight = np.exp2(s - s.max())
+            want = weight @ v / weight.sum() + b.center[r, 0].double().cpu().numpy()
+            # a weight is 1, 0 or off by 2^-14 of itself; two-part probabilities are off by 2^-20,
+            # one-part ones by 2^-11, sums by T / 16 + 64 float32 roundings
+            bound = (2.0 ** -13 + 2.0 ** -11 + len(k) * 2.0 ** -28) * np.abs(v).max()
+            got = out[r, row].double().cpu().numpy()
+            assert (np.abs(got - want) <= bound + np.abs(want) * 2.0 ** -11 + 2.0 ** -24).all(), (r, row)
+            want_lse = s.max() + np.log2(weight.sum())
+            assert abs(float(lse[r, row]) - want_lse) <= 2.0 ** -21 * abs(want_lse) + 2.0 ** -12, (r, row)
+
+
+def test_softmax_scales_past_float32_are_refused(cuda):
+    """Scores of INT8 pages reach 2^46, times 2^80 and log2(e) still float32."""
+    b = Batch(cuda, [(0, 2, 40)], [20, 3], [5, 5], 2, 4)
+    decode = planned(b, cuda)
+    for sm_scale in (2.0 ** 80, 2.0 ** 99):
+        with pytest.raises(RuntimeError, match="sm_scale"):
+            run(decode, b, sm_scale=sm_scale)
+
+
+def test_selected_pages_with_scores_of_any_size(cuda):
+    """Codes, scales and queries at their largest: the exact tail's scores are far below."""
+    b = Batch(cuda, [], [1000, 90], [40, 0], 1, 4)
+    b.q = torch.full_like(b.q, 2.0 ** 15)
+    b.cache[0].fill_(-128)
+    b.cache[0][b.ids[::2].long()] = 127
+    b.scales[0].fill_(2.0 ** 15)
+    decode = selecting.planned(b, cuda, 8)
+    selected = decode.select(b.q, selecting.bounds_of(b, cuda), b.scales[0])
+    for sm_scale in (128 ** -0.5, 2.0 ** 79):
+        out, lse = selecting.run(decode, b, selected, sm_scale=sm_scale)
+        seen = b.keys_and_values(selected.cpu().numpy())
+        for r in range(2):
+            k, v = seen(r, 0)
+            top = k[:, 0] == k[:, 0].max()
+            want = v[top].mean(0) + b.center[r, 0].double().cpu().numpy()
+            got = out[r].double().cpu().numpy()
+            assert (np.abs(got - want) <= 2.0 ** -10 * np.abs(v).max() + np.abs(want) * 2.0 ** -11).all()
+            s = 128 * 2.0 ** 15 * k[:, 0].max() * np.float64(np.float32(sm_scale)) * LOG2E
+            assert np.allclose(lse[r].cpu().numpy(), s + np.log2(top.sum()), rtol=2.0 ** -21, atol=0)
