@@ -134,8 +134,9 @@ __device__ __forceinline__ void scale_sums(RowState& st, const float (&f)[4]) {
 // pages' V scales (with kScaled), ``scale`` the softmax scale in base 2, ``exponent`` that
 // of the sums.  The base comes off the scores before they are scaled: past 2^24 a product less
 // the rounded product of the base could be anything (fused the other way an operation less per
-// score: 61 requests over FP16 pages 33.5 us, 34.1 so; over INT8 pages the same).  p: the lane's rows of the A operand of P V; the FP16 part and the remainder in
-// one, or with kWide in one after the other.
+// score: 61 requests over FP16 pages 33.5 us, 34.1 so; over INT8 pages the same).
+// p: the lane's rows of the A operand of P V; the FP16 part and the remainder in one, or with
+// kWide in one after the other.
 template <int kPages, bool kScaled, bool kWide>
 __device__ __forceinline__ void softmax_step(RowState& st, const float (&s)[kPages][4],
                                              const float (&v_scale)[kPages], float scale, float slack,
