@@ -85,6 +85,7 @@ struct Int4Args {
   uint16_t* out;
   float* lse;
   float sm_scale_log2;
+  float slack;                     // how far a score, not yet scaled, may pass the base
   int num_qo_heads, num_kv_heads, group;
 };
 
@@ -124,11 +125,10 @@ __device__ __forceinline__ float times_half(float x, uint32_t pair, int which) {
 constexpr float kSlack = 4.0f;     // how far (base 2) a score may pass the base
 
 // Running state of one wave.  Lane (kg, n) has head n % 8's (kWide: n's): base (before the
-// softmax scale), limit past which it moves, and offset, the exponent of the sums
-// minus the scaled base; l sums the lane's own tokens.  acc[nb][r] is row 4 kg + r of
-// the product, channel 8 n + nb.
+// softmax scale), and shift, which is the base or 0 before there is one; l sums the
+// lane's own tokens.  acc[nb][r] is row 4 kg + r of the product, channel 8 n + nb.
 struct State {
-  float base, limit, offset;
+  float base, shift;
   float l[2];                      // of tokens 4 kg, 4 kg + 1 and of the other two
   v4f acc[8];
 };
@@ -142,28 +142,28 @@ __device__ __forceinline__ void scale_sums(State& st, const float (&f)[4]) {
 
 // Softmax step over kPages pages: s are the lane's scores, masked ones -inf,
 // v_scale pairs of V's scales (FP16; 0 where masked), ``scale`` the softmax scale
-// in base 2, ``exponent`` that of the sums.  p: the lane's rows of the A operand
+// in base 2, ``exponent`` that of the sums.  The base comes off the scores before they are
+// scaled: past 2^24 a product less the rounded product of the base could be anything.  p: the lane's rows of the A operand
 // of P V, with kCodes times V's scales; rows of the FP16 part and of the remainder in
 // one, or with kWide in one after the other.
 template <int kPages, bool kCodes, bool kWide>
 __device__ __forceinline__ void softmax_step(State& st, const float (&s)[kPages][4],
                                              const uint32_t (&v_scale)[kPages][2], float scale,
-                                             float exponent, float low_part, int lane,
-                                             v8h (&p)[1 + kWide][kPages / 2]) {
+                                             float slack, float exponent, float low_part,
+                                             int lane, v8h (&p)[1 + kWide][kPages / 2]) {
   float top = kNegInf;
 #pragma unroll
   for (int i = 0; i < kPages; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][r]);
-  if (__builtin_amdgcn_ballot_w64(top > st.limit)) {
+  if (__builtin_amdgcn_ballot_w64(top - st.base > slack)) {
     top = fmaxf(top, __shfl_xor(top, 16, kWave));
     top = fmaxf(top, __shfl_xor(top, 32, kWave));
     const float base = fmaxf(st.base, top);
-    // a head with nothing visible yet keeps a base of -inf and an offset of 0
+    // a head with nothing visible yet keeps a base of -inf
     const float alpha = base == kNegInf ? 1.0f : __builtin_amdgcn_exp2f((st.base - base) * scale);
     st.base = base;
-    st.limit = base + kSlack / scale;
-    st.offset = base == kNegInf ? exponent : fmaf(-base, scale, exponent);
+    st.shift = base == kNegInf ? 0.0f : base;
     st.l[0] *= alpha;
     st.l[1] *= alpha;
     const int kg = lane >> 4;
@@ -178,8 +178,8 @@ __device__ __forceinline__ void softmax_step(State& st, const float (&s)[kPages]
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
       const int page = 2 * j + (h >> 1), r = 2 * (h & 1);
-      const float x0 = __builtin_amdgcn_exp2f(fmaf(s[page][r], scale, st.offset));
-      const float x1 = __builtin_amdgcn_exp2f(fmaf(s[page][r + 1], scale, st.offset));
+      const float x0 = __builtin_amdgcn_exp2f(fmaf(s[page][r] - st.shift, scale, exponent));
+      const float x1 = __builtin_amdgcn_exp2f(fmaf(s[page][r + 1] - st.shift, scale, exponent));
       st.l[h & 1] += x0 + x1;
       const float w0 = kCodes ? times_half(x0, v_scale[page][h & 1], 0) : x0;
       const float w1 = kCodes ? times_half(x1, v_scale[page][h & 1], 1) : x1;
@@ -241,8 +241,8 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
   const float low_part = kWide || n >= kHeads ? 1.0f : 0.0f;
 
   State st;
-  st.base = st.limit = kNegInf;
-  st.offset = st.l[0] = st.l[1] = 0.0f;
+  st.base = kNegInf;
+  st.shift = st.l[0] = st.l[1] = 0.0f;
 #pragma unroll
   for (int nb = 0; nb < 8; ++nb) st.acc[nb] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   float exponent = 0.0f;           // of the sums l and acc
@@ -304,7 +304,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
       largest = fmaxf(largest, __shfl_xor(largest, 32, kWave));
       int e = 0;
       if (largest > 0.0f) frexpf(largest, &e);
-      exponent = st.offset = static_cast<float>(10 - e);
+      exponent = static_cast<float>(10 - e);
     }
 
     const Exponents at;
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
         }
       }
       v8h p[1 + kWide][kInt4GroupPages / 2];
-      softmax_step<kInt4GroupPages, true, kWide>(st, s, v_scale, a.sm_scale_log2, exponent, low_part, lane, p);
+      softmax_step<kInt4GroupPages, true, kWide>(st, s, v_scale, a.sm_scale_log2, a.slack, exponent, low_part, lane, p);
 #pragma unroll
       for (int i = 0; i < kInt4GroupPages; ++i) consume_point(cur.v[i]);
       auto product = [&](const v8h (&rows)[1 + kWide], v8h columns, v4f sum) {
@@ -395,7 +395,6 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
     const float change = __builtin_amdgcn_exp2f(10.0f - exponent);
     st.l[0] *= change;
     st.l[1] *= change;
-    st.offset += 10.0f - exponent;
     const float f[4] = {change, change, change, change};
     scale_sums(st, f);
     exponent = 10.0f;
@@ -432,7 +431,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4Args a) {
       }
       v8h p[1 + kWide][1];
       const uint32_t unscaled[2][2] = {};
-      softmax_step<2, false, kWide>(st, s, unscaled, a.sm_scale_log2, exponent, low_part, lane, p);
+      softmax_step<2, false, kWide>(st, s, unscaled, a.sm_scale_log2, a.slack, exponent, low_part, lane, p);
 #pragma unroll
       for (int nb = 0; nb < 8; ++nb) {
         v4u cols;
@@ -571,9 +570,9 @@ extern "C" int32_t pg_int4_decode_run(const pg_int4_plan_t* plan, const void* qu
     return fail(PG_ERROR_INVALID_ARGUMENT, "history segment tensors missing");
   if (plan->has_tail && (!tail_k || !tail_v || !tail_indices || !tail_last_len))
     return fail(PG_ERROR_INVALID_ARGUMENT, "tail segment tensors missing");
-  // the kernel multiplies it by log2(e), and scores of any FP16 values by that
-  if (!(sm_scale > 0.0f) || !(sm_scale < 0x1p100f))
-    return fail(PG_ERROR_INVALID_ARGUMENT, "sm_scale must be positive and below 2^100");
+  // times log2(e) and a score, which comes to 2^42 with codes and scales, it stays in float32
+  if (!(sm_scale > 0.0f) || !(sm_scale < 0x1p80f))
+    return fail(PG_ERROR_INVALID_ARGUMENT, "sm_scale must be positive and below 2^80");
   for (const void* p : {query, codes, scales, tail_k, tail_v})
     if (reinterpret_cast<uintptr_t>(p) % 16)
       return fail(PG_ERROR_INVALID_ARGUMENT, "queries and pages must be 16-byte aligned");
@@ -606,6 +605,7 @@ extern "C" int32_t pg_int4_decode_run(const pg_int4_plan_t* plan, const void* qu
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
   a.sm_scale_log2 = sm_scale * 1.4426950408889634f;
+  a.slack = std::min(kSlack / a.sm_scale_log2, __FLT_MAX__);
   a.num_qo_heads = plan->num_qo_heads;
   a.num_kv_heads = plan->num_kv_heads;
   a.group = plan->num_qo_heads / plan->num_kv_heads;

@@ -323,3 +323,38 @@ def test_gradients_are_refused(cuda):
             c.run(**{name: t})
         with torch.no_grad():
             assert torch.equal(c.run(**{name: t})[0], want[0])
+
+
+@pytest.mark.parametrize("kv_heads,group", [(2, 4), (1, 16)])
+@pytest.mark.parametrize("sm_scale", [128 ** -0.5, 2.0 ** 30, 2.0 ** 79])
+@pytest.mark.parametrize("with_tail", [True, False])
+def test_scores_of_any_size(cuda, kv_heads, group, sm_scale, with_tail):
+    """Queries of +-2^15 and scales of 2^15: a score is 2^30 times a whole number, exact, so a
+    weight is 1 or 0.  With a tail, whose keys are +-2^15 in all dims, it has the largest ones."""
+    c = Case(cuda, [1000, 3000, 40, 0], [40, 0, 16, 300], kv_heads, group, with_tail=with_tail)
+    c.q = torch.where(c.q[:, :, :1] > 0, 2.0 ** 15, -2.0 ** 15).half().expand(c.q.shape).contiguous()
+    c.scales[:, :, :, 0] = 2.0 ** 15
+    c.exact[0] = torch.where(c.exact[0][..., :1] > 0, 2.0 ** 15, -2.0 ** 15).half().expand(c.exact[0].shape).contiguous()
+    out, lse = c.run(sm_scale=sm_scale)
+    (kc, ks), (vc, vs) = unpack(c.codes, c.scales)
+    pools = [(kc * ks.astype(np.float64)[..., None], vc * vs.astype(np.float64)[..., None]),
+             tuple(t.double().cpu().numpy() for t in c.exact)]
+    for b in range(c.batch):
+        rows = [[p[ids.cpu().numpy()[indptr[b]:indptr[b + 1]]].reshape(-1, kv_heads, 128)[:tokens[b]] for p in pool]
+                for tokens, (indptr, ids, _), pool in zip((c.history, c.tail)[:1 + with_tail], c.tables, pools)]
+        k, v = (np.concatenate(x) for x in zip(*rows))
+        for head in range(kv_heads * group):
+            h = head // group
+            center = c.center[b, h].double().cpu().numpy()
+            got = out[b, head].double().cpu().numpy()
+            if not len(k):
+                assert np.array_equal(got, center) and float(lse[b, head]) == -np.inf
+                continue
+            s = k[:, h] @ c.q[b, head].double().cpu().numpy()
+            top = s == s.max()
+            want = v[top, h].mean(0) + center
+            # equal weights in two parts (2^-20), sums of float32, the output's half step
+            bound = (2.0 ** -19 + len(k) * 2.0 ** -24) * np.abs(v[:, h]).max()
+            assert (np.abs(got - want) <= bound + np.abs(want) * 2.0 ** -11 + 2.0 ** -24).all(), (b, head)
+            want_lse = s.max() * np.float64(np.float32(sm_scale)) * np.log2(np.e) + np.log2(top.sum())
+            assert abs(float(lse[b, head]) - want_lse) <= 2.0 ** -21 * abs(want_lse), (b, head)
