@@ -907,7 +907,8 @@ int32_t pg_prefix_run(const pg_segment_plan_t* plan, const void* query, int64_t 
 
 /* bounds int8 [pool_pages, Hkv, 2, 128]: the least and the largest code of each channel
  * of pages page_ids[i], i < count (NULL: page i), over their first lengths[i] tokens
- * (NULL: 16; 127 and -128 where that is 0).  Ids outside the pool are skipped, the
+ * (NULL: 16; 127 and -128 where that is 0, which score least of all bounds under the
+ * same scale above 0).  Ids outside the pool are skipped, the
  * others must differ from each other. */
 int32_t pg_sparse_key_bounds(const void* key_codes, void* bounds, int64_t pool_pages,
                              const int32_t* page_ids, const int32_t* lengths, int64_t count,
@@ -925,7 +926,7 @@ int32_t pg_sparse_plan(const int32_t* host_indptr, const int32_t* host_tail_indp
  * to even, at most 127 of them, where its largest magnitude is f 2^x with f in [0.5, 1),
  * a page scores
  *   max over the KV head's query heads of
- *     f32(sum_d max(q'_d lo_d, q'_d hi_d) * key_scale) * 2^(x - 7),
+ *     f32(sum_d (max(q'_d, 0) hi_d + min(q'_d, 0) lo_d) * key_scale) * 2^(x - 7),
  * -inf for a row with an infinity or NaN, where the score is NaN, and for a page id below
  * 0.  Taken are the first and last pages, and of the others those with the highest
  * scores, among equal ones the lowest positions. */

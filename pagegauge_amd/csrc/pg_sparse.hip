@@ -2,7 +2,7 @@
 // the bounds, the scores that they give, the choice, and the attention over it.
 //
 // Bounds are the least and the largest K code of each channel of a (page, KV head).  For a
-// query row q, the largest product that a key between them could have is
+// query row q, the largest product that a key between them (lo <= hi) could have is
 //   sum_d max(q_d hi_d, q_d lo_d) = sum_d q+_d hi_d + q-_d lo_d,   q+ = max(q, 0), q- = min(q, 0),
 // a product of 256 terms, and with q in whole steps of a power of two, one of 8-bit integers
 // on the matrix cores: exact, so that the choice does not depend on an order of additions.

@@ -41,8 +41,10 @@ def key_bounds(key_codes: torch.Tensor, bounds: torch.Tensor, *, page_ids: Optio
     """Write the bounds of pages ``page_ids`` (device int32 [n]; None: the whole pool)
     of ``key_codes`` int8 [pages, 16, Hkv, 128] into ``bounds`` [pages, Hkv, 2, 128].
     ``lengths`` (device int32 [n]) is the tokens that each page holds, 16 if not given;
-    a page without tokens gets 127 and -128, the lowest of all scores.  Ids outside the
-    pool (-1) are skipped; the others must differ from each other."""
+    a page without tokens gets 127 and -128, whose score is the lowest that bounds under
+    the same K scale (above 0) can have: a page that was never written and has a scale of 0
+    scores 0.  Ids outside the pool (-1) are skipped; the others must differ from each
+    other."""
     if key_codes.dim() != 4 or key_codes.shape[2] == 0:
         raise ValueError("key_codes must be contiguous int8 [pages,16,Hkv,128]")
     pages, _, heads, _ = key_codes.shape

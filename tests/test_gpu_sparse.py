@@ -277,3 +277,28 @@ def test_refuses(cuda):
             (b.cache[0], bounds, dict(page_ids=b.ids, lengths=b.ids[:3]), "lengths")):
         with pytest.raises(ValueError, match=message):
             sparse.key_bounds(codes, x, **over)
+
+
+def test_scores_are_the_headers(cuda):
+    """Pages without tokens and scales of 0, both at once, and below it: the C header's formula
+    as it stands, sum_d (max(q', 0) hi + min(q', 0) lo), for any bounds."""
+    b = Batch(cuda, [], [3000, 1000], [0, 0], 2, 4)
+    bounds = bounds_of(b, cuda)
+    at = b.ids.long()
+    for every, first in ((5, 1), (7, 2)):                 # some with a scale, some without
+        bounds[at[first::every], :, 0], bounds[at[first::every], :, 1] = 127, -128
+    b.scales[0][at[2::7]] = 0
+    b.scales[0][at[3::11]] *= -1
+    got = planned(b, cuda, 40, 0, 0, with_tail=False).select(b.q, bounds, b.scales[0]).cpu().numpy()
+    q, low, high = b.q.double().cpu().numpy(), *bounds.cpu().numpy().astype(np.int64).transpose(2, 0, 1, 3)
+    scale = b.scales[0].float().cpu().numpy()
+    for i in range(2):
+        ids = at[int(b.own_ptr[i]):int(b.own_ptr[i + 1])].cpu().numpy()
+        for h in range(2):
+            best = np.full(len(ids), -np.inf, np.float32)
+            for row in q[i, 4 * h:4 * h + 4]:
+                x = int(np.frexp(np.abs(row).max())[1])
+                steps = np.clip(np.rint(np.ldexp(row, 7 - x)), -127, 127).astype(np.int64)
+                total = (np.maximum(steps, 0) * high[ids, h] + np.minimum(steps, 0) * low[ids, h]).sum(1)
+                best = np.maximum(best, np.float32(total) * scale[ids, h] * np.float32(2.0 ** (x - 7)))
+            assert got[i, h].tolist() == sorted(np.argsort(-best, kind="stable")[:40])
