@@ -276,7 +276,11 @@ class SharedPrefixDecode(_SegmentDecode):
         (K, V) pages of prefixes and own tables, with INT8 pages their scales
         [pages, Hkv]; ``exact_cache`` the (K, V) pages of the tail, ``value_center``
         [B, Hkv, 128].  A request without tokens gives its center (or zeros) and an lse
-        of -inf.  Tensors that autograd follows are refused: there is no backward pass."""
+        of -inf.  Weights of prefixes with up to 32 query rows (requests times heads of a
+        KV head's group), of own pages and of the tail are good to 2^-20 of themselves
+        beside their scores' rounding, those of larger prefixes to 2^-11, so that an output
+        is off by that part of the weighted mean of |V|.  Tensors that autograd follows are
+        refused: there is no backward pass."""
         if not self._planned:
             raise RuntimeError("plan() must be called before run()")
         cache_at, exact_at, center_at, out, lse, out_at, lse_at, stream = self._run_args(
