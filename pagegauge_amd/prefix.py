@@ -67,6 +67,11 @@ class _PageIds:
         found = _page_id_range(self._indices, self._indptr)
         self._range = None if found is None else tuple(max(i, 0) for i in found)
 
+    @property
+    def need(self) -> int:
+        """The fewest pages of a pool that ``check`` takes without another look."""
+        return 0 if self._empty else 1 if self._range is None else self._range[1] + 1
+
     def check(self, pool_pages: int, what: str) -> None:
         """All ids are of a pool of so many pages.  Tables may be rewritten in place after the
         plan: one whose ids were too large is looked at again before it is refused, which waits
@@ -167,7 +172,19 @@ class _SegmentDecode:
         self._sm_scale = sm_scale if sm_scale is not None else 1.0 / math.sqrt(DIM)
         self._tables = tables                       # alive, and where the kernels read
         self._table_ptrs = tuple(_ptr(t) for t in tables)
-        self._page_ids, self._tail_ids = page_ids, tail_ids
+        self._page_ids, self._tail_ids = page_ids, () if tail_ids is None else (tail_ids,)
+        self._need, self._tail_need = (max((ids.need for ids in t), default=0) for t in (page_ids, self._tail_ids))
+
+    def _check_pool(self, pool_pages: int, what: str) -> None:
+        """A pool with fewer pages than the tables needed when last looked at."""
+        for ids in self._page_ids:
+            ids.check(pool_pages, what)
+        self._need = max(ids.need for ids in self._page_ids)
+
+    def _check_exact(self, pool_pages: int) -> None:
+        for ids in self._tail_ids:
+            ids.check(pool_pages, "exact tail")
+            self._tail_need = ids.need
 
     def _run_args(self, q, kv_cache, k_page_scale, v_page_scale, exact_cache, value_center, out, lse, return_lse):
         """Checked pointers of a run, and its outputs."""
@@ -188,8 +205,8 @@ class _SegmentDecode:
             cache_at[3] = _capi.pointer(v_page_scale, torch.float16, (v_pages, hkv), device, _SCALES)
         elif k_page_scale is not None or v_page_scale is not None:
             raise ValueError("FP16 pages have no scales")
-        for ids in self._page_ids:
-            ids.check(min(k_pages, v_pages), "KV")
+        if min(k_pages, v_pages) < self._need:
+            self._check_pool(min(k_pages, v_pages), "KV")
         exact_at = (None, None)
         if self._tables[-1] is not None:
             if exact_cache is None:
@@ -201,7 +218,8 @@ class _SegmentDecode:
             k_pages, v_pages = exact_k.shape[0], exact_v.shape[0]
             exact_at = (_capi.pointer(exact_k, torch.float16, (k_pages, PAGE, hkv, DIM), device, _EXACT),
                         _capi.pointer(exact_v, torch.float16, (v_pages, PAGE, hkv, DIM), device, _EXACT))
-            self._tail_ids.check(min(k_pages, v_pages), "exact tail")
+            if min(k_pages, v_pages) < self._tail_need:
+                self._check_exact(min(k_pages, v_pages))
         center_at = lse_at = None
         if value_center is not None:
             center_at = _capi.pointer(value_center, torch.float16, (batch, hkv, DIM), device, _CENTERS)

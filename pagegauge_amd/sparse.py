@@ -115,8 +115,8 @@ class SelectedPagesDecode(_SegmentDecode):
         _check_scale(k_page_scale, "k_page_scale", pool, self._num_kv_heads)
         if k_page_scale.get_device() != device or self._device != device:
             raise ValueError(_capi.DEVICE_ERROR)
-        for ids in self._page_ids:
-            ids.check(pool, "bounds'")
+        if pool < self._need:
+            self._check_pool(pool, "bounds'")
         out_at = None if out is None else self._selection(out, device)
         stream = _capi.launch_stream(device)
         if out is None:
