@@ -26,8 +26,8 @@
 //
 // Bound by HBM once a wave has several groups, by a chain of trips to memory (work item, page
 // ids, pages, partial rows) before: 512 workgroups over 256 picked pages of 8 requests' 8 heads
-// and their 128 exact pages, 75 MB, 18.8 us (4.0 TB/s: a head's rows are lines of 128 bytes apart from each
-// other); 256 requests of 6 to 63 INT8 and 16 exact pages, 558 MB, about 125 us (4.5 TB/s);
+// and their 128 exact pages, 75 MB, 19 to 21 us (3.5 to 4.0 TB/s: a head's rows are lines of 128 bytes apart
+// from each other); 256 requests of 6 to 63 INT8 and 16 exact pages, 558 MB, about 125 us (4.5 TB/s);
 // 2000 tokens of 4 requests 8.3 us.  Measured and not taken: partial rows' slots requested
 // ahead of the pages (the first of these 19.3 us: registers).
 #pragma once

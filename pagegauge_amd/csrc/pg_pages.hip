@@ -69,7 +69,7 @@ __device__ __forceinline__ void copy_block(const CopyArgs& a, const CopyPlane& p
 // 1024 vectors of 16 bytes (or what the page's size and place allow).  Bound by HBM: 540
 // exact pages of K and V in 8 layers, 566 MB read and written, 95 to 101 us (5.6 to 6.0 TB/s;
 // a copy of 1 GiB reaches 5.1), 8 pages 3.8 us; a list with empty entries costs their
-// workgroups (4096 moves of an INT8 pool in 8192 entries, 268 MB, 59 us: 4.5 TB/s).
+// workgroups (4096 moves of an INT8 pool in 8192 entries, 268 MB, 67 us: 4.0 TB/s).
 __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyArgs a) {
   int plane = 0;
   while (plane + 1 < a.planes_used && blockIdx.x >= a.planes[plane + 1].first_block) ++plane;

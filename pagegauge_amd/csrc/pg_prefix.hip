@@ -61,10 +61,11 @@ struct SharedTiles {
 // Tiles go from memory to registers a whole iteration before they are put in LDS.
 //
 // Bound by the matrix cores and the VALU together: of the cycles of 256 requests (1024 query
-// rows per KV head) over 16384 tokens MFMA takes 32 %, the VALU 49 % (35 % over FP16 pages),
-// LDS 35 %, and the two waves of a SIMD hide little of one behind the other.  69 GFLOP, 8
-// parts: 91 us over INT8 pages (753 TFLOP/s), 84 over FP16 ones (818; a library product of 8192
-// cubed reaches 1194); 48 query rows per KV head 19 us.  Measured and not taken: the scores of
+// rows per KV head) over 16384 tokens MFMA takes 32 %, the VALU 48 % (36 and 39 % over FP16
+// pages), LDS 35 %, and the two waves of a SIMD hide little of one behind the other.  69 GFLOP,
+// 8 parts: 95 us over INT8 pages (723 TFLOP/s; the median of 30 in a row 102), 86 over FP16
+// ones (797; 98; a library product of 8192 cubed reaches 1194); 48 query rows per KV head 19 us.
+// Measured and not taken, beside 91 us at the time: the scores of
 // tile j + 1 beside the softmax of tile j (one wave's 256 registers just hold it: 102 us),
 // orders of instructions for the scheduler (97 to 104), no wave priority (93.8), priority to
 // one of a CU's workgroups (96), V's scales in the exponents (the same with an eighth fewer
@@ -380,7 +381,7 @@ __device__ __forceinline__ void shared_attention(const PageAttentionArgs& a, con
 
 // The forms share a launch, so that the matrix cores' work on shared prefixes and the
 // reading of requests' own pages run side by side: 256 requests on 16384 tokens with 100 to
-// 1000 of their own and 256 exact ones, 587 MB and 72 GFLOP, 160 us, where the prefix takes 91
+// 1000 of their own and 256 exact ones, 587 MB and 72 GFLOP, 162 to 180 us, where the prefix takes 95
 // alone and the rest about 125.
 template <bool kCodes>
 __global__ __launch_bounds__(kAttentionThreads, 2) void prefix_attention_kernel(PageAttentionArgs a) {
