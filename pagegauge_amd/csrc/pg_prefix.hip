@@ -19,7 +19,7 @@ constexpr float kRescaleLimit = 8.0f;                    // log2
 // lags: as far up in FP16's range as goes, for the small ones' sake.
 constexpr float kProbabilityExponent = 7.0f;
 // A maximum past which scores are scaled before it comes off them: the product that it was
-// rounded from may be further above it than FP16's range allows, from 2^26 on.
+// rounded from may be further above it than FP16's range allows, from 2^24 on.
 // A row that has seen nothing, or an infinity, has no part in that: other rows keep their bits.
 constexpr float kLargeScore = 0x1p20f;
 constexpr float kNoSuchScore = 0x1p127f;
